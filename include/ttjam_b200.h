@@ -317,6 +317,95 @@ int tt_test_arm_wait_timeout(int budget_log2);
  * arguments. Returns TT_OK, TT_ERR_INVALID_ARGUMENT or TT_ERR_CUDA. */
 int tt_test_gelu(const float *x, float *y, int64_t n, void *stream);
 
+/* ---------------------------------------------------------------------------
+ * The 8-bit paged key/value cache: incremental use of the causal attention.
+ * The reference recomputes every key and value on every forward
+ * (BaselineSelfAttention.forward, torch_transformer_benchmark.py:93-121); with
+ * a cache, a call on new tokens reads those of the earlier ones instead. These
+ * entry points have no counterpart in the reference.
+ *
+ * Layout. A layer's keys and values are 8-bit codes in two pools of pages,
+ * [num_pages, kv_heads, page_size, head_dim], with one fp32 scale for each page
+ * and head, [num_pages, kv_heads]: value = code * scale. Tokens
+ * [c * page_size, (c + 1) * page_size) of sequence b lie in page
+ * block_table[b * table_columns + c]; lengths[b] counts the tokens of sequence
+ * b, the new ones of the call included. Sequences may share pages that are only
+ * read; a page that new tokens land in belongs to one sequence.
+ *
+ * Scales are powers of two, 2^E with E >= -64 the smallest that brings the
+ * largest magnitude of the page and head (448 for e4m3, 127 for int8) into the
+ * code's range. A value is rounded to the nearest code, ties to even. When
+ * tokens appended to a page need a larger scale than it has, its old codes are
+ * rounded again to the larger one. A NaN, an infinity or a magnitude beyond the
+ * largest code * 2^63 makes the scale of its page and head NaN: every token
+ * there then reads as NaN, until the page is written anew from its first slot.
+ *
+ * Device checks. A length, a count or a block-table entry out of its range is
+ * latched as TT_ERR_DEVICE_FAULT in *status (detail 0x5100, 0x5200 or 0x5300)
+ * and never followed: lengths and counts are clamped, tokens of a page that
+ * does not exist are dropped when written, zero when read and unseen by the
+ * attention.
+ * ------------------------------------------------------------------------ */
+
+#define TT_KV_E4M3 0 /* float8 e4m3 (torch.float8_e4m3fn) */
+#define TT_KV_INT8 1 /* int8, -127 to 127 */
+
+/* One layer's cache, all pointers to device memory that the caller owns. */
+typedef struct tt_kv_cache {
+  void *k_codes, *v_codes;       /* [num_pages, kv_heads, page_size, head_dim] bytes,
+                                    16-byte aligned */
+  float *k_scale, *v_scale;      /* [num_pages, kv_heads] */
+  const int32_t *block_table;    /* [batch, table_columns] */
+  const int32_t *lengths;        /* [batch] */
+  int32_t *status;               /* two ints (code, detail), zeroed by the caller, or NULL */
+  int32_t num_pages, page_size;  /* page_size: 16, 32, 64 or 128 */
+  int32_t kv_heads, head_dim;    /* head_dim: a multiple of 16, at most 256 */
+  int32_t batch, table_columns;
+  int32_t format;                /* TT_KV_E4M3 or TT_KV_INT8 */
+  int32_t reserved;              /* must be 0 */
+} tt_kv_cache;
+
+/* Writes the keys and values of new tokens. k and v are [batch, tokens, kv_heads,
+ * head_dim] of element type `dtype` (TT_DTYPE_*), head_dim contiguous, the
+ * three other strides in elements in k_strides and v_strides (slices of a
+ * fused projection need no copy; pointers and strides that are multiples of
+ * 16 bytes are fastest). Sequence b's first counts[b] rows are new tokens
+ * (counts NULL: all `tokens` rows), at positions lengths[b] - counts[b] up to
+ * lengths[b] - 1; the rows behind them are not read. Slots of a page behind the
+ * last token are left as they are. One launch on `stream`. */
+int tt_kv_write(const tt_kv_cache *cache, int dtype, const void *k, const void *v,
+                const int64_t *k_strides, const int64_t *v_strides, int64_t tokens,
+                const int32_t *counts, void *stream);
+
+/* Reads the first max_tokens tokens of every sequence back: k and v,
+ * [batch, max_tokens, kv_heads, head_dim] of element type `dtype`, contiguous and
+ * 16-byte aligned, receive code * scale rounded once; rows at or behind
+ * lengths[b] are 0. One launch on `stream`. */
+int tt_kv_read(const tt_kv_cache *cache, int dtype, void *k, void *v, int64_t max_tokens,
+               void *stream);
+
+/* Bytes of scratch tt_kv_attention needs for `tokens` rows of `heads` query heads
+ * on the current device (0 when it needs none, or for invalid arguments). */
+size_t tt_kv_attention_workspace_bytes(const tt_kv_cache *cache, int64_t tokens, int32_t heads);
+
+/* Causal attention of new tokens over the cache, which holds their keys and
+ * values already (tt_kv_write). q is [batch, tokens, heads, head_dim] with
+ * strides as in tt_kv_write; heads is a multiple of kv_heads, and query head h
+ * reads key head h / (heads / kv_heads). Row i < counts[b] of sequence b stands at
+ * position lengths[b] - counts[b] + i and sees the tokens up to its own:
+ * out = softmax(scale * q k^T) v, computed to fp32 accuracy and rounded once to
+ * `dtype`. out is [batch, tokens, heads, head_dim], contiguous, 16-byte aligned,
+ * written in full: rows at or behind counts[b], and rows that see no token, are
+ * 0. The workspace needs no initial value and holds nothing after the call;
+ * calls whose GPU work overlaps need one each. */
+int tt_kv_attention(const tt_kv_cache *cache, int dtype, const void *q, const int64_t *q_strides,
+                    int64_t tokens, int32_t heads, const int32_t *counts, float scale, void *out,
+                    void *workspace, size_t workspace_bytes, void *stream);
+
+/* Synchronises `stream`, reads and clears the cache's status word: *code receives
+ * TT_OK or the first latched TT_ERR_DEVICE_*, *detail which check it was. */
+int tt_kv_read_status(const tt_kv_cache *cache, int32_t *code, int32_t *detail, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

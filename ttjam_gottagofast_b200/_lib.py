@@ -43,6 +43,8 @@ EXPORTED = (
     "tt_launch_probe_start", "tt_launch_probe_read", "tt_test_arm_wait_timeout",
     "tt_pack_image_typed", "tt_typed_workspace_bytes", "tt_forward_typed",
     "tt_host_workspace_bytes", "tt_forward_host", "tt_test_gelu",
+    "tt_kv_write", "tt_kv_read", "tt_kv_attention", "tt_kv_attention_workspace_bytes",
+    "tt_kv_read_status",
 )
 
 # Element types of the typed entry points (TT_DTYPE_*), by torch dtype name.
@@ -50,6 +52,9 @@ TT_DTYPE_F32 = 0
 TT_DTYPE_F16 = 1
 TT_DTYPE_BF16 = 2
 DTYPE_CODES = {"float32": TT_DTYPE_F32, "float16": TT_DTYPE_F16, "bfloat16": TT_DTYPE_BF16}
+
+# Code formats of the 8-bit key/value cache (TT_KV_*).
+KV_FORMATS = {"e4m3": 0, "int8": 1}
 
 # TT_KERNEL_* launch kinds reported by tt_launch_probe_read.
 KERNEL_KINDS = {1: "layernorm", 2: "qkv", 3: "attention", 4: "out_proj", 5: "ffn_in",
@@ -68,6 +73,14 @@ class TTLayerParams(ctypes.Structure):
         "norm1_weight", "norm1_bias", "q_weight", "q_bias", "k_weight", "k_bias",
         "v_weight", "v_bias", "out_weight", "out_bias", "norm2_weight", "norm2_bias",
         "ffn_in_weight", "ffn_in_bias", "ffn_out_weight", "ffn_out_bias")]
+
+
+class TTKVCache(ctypes.Structure):
+    _fields_ = [*((name, ctypes.c_void_p) for name in (
+        "k_codes", "v_codes", "k_scale", "v_scale", "block_table", "lengths", "status")),
+        *((name, ctypes.c_int32) for name in (
+            "num_pages", "page_size", "kv_heads", "head_dim", "batch", "table_columns", "format",
+            "reserved"))]
 
 
 _lock = threading.Lock()
@@ -137,6 +150,18 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
         lib.tt_test_gelu.argtypes = [vp, vp, i64, vp]
         lib.tt_test_arm_wait_timeout.restype = ctypes.c_int
         lib.tt_test_arm_wait_timeout.argtypes = [ctypes.c_int]
+        kvp, i64p = ctypes.POINTER(TTKVCache), ctypes.POINTER(i64)
+        lib.tt_kv_write.restype = ctypes.c_int
+        lib.tt_kv_write.argtypes = [kvp, ctypes.c_int, vp, vp, i64p, i64p, i64, vp, vp]
+        lib.tt_kv_read.restype = ctypes.c_int
+        lib.tt_kv_read.argtypes = [kvp, ctypes.c_int, vp, vp, i64, vp]
+        lib.tt_kv_attention_workspace_bytes.restype = sz
+        lib.tt_kv_attention_workspace_bytes.argtypes = [kvp, i64, i32]
+        lib.tt_kv_attention.restype = ctypes.c_int
+        lib.tt_kv_attention.argtypes = [kvp, ctypes.c_int, vp, i64p, i64, i32, vp,
+                                        ctypes.c_float, vp, vp, sz, vp]
+        lib.tt_kv_read_status.restype = ctypes.c_int
+        lib.tt_kv_read_status.argtypes = [kvp, ctypes.POINTER(i32), ctypes.POINTER(i32), vp]
         if lib.tt_abi_version() != TT_ABI_VERSION:
             raise RuntimeError("libttjam_b200.so ABI version mismatch; rebuild it")
         _lib = lib

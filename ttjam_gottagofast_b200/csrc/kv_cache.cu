@@ -1,0 +1,402 @@
+// Writing new tokens into the 8-bit key/value cache and reading tokens back
+// (the format: kv_cache.cuh), and the C entry points of the cache.
+#include <algorithm>
+#include <cmath>
+
+#include "kv_cache.cuh"
+
+namespace tt {
+namespace {
+
+// 16 consecutive elements as fp32: four 16-byte loads (fp32) or two (16-bit).
+template <typename T, bool VEC>
+__device__ __forceinline__ void load16(const T *p, float *x) {
+  if constexpr (VEC) {
+    constexpr int N = 16 * sizeof(T) / 16, E = 16 / sizeof(T);
+    uint4 raw[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) raw[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const T *e = reinterpret_cast<const T *>(&raw[i]);
+#pragma unroll
+      for (int j = 0; j < E; ++j) x[i * E + j] = kv_to_float(e[j]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = kv_to_float(p[i]);
+  }
+}
+
+// One block per (sequence, page that new tokens of it land in, head, keys or
+// values): the block's chunks of 16 elements stay in registers between the
+// maximum and the rounding, so each new element is read once. The maximum is
+// taken on the bits of |x| (ordered like the values; infinities and NaN on
+// top), so it does not hang on the order of the reduction.
+template <typename T, int FMT, int THREADS, int NC, bool VEC>
+__global__ void __launch_bounds__(THREADS) kv_write_kernel(KvView c, const T *k, const T *v,
+                                                           KvStrides kst, KvStrides vst,
+                                                           int tokens, const int32_t *counts,
+                                                           int touched) {
+  __shared__ uint32_t s_max[THREADS / 32];
+  pdl_trigger();
+  int item = blockIdx.x;
+  const bool is_v = item & 1;
+  item >>= 1;
+  const int h = item % c.heads;
+  item /= c.heads;
+  const int b = item / touched, j = item % touched;
+  pdl_wait();
+  const int len = c.length(b), count = c.count(counts, b, tokens, len);
+  const int start = len - count, page = 1 << c.page_log2;
+  const int col = (start >> c.page_log2) + j;
+  const int lo = max(start, col << c.page_log2), hi = min(len, (col + 1) << c.page_log2);
+  if (lo >= hi) return;  // no new token of this sequence in that page
+  const int pg = c.page_of(b, col);
+  if (pg < 0) return;  // tokens of a page that does not exist are dropped
+  const T *src = is_v ? v : k;
+  const KvStrides st = is_v ? vst : kst;
+  src += b * st.batch + h * st.head;
+  uint8_t *dst = (is_v ? c.v : c.k) + c.tile(pg, h);
+  float *scale_p = (is_v ? c.vs : c.ks) + (int64_t)pg * c.heads + h;
+  const int slot = lo & (page - 1);  // tokens the page held before
+  const float old = slot > 0 ? *scale_p : 0.f;
+  const int hd16 = c.hd >> 4, chunks = (hi - lo) * hd16;
+
+  float x[NC][16];
+  uint32_t mx = 0;
+#pragma unroll
+  for (int u = 0; u < NC; ++u) {
+    const int i = threadIdx.x + u * THREADS;
+    if (i < chunks) {
+      const int t = i / hd16, d = (i - t * hd16) << 4;
+      load16<T, VEC>(src + (int64_t)(lo - start + t) * st.token + d, x[u]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[u][e] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < NC; ++u)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) mx = max(mx, __float_as_uint(x[u][e]) & 0x7fffffffu);
+  mx = __reduce_max_sync(0xffffffffu, mx);
+  if constexpr (THREADS > 32) {
+    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) mx = max(mx, s_max[w]);
+  } else {
+    __syncwarp();
+  }
+  // the exponent: |x| = 1.m * 2^e; 448 = 1.75 * 2^8, 127 = 1.984375 * 2^6
+  constexpr int TOP_E = FMT == TT_KV_INT8 ? 6 : 8;
+  constexpr uint32_t TOP_M = FMT == TT_KV_INT8 ? 0x7e0000u : 0x600000u;
+  int e = (int)(mx >> 23) - 127 - TOP_E + ((mx & 0x7fffffu) > TOP_M);
+  const bool bad = mx >= 0x7f800000u || e > kKvMostExponent || !(old == old);
+  e = max(e, kKvLeastExponent);
+  float scale = kv_pow2(bad ? 0 : e);
+  if (!bad) scale = fmaxf(scale, old);
+  const float inv = bad ? 0.f : 1.f / scale;  // a power of two: exact
+  if (threadIdx.x == 0) *scale_p = bad ? __int_as_float(0x7fc00000) : scale;
+  if (slot > 0 && !bad && scale != old) {
+    // the page's scale grew: its old codes move to the new one
+    const float ratio = old * inv;
+    for (int i = threadIdx.x; i < slot * hd16; i += THREADS) {
+      uint4 w = reinterpret_cast<uint4 *>(dst)[i];
+      uint32_t *ww = &w.x;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float y[4];
+        kv_decode4<FMT>(ww[q], y);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] *= ratio;
+        ww[q] = kv_encode4<FMT>(y);
+      }
+      reinterpret_cast<uint4 *>(dst)[i] = w;
+    }
+  }
+  uint4 *out = reinterpret_cast<uint4 *>(dst + slot * c.hd);
+#pragma unroll
+  for (int u = 0; u < NC; ++u) {
+    const int i = threadIdx.x + u * THREADS;
+    if (i >= chunks) break;
+    uint32_t w[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float y[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) y[r] = bad ? 0.f : x[u][4 * q + r] * inv;
+      w[q] = kv_encode4<FMT>(y);
+    }
+    out[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// One thread per 16 codes of (keys or values, sequence, token, head); rows
+// behind a sequence's end, and of pages that do not exist, are zero.
+template <typename T, int FMT>
+__global__ void __launch_bounds__(256) kv_read_kernel(KvView c, T *k, T *v, uint32_t per_seq) {
+  pdl_trigger();
+  pdl_wait();
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+  if (i >= per_seq) return;
+  const int b = blockIdx.y;
+  const uint32_t hd16 = c.hd >> 4;
+  const uint32_t d16 = i % hd16, r = i / hd16;
+  const int h = r % c.heads, t = r / c.heads;
+  float x[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) x[e] = 0.f;
+  if (t < c.length(b)) {
+    const int pg = c.page_of(b, t >> c.page_log2);
+    if (pg >= 0) {
+      const int64_t off = c.tile(pg, h) + (int64_t)(t & ((1 << c.page_log2) - 1)) * c.hd + 16 * d16;
+      const uint4 w = *reinterpret_cast<const uint4 *>((blockIdx.z ? c.v : c.k) + off);
+      const float s = (blockIdx.z ? c.vs : c.ks)[(int64_t)pg * c.heads + h];
+      kv_decode4<FMT>(w.x, x);
+      kv_decode4<FMT>(w.y, x + 4);
+      kv_decode4<FMT>(w.z, x + 8);
+      kv_decode4<FMT>(w.w, x + 12);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] *= s;
+    }
+  }
+  T *out = (blockIdx.z ? v : k) + ((int64_t)b * per_seq + i) * 16;
+  constexpr int N = 16 * sizeof(T) / 16, E = 16 / sizeof(T);
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    uint4 raw;
+    T *e = reinterpret_cast<T *>(&raw);
+#pragma unroll
+    for (int q = 0; q < E; ++q) kv_store(e + q, x[n * E + q]);
+    __stcs(reinterpret_cast<uint4 *>(out) + n, raw);
+  }
+}
+
+bool vec_ok(const void *p, const KvStrides &s, int size) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (s.batch * size) % 16 == 0 &&
+         (s.token * size) % 16 == 0 && (s.head * size) % 16 == 0;
+}
+
+template <typename T, int FMT, int THREADS, int NC>
+int write_nc(const KvView &c, const void *k, const void *v, KvStrides ks, KvStrides vs,
+             int tokens, const int32_t *counts, int touched, unsigned items,
+             cudaStream_t stream) {
+  const bool vec = vec_ok(k, ks, sizeof(T)) && vec_ok(v, vs, sizeof(T));
+  auto *kern = vec ? kv_write_kernel<T, FMT, THREADS, NC, true>
+                   : kv_write_kernel<T, FMT, THREADS, NC, false>;
+  TT_CUDA_TRY(launch_kernel(kern, dim3(items), dim3(THREADS), 0, stream, 1, c,
+                            static_cast<const T *>(k), static_cast<const T *>(v), ks, vs, tokens,
+                            counts, touched));
+  return TT_OK;
+}
+
+template <typename T, int FMT>
+int write_typed(const KvView &c, const void *k, const void *v, KvStrides ks, KvStrides vs,
+                int tokens, const int32_t *counts, cudaStream_t stream) {
+  const int page = 1 << c.page_log2;
+  const int touched = (tokens + page - 2) / page + 1;  // pages that `tokens` in a row can touch
+  const int64_t items = (int64_t)2 * c.heads * touched * c.batch;
+  if (items > INT32_MAX) return fail(TT_ERR_UNSUPPORTED, "tt_kv_write: too many tokens");
+  const int chunks = std::min(tokens, page) * (c.hd >> 4);  // of 16 elements, in one page
+#define TT_KV_WRITE(THREADS, NC) \
+  return write_nc<T, FMT, THREADS, NC>(c, k, v, ks, vs, tokens, counts, touched, (unsigned)items, stream)
+  if (chunks <= 32) TT_KV_WRITE(32, 1);
+  if (chunks <= 256) TT_KV_WRITE(256, 1);
+  if (chunks <= 512) TT_KV_WRITE(256, 2);
+  if (chunks <= 1024) TT_KV_WRITE(256, 4);
+  TT_KV_WRITE(256, 8);  // 128 tokens of 256 elements, the largest page
+#undef TT_KV_WRITE
+}
+
+}  // namespace
+
+int launch_kv_write(const KvView &c, int dtype, const void *k, const void *v, KvStrides ks,
+                    KvStrides vs, int64_t tokens, const int32_t *counts, cudaStream_t stream) {
+  const bool i8 = c.format == TT_KV_INT8;
+  const int n = (int)tokens;
+  switch (dtype) {
+    case TT_DTYPE_F32:
+      return i8 ? write_typed<float, TT_KV_INT8>(c, k, v, ks, vs, n, counts, stream)
+                : write_typed<float, TT_KV_E4M3>(c, k, v, ks, vs, n, counts, stream);
+    case TT_DTYPE_F16:
+      return i8 ? write_typed<__half, TT_KV_INT8>(c, k, v, ks, vs, n, counts, stream)
+                : write_typed<__half, TT_KV_E4M3>(c, k, v, ks, vs, n, counts, stream);
+    default:
+      return i8 ? write_typed<__nv_bfloat16, TT_KV_INT8>(c, k, v, ks, vs, n, counts, stream)
+                : write_typed<__nv_bfloat16, TT_KV_E4M3>(c, k, v, ks, vs, n, counts, stream);
+  }
+}
+
+template <typename T>
+static int read_typed(const KvView &c, void *k, void *v, int64_t max_tokens, cudaStream_t stream) {
+  const int64_t per_seq = max_tokens * c.heads * (c.hd >> 4);
+  if (per_seq > UINT32_MAX - 256 || c.batch > 65535)
+    return fail(TT_ERR_UNSUPPORTED, "tt_kv_read: too many tokens or sequences");
+  auto *kern = c.format == TT_KV_INT8 ? kv_read_kernel<T, TT_KV_INT8> : kv_read_kernel<T, TT_KV_E4M3>;
+  TT_CUDA_TRY(launch_kernel(kern, dim3((unsigned)ceil_div(per_seq, 256), c.batch, 2), dim3(256), 0,
+                            stream, 1, c, static_cast<T *>(k), static_cast<T *>(v),
+                            (uint32_t)per_seq));
+  return TT_OK;
+}
+
+int launch_kv_read(const KvView &c, int dtype, void *k, void *v, int64_t max_tokens,
+                   cudaStream_t stream) {
+  switch (dtype) {
+    case TT_DTYPE_F32: return read_typed<float>(c, k, v, max_tokens, stream);
+    case TT_DTYPE_F16: return read_typed<__half>(c, k, v, max_tokens, stream);
+    default: return read_typed<__nv_bfloat16>(c, k, v, max_tokens, stream);
+  }
+}
+
+// The checks every entry point makes of a cache; fills *v.
+static int kv_view(const tt_kv_cache *c, const char *what, KvView *v) {
+  auto no = [&](int code, const std::string &m) { return fail(code, std::string(what) + ": " + m); };
+  if (c == nullptr) return no(TT_ERR_INVALID_ARGUMENT, "cache is NULL");
+  if (c->format != TT_KV_E4M3 && c->format != TT_KV_INT8)
+    return no(TT_ERR_INVALID_ARGUMENT, "format must be TT_KV_E4M3 or TT_KV_INT8");
+  if (c->reserved != 0) return no(TT_ERR_INVALID_ARGUMENT, "reserved field must be 0");
+  if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128)
+    return no(TT_ERR_UNSUPPORTED, "page_size must be 16, 32, 64 or 128");
+  if (c->head_dim < 16 || c->head_dim > 256 || c->head_dim % 16 != 0)
+    return no(TT_ERR_UNSUPPORTED, "head_dim must be a multiple of 16, at most 256");
+  if (c->kv_heads <= 0 || c->num_pages <= 0 || c->batch < 0 || c->table_columns <= 0)
+    return no(TT_ERR_INVALID_ARGUMENT, "kv_heads, num_pages and table_columns must be positive");
+  if ((int64_t)c->table_columns * c->page_size > INT32_MAX)
+    return no(TT_ERR_UNSUPPORTED, "table_columns * page_size must fit 32 bits");
+  if (c->batch > 0 && (c->k_codes == nullptr || c->v_codes == nullptr || c->k_scale == nullptr ||
+                       c->v_scale == nullptr || c->block_table == nullptr || c->lengths == nullptr))
+    return no(TT_ERR_INVALID_ARGUMENT, "a cache pointer is NULL");
+  if (((reinterpret_cast<uintptr_t>(c->k_codes) | reinterpret_cast<uintptr_t>(c->v_codes)) & 15) ||
+      ((reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale) |
+        reinterpret_cast<uintptr_t>(c->block_table) | reinterpret_cast<uintptr_t>(c->lengths) |
+        reinterpret_cast<uintptr_t>(c->status)) & 3))
+    return no(TT_ERR_INVALID_ARGUMENT, "a cache pointer is misaligned (codes: 16 bytes)");
+  v->k = static_cast<uint8_t *>(c->k_codes);
+  v->v = static_cast<uint8_t *>(c->v_codes);
+  v->ks = c->k_scale;
+  v->vs = c->v_scale;
+  v->table = c->block_table;
+  v->lengths = c->lengths;
+  v->status = reinterpret_cast<DeviceStatus *>(c->status);
+  v->pages = c->num_pages;
+  v->page_log2 = c->page_size == 16 ? 4 : c->page_size == 32 ? 5 : c->page_size == 64 ? 6 : 7;
+  v->heads = c->kv_heads;
+  v->hd = c->head_dim;
+  v->batch = c->batch;
+  v->columns = c->table_columns;
+  v->format = c->format;
+  return TT_OK;
+}
+
+static bool dtype_ok(int dtype) {
+  return dtype == TT_DTYPE_F32 || dtype == TT_DTYPE_F16 || dtype == TT_DTYPE_BF16;
+}
+
+}  // namespace tt
+
+using namespace tt;
+
+extern "C" {
+
+int tt_kv_write(const tt_kv_cache *cache, int dtype, const void *k, const void *v,
+                const int64_t *k_strides, const int64_t *v_strides, int64_t tokens,
+                const int32_t *counts, void *stream) {
+  KvView c;
+  const int rc = kv_view(cache, "tt_kv_write", &c);
+  if (rc != TT_OK) return rc;
+  if (!dtype_ok(dtype))
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_write: dtype must be a TT_DTYPE_* value");
+  if (tokens < 0 || tokens > INT32_MAX)
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_write: tokens must be >= 0 and fit 32 bits");
+  if (tokens == 0 || c.batch == 0) return TT_OK;
+  if (k == nullptr || v == nullptr || k_strides == nullptr || v_strides == nullptr)
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_write: NULL k, v or strides");
+  const int64_t room = (int64_t)c.columns << c.page_log2;
+  if (counts == nullptr && tokens > room)
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_write: more tokens than a sequence has room for");
+  tokens = std::min(tokens, room);  // rows behind those are behind every count
+  return launch_kv_write(c, dtype, k, v, {k_strides[0], k_strides[1], k_strides[2]},
+                         {v_strides[0], v_strides[1], v_strides[2]}, tokens, counts,
+                         static_cast<cudaStream_t>(stream));
+}
+
+int tt_kv_read(const tt_kv_cache *cache, int dtype, void *k, void *v, int64_t max_tokens,
+               void *stream) {
+  KvView c;
+  const int rc = kv_view(cache, "tt_kv_read", &c);
+  if (rc != TT_OK) return rc;
+  if (!dtype_ok(dtype))
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_read: dtype must be a TT_DTYPE_* value");
+  if (max_tokens < 0 || max_tokens > INT32_MAX)
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_read: max_tokens must be >= 0 and fit 32 bits");
+  if (max_tokens == 0 || c.batch == 0) return TT_OK;
+  if (k == nullptr || v == nullptr)
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_read: NULL k or v");
+  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15)
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_read: k and v must be 16-byte aligned");
+  return launch_kv_read(c, dtype, k, v, max_tokens, static_cast<cudaStream_t>(stream));
+}
+
+size_t tt_kv_attention_workspace_bytes(const tt_kv_cache *cache, int64_t tokens, int32_t heads) {
+  KvView c;
+  if (kv_view(cache, "tt_kv_attention_workspace_bytes", &c) != TT_OK) return 0;
+  if (tokens <= 0 || tokens > INT32_MAX || c.batch == 0 || heads <= 0 || heads % c.heads != 0)
+    return 0;
+  return kv_attention_ws_bytes(c, tokens, heads);
+}
+
+int tt_kv_attention(const tt_kv_cache *cache, int dtype, const void *q, const int64_t *q_strides,
+                    int64_t tokens, int32_t heads, const int32_t *counts, float scale, void *out,
+                    void *workspace, size_t workspace_bytes, void *stream) {
+  KvView c;
+  const int rc = kv_view(cache, "tt_kv_attention", &c);
+  if (rc != TT_OK) return rc;
+  if (!dtype_ok(dtype))
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_attention: dtype must be a TT_DTYPE_* value");
+  if (tokens < 0 || tokens > INT32_MAX)
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_attention: tokens must be >= 0 and fit 32 bits");
+  if (heads <= 0 || heads % c.heads != 0)
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_attention: heads must be a multiple of kv_heads");
+  if (!(scale > 0.f) || !std::isfinite(scale))
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_attention: scale must be positive and finite");
+  if (tokens == 0 || c.batch == 0) return TT_OK;
+  if (q == nullptr || q_strides == nullptr || out == nullptr)
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_attention: NULL q, strides or out");
+  if (q == out) return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_attention: out may not alias q");
+  if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15)
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_attention: out and workspace must be 16-byte aligned");
+  const size_t need = kv_attention_ws_bytes(c, tokens, heads);
+  if (workspace_bytes < need || (need > 0 && workspace == nullptr))
+    return fail(TT_ERR_WORKSPACE, "tt_kv_attention: workspace smaller than "
+                                  "tt_kv_attention_workspace_bytes (" + std::to_string(need) + " bytes)");
+  KvAttentionArgs a{};
+  a.c = c;
+  a.q = q;
+  a.qs = {q_strides[0], q_strides[1], q_strides[2]};
+  a.out = out;
+  a.counts = counts;
+  a.ws = static_cast<float *>(workspace);
+  a.dtype = dtype;
+  a.tokens = (int)tokens;
+  a.heads = heads;
+  a.group = heads / c.heads;
+  a.scale = scale;
+  return launch_kv_attention(a, static_cast<cudaStream_t>(stream));
+}
+
+int tt_kv_read_status(const tt_kv_cache *cache, int32_t *code, int32_t *detail, void *stream_) {
+  if (cache == nullptr || cache->status == nullptr || code == nullptr)
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_read_status: NULL cache, status or code");
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  int32_t st[2] = {0, 0};
+  TT_CUDA_TRY(cudaMemcpyAsync(st, cache->status, sizeof st, cudaMemcpyDeviceToHost, stream));
+  TT_CUDA_TRY(cudaStreamSynchronize(stream));
+  TT_CUDA_TRY(cudaMemsetAsync(cache->status, 0, sizeof st, stream));
+  *code = st[0];
+  if (detail) *detail = st[1];
+  return TT_OK;
+}
+
+}  // extern "C"

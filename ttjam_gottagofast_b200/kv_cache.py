@@ -1,0 +1,281 @@
+"""An 8-bit paged key/value cache and the attention over it.
+
+`KVCache` holds the keys and values of a batch of sequences as float8 e4m3 or
+int8 codes, in pages of `page_size` tokens, with one power-of-two scale for each
+page and head (include/ttjam_b200.h states the format). Three calls work on one
+layer of it, each on `torch.cuda.current_stream()` without a host sync:
+
+* `write(k, v)` quantises the keys and values of new tokens into it;
+* `attend(q)` is the causal attention of the new tokens over it;
+* `read()` gives the tokens back as dense tensors.
+
+`advance(tokens)` makes room first: it adds the new tokens to `lengths`, and the
+calls on all layers then take row i of a sequence's `count` new ones to stand at
+position `lengths - count + i`. `UserOptimizedTransformer.forward_cached` does
+all of this for a whole model.
+
+There is no CPU path and no autograd: the cache is for running a model, and
+CPU tensors raise. The reference has no counterpart; it computes every key and
+value anew on each forward (torch_transformer_benchmark.py:93-121).
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+
+FORMATS = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+PAGE_SIZES = (16, 32, 64, 128)
+
+
+def _dtype_code(t: torch.Tensor, what: str) -> int:
+    code = _lib.DTYPE_CODES.get(str(t.dtype).split(".")[-1])
+    if code is None:
+        raise ValueError(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
+    return code
+
+
+class KVCache:
+    """Keys and values of `batch` sequences of up to `max_tokens` tokens, for
+    `num_layers` layers of `kv_heads` heads.
+
+    The tensors are public: `k` and `v` are [num_layers, num_pages, kv_heads,
+    page_size, head_dim] codes (torch.float8_e4m3fn or torch.int8), `k_scale`
+    and `v_scale` [num_layers, num_pages, kv_heads] float32, `block_table`
+    [batch, max_tokens / page_size, rounded up] int32 and `lengths` [batch] int32.
+    The constructor gives every sequence pages of its own; a program with its
+    own page allocator writes into `block_table` and `lengths`, or brings its
+    tensors (`from_tensors`). Sequences may share pages that are only read.
+    The tensors themselves are fixed for the cache's life (their contents change)."""
+
+    def __init__(self, batch: int, max_tokens: int, kv_heads: int, head_dim: int, *,
+                 num_layers: int = 1, page_size: int = 64, fmt: str = "e4m3",
+                 device=None) -> None:
+        if fmt not in FORMATS:
+            raise ValueError(f"fmt must be one of {sorted(FORMATS)}, got {fmt!r}")
+        for name, n in (("batch", batch), ("max_tokens", max_tokens), ("kv_heads", kv_heads),
+                        ("head_dim", head_dim), ("num_layers", num_layers)):
+            if n <= 0:
+                raise ValueError(f"{name} must be positive")
+        if page_size not in PAGE_SIZES:
+            raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
+        device = torch.device("cuda" if device is None else device)
+        if device.type != "cuda":
+            raise RuntimeError("KVCache runs on CUDA only (no CPU path)")
+        columns = -(-max_tokens // page_size)
+        pages = batch * columns
+        shape = (num_layers, pages, kv_heads, page_size, head_dim)
+        codes = [torch.zeros(shape, dtype=torch.uint8, device=device).view(FORMATS[fmt])
+                 for _ in range(2)]
+        scales = [torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)]
+        table = torch.arange(pages, dtype=torch.int32, device=device).view(batch, columns)
+        self._setup(*codes, *scales, table,
+                    torch.zeros(batch, dtype=torch.int32, device=device), max_tokens)
+        self._longest = 0
+
+    @classmethod
+    def from_tensors(cls, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor,
+                     v_scale: torch.Tensor, block_table: torch.Tensor,
+                     lengths: torch.Tensor) -> "KVCache":
+        """A cache over the caller's tensors, of the shapes and types the class
+        names (all contiguous, on one device). Scales are powers of two: those
+        that `write` made, or a copy of them."""
+        self = cls.__new__(cls)
+        if block_table.dim() != 2 or k.dim() != 5:
+            raise ValueError("k must be [layers, pages, kv_heads, page_size, head_dim] and "
+                             "block_table [batch, columns]")
+        self._setup(k, v, k_scale, v_scale, block_table, lengths,
+                    block_table.shape[1] * k.shape[3])
+        return self
+
+    def _setup(self, k, v, k_scale, v_scale, block_table, lengths, max_tokens) -> None:
+        fmt = {t: f for f, t in FORMATS.items()}.get(k.dtype)
+        if fmt is None:
+            raise ValueError(f"codes must be torch.float8_e4m3fn or torch.int8, got {k.dtype}")
+        layers, pages, heads, page, hd = k.shape
+        batch, columns = block_table.shape
+        if page not in PAGE_SIZES:
+            raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page}")
+        want = {"v": (v, k.shape, k.dtype), "k_scale": (k_scale, k.shape[:3], torch.float32),
+                "v_scale": (v_scale, k.shape[:3], torch.float32),
+                "block_table": (block_table, (batch, columns), torch.int32),
+                "lengths": (lengths, (batch,), torch.int32)}
+        for name, (t, shape, dtype) in {"k": (k, k.shape, k.dtype), **want}.items():
+            if t.device.type != "cuda":
+                raise RuntimeError("KVCache runs on CUDA only (no CPU path)")
+            if (tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != k.device
+                    or not t.is_contiguous()):
+                raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape "
+                                 f"{tuple(shape)} on {k.device}, got {t.dtype} of "
+                                 f"{tuple(t.shape)} on {t.device}")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.block_table, self.lengths = block_table, lengths
+        self.fmt, self.device = fmt, k.device
+        self.num_layers, self.num_pages = layers, pages
+        self.kv_heads, self.page_size, self.head_dim = heads, page, hd
+        self.batch, self.max_tokens = batch, max_tokens
+        self._longest = None  # an upper bound on lengths known to the host, or None
+        self._status = torch.zeros(2, dtype=torch.int32, device=k.device)
+        self._lib = _lib.load()
+        self._ws_bytes = {}
+        self._structs = []
+        for i in range(layers):
+            c = _lib.TTKVCache()
+            c.k_codes, c.v_codes = k[i].data_ptr(), v[i].data_ptr()
+            c.k_scale, c.v_scale = k_scale[i].data_ptr(), v_scale[i].data_ptr()
+            c.block_table, c.lengths = block_table.data_ptr(), lengths.data_ptr()
+            c.status = self._status.data_ptr()
+            c.num_pages, c.page_size, c.kv_heads, c.head_dim = pages, page, heads, hd
+            c.batch, c.table_columns, c.format = batch, columns, _lib.KV_FORMATS[fmt]
+            # an empty write makes every check of the shape and touches nothing
+            _lib.check(self._lib.tt_kv_write(ctypes.byref(c), 0, None, None, None, None, 0, None,
+                                             None), "KVCache", self._lib)
+            self._structs.append(ctypes.pointer(c))
+
+    # ---- lengths ------------------------------------------------------------
+    def advance(self, tokens: int, new_tokens: Optional[torch.Tensor] = None) -> None:
+        """Add `tokens` new tokens to every sequence, or new_tokens[b] of at most
+        `tokens` to sequence b. Refuses what `max_tokens` has no room for. (While
+        a CUDA graph is captured, and in its replays, the host cannot know the
+        lengths; a length beyond the room is then latched on the device.)"""
+        if tokens < 0:
+            raise ValueError("tokens must be >= 0")
+        new_tokens = self._counts(new_tokens)
+        if not torch.cuda.is_current_stream_capturing():
+            if self._longest is None or self._longest + tokens > self.max_tokens:
+                grown = self.lengths + (tokens if new_tokens is None else new_tokens)
+                longest = int(grown.max())
+                if longest > self.max_tokens:
+                    raise ValueError(f"cache is full: a sequence would hold {longest} tokens of "
+                                     f"at most {self.max_tokens}")
+                self._longest = longest
+            else:
+                self._longest += tokens
+        else:
+            self._longest = None
+        self.lengths.add_(tokens if new_tokens is None else new_tokens)
+
+    def reset(self) -> None:
+        """Forget every token (lengths 0); the pages stay where they are."""
+        self.lengths.zero_()
+        self._longest = None
+
+    # ---- the operators ------------------------------------------------------
+    def write(self, k: torch.Tensor, v: torch.Tensor, new_tokens: Optional[torch.Tensor] = None,
+              layer: int = 0) -> None:
+        """Quantise the keys and values of new tokens into layer `layer`: k and
+        v are [batch, tokens, kv_heads, head_dim] float32, float16 or bfloat16
+        (any strides with head_dim contiguous). new_tokens, [batch] int32, says
+        how many leading rows of each sequence are new tokens (default: all);
+        `lengths` counts them already."""
+        for name, t in (("k", k), ("v", v)):
+            self._check(t, name, self.kv_heads)
+        if k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError(f"k and v must agree in shape and type, got {tuple(k.shape)} "
+                             f"{k.dtype} and {tuple(v.shape)} {v.dtype}")
+        k, v = self._rows(k), self._rows(v)
+        counts = self._counts(new_tokens)
+        self._call("tt_kv_write", layer, _dtype_code(k, "k"), k.data_ptr(), v.data_ptr(),
+                   _strides(k), _strides(v), k.shape[1],
+                   None if counts is None else counts.data_ptr())
+
+    def read(self, dtype: torch.dtype = torch.float32, max_tokens: Optional[int] = None,
+             layer: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The first max_tokens (default: as many as there is room for) tokens
+        of every sequence in layer `layer`: k and v, [batch, max_tokens,
+        kv_heads, head_dim] of `dtype`, zero behind each sequence's end."""
+        n = self.max_tokens if max_tokens is None else max_tokens
+        if n < 0:
+            raise ValueError("max_tokens must be >= 0")
+        shape = (self.batch, n, self.kv_heads, self.head_dim)
+        k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
+        self._call("tt_kv_read", layer, _dtype_code(k, "dtype"), k.data_ptr(), v.data_ptr(), n)
+        return k, v
+
+    def attend(self, q: torch.Tensor, new_tokens: Optional[torch.Tensor] = None, layer: int = 0,
+               scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Causal attention of the new tokens over layer `layer`, which holds
+        their keys and values already. q is [batch, tokens, heads, head_dim]
+        (strides as in `write`), heads a multiple of kv_heads: query head h
+        reads key head h // (heads // kv_heads). Row i < new_tokens[b] stands at
+        position lengths[b] - new_tokens[b] + i and sees the tokens up to its
+        own. `scale` (default head_dim ** -0.5) multiplies the scores. Returns
+        (or writes to `out`, contiguous) [batch, tokens, heads, head_dim] of
+        q's type, computed to fp32 accuracy; rows behind new_tokens[b] are 0."""
+        if q.dim() != 4 or q.shape[2] % self.kv_heads or q.shape[2] == 0:
+            raise ValueError(f"q must be [batch, tokens, heads, head_dim] with heads a multiple of "
+                             f"{self.kv_heads}, got {tuple(q.shape)}")
+        self._check(q, "q", q.shape[2])
+        q = self._rows(q)
+        n, heads = q.shape[1], q.shape[2]
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        elif (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device
+              or not out.is_contiguous()):
+            raise ValueError("out must be a contiguous tensor of q's shape, type and device")
+        counts = self._counts(new_tokens)
+        scale = self.head_dim ** -0.5 if scale is None else float(scale)
+        nbytes = self._ws_bytes.get((n, heads))
+        if nbytes is None:
+            with torch.cuda.device(self.device):
+                nbytes = self._lib.tt_kv_attention_workspace_bytes(self._structs[0], n, heads)
+            self._ws_bytes[(n, heads)] = nbytes
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        self._call("tt_kv_attention", layer, _dtype_code(q, "q"), q.data_ptr(), _strides(q), n,
+                   heads, None if counts is None else counts.data_ptr(), scale, out.data_ptr(),
+                   None if ws is None else ws.data_ptr(), nbytes)
+        return out
+
+    def read_device_status(self) -> Tuple[int, int]:
+        """Synchronise and return (code, detail) latched by the kernels' checks
+        of lengths, counts and block-table entries; (0, 0) when all were in range."""
+        code, detail = ctypes.c_int32(0), ctypes.c_int32(0)
+        stream = torch.cuda.current_stream(self.device).cuda_stream
+        _lib.check(self._lib.tt_kv_read_status(self._structs[0], ctypes.byref(code),
+                                               ctypes.byref(detail), stream),
+                   "tt_kv_read_status", self._lib)
+        return code.value, detail.value
+
+    # ---- checks -------------------------------------------------------------
+    def _check(self, t: torch.Tensor, name: str, heads: int) -> None:
+        if not t.is_cuda:
+            raise RuntimeError("KVCache runs on CUDA only (no CPU path)")
+        if t.device != self.device:
+            raise ValueError(f"{name} must be on {self.device}, got {t.device}")
+        if t.dim() != 4 or t.shape[0] != self.batch or t.shape[2] != heads or \
+                t.shape[3] != self.head_dim:
+            raise ValueError(f"{name} must be [{self.batch}, tokens, {heads}, {self.head_dim}], "
+                             f"got {tuple(t.shape)}")
+
+    @staticmethod
+    def _rows(t: torch.Tensor) -> torch.Tensor:
+        return t if t.stride(3) == 1 else t.contiguous()
+
+    def _counts(self, new_tokens: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+        if new_tokens is None:
+            return None
+        if (new_tokens.shape != (self.batch,) or new_tokens.dtype != torch.int32
+                or new_tokens.device != self.device):
+            raise ValueError(f"new_tokens must be an int32 tensor of shape ({self.batch},) on "
+                             f"{self.device}, got {new_tokens.dtype} of "
+                             f"{tuple(new_tokens.shape)} on {new_tokens.device}")
+        return new_tokens.contiguous()
+
+    def _call(self, name: str, layer: int, *args) -> None:
+        if not 0 <= layer < self.num_layers:
+            raise ValueError(f"layer must be in [0, {self.num_layers}), got {layer}")
+        if self.device.index != torch.cuda.current_device():
+            with torch.cuda.device(self.device):
+                return self._call(name, layer, *args)
+        stream = torch.cuda.current_stream(self.device).cuda_stream
+        rc = getattr(self._lib, name)(self._structs[layer], *args, stream)
+        if rc != 0:
+            _lib.check(rc, name, self._lib)
+
+
+def _strides(t: torch.Tensor):
+    s = t.stride()
+    return (ctypes.c_int64 * 3)(s[0], s[1], s[2])
