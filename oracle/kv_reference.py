@@ -97,13 +97,15 @@ def read(cache, name, b):
 
 
 def attend(cache, q, counts, scale):
-    """(out, size, reach): out [batch, tokens, heads, head_dim] float64; size =
-    sum_j p_j |v_j| per element and reach = max_j scale * sum_d |q_d k_jd| per
-    (batch, token, head), which bounds of rounding errors go by."""
+    """(out, size, total, reach): out [batch, tokens, heads, head_dim] float64;
+    size = sum_j p_j |v_j| and total = sum_j |v_j| per element, and reach =
+    max_j scale * sum_d (|q_d| + max|q| / 8) |k_jd| per (batch, token, head), which
+    bounds of rounding errors go by."""
     batch, n, heads, hd = q.shape
     q = q.double()
     out = torch.zeros(q.shape, dtype=torch.float64)
-    size, reach = torch.zeros_like(out), torch.zeros(q.shape[:3], dtype=torch.float64)
+    size, total = torch.zeros_like(out), torch.zeros_like(out)
+    reach = torch.zeros(q.shape[:3], dtype=torch.float64)
     group = heads // cache["k"].shape[1]
     for b in range(batch):
         k, there = read(cache, "k", b)
@@ -118,5 +120,7 @@ def attend(cache, q, counts, scale):
                 p = torch.softmax(scale * (kk @ q[b, i, h]), 0)
                 out[b, i, h] = p @ vv
                 size[b, i, h] = p @ vv.abs()
-                reach[b, i, h] = scale * float((kk.abs() @ q[b, i, h].abs()).max())
-    return out, size, reach
+                total[b, i, h] = vv.abs().sum(0)
+                qq = q[b, i, h].abs()
+                reach[b, i, h] = scale * float((kk.abs() @ (qq + qq.max() / 8)).max())
+    return out, size, total, reach

@@ -52,24 +52,32 @@ def same_bits(a, b):
     return torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
 
 
-def attention_bound(size, reach, hd, tokens, dtype):
+def attention_bound(size, total, reach, hd, tokens, dtype):
     """How far an element may be from the 64-bit value, by counting roundings.
 
     A score's products are exact (11-bit pieces of q times a code); q's split
-    loses 2^-22 of each, and each of the hd / 16 additions of a tensor-core step
+    loses 2^-22 of each, or 2^-25 of the row's largest element where that is more
+    (an fp16 piece has no step below 2^-24; reach counts 2^-25 of it), and each of the hd / 16 additions of a tensor-core step
     at most 2^-22 of the sum of magnitudes: (hd / 16 + 2) 2^-22 reach. The
     exponent's fused multiply-add rounds a number of up to 2^5 where p matters
     (2^-19 of p after ln 2), exp2 and p's split add less than 2^-21 together.
     Sums of up to `tokens` terms lose at most tokens * 2^-24 in all, /4 because
     four warps share them. Each relative error of p_j counts once in the sum of
-    p v and once in the sum of p.
+    p v and once in the sum of p. 16-bit rows may round p to fp16 for its product
+    with v (not in the sum): float16's steps are 2^-10 of a power of two, so half
+    a step is at most eps / 2 = 2^-11 of p, once.
+
+    p's pieces have no step below 2^-24 either, and p is scaled to have its largest
+    value at 2^6 at least: each p_j is off by up to 2^-31 of the largest, whatever
+    its own size, which is 2^-31 of `total` in the sum of p v.
 
     The output's own rounding adds half a step of its type: eps / 2 of the value,
     and below the type's smallest normal number, where the steps stay as they are
     there, half of smallest_normal * eps (float16: 2^-14 2^-10 / 2 = 2^-25)."""
     eps = (hd / 16 + 2) * 2.0 ** -22 * reach + 2.0 ** -18 + tokens * 2.0 ** -26
     info = torch.finfo(dtype)
-    return 2 * eps[..., None] * size + info.smallest_normal * info.eps / 2, info.eps / 2
+    once = 2.0 ** -11 if info.bits == 16 else 0.0
+    return (2 * eps[..., None] + once) * size + 2.0 ** -31 * total + info.smallest_normal * info.eps / 2, info.eps / 2
 
 
 def worst(got, exact, bound, half_step):

@@ -162,7 +162,7 @@ def test_oracle_attention_is_softmax_over_the_seen_tokens():
         cache[name] = torch.randint(-127, 128, (2, 2, 16, 16), generator=g).double()
         cache[name + "_scale"] = torch.tensor([[0.5, 1.0], [2.0, 0.25]], dtype=torch.float64) / 64
     q = torch.randn(1, 3, 4, 16, generator=g)
-    out, _, _ = ref.attend(cache, q, [2], 0.25)
+    out, _, _, _ = ref.attend(cache, q, [2], 0.25)
     k, v = (ref.read(cache, n, 0)[0].transpose(0, 1) for n in ("k", "v"))
     want = torch.nn.functional.scaled_dot_product_attention(
         q[0, :2].double().transpose(0, 1), k.repeat_interleave(2, 0), v.repeat_interleave(2, 0),

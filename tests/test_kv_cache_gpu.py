@@ -168,6 +168,11 @@ ATTENDS = [  # batch, tokens, heads, kv_heads, head_dim, page, lengths, counts
     (2, 130, 4, 2, 64, 64, [400, 130], [130, 7]),
     (2, 200, 2, 2, 128, 16, [200, 333], None),
     (1, 129, 3, 1, 16, 128, [640], None),
+    (1, 300, 2, 1, 256, 64, [300], None),
+    (2, 90, 3, 3, 80, 32, [900, 90], None),
+    (1, 140, 1, 1, 64, 64, [2000], None),
+    (1, 100, 2, 2, 128, 16, [1500], None),
+    (3, 300, 1, 1, 48, 32, [300, 0, 1111], [40, 0, 300]),
 ]
 
 
@@ -183,8 +188,8 @@ def test_attend_matches_64_bits(case, dtype, fmt):
     got = cache.attend(q, new_tokens=None if counts is None else _counts(counts), out=out)
     assert got is out
     counts = counts or [n] * batch
-    exact, size, reach = ref.attend(want, q.cpu(), counts, hd ** -0.5)
-    bound, half_step = kh.attention_bound(size, reach, hd, max(lengths), q.dtype)
+    exact, size, total, reach = ref.attend(want, q.cpu(), counts, hd ** -0.5)
+    bound, half_step = kh.attention_bound(size, total, reach, hd, max(lengths), q.dtype)
     assert not torch.isnan(got).any() and kh.worst(got, exact, bound, half_step) <= 1
     for b in range(batch):
         assert not got[b, counts[b]:].any()
@@ -209,16 +214,32 @@ def test_attend_bad_pages_nan_pages_and_own_scale(fmt, tokens):
     g = torch.Generator().manual_seed(3)
     q = torch.randn((4, tokens, 4, 64), generator=g).cuda()
     got = cache.attend(q, scale=0.3).cpu().double()
-    exact, size, reach = ref.attend(want, q.cpu(), [tokens] * 4, 0.3)
+    exact, size, total, reach = ref.attend(want, q.cpu(), [tokens] * 4, 0.3)
     assert torch.equal(torch.isnan(got), torch.isnan(exact))
     assert torch.isnan(got[3, :, 2:]).all() and not torch.isnan(got[3, :, :2]).any()
     assert not got[2].any()
-    bound, half_step = kh.attention_bound(size, reach, 64, max(lengths), torch.float32)
+    bound, half_step = kh.attention_bound(size, total, reach, 64, max(lengths), torch.float32)
     assert kh.worst(got, exact, bound, half_step) <= 1
     assert cache.read_device_status()[0] != 0  # the entries were latched
     assert cache.read_device_status() == (0, 0)
     k, _ = cache.read(max_tokens=80)
     assert not k[1, 48:64].any() and not k[1, 80:96].any() and k[1, 64:80].any()
+
+
+@pytest.mark.parametrize("tokens", [20, 150])
+def test_attend_nan_pages_reach_only_the_rows_that_see_them(tokens):
+    """A page of the new tokens themselves: the rows before it stay numbers."""
+    cache, _ = kh.make(65, "int8", 2, 16, 1, 32, 16, [tokens, tokens + 40])
+    for b, name in ((0, "v_scale"), (1, "k_scale")):
+        getattr(cache, name)[0, int(cache.block_table[b, (tokens + 40 * b - 1) // 16])] = float("nan")
+    want = kh.mirror(cache)
+    q = torch.randn((2, tokens, 1, 32), generator=torch.Generator().manual_seed(2)).cuda()
+    got = cache.attend(q)
+    exact, size, total, reach = ref.attend(want, q.cpu(), [tokens] * 2, 32 ** -0.5)
+    assert torch.isnan(exact).any() and not torch.isnan(exact).all(-1).all()
+    assert torch.equal(torch.isnan(got).cpu(), torch.isnan(exact))
+    bound, half_step = kh.attention_bound(size, total, reach, 32, tokens + 40, torch.float32)
+    assert kh.worst(got, exact, bound, half_step) <= 1
 
 
 def test_attend_large_scores_and_far_apart_value_scales():
@@ -232,8 +253,8 @@ def test_attend_large_scores_and_far_apart_value_scales():
     q = torch.randn((1, 2, 3, 64), generator=torch.Generator().manual_seed(1)).cuda() * 0.5
     q[0, 1] = 0
     got = cache.attend(q)
-    exact, size, reach = ref.attend(want, q.cpu(), [2], 64 ** -0.5)
-    bound, half_step = kh.attention_bound(size, reach, 64, 300, torch.float32)
+    exact, size, total, reach = ref.attend(want, q.cpu(), [2], 64 ** -0.5)
+    bound, half_step = kh.attention_bound(size, total, reach, 64, 300, torch.float32)
     assert not torch.isnan(got).any() and kh.worst(got, exact, bound, half_step) <= 1
 
 

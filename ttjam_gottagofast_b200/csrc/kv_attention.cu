@@ -31,6 +31,7 @@
 #include <algorithm>
 
 #include "kv_cache.cuh"
+#include "kv_codes.cuh"
 
 namespace tt {
 namespace {
@@ -49,11 +50,6 @@ struct RowShape {
   static constexpr int kSlot = kRows * HD + 2 * kRows;  // floats of a partial result
 };
 
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void mma16816(float *c, uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -61,62 +57,6 @@ __device__ __forceinline__ void mma16816(float *c, uint32_t a0, uint32_t a1, uin
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// Codes to fp16 pairs, exact, by integer operations, so that no bit pattern
-// (a slot that was never written) turns into a NaN. int8: 1024 + (code + 128)
-// is the fp16 with that low byte, minus 1152. e4m3: the bits put in place under
-// the fp16 exponent are the value * 2^-8, for normal and subnormal codes alike.
-template <int FMT>
-constexpr float kCodeUnit = FMT == TT_KV_INT8 ? 1.f : 256.f;
-
-__device__ __forceinline__ uint32_t i8_pair(uint32_t biased, uint32_t sel) {
-  uint32_t r = __byte_perm(biased, 0x64646464u, sel);
-  asm("sub.f16x2 %0, %0, %1;" : "+r"(r) : "r"(0x64806480u));
-  return r;
-}
-__device__ __forceinline__ uint32_t e4m3_pair(uint32_t t) {  // codes in bits 8-15 and 24-31
-  return (t & 0x80008000u) | ((t >> 1) & 0x3f803f80u);
-}
-// four consecutive codes -> (0, 1), (2, 3)
-template <int FMT>
-__device__ __forceinline__ void codes_along(uint32_t w, uint32_t &a, uint32_t &b) {
-  if constexpr (FMT == TT_KV_INT8) {
-    const uint32_t u = w ^ 0x80808080u;
-    a = i8_pair(u, 0x4140);
-    b = i8_pair(u, 0x4342);
-  } else {
-    a = e4m3_pair(__byte_perm(w, 0, 0x1000));
-    b = e4m3_pair(__byte_perm(w, 0, 0x3020));
-  }
-}
-// four codes of each of two tokens -> the pair (x, y) of each code
-template <int FMT>
-__device__ __forceinline__ void codes_across(uint32_t x, uint32_t y, uint32_t *r) {
-  if constexpr (FMT == TT_KV_INT8) {
-    const uint32_t lo = __byte_perm(x, y, 0x5140) ^ 0x80808080u;
-    const uint32_t hi = __byte_perm(x, y, 0x7362) ^ 0x80808080u;
-    r[0] = i8_pair(lo, 0x4140);
-    r[1] = i8_pair(lo, 0x4342);
-    r[2] = i8_pair(hi, 0x4140);
-    r[3] = i8_pair(hi, 0x4342);
-  } else {
-    r[0] = e4m3_pair(__byte_perm(x, y, 0x4000));
-    r[1] = e4m3_pair(__byte_perm(x, y, 0x5010));
-    r[2] = e4m3_pair(__byte_perm(x, y, 0x6020));
-    r[3] = e4m3_pair(__byte_perm(x, y, 0x7030));
-  }
-}
-
-__device__ __forceinline__ float load_q(const KvAttentionArgs &a, int64_t i) {
-  if (a.dtype == TT_DTYPE_F32) return static_cast<const float *>(a.q)[i];
-  if (a.dtype == TT_DTYPE_F16) return __half2float(static_cast<const __half *>(a.q)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16 *>(a.q)[i]);
-}
-__device__ __forceinline__ void store_out(const KvAttentionArgs &a, int64_t i, float x) {
-  if (a.dtype == TT_DTYPE_F32) static_cast<float *>(a.out)[i] = x;
-  else if (a.dtype == TT_DTYPE_F16) static_cast<__half *>(a.out)[i] = __float2half_rn(x);
-  else static_cast<__nv_bfloat16 *>(a.out)[i] = __float2bfloat16_rn(x);
 }
 
 // Units of sequence b for one (key head, row block): at least one, which writes
@@ -288,7 +228,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_rows_kernel(KvAttention
         const int d = HD == 32 ? 8 * tig + 4 * w : 64 * (w / 4) + 16 * tig + 4 * (w % 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x[w][i] = live && d < c.hd ? load_q(a, off + d + i) : 0.f;
+          x[w][i] = live && d < c.hd ? kv_load_in(a.dtype, a.q, off + d + i) : 0.f;
           mx = fmaxf(mx, fabsf(x[w][i]));
         }
       }
@@ -400,7 +340,8 @@ __global__ void __launch_bounds__(kThreads) kv_attention_rows_kernel(KvAttention
               p[x][q] = v;
               sum += v;
             }
-          l = fmaf(sum, 1.f / cur[g].vs, l);
+          // a NaN scale counts only where a token of its page is seen
+          if (sum != 0.f) l = fmaf(sum, 1.f / cur[g].vs, l);
           uint32_t pa[4];
           f16_split2(p[0][0], p[0][1], pa[0], pa[1]);
           f16_split2(p[1][0], p[1][1], pa[2], pa[3]);
@@ -452,7 +393,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_rows_kernel(KvAttention
         const int row = rb * kRows + rr, ti = row / a.group;
         if (d < c.hd) {
           const float v = ti >= count || ll == 0.f ? 0.f : oo * kCodeUnit<FMT> / ll;
-          store_out(a, (((int64_t)b * a.tokens + ti) * a.heads + h * a.group + row % a.group) * c.hd + d, v);
+          kv_store_out(a.dtype, a.out, (((int64_t)b * a.tokens + ti) * a.heads + h * a.group + row % a.group) * c.hd + d, v);
         }
       } else {
         slot[rr * HD + d] = oo;
@@ -519,7 +460,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_join_kernel(KvAttention
       oo = fmaf(s[rr * HD + d], f, oo);
     }
     const float v = ti >= count || ll == 0.f ? 0.f : oo * kCodeUnit<FMT> / ll;
-    store_out(a, (((int64_t)b * a.tokens + ti) * a.heads + h * a.group + row % a.group) * c.hd + d, v);
+    kv_store_out(a.dtype, a.out, (((int64_t)b * a.tokens + ti) * a.heads + h * a.group + row % a.group) * c.hd + d, v);
   }
 }
 
@@ -597,7 +538,13 @@ int for_shape(const KvView &c, F &&f) {
 
 }  // namespace
 
+// Rows of a key head from which the tile kernel takes over.
+static bool use_tiles(const KvView &c, int64_t tokens, int heads) {
+  return tokens * (heads / c.heads) >= 64;
+}
+
 size_t kv_attention_ws_bytes(const KvView &c, int64_t tokens, int heads) {
+  if (use_tiles(c, tokens, heads)) return kv_attention_tiles_ws_bytes(c, tokens, heads);
   RowPlan p{};
   const int rc = for_shape(c, [&](auto hd, auto fmt) {
     return rows_plan<decltype(hd)::value, decltype(fmt)::value>(c, tokens, heads, &p);
@@ -606,6 +553,7 @@ size_t kv_attention_ws_bytes(const KvView &c, int64_t tokens, int heads) {
 }
 
 int launch_kv_attention(const KvAttentionArgs &a, cudaStream_t stream) {
+  if (use_tiles(a.c, a.tokens, a.heads)) return launch_kv_attention_tiles(a, stream);
   return for_shape(a.c, [&](auto hd, auto fmt) {
     return launch_rows<decltype(hd)::value, decltype(fmt)::value>(a, stream);
   });

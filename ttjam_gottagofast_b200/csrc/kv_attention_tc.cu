@@ -1,0 +1,764 @@
+// Causal attention of new tokens over the 8-bit paged key/value cache, for many
+// query rows (prompts): tcgen05 products of 128-row tiles. The mathematics is
+// kv_attention.cu's: the key scale multiplies the score, the value scale 2^e
+// joins the exponent, p = 2^(s' + e - M + 7) with a whole-number reference M,
+// out = sum p code / sum p 2^-e; the codes, exact in fp16, are the B operands.
+//
+// PIECES: how many fp16 pieces q and p are split into. fp32 rows take two (22
+// significant bits). 16-bit rows take one: q, scaled by a power of two to have
+// its largest element in [1, 2), is exact in it (bf16 elements below 2^-17 of the
+// row's largest lose at most 2^-25 of that), and rounding p to 11 bits moves the
+// output by less than rounding it to its own type does; the sum of p is taken
+// before that rounding, in fp32.
+//
+// CTA = (row tile, key head, sequence, split of the tokens): MT tiles of 128 query
+// rows (row = token * group + head of the group) against tiles of TOK tokens.
+//   warps 0 .. 4 MT - 1   softmax: tensor-memory lane t of tile x is one thread's
+//             row. Two passes over the TOK scores (the row maximum, then p, which
+//             replaces the scores 32 columns at a time); O is rescaled in tensor
+//             memory only when the maximum grows by more than 2^8.
+//   4 warps   conversion: 16 codes a load, eight fp16 pairs by integer operations,
+//             stored as 128-byte-swizzled rows of 64 dims, K-major for K and, the
+//             same bytes read the other way, MN-major for V; one tile ahead in
+//             registers. The tile's scales go to shared memory.
+//   1 warp    allocates tensor memory; its lane 0 issues the MMAs: S_x = q_x K^T,
+//             O_x += P_x V (A = P from tensor memory), the tiles in turn, so that
+//             one's softmax runs under the other's products.
+// K and V tiles share a ring of NS slots (K_0 V_0 K_1 ...). Every wait is bounded;
+// one that gives up latches TT_ERR_DEVICE_TIMEOUT in the cache's status word, and
+// the kernel frees its tensor memory and returns.
+#include <math_constants.h>
+
+#include <algorithm>
+
+#include "kv_cache.cuh"
+#include "kv_codes.cuh"
+
+namespace tt {
+namespace {
+
+constexpr int kConvWarps = 4, kConvThreads = 32 * kConvWarps;
+
+template <int HD_, int PIECES>
+struct TcShape {
+  static constexpr int HD = HD_;
+  static constexpr int MT = HD <= 128 ? 2 : 1;    // 128-row tiles per CTA
+  static constexpr int TOK = HD <= 128 ? 128 : 64;  // tokens per tile
+  static constexpr bool QT = HD == 64;            // q in tensor memory (else shared memory)
+  static constexpr int BOXES = HD / 64;           // 64-dim boxes of an operand tile
+  static constexpr uint32_t BOX = TOK * 128;      // bytes
+  static constexpr uint32_t SLOT = BOXES * BOX;
+  static constexpr uint32_t QBOX = 128 * 128;
+  static constexpr uint32_t QBYTES = QT ? 0 : MT * PIECES * BOXES * QBOX;
+  static constexpr int NS = (int)std::min<uint32_t>(6, (224 * 1024 - QBYTES) / SLOT);
+  static constexpr uint32_t BARS = QBYTES + NS * SLOT;  // barriers, after the operands
+  static constexpr size_t SMEM = BARS + 1024 + 1024;    // alignment of the base, barriers
+  static constexpr int SOFT_WARPS = 4 * MT;
+  static constexpr int THREADS = 32 * (SOFT_WARPS + kConvWarps + 1);
+  // tensor-memory columns
+  static constexpr uint32_t T_O = 0, T_S = MT * HD, T_Q = MT * (HD + TOK);
+  static_assert(T_Q + (QT ? MT * PIECES * HD / 2 : 0) <= 512, "tensor memory");
+  static_assert(NS >= 3 && SMEM <= 227 * 1024, "shared memory");
+  static constexpr int GROUPS = TOK / 16;  // of 16 tokens, each in one page
+  static constexpr int NCH = TOK * HD / 16 / kConvThreads;  // 16-code chunks a converter thread
+  static constexpr uint32_t IDESC_S =
+      (1u << 4) | ((uint32_t)(TOK >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+  static constexpr uint32_t IDESC_PV =  // B is MN-major
+      (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// Bounded wait: false after about 2^28 cycles (latching TT_ERR_DEVICE_TIMEOUT and
+// setting the CTA's abort word), or soon after another thread's gave up.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort_w,
+                                          DeviceStatus *st, int detail) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 31) == 0) {
+      if (*abort_w != 0) return false;
+      if (clock64() - t0 > (1LL << 28)) {
+        *abort_w = 1;
+        raise_status(st, TT_ERR_DEVICE_TIMEOUT, detail);
+        return false;
+      }
+    }
+  }
+}
+// Shared-memory matrix descriptor, 128-byte swizzle: 8-row groups 1024 bytes
+// apart, and (MN-major) 64-element blocks `lead` bytes apart.
+__device__ __forceinline__ uint64_t sdesc(uint32_t saddr, uint32_t lead) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFF);
+  d |= (uint64_t)((lead >> 4) & 0x3FFF) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accum)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accum)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void fence_async() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+      "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *v) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+// Two non-negative values below 65504 to one fp16 pair, or to two (high, rest).
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+__device__ __forceinline__ float widen_nonneg(uint32_t h16) {
+  // an fp16's bits under the fp32 exponent are its value * 2^-112 (subnormals too)
+  float r;
+  asm("mul.rn.f32 %0, %1, 0f77800000;" : "=f"(r) : "f"(__uint_as_float(h16 << 13)));
+  return r;
+}
+
+template <int HD, int FMT, int PIECES>
+__global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
+    kv_attention_tiles_kernel(KvAttentionArgs a, int row_tiles, int splits) {
+  using Sh = TcShape<HD, PIECES>;
+  constexpr int MT = Sh::MT, TOK = Sh::TOK, NS = Sh::NS, GROUPS = Sh::GROUPS;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ float s_ks[4][GROUPS], s_ve[4][GROUPS];  // of tile j in [j & 3]
+  __shared__ uint32_t s_ok[4];                        // groups whose page exists
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t *const smem = smem_raw + (base - raw);
+  const uint32_t bars = base + Sh::BARS;
+  auto slot_full = [&](int s) { return bars + 8u * s; };
+  auto slot_empty = [&](int s) { return bars + 8u * (NS + s); };
+  auto s_full = [&](int x) { return bars + 8u * (2 * NS + x); };
+  auto p_full = [&](int x) { return bars + 8u * (2 * NS + MT + x); };
+  auto o_done = [&](int x) { return bars + 8u * (2 * NS + 2 * MT + x); };
+  constexpr uint32_t XB = 2 * NS + 3 * MT;
+  auto sc_full = [&](int i) { return bars + 8u * (XB + i); };
+  const uint32_t q_ready = bars + 8u * (XB + 4), drain_bar = bars + 8u * (XB + 5);
+  const uint32_t tmem_slot = bars + 8u * (XB + 6);
+  volatile uint32_t *tmem_slot_p = reinterpret_cast<volatile uint32_t *>(smem + (tmem_slot - base));
+  volatile int *abort_w = reinterpret_cast<volatile int *>(smem + (tmem_slot + 4 - base));
+
+  const KvView &c = a.c;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_trigger();
+  pdl_wait();
+  // latest row tiles (the longest, causally) first
+  const int rt = row_tiles - 1 - (int)(blockIdx.x / c.heads), h = blockIdx.x % c.heads;
+  const int b = blockIdx.y, split = blockIdx.z;
+  const int rows_all = a.tokens * a.group, row0 = rt * 128 * MT;
+  const int len = c.length(b), count = c.count(a.counts, b, a.tokens, len);
+  const int live = min(rows_all, count * a.group) - row0;  // live rows from row0 on
+  // tokens that the CTA's last live row sees, and this split's tiles of them
+  const int any_end = live > 0 ? len - count + (row0 + min(live, 128 * MT) - 1) / a.group + 1 : 0;
+  const int tiles = (any_end + TOK - 1) / TOK;
+  const int j0 = (int)((int64_t)tiles * split / splits);
+  const int nj = (int)((int64_t)tiles * (split + 1) / splits) - j0;
+  const int active = min(MT, (live + 127) / 128);
+
+  // results of this thread's row, written where they belong
+  const int64_t rows_padded = (int64_t)row_tiles * 128 * MT;
+  auto part = [&](int r) {  // partial result of row r
+    return (((int64_t)split * c.batch + b) * c.heads + h) * rows_padded + r;
+  };
+  float *const part_ml = a.ws + (int64_t)splits * c.batch * c.heads * rows_padded * HD;
+  auto out_row = [&](int r) {
+    return (((int64_t)b * a.tokens + r / a.group) * a.heads + h * a.group + r % a.group) * c.hd;
+  };
+  if (nj <= 0) {  // no token for any row: zeros (the same for the whole CTA)
+    if (warp < Sh::SOFT_WARPS) {
+      const int r = row0 + threadIdx.x;
+      if (splits > 1) {
+        part_ml[2 * part(r)] = -CUDART_INF_F;
+        part_ml[2 * part(r) + 1] = 0.f;
+      } else if (r < rows_all) {
+        const float z[16] = {};
+        for (int d = 0; d < c.hd; d += 16) kv_store_row16(a.dtype, a.out, out_row(r) + d, z);
+      }
+    }
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(slot_full(s), kConvWarps);
+      mbar_init(slot_empty(s), 1);
+    }
+    for (int x = 0; x < MT; ++x) {
+      mbar_init(s_full(x), 1);
+      mbar_init(p_full(x), 4);
+      mbar_init(o_done(x), 1);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(sc_full(i), 1);
+    mbar_init(q_ready, 4 * active);
+    mbar_init(drain_bar, 1);
+    *abort_w = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  constexpr int kMmaWarp = Sh::SOFT_WARPS + kConvWarps;
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tmem_slot)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tm = *tmem_slot_p;
+
+  if (warp == kMmaWarp) {
+    if (lane == 0) {
+      // ---- MMA issuer ------------------------------------------------------
+      auto slot_addr = [&](int i) { return base + Sh::QBYTES + (uint32_t)(i % NS) * Sh::SLOT; };
+      auto wait_slot = [&](int i) {
+        return mbar_wait(slot_full(i % NS), (i / NS) & 1, abort_w, c.status, 0x6100);
+      };
+      auto issue_s = [&](int x, int i) {
+        const uint32_t k = slot_addr(i), d = tm + Sh::T_S + (uint32_t)(TOK * x);
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const uint64_t kd = sdesc(k + (kk / 4) * Sh::BOX, 16) + 2 * (kk % 4);
+#pragma unroll
+          for (int w = 0; w < PIECES; ++w) {
+            if constexpr (Sh::QT) {
+              mma_ts(d, tm + Sh::T_Q + (uint32_t)((x * PIECES + w) * (HD / 2) + 8 * kk), kd,
+                     Sh::IDESC_S, (kk | w) != 0);
+            } else {
+              const uint32_t q = base + (uint32_t)((x * PIECES + w) * Sh::BOXES + kk / 4) * Sh::QBOX;
+              mma_ss(d, sdesc(q, 16) + 2 * (kk % 4), kd, Sh::IDESC_S, (kk | w) != 0);
+            }
+          }
+        }
+        mma_commit(s_full(x));
+      };
+      bool ok = mbar_wait(q_ready, 0, abort_w, c.status, 0x6000) && wait_slot(0);
+      fence_after();
+      if (ok) {
+        for (int x = 0; x < active; ++x) issue_s(x, 0);
+        mma_commit(slot_empty(0));
+      }
+      for (int j = 0; ok && j < nj; ++j) {
+        const int vi = 2 * j + 1, ki = 2 * j + 2;
+        ok = wait_slot(vi);
+        for (int x = 0; ok && x < active; ++x) {
+          if (!(ok = mbar_wait(p_full(x), j & 1, abort_w, c.status, 0x6200))) break;
+          fence_after();
+          const uint32_t v = slot_addr(vi), p = tm + Sh::T_S + (uint32_t)(TOK * x);
+#pragma unroll
+          for (int kk = 0; kk < TOK / 16; ++kk) {
+            const uint64_t vd = sdesc(v, Sh::BOX) + 128 * kk;
+#pragma unroll
+            for (int w = 0; w < PIECES; ++w)
+              mma_ts(tm + Sh::T_O + (uint32_t)(HD * x),
+                     p + 32u * (kk >> 1) + 8u * (kk & 1) + 16u * w, vd, Sh::IDESC_PV,
+                     (j | kk | w) != 0);
+          }
+          mma_commit(o_done(x));
+          if (j + 1 < nj) {
+            if (x == 0 && !(ok = wait_slot(ki))) break;
+            fence_after();
+            issue_s(x, ki);
+          }
+        }
+        if (ok) {
+          mma_commit(slot_empty(vi % NS));
+          if (j + 1 < nj) mma_commit(slot_empty(ki % NS));
+        }
+      }
+      // every MMA issued above has completed before the tensor memory is freed
+      mma_commit(drain_bar);
+      const long long t0 = clock64();
+      for (uint32_t i = 0; !mbar_try_wait(drain_bar, 0); ++i)
+        if ((i & 31) == 31 && clock64() - t0 > (1LL << 28)) {
+          raise_status(c.status, TT_ERR_DEVICE_TIMEOUT, 0x6F00);
+          break;
+        }
+    }
+    __syncwarp();
+  } else if (warp >= Sh::SOFT_WARPS) {
+    // ---- conversion of the codes -------------------------------------------
+    constexpr int NCH = Sh::NCH, CPR = HD / 16;  // chunks per thread, per token
+    const int ct = threadIdx.x - 32 * Sh::SOFT_WARPS;
+    const int cw = warp - Sh::SOFT_WARPS;
+    auto pages_of = [&](int j) {  // lane g < GROUPS: the page of group g
+      const int t = (j0 + j) * TOK + 16 * lane;
+      return j < nj && lane < GROUPS && t < any_end ? c.page_of(b, t >> c.page_log2) : -1;
+    };
+    uint4 raw_k[NCH], raw_v[NCH];
+    auto load = [&](const uint8_t *pool, int ids, int j, uint4 *r) {
+#pragma unroll
+      for (int u = 0; u < NCH; ++u) {
+        const int i = u * kConvThreads + ct, t = i / CPR, d = (i % CPR) * 16;
+        const int pg = __shfl_sync(0xffffffffu, ids, t >> 4);
+        r[u] = make_uint4(0, 0, 0, 0);
+        if (pg >= 0 && d < c.hd) {
+          const int in_page = ((j0 + j) * TOK + t) & ((1 << c.page_log2) - 1);
+          r[u] = *reinterpret_cast<const uint4 *>(pool + c.tile(pg, h) + (int64_t)in_page * c.hd + d);
+        }
+      }
+    };
+    auto store = [&](int i_slot, const uint4 *r) {
+      uint8_t *dst = smem + Sh::QBYTES + (uint32_t)(i_slot % NS) * Sh::SLOT;
+#pragma unroll
+      for (int u = 0; u < NCH; ++u) {
+        const int i = u * kConvThreads + ct, t = i / CPR, ch = i % CPR;
+        uint32_t f[8];
+        codes_along<FMT>(r[u].x, f[0], f[1]);
+        codes_along<FMT>(r[u].y, f[2], f[3]);
+        codes_along<FMT>(r[u].z, f[4], f[5]);
+        codes_along<FMT>(r[u].w, f[6], f[7]);
+        uint8_t *row = dst + (ch / 4) * Sh::BOX + t * 128;
+        const int c0 = (2 * ch) % 8;
+        *reinterpret_cast<uint4 *>(row + ((c0 ^ (t & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
+        *reinterpret_cast<uint4 *>(row + (((c0 + 1) ^ (t & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
+      }
+      fence_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(slot_full(i_slot % NS));
+    };
+    int ids = pages_of(0), ids_next = pages_of(1);
+    load(c.k, ids, 0, raw_k);
+    load(c.v, ids, 0, raw_v);
+    bool ok = true;
+    for (int j = 0; ok && j < nj; ++j) {
+      if (cw == 0) {
+        // scales of the tile's groups; tile j - 4's were read before slot V_{j-2}
+        // was handed back, which this warp has waited for
+        if (lane < GROUPS) {
+          const int64_t at = (int64_t)(ids < 0 ? 0 : ids) * c.heads + h;
+          const float ks = c.ks[at], vs = c.vs[at];
+          s_ks[j & 3][lane] = ids < 0 ? 1.f : ks;
+          s_ve[j & 3][lane] = ids < 0 ? 0.f : vs == vs ? (float)((__float_as_int(vs) >> 23) - 127) : vs;
+        }
+        const uint32_t okm = __ballot_sync(0xffffffffu, lane < GROUPS && ids >= 0);
+        if (lane == 0) s_ok[j & 3] = okm;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sc_full(j & 3));
+      }
+      const int ki = 2 * j, vi = 2 * j + 1;
+      if (ki >= NS && !mbar_wait(slot_empty(ki % NS), (ki / NS - 1) & 1, abort_w, c.status, 0x6300)) break;
+      store(ki, raw_k);
+      if (j + 1 < nj) load(c.k, ids_next, j + 1, raw_k);
+      if (vi >= NS && !mbar_wait(slot_empty(vi % NS), (vi / NS - 1) & 1, abort_w, c.status, 0x6400)) break;
+      store(vi, raw_v);
+      if (j + 1 < nj) load(c.v, ids_next, j + 1, raw_v);
+      ids = ids_next;
+      ids_next = pages_of(j + 2);
+    }
+  } else if (warp / 4 < active) {
+    // ---- softmax -----------------------------------------------------------
+    const int x = warp / 4, t = threadIdx.x & 127;
+    const int r = row0 + 128 * x + t;
+    const int tok = r / a.group;
+    const bool alive = r < rows_all && tok < count;
+    const int end = alive ? len - count + tok + 1 : 0;
+    const int first = row0 + 128 * x;
+    const int all_end = len - count + first / a.group + 1;  // tokens that every live row sees
+    const uint32_t lane_base = tm + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t t_s = lane_base + Sh::T_S + (uint32_t)(TOK * x);
+    const uint32_t t_o = lane_base + Sh::T_O + (uint32_t)(HD * x);
+    float sc;
+    {
+      // q: the row's largest magnitude, then scaled and split
+      const int64_t off = b * a.qs.batch + (int64_t)tok * a.qs.token +
+                          (int64_t)(h * a.group + r % a.group) * a.qs.head;
+      float mx = 0.f, v[16];
+      for (int d = 0; d < c.hd; d += 16) {
+        if (alive) kv_load_row16(a.dtype, a.q, off + d, a.q_vec, v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, alive ? fabsf(v[i]) : 0.f);
+      }
+      int e = (__float_as_int(mx) >> 23) - 127;
+      e = mx > 0.f ? min(max(e, -126), 126) : 0;
+      const float f = kv_pow2(-e);
+#pragma unroll
+      for (int d = 0; d < HD; d += 16) {
+        if (alive && d < c.hd) {
+          kv_load_row16(a.dtype, a.q, off + d, a.q_vec, v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = 0.f;
+        }
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if constexpr (PIECES == 2) f16_split2(v[2 * i] * f, v[2 * i + 1] * f, hi[i], lo[i]);
+          else hi[i] = pack_f16(v[2 * i] * f, v[2 * i + 1] * f);
+        }
+#pragma unroll
+        for (int w = 0; w < PIECES; ++w) {
+          const uint32_t *p = w ? lo : hi;
+          if constexpr (Sh::QT) {
+            asm volatile(
+                "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(
+                    lane_base + Sh::T_Q + (uint32_t)((x * PIECES + w) * (HD / 2) + d / 2)),
+                "r"(p[0]), "r"(p[1]), "r"(p[2]), "r"(p[3]), "r"(p[4]), "r"(p[5]), "r"(p[6]),
+                "r"(p[7])
+                : "memory");
+          } else {
+            uint8_t *row = smem + (uint32_t)((x * PIECES + w) * Sh::BOXES + d / 64) * Sh::QBOX + t * 128;
+            const int c0 = (d % 64) / 8;
+            *reinterpret_cast<uint4 *>(row + ((c0 ^ (t & 7)) << 4)) = make_uint4(p[0], p[1], p[2], p[3]);
+            *reinterpret_cast<uint4 *>(row + (((c0 + 1) ^ (t & 7)) << 4)) = make_uint4(p[4], p[5], p[6], p[7]);
+          }
+        }
+      }
+      sc = a.scale * 1.4426950408889634f * kCodeUnit<FMT> * kv_pow2(e);
+      if constexpr (Sh::QT) tmem_wait_st();
+      else fence_async();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_ready);
+    }
+    float m = -CUDART_INF_F, l = 0.f;
+    for (int j = 0; j < nj; ++j) {
+      const int t0 = (j0 + j) * TOK;
+      mbar_wait(sc_full(j & 3), (j >> 2) & 1, abort_w, c.status, 0x6500);
+      const uint32_t okm = s_ok[j & 3];
+      const bool open = t0 + TOK <= all_end && okm == (1u << GROUPS) - 1u;  // the same for the warp
+      const float *ks = s_ks[j & 3], *ve = s_ve[j & 3];
+      mbar_wait(s_full(x), j & 1, abort_w, c.status, 0x6600);
+      fence_after();
+      // bits of the columns this row sees, in its 16-token group g
+      auto seen = [&](int g) -> uint32_t {
+        const int n = end - t0 - 16 * g;
+        const uint32_t mask = n >= 16 ? 0xffffu : n <= 0 ? 0u : (1u << n) - 1u;
+        return (okm >> g) & 1u ? mask : 0u;
+      };
+      float top = -CUDART_INF_F;
+#pragma unroll
+      for (int q = 0; q < TOK / 32; ++q) {
+        float s[32];
+        tmem_ld32(t_s + 32u * q, s);
+        tmem_wait_ld();
+#pragma unroll
+        for (int g2 = 0; g2 < 2; ++g2) {
+          const int g = 2 * q + g2;
+          float *sg = s + 16 * g2;
+          if (!open) {
+            const uint32_t mk = seen(g);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sg[i] = (mk >> i) & 1u ? sg[i] : -CUDART_INF_F;
+          }
+          float mx = fmaxf(fmax3(sg[0], sg[1], sg[2]), sg[3]);
+#pragma unroll
+          for (int i = 4; i < 16; i += 2) mx = fmax3(mx, sg[i], sg[i + 1]);
+          top = fmaxf(top, fmaf(mx, ks[g] * sc, ve[g]));
+        }
+      }
+      constexpr float kLazy = 8.f;
+      const bool raise = top > m + kLazy || (m == -CUDART_INF_F && top > m);
+      const float mn = raise ? ceilf(top) : m;
+      const float alpha = raise ? exp2_approx(m - mn) : 1.f;  // 0 from -inf
+      if (j > 0 && __any_sync(0xffffffffu, raise && m != -CUDART_INF_F)) {
+        mbar_wait(o_done(x), (j - 1) & 1, abort_w, c.status, 0x6700);
+        fence_after();
+#pragma unroll 1
+        for (int d = 0; d < HD; d += 16) {
+          uint32_t o[16];
+          tmem_ld16(t_o + d, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          tmem_st16(t_o + d, o);
+        }
+      }
+      l *= alpha;
+      m = mn;
+      const float ref = m == -CUDART_INF_F ? 0.f : m;
+#pragma unroll
+      for (int q = 0; q < TOK / 32; ++q) {
+        float s[32];
+        tmem_ld32(t_s + 32u * q, s);
+        tmem_wait_ld();
+        uint32_t w[32];
+#pragma unroll
+        for (int g2 = 0; g2 < 2; ++g2) {
+          const int g = 2 * q + g2;
+          const float kc = ks[g] * sc, bs = ve[g] - ref + 7.f;
+          const uint32_t mk = open ? 0xffffu : seen(g);
+          float sum[2] = {0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float p0 = exp2_approx(fmaf(s[16 * g2 + 2 * i], kc, bs));
+            float p1 = exp2_approx(fmaf(s[16 * g2 + 2 * i + 1], kc, bs));
+            if (!open) {
+              p0 = (mk >> (2 * i)) & 1u ? p0 : 0.f;
+              p1 = (mk >> (2 * i + 1)) & 1u ? p1 : 0.f;
+            }
+            sum[0] += p0;
+            sum[1] += p1;
+            const uint32_t hp = pack_f16(p0, p1);
+            w[8 * g2 + i] = hp;
+            if constexpr (PIECES == 2)
+              w[16 + 8 * g2 + i] = pack_f16(__fsub_rn(p0, widen_nonneg(hp & 0xffffu)),
+                                            __fsub_rn(p1, widen_nonneg(hp >> 16)));
+          }
+          // 2^-e from the exponent; a NaN counts only where a token of it is seen
+          const float both = sum[0] + sum[1];
+          if (both != 0.f) l = fmaf(both, exp2_approx(-ve[g]), l);
+        }
+        tmem_st16(t_s + 32u * q, w);
+        if constexpr (PIECES == 2) tmem_st16(t_s + 32u * q + 16u, w + 16);
+      }
+      tmem_wait_st();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full(x));
+    }
+    mbar_wait(o_done(x), (nj - 1) & 1, abort_w, c.status, 0x6800);
+    fence_after();
+    const float inv = l == 0.f ? 0.f : kCodeUnit<FMT> / l;
+    const int64_t at = out_row(r < rows_all ? r : 0);
+#pragma unroll
+    for (int d = 0; d < HD; d += 16) {
+      uint32_t o[16];
+      tmem_ld16(t_o + d, o);
+      tmem_wait_ld();
+      float v[16];
+      if (splits > 1) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<uint4 *>(a.ws + part(r) * HD + d + i) =
+              make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+      } else if (d < c.hd && r < rows_all) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = end > 0 && l != 0.f ? __uint_as_float(o[i]) * inv : 0.f;
+        kv_store_row16(a.dtype, a.out, at + d, v);
+      }
+    }
+    if (splits > 1) {
+      part_ml[2 * part(r)] = m;
+      part_ml[2 * part(r) + 1] = end > 0 ? l : 0.f;
+    }
+    fence_before();
+  } else {
+    // a tile without a live row: zeros
+    const int r = row0 + threadIdx.x;
+    if (splits > 1) {
+      part_ml[2 * part(r)] = -CUDART_INF_F;
+      part_ml[2 * part(r) + 1] = 0.f;
+    } else if (r < rows_all) {
+      const float z[16] = {};
+      for (int d = 0; d < c.hd; d += 16) kv_store_row16(a.dtype, a.out, out_row(r) + d, z);
+    }
+  }
+  __syncthreads();
+  if (warp == kMmaWarp)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm));
+}
+
+// Joins the splits of each row, in their order; one thread per 4 dims.
+template <int HD, int FMT>
+__global__ void __launch_bounds__(256) kv_attention_tiles_join_kernel(KvAttentionArgs a,
+                                                                      int64_t rows_padded,
+                                                                      int splits) {
+  pdl_trigger();
+  pdl_wait();
+  const KvView &c = a.c;
+  const int rows_all = a.tokens * a.group;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int d = (int)(i % (HD / 4)) * 4;
+  const int64_t r64 = i / (HD / 4);
+  if (r64 >= rows_all || d >= c.hd) return;
+  const int r = (int)r64, h = blockIdx.y, b = blockIdx.z;
+  const float *ml = a.ws + (int64_t)splits * c.batch * c.heads * rows_padded * HD;
+  auto part = [&](int s) { return (((int64_t)s * c.batch + b) * c.heads + h) * rows_padded + r; };
+  float m = -CUDART_INF_F;
+  for (int s = 0; s < splits; ++s) m = fmaxf(m, ml[2 * part(s)]);
+  float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < splits; ++s) {
+    const float ms = ml[2 * part(s)], ls = ml[2 * part(s) + 1];
+    if (ls == 0.f) continue;  // a split that the row sees nothing of (its O may not exist)
+    const float f = ms == m || !(ls == ls) ? 1.f : exp2_approx(ms - m);
+    const float4 v = *reinterpret_cast<const float4 *>(a.ws + part(s) * HD + d);
+    l = fmaf(ls, f, l);
+    o[0] = fmaf(v.x, f, o[0]), o[1] = fmaf(v.y, f, o[1]);
+    o[2] = fmaf(v.z, f, o[2]), o[3] = fmaf(v.w, f, o[3]);
+  }
+  const float inv = l == 0.f ? 0.f : kCodeUnit<FMT> / l;
+  const int64_t at = (((int64_t)b * a.tokens + r / a.group) * a.heads + h * a.group + r % a.group) * c.hd + d;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) kv_store_out(a.dtype, a.out, at + k, o[k] * inv);
+}
+
+struct TilePlan {
+  int row_tiles, splits;
+  int64_t rows_padded;
+  size_t ws_bytes;
+};
+
+template <int HD, int PIECES>
+TilePlan tile_plan(const KvView &c, int64_t tokens, int heads, int sms) {
+  using Sh = TcShape<HD, PIECES>;
+  TilePlan p{};
+  const int64_t rows = tokens * (heads / c.heads);
+  p.row_tiles = (int)ceil_div(rows, 128 * Sh::MT);
+  p.rows_padded = (int64_t)p.row_tiles * 128 * Sh::MT;
+  const int64_t ctas = (int64_t)p.row_tiles * c.heads * c.batch;
+  const int64_t tiles = ceil_div((int64_t)c.columns << c.page_log2, Sh::TOK);
+  // one CTA an SM: too few of them share the tokens, four tiles each at least
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(sms / std::max<int64_t>(ctas, 1), tiles / 4));
+  p.ws_bytes = p.splits > 1 ? (size_t)p.splits * c.batch * c.heads * p.rows_padded * (HD + 2) * sizeof(float)
+                            : 0;
+  return p;
+}
+
+int sm_count(int *out) {
+  int dev = 0;
+  TT_CUDA_TRY(cudaGetDevice(&dev));
+  TT_CUDA_TRY(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev));
+  return TT_OK;
+}
+
+template <int HD, int FMT, int PIECES>
+int launch_tiles(const KvAttentionArgs &a, cudaStream_t stream) {
+  using Sh = TcShape<HD, PIECES>;
+  int sms = 0;
+  const int rc = sm_count(&sms);
+  if (rc != TT_OK) return rc;
+  if ((int64_t)a.tokens * a.group > INT32_MAX || a.c.batch > 65535 || a.c.heads > 65535)
+    return fail(TT_ERR_UNSUPPORTED, "tt_kv_attention: too many rows, heads or sequences");
+  const TilePlan p = tile_plan<HD, PIECES>(a.c, a.tokens, a.heads, sms);
+  if ((int64_t)p.row_tiles * a.c.heads > INT32_MAX)
+    return fail(TT_ERR_UNSUPPORTED, "tt_kv_attention: too many rows");
+  auto *kern = kv_attention_tiles_kernel<HD, FMT, PIECES>;
+  static bool set[64] = {};
+  int dev = 0;
+  TT_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev >= 64 || !set[dev]) {
+    TT_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::SMEM));
+    if (dev < 64) set[dev] = true;
+  }
+  TT_CUDA_TRY(launch_kernel(kern, dim3(p.row_tiles * a.c.heads, a.c.batch, p.splits), dim3(Sh::THREADS),
+                            Sh::SMEM, stream, 1, a, p.row_tiles, p.splits));
+  if (p.splits > 1)
+    TT_CUDA_TRY(launch_kernel(kv_attention_tiles_join_kernel<HD, FMT>,
+                              dim3((unsigned)ceil_div((int64_t)a.tokens * a.group * (HD / 4), 256),
+                                   a.c.heads, a.c.batch),
+                              dim3(256), 0, stream, 1, a, p.rows_padded, p.splits));
+  return TT_OK;
+}
+
+template <class F>
+int for_tiles(const KvView &c, int dtype, F &&f) {
+  const bool i8 = c.format == TT_KV_INT8, two = dtype == TT_DTYPE_F32;
+  using std::integral_constant;
+#define TT_KV_TILES(HD, P)                                                                            \
+  return i8 ? f(integral_constant<int, HD>(), integral_constant<int, TT_KV_INT8>(), integral_constant<int, P>()) \
+            : f(integral_constant<int, HD>(), integral_constant<int, TT_KV_E4M3>(), integral_constant<int, P>())
+  if (c.hd <= 64) {
+    if (two) TT_KV_TILES(64, 2);
+    TT_KV_TILES(64, 1);
+  }
+  if (c.hd <= 128) {
+    if (two) TT_KV_TILES(128, 2);
+    TT_KV_TILES(128, 1);
+  }
+  if (two) TT_KV_TILES(256, 2);
+  TT_KV_TILES(256, 1);
+#undef TT_KV_TILES
+}
+
+}  // namespace
+
+size_t kv_attention_tiles_ws_bytes(const KvView &c, int64_t tokens, int heads) {
+  int sms = 0;
+  if (sm_count(&sms) != TT_OK) return 0;
+  size_t n = 0;
+  for_tiles(c, TT_DTYPE_F32, [&](auto hd, auto, auto pieces) {  // the same for every type
+    n = tile_plan<decltype(hd)::value, decltype(pieces)::value>(c, tokens, heads, sms).ws_bytes;
+    return TT_OK;
+  });
+  return n;
+}
+
+int launch_kv_attention_tiles(const KvAttentionArgs &a, cudaStream_t stream) {
+  return for_tiles(a.c, a.dtype, [&](auto hd, auto fmt, auto pieces) {
+    return launch_tiles<decltype(hd)::value, decltype(fmt)::value, decltype(pieces)::value>(a, stream);
+  });
+}
+
+}  // namespace tt

@@ -383,6 +383,7 @@ int tt_kv_attention(const tt_kv_cache *cache, int dtype, const void *q, const in
   a.heads = heads;
   a.group = heads / c.heads;
   a.scale = scale;
+  a.q_vec = vec_ok(q, a.qs, dtype == TT_DTYPE_F32 ? 4 : 2);
   return launch_kv_attention(a, static_cast<cudaStream_t>(stream));
 }
 

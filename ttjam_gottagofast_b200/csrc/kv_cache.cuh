@@ -138,10 +138,14 @@ struct KvAttentionArgs {
   float *ws;  // partial results
   int dtype, tokens, heads, group;
   float scale;
+  bool q_vec;  // q's rows are 16-byte aligned
 };
 
 // kv_attention.cu
 size_t kv_attention_ws_bytes(const KvView &c, int64_t tokens, int heads);
 int launch_kv_attention(const KvAttentionArgs &a, cudaStream_t stream);
+// kv_attention_tc.cu
+size_t kv_attention_tiles_ws_bytes(const KvView &c, int64_t tokens, int heads);
+int launch_kv_attention_tiles(const KvAttentionArgs &a, cudaStream_t stream);
 
 }  // namespace tt

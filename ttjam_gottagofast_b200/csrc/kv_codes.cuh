@@ -1,0 +1,113 @@
+// Codes of the 8-bit key/value cache as tensor-core operands, and typed rows:
+// shared by the two attention kernels over it.
+#pragma once
+
+#include "kv_cache.cuh"
+
+namespace tt {
+
+// Codes to fp16 pairs, exact, by integer operations, so that no bit pattern
+// (a slot that was never written) turns into a NaN. int8: 1024 + (code + 128)
+// is the fp16 with that low byte, minus 1152. e4m3: the bits put in place under
+// the fp16 exponent are the value * 2^-8, for normal and subnormal codes alike;
+// kCodeUnit gives the factor back.
+template <int FMT>
+constexpr float kCodeUnit = FMT == TT_KV_INT8 ? 1.f : 256.f;
+
+__device__ __forceinline__ uint32_t i8_pair(uint32_t biased, uint32_t sel) {
+  uint32_t r = __byte_perm(biased, 0x64646464u, sel);
+  asm("sub.f16x2 %0, %0, %1;" : "+r"(r) : "r"(0x64806480u));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t t) {  // codes in bits 8-15 and 24-31
+  return (t & 0x80008000u) | ((t >> 1) & 0x3f803f80u);
+}
+// four consecutive codes -> (0, 1), (2, 3)
+template <int FMT>
+__device__ __forceinline__ void codes_along(uint32_t w, uint32_t &a, uint32_t &b) {
+  if constexpr (FMT == TT_KV_INT8) {
+    const uint32_t u = w ^ 0x80808080u;
+    a = i8_pair(u, 0x4140);
+    b = i8_pair(u, 0x4342);
+  } else {
+    a = e4m3_pair(__byte_perm(w, 0, 0x1000));
+    b = e4m3_pair(__byte_perm(w, 0, 0x3020));
+  }
+}
+// four codes of each of two tokens -> the pair (x, y) of each code
+template <int FMT>
+__device__ __forceinline__ void codes_across(uint32_t x, uint32_t y, uint32_t *r) {
+  if constexpr (FMT == TT_KV_INT8) {
+    const uint32_t lo = __byte_perm(x, y, 0x5140) ^ 0x80808080u;
+    const uint32_t hi = __byte_perm(x, y, 0x7362) ^ 0x80808080u;
+    r[0] = i8_pair(lo, 0x4140);
+    r[1] = i8_pair(lo, 0x4342);
+    r[2] = i8_pair(hi, 0x4140);
+    r[3] = i8_pair(hi, 0x4342);
+  } else {
+    r[0] = e4m3_pair(__byte_perm(x, y, 0x4000));
+    r[1] = e4m3_pair(__byte_perm(x, y, 0x5010));
+    r[2] = e4m3_pair(__byte_perm(x, y, 0x6020));
+    r[3] = e4m3_pair(__byte_perm(x, y, 0x7030));
+  }
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float kv_load_in(int dtype, const void *p, int64_t i) {
+  if (dtype == TT_DTYPE_F32) return static_cast<const float *>(p)[i];
+  if (dtype == TT_DTYPE_F16) return __half2float(static_cast<const __half *>(p)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+}
+__device__ __forceinline__ void kv_store_out(int dtype, void *p, int64_t i, float x) {
+  if (dtype == TT_DTYPE_F32) static_cast<float *>(p)[i] = x;
+  else if (dtype == TT_DTYPE_F16) static_cast<__half *>(p)[i] = __float2half_rn(x);
+  else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(x);
+}
+
+// 16 consecutive elements from element i on; `vec`: the address is a multiple of 16 bytes.
+template <typename T>
+__device__ __forceinline__ void load_row16(const T *p, bool vec, float *x) {
+  constexpr int N = 16 * sizeof(T) / 16, E = 16 / sizeof(T);
+  if (vec) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const uint4 raw = reinterpret_cast<const uint4 *>(p)[n];
+      const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[n * E + i] = kv_to_float(e[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = kv_to_float(p[i]);
+  }
+}
+__device__ __forceinline__ void kv_load_row16(int dtype, const void *p, int64_t i, bool vec, float *x) {
+  if (dtype == TT_DTYPE_F32) load_row16(static_cast<const float *>(p) + i, vec, x);
+  else if (dtype == TT_DTYPE_F16) load_row16(static_cast<const __half *>(p) + i, vec, x);
+  else load_row16(static_cast<const __nv_bfloat16 *>(p) + i, vec, x);
+}
+// 16 consecutive elements at a 16-byte-aligned address.
+template <typename T>
+__device__ __forceinline__ void store_row16(T *p, const float *x) {
+  constexpr int N = 16 * sizeof(T) / 16, E = 16 / sizeof(T);
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    uint4 raw;
+    T *e = reinterpret_cast<T *>(&raw);
+#pragma unroll
+    for (int i = 0; i < E; ++i) kv_store(e + i, x[n * E + i]);
+    reinterpret_cast<uint4 *>(p)[n] = raw;
+  }
+}
+__device__ __forceinline__ void kv_store_row16(int dtype, void *p, int64_t i, const float *x) {
+  if (dtype == TT_DTYPE_F32) store_row16(static_cast<float *>(p) + i, x);
+  else if (dtype == TT_DTYPE_F16) store_row16(static_cast<__half *>(p) + i, x);
+  else store_row16(static_cast<__nv_bfloat16 *>(p) + i, x);
+}
+
+}  // namespace tt
