@@ -275,6 +275,7 @@ int tt_last_error(char *buf, size_t len);
 #define TT_KERNEL_ROW_SCAN 9      /* valid lengths and live row tiles of a padded batch */
 #define TT_KERNEL_CONVERT 10      /* 16-bit x widened to fp32, fp32 y rounded to 16 bits, or a
                                      copy kernel of tt_forward_host (x, mask in; y out) */
+#define TT_KERNEL_KV_WRITE 11     /* keys and values into the cache (tt_forward_cached) */
 
 /* Launch timing probe, a measurement aid with no counterpart in the
  * reference. tt_launch_probe_start(capacity) creates 2 * capacity timing
@@ -401,6 +402,27 @@ size_t tt_kv_attention_workspace_bytes(const tt_kv_cache *cache, int64_t tokens,
 int tt_kv_attention(const tt_kv_cache *cache, int dtype, const void *q, const int64_t *q_strides,
                     int64_t tokens, int32_t heads, const int32_t *counts, float scale, void *out,
                     void *workspace, size_t workspace_bytes, void *stream);
+
+/* Bytes of scratch tt_forward_cached needs on the current device (0 for
+ * arguments it refuses). */
+size_t tt_cached_workspace_bytes(const tt_config *cfg, int dtype, const tt_kv_cache *caches,
+                                 int64_t batch, int64_t tokens);
+
+/* The forward pass of a causal model on new tokens alone: x and y are [batch,
+ * tokens, d_model] of element type `dtype` (as in tt_forward_typed), caches one
+ * entry for each layer, all of one batch, page size and table shape, with
+ * num_heads heads of the model's head_dim. Row i < counts[b] (counts NULL: every
+ * row) of sequence b stands at position lengths[b] - counts[b] + i; each layer
+ * writes its keys and values into its cache and attends over it, so tokens are
+ * given once, in one call or many. Rows at or behind counts[b] give zero rows of
+ * y. Runs the per-op schedules (TT_PLAN_AUTO, TT_PLAN_OPS_FFMA or
+ * TT_PLAN_OPS_TC) with direct launches on `stream`; capture it in a CUDA graph
+ * to replay it. The split-precision schedule holds the attention's contexts as
+ * fp16 pieces, and rounding to a code can enlarge a value by 2^-4: set
+ * TT_FLAG_FP32_ONLY unless 1.0625 * tt_fp16_operand_bound is below TT_FP16_MAX. */
+int tt_forward_cached(const tt_config *cfg, const void *image, int dtype, const void *x,
+                      const tt_kv_cache *caches, const int32_t *counts, int64_t batch, int64_t tokens,
+                      void *y, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Synchronises `stream`, reads and clears the cache's status word: *code receives
  * TT_OK or the first latched TT_ERR_DEVICE_*, *detail which check it was. */

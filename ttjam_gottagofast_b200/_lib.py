@@ -44,7 +44,7 @@ EXPORTED = (
     "tt_pack_image_typed", "tt_typed_workspace_bytes", "tt_forward_typed",
     "tt_host_workspace_bytes", "tt_forward_host", "tt_test_gelu",
     "tt_kv_write", "tt_kv_read", "tt_kv_attention", "tt_kv_attention_workspace_bytes",
-    "tt_kv_read_status",
+    "tt_kv_read_status", "tt_forward_cached", "tt_cached_workspace_bytes",
 )
 
 # Element types of the typed entry points (TT_DTYPE_*), by torch dtype name.
@@ -58,7 +58,8 @@ KV_FORMATS = {"e4m3": 0, "int8": 1}
 
 # TT_KERNEL_* launch kinds reported by tt_launch_probe_read.
 KERNEL_KINDS = {1: "layernorm", 2: "qkv", 3: "attention", 4: "out_proj", 5: "ffn_in",
-                6: "ffn_out", 7: "final_norm", 8: "whole_forward", 9: "row_scan", 10: "convert"}
+                6: "ffn_out", 7: "final_norm", 8: "whole_forward", 9: "row_scan", 10: "convert",
+                11: "kv_write"}
 
 
 class TTConfig(ctypes.Structure):
@@ -160,6 +161,10 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
         lib.tt_kv_attention.restype = ctypes.c_int
         lib.tt_kv_attention.argtypes = [kvp, ctypes.c_int, vp, i64p, i64, i32, vp,
                                         ctypes.c_float, vp, vp, sz, vp]
+        lib.tt_cached_workspace_bytes.restype = sz
+        lib.tt_cached_workspace_bytes.argtypes = [cfgp, ctypes.c_int, kvp, i64, i64]
+        lib.tt_forward_cached.restype = ctypes.c_int
+        lib.tt_forward_cached.argtypes = [cfgp, vp, ctypes.c_int, vp, kvp, vp, i64, i64, vp, vp, sz, vp]
         lib.tt_kv_read_status.restype = ctypes.c_int
         lib.tt_kv_read_status.argtypes = [kvp, ctypes.POINTER(i32), ctypes.POINTER(i32), vp]
         if lib.tt_abi_version() != TT_ABI_VERSION:

@@ -9,6 +9,7 @@
 #include "cluster_forward.cuh"
 #include "gemm_tc.cuh"
 #include "image.cuh"
+#include "kv_cache.cuh"
 #include "tile_forward.cuh"
 #include "tt_common.cuh"
 
@@ -149,6 +150,33 @@ int timed_launch(int kind, cudaStream_t stream, F &&launch) {
     pr.count = i + 1;
   }
   return rc;
+}
+
+// The cached form of a layer's attention: k and v of the fp32 q|k|v rows into
+// the cache, then q over it.
+int cached_attention(const CachedStep &step, int layer, const float *qkv, int64_t batch, int64_t seq,
+                     int D, int H, float scale, KvOut out, cudaStream_t stream) {
+  const KvView &c = step.caches[layer];
+  const KvStrides st{seq * 3 * D, 3 * D, D / H};
+  int rc;
+  if ((rc = timed_launch(TT_KERNEL_KV_WRITE, stream, [&] {
+         return launch_kv_write(c, TT_DTYPE_F32, qkv + D, qkv + 2 * D, st, st, seq, step.counts, stream);
+       })))
+    return rc;
+  KvAttentionArgs a{};
+  a.c = c;
+  a.q = qkv;
+  a.qs = st;
+  a.out = out;
+  a.counts = step.counts;
+  a.ws = step.attention_ws;
+  a.dtype = TT_DTYPE_F32;
+  a.tokens = (int)seq;
+  a.heads = H;
+  a.group = 1;
+  a.scale = scale;
+  a.q_vec = (D / H) % 4 == 0 && D % 4 == 0;
+  return timed_launch(TT_KERNEL_ATTENTION, stream, [&] { return launch_kv_attention(a, stream); });
 }
 
 }  // namespace
@@ -300,7 +328,8 @@ int forward_tile(const tt_config &cfg, const ImageLayout &L, const char *image, 
 
 int forward_ops(const tt_config &cfg, const ImageLayout &L, const char *image, const float *x,
                 const uint8_t *mask, int64_t batch, int64_t seq, float *y,
-                const WorkspaceLayout &W, char *ws, cudaStream_t stream) {
+                const WorkspaceLayout &W, char *ws, cudaStream_t stream,
+                const CachedStep *cached) {
   const int D = cfg.d_model, F = cfg.ffn_dim, H = cfg.num_heads, hd = D / H;
   const int64_t T = batch * seq;
   float *qkv = reinterpret_cast<float *>(ws + W.qkv);
@@ -324,9 +353,14 @@ int forward_ops(const tt_config &cfg, const ImageLayout &L, const char *image, c
     a.qkv = qkv; a.ctx = ctx; a.mask = mask; a.batch = batch; a.seq = (int)seq;
     a.d_model = D; a.num_heads = H; a.head_dim = hd; a.causal = cfg.causal;
     a.scale = (float)(1.0 / std::sqrt((double)hd));
-    if ((rc = timed_launch(TT_KERNEL_ATTENTION, stream,
-                           [&] { return launch_attention_ffma(a, stream); })))
+    if (cached != nullptr) {
+      if ((rc = cached_attention(*cached, l, qkv, batch, seq, D, H, a.scale,
+                                 {ctx, nullptr, TT_DTYPE_F32}, stream)))
+        return rc;
+    } else if ((rc = timed_launch(TT_KERNEL_ATTENTION, stream,
+                                  [&] { return launch_attention_ffma(a, stream); }))) {
       return rc;
+    }
     // y = x + masked(context . Wo^T + bo)
     GemmParams go{};
     go.A = ctx; go.lda = D; go.W = P(o.wo); go.bias = P(o.bo); go.R = xin; go.C = y;
@@ -382,7 +416,8 @@ bool ops_tc_skips_dead_rows(const tt_config &cfg, int64_t tokens) {
 
 int forward_ops_tc(const tt_config &cfg, const ImageLayout &L, const char *image, const float *x,
                    const uint8_t *mask, int64_t batch, int64_t seq, float *y,
-                   const WorkspaceLayout &W, char *ws, cudaStream_t stream) {
+                   const WorkspaceLayout &W, char *ws, cudaStream_t stream,
+                   const CachedStep *cached) {
   const int D = cfg.d_model, F = cfg.ffn_dim, H = cfg.num_heads, hd = D / H;
   const int64_t T = batch * seq;
   if (T > INT32_MAX) return fail(TT_ERR_UNSUPPORTED, "tensor-core schedule: too many tokens");
@@ -463,6 +498,10 @@ int forward_ops_tc(const tt_config &cfg, const ImageLayout &L, const char *image
       a.head_dim = hd; a.causal = cfg.causal; a.scale = scale; a.counter = attn_counter;
       if ((rc = timed_launch(TT_KERNEL_ATTENTION, stream,
                              [&] { return launch_attention_tc(a, stream); })))
+        return rc;
+    } else if (cached != nullptr) {
+      if ((rc = cached_attention(*cached, l, qkv, batch, seq, D, H, scale, {ctx_hi, ctx_lo, kKvSplit},
+                                 stream)))
         return rc;
     } else {
       AttentionParams a{};
@@ -744,6 +783,114 @@ int tt_forward_typed(const tt_config *cfg, const void *image, int dtype, const v
   if ((rc = tt_forward(cfg, image, x32, mask, batch, seq, y32, ws + 2 * io,
                        workspace_bytes - 2 * io, stream_)))
     return rc;
+  return timed_launch(TT_KERNEL_CONVERT, stream,
+                      [&] { return launch_narrow(dtype, y32, y, n, stream); });
+}
+
+// The per-op schedule of a step over the cache, its buffers, and where they lie
+// in the workspace: [x, y in fp32, for a 16-bit dtype] [W] [row mask] [attention].
+struct CachedLayout {
+  tt_config ops;
+  int plan = 0;
+  size_t io = 0, w = 0, mask = 0, attention = 0, total = 0;
+};
+
+// The checks of a cached step, and its layout. `caches` has one entry a layer.
+static int cached_layout(const tt_config *cfg, int dtype, const tt_kv_cache *caches, int64_t batch,
+                         int64_t tokens, std::vector<KvView> *views, CachedLayout *C) {
+  int rc = validate_config(cfg);
+  if (rc != TT_OK) return rc;
+  if (cfg->causal != 1)
+    return fail(TT_ERR_UNSUPPORTED, "tt_forward_cached: only a causal model runs token by token");
+  if (dtype != TT_DTYPE_F32 && dtype != TT_DTYPE_F16 && dtype != TT_DTYPE_BF16)
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_forward_cached: dtype must be a TT_DTYPE_* value");
+  if (batch < 0 || tokens < 0)
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_forward_cached: batch and tokens must be >= 0");
+  if (tokens > INT32_MAX || batch > 65535 || batch * tokens > INT32_MAX)
+    return fail(TT_ERR_UNSUPPORTED, "tt_forward_cached: batch * tokens too large");
+  if (caches == nullptr) return fail(TT_ERR_INVALID_ARGUMENT, "tt_forward_cached: caches is NULL");
+  if (cfg->plan == TT_PLAN_CLUSTER || cfg->plan == TT_PLAN_TILE)
+    return fail(TT_ERR_UNSUPPORTED, "tt_forward_cached runs the per-op schedules");
+  views->resize(cfg->num_layers);
+  for (int l = 0; l < cfg->num_layers; ++l) {
+    KvView &v = (*views)[l];
+    if ((rc = kv_view(&caches[l], "tt_forward_cached", &v)) != TT_OK) return rc;
+    if (v.batch != batch || v.heads != cfg->num_heads || v.hd * cfg->num_heads != cfg->d_model)
+      return fail(TT_ERR_INVALID_ARGUMENT,
+                  "tt_forward_cached: layer " + std::to_string(l) +
+                      "'s cache has another batch, number of heads or head_dim than the model");
+    if (v.columns != (*views)[0].columns || v.page_log2 != (*views)[0].page_log2)
+      return fail(TT_ERR_INVALID_ARGUMENT,
+                  "tt_forward_cached: the layers' caches have unlike page sizes or tables");
+  }
+  C->ops = *cfg;
+  if (C->ops.plan == TT_PLAN_AUTO) C->ops.plan = auto_ops_plan(*cfg);
+  C->plan = forward_plan(&C->ops, batch, tokens);
+  if (C->plan < 0) return C->plan;
+  const size_t T = (size_t)batch * (size_t)tokens;
+  C->io = dtype == TT_DTYPE_F32 ? 0 : align_up(T * (size_t)cfg->d_model * sizeof(float), 256);
+  C->w = 2 * C->io;
+  C->mask = C->w + WorkspaceLayout(C->ops, batch, tokens, true).total;
+  C->attention = C->mask + align_up(T, 256);
+  C->total = C->attention + (T > 0 ? kv_attention_ws_bytes((*views)[0], tokens, cfg->num_heads) : 0);
+  return TT_OK;
+}
+
+size_t tt_cached_workspace_bytes(const tt_config *cfg, int dtype, const tt_kv_cache *caches,
+                                 int64_t batch, int64_t tokens) {
+  std::vector<KvView> views;
+  CachedLayout C;
+  return cached_layout(cfg, dtype, caches, batch, tokens, &views, &C) == TT_OK ? C.total : 0;
+}
+
+int tt_forward_cached(const tt_config *cfg, const void *image, int dtype, const void *x,
+                      const tt_kv_cache *caches, const int32_t *counts, int64_t batch, int64_t tokens,
+                      void *y, void *workspace, size_t workspace_bytes, void *stream_) {
+  std::vector<KvView> views;
+  CachedLayout C;
+  int rc = cached_layout(cfg, dtype, caches, batch, tokens, &views, &C);
+  if (rc != TT_OK) return rc;
+  if (batch == 0 || tokens == 0) return TT_OK;
+  if (image == nullptr || x == nullptr || y == nullptr || workspace == nullptr)
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_forward_cached: NULL image, x, y or workspace");
+  if (x == y) return fail(TT_ERR_INVALID_ARGUMENT, "tt_forward_cached: y may not alias x");
+  if (misaligned(image) || misaligned(x) || misaligned(y) || misaligned(workspace))
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_forward_cached: pointers must be 16-byte aligned");
+  if (tokens > ((int64_t)views[0].columns << views[0].page_log2))
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_forward_cached: more tokens than a sequence has room for");
+  if (workspace_bytes < C.total)
+    return fail(TT_ERR_WORKSPACE, "tt_forward_cached: workspace smaller than "
+                                  "tt_cached_workspace_bytes (" + std::to_string(C.total) + " bytes)");
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  char *ws = static_cast<char *>(workspace);
+  const int64_t n = batch * tokens * (int64_t)cfg->d_model;
+  const float *x32 = static_cast<const float *>(x);
+  float *y32 = static_cast<float *>(y);
+  if (dtype != TT_DTYPE_F32) {
+    float *wide = reinterpret_cast<float *>(ws);
+    x32 = wide;
+    y32 = reinterpret_cast<float *>(ws + C.io);
+    if ((rc = timed_launch(TT_KERNEL_CONVERT, stream,
+                           [&] { return launch_widen(dtype, x, wide, n, stream); })))
+      return rc;
+  }
+  const uint8_t *mask = nullptr;
+  if (counts != nullptr) {
+    uint8_t *m = reinterpret_cast<uint8_t *>(ws + C.mask);
+    if ((rc = timed_launch(TT_KERNEL_ROW_SCAN, stream, [&] {
+           return launch_kv_mask(views[0], counts, tokens, m, stream);
+         })))
+      return rc;
+    mask = m;
+  }
+  const CachedStep step{views.data(), counts, reinterpret_cast<float *>(ws + C.attention)};
+  const ImageLayout L(*cfg);
+  const WorkspaceLayout W(C.ops, batch, tokens, true);
+  const char *img = static_cast<const char *>(image);
+  rc = C.plan == PLAN_OPS_TC
+           ? forward_ops_tc(C.ops, L, img, x32, mask, batch, tokens, y32, W, ws + C.w, stream, &step)
+           : forward_ops(C.ops, L, img, x32, mask, batch, tokens, y32, W, ws + C.w, stream, &step);
+  if (rc != TT_OK || dtype == TT_DTYPE_F32) return rc;
   return timed_launch(TT_KERNEL_CONVERT, stream,
                       [&] { return launch_narrow(dtype, y32, y, n, stream); });
 }

@@ -103,7 +103,9 @@ struct WorkspaceLayout {
   bool tensor = false;        // buffers of the tensor-core schedule
   bool tc_attention = false;  // ... whose attention also runs on tensor cores
 
-  WorkspaceLayout(const tt_config &cfg, int64_t batch, int64_t seq) {
+  // cached: of a step over the key/value cache, whose attention reads fp32
+  // q|k|v and keeps its partial results after everything else
+  WorkspaceLayout(const tt_config &cfg, int64_t batch, int64_t seq, bool cached = false) {
     const size_t T = (size_t)batch * (size_t)seq, D = cfg.d_model, F = cfg.ffn_dim;
     const size_t f4 = sizeof(float);
     // the buffers of the schedule the call runs: forced, or what TT_PLAN_AUTO
@@ -118,7 +120,7 @@ struct WorkspaceLayout {
       return off;
     };
     const int hd = cfg.d_model / cfg.num_heads;
-    tc_attention = tensor && attention_tc_supported(hd, cfg.d_model);
+    tc_attention = tensor && !cached && attention_tc_supported(hd, cfg.d_model);
     if (tc_attention) {
       // q|k as an fp16 split, and v transposed per (sequence, head) with keys
       // contiguous (rows of seq_pad fp16 values, a multiple of 16 bytes), for
@@ -142,6 +144,15 @@ struct WorkspaceLayout {
     }
     total = cur;
   }
+};
+
+// The attention of a step on new tokens (tt_forward_cached): layer l writes its
+// keys and values into caches[l] and attends over it.
+struct KvView;
+struct CachedStep {
+  const KvView *caches;
+  const int32_t *counts;
+  float *attention_ws;
 };
 
 // Everything a per-op forward's launch sequence depends on (graph_cache.cu):
@@ -170,12 +181,14 @@ int auto_ops_plan(const tt_config &cfg);
 int noalloc_scratch_address(void **out);
 int forward_ops(const tt_config &cfg, const ImageLayout &L, const char *image, const float *x,
                 const uint8_t *mask, int64_t batch, int64_t seq, float *y,
-                const WorkspaceLayout &W, char *ws, cudaStream_t stream);
+                const WorkspaceLayout &W, char *ws, cudaStream_t stream,
+                const CachedStep *cached = nullptr);
 // Whether the tensor-core schedule lists the live row tiles of the batch and
 // lets its GEMMs skip the rest (one extra launch): GEMM-heavy shapes only.
 bool ops_tc_skips_dead_rows(const tt_config &cfg, int64_t tokens);
 int forward_ops_tc(const tt_config &cfg, const ImageLayout &L, const char *image, const float *x,
                    const uint8_t *mask, int64_t batch, int64_t seq, float *y,
-                   const WorkspaceLayout &W, char *ws, cudaStream_t stream);
+                   const WorkspaceLayout &W, char *ws, cudaStream_t stream,
+                   const CachedStep *cached = nullptr);
 
 }  // namespace tt

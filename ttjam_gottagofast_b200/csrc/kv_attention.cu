@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_rows_kernel(KvAttention
         const int row = rb * kRows + rr, ti = row / a.group;
         if (d < c.hd) {
           const float v = ti >= count || ll == 0.f ? 0.f : oo * kCodeUnit<FMT> / ll;
-          kv_store_out(a.dtype, a.out, (((int64_t)b * a.tokens + ti) * a.heads + h * a.group + row % a.group) * c.hd + d, v);
+          kv_store_out(a.out, (((int64_t)b * a.tokens + ti) * a.heads + h * a.group + row % a.group) * c.hd + d, v);
         }
       } else {
         slot[rr * HD + d] = oo;
@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_join_kernel(KvAttention
       oo = fmaf(s[rr * HD + d], f, oo);
     }
     const float v = ti >= count || ll == 0.f ? 0.f : oo * kCodeUnit<FMT> / ll;
-    kv_store_out(a.dtype, a.out, (((int64_t)b * a.tokens + ti) * a.heads + h * a.group + row % a.group) * c.hd + d, v);
+    kv_store_out(a.out, (((int64_t)b * a.tokens + ti) * a.heads + h * a.group + row % a.group) * c.hd + d, v);
   }
 }
 

@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
         part_ml[2 * part(r) + 1] = 0.f;
       } else if (r < rows_all) {
         const float z[16] = {};
-        for (int d = 0; d < c.hd; d += 16) kv_store_row16(a.dtype, a.out, out_row(r) + d, z);
+        for (int d = 0; d < c.hd; d += 16) kv_store_row16(a.out, out_row(r) + d, z);
       }
     }
     return;
@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       } else if (d < c.hd && r < rows_all) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = end > 0 && l != 0.f ? __uint_as_float(o[i]) * inv : 0.f;
-        kv_store_row16(a.dtype, a.out, at + d, v);
+        kv_store_row16(a.out, at + d, v);
       }
     }
     if (splits > 1) {
@@ -622,7 +622,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       part_ml[2 * part(r) + 1] = 0.f;
     } else if (r < rows_all) {
       const float z[16] = {};
-      for (int d = 0; d < c.hd; d += 16) kv_store_row16(a.dtype, a.out, out_row(r) + d, z);
+      for (int d = 0; d < c.hd; d += 16) kv_store_row16(a.out, out_row(r) + d, z);
     }
   }
   __syncthreads();
@@ -661,7 +661,7 @@ __global__ void __launch_bounds__(256) kv_attention_tiles_join_kernel(KvAttentio
   const float inv = l == 0.f ? 0.f : kCodeUnit<FMT> / l;
   const int64_t at = (((int64_t)b * a.tokens + r / a.group) * a.heads + h * a.group + r % a.group) * c.hd + d;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) kv_store_out(a.dtype, a.out, at + k, o[k] * inv);
+  for (int k = 0; k < 4; ++k) kv_store_out(a.out, at + k, o[k] * inv);
 }
 
 struct TilePlan {

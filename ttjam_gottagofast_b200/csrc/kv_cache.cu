@@ -174,6 +174,15 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvView c, T *k, T *v, uint
   }
 }
 
+__global__ void __launch_bounds__(256) kv_mask_kernel(KvView c, const int32_t *counts, int tokens,
+                                                      uint8_t *mask) {
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x;
+  const int count = c.count(counts, b, tokens, c.length(b));
+  if (i < tokens) mask[(int64_t)b * tokens + i] = i < count;
+}
+
 bool vec_ok(const void *p, const KvStrides &s, int size) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (s.batch * size) % 16 == 0 &&
          (s.token * size) % 16 == 0 && (s.head * size) % 16 == 0;
@@ -229,6 +238,13 @@ int launch_kv_write(const KvView &c, int dtype, const void *k, const void *v, Kv
   }
 }
 
+int launch_kv_mask(const KvView &c, const int32_t *counts, int64_t tokens, uint8_t *mask,
+                   cudaStream_t stream) {
+  TT_CUDA_TRY(launch_kernel(kv_mask_kernel, dim3((unsigned)ceil_div(tokens, 256), c.batch), dim3(256),
+                            0, stream, 1, c, counts, (int)tokens, mask));
+  return TT_OK;
+}
+
 template <typename T>
 static int read_typed(const KvView &c, void *k, void *v, int64_t max_tokens, cudaStream_t stream) {
   const int64_t per_seq = max_tokens * c.heads * (c.hd >> 4);
@@ -250,8 +266,7 @@ int launch_kv_read(const KvView &c, int dtype, void *k, void *v, int64_t max_tok
   }
 }
 
-// The checks every entry point makes of a cache; fills *v.
-static int kv_view(const tt_kv_cache *c, const char *what, KvView *v) {
+int kv_view(const tt_kv_cache *c, const char *what, KvView *v) {
   auto no = [&](int code, const std::string &m) { return fail(code, std::string(what) + ": " + m); };
   if (c == nullptr) return no(TT_ERR_INVALID_ARGUMENT, "cache is NULL");
   if (c->format != TT_KV_E4M3 && c->format != TT_KV_INT8)
@@ -375,7 +390,7 @@ int tt_kv_attention(const tt_kv_cache *cache, int dtype, const void *q, const in
   a.c = c;
   a.q = q;
   a.qs = {q_strides[0], q_strides[1], q_strides[2]};
-  a.out = out;
+  a.out = {out, nullptr, dtype};
   a.counts = counts;
   a.ws = static_cast<float *>(workspace);
   a.dtype = dtype;

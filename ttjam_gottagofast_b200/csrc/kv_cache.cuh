@@ -124,19 +124,33 @@ __device__ __forceinline__ uint32_t kv_encode4(const float *x) {
 }
 
 // kv_cache.cu
+// The checks every entry point makes of a cache; fills *v.
+int kv_view(const tt_kv_cache *c, const char *what, KvView *v);
+// mask[b * tokens + i] = i < counts[b]
+int launch_kv_mask(const KvView &c, const int32_t *counts, int64_t tokens, uint8_t *mask,
+                   cudaStream_t stream);
 int launch_kv_write(const KvView &c, int dtype, const void *k, const void *v, KvStrides ks,
                     KvStrides vs, int64_t tokens, const int32_t *counts, cudaStream_t stream);
 int launch_kv_read(const KvView &c, int dtype, void *k, void *v, int64_t max_tokens,
                    cudaStream_t stream);
 
+// Where attention writes [batch, tokens, heads, head_dim], contiguous: elements
+// of a TT_DTYPE_*, or (kKvSplit) their fp16 split, the high pieces at p and the
+// low ones at lo, which the split-precision out_proj reads.
+constexpr int kKvSplit = -1;
+struct KvOut {
+  void *p, *lo;
+  int dtype;
+};
+
 struct KvAttentionArgs {
   KvView c;
   const void *q;
   KvStrides qs;
-  void *out;  // [batch, tokens, heads, head_dim], contiguous
+  KvOut out;
   const int32_t *counts;
   float *ws;  // partial results
-  int dtype, tokens, heads, group;
+  int dtype, tokens, heads, group;  // dtype: of q
   float scale;
   bool q_vec;  // q's rows are 16-byte aligned
 };

@@ -63,10 +63,11 @@ __device__ __forceinline__ float kv_load_in(int dtype, const void *p, int64_t i)
   if (dtype == TT_DTYPE_F16) return __half2float(static_cast<const __half *>(p)[i]);
   return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
 }
-__device__ __forceinline__ void kv_store_out(int dtype, void *p, int64_t i, float x) {
-  if (dtype == TT_DTYPE_F32) static_cast<float *>(p)[i] = x;
-  else if (dtype == TT_DTYPE_F16) static_cast<__half *>(p)[i] = __float2half_rn(x);
-  else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(x);
+__device__ __forceinline__ void kv_store_out(const KvOut &o, int64_t i, float x) {
+  if (o.dtype == TT_DTYPE_F32) static_cast<float *>(o.p)[i] = x;
+  else if (o.dtype == TT_DTYPE_F16) static_cast<__half *>(o.p)[i] = __float2half_rn(x);
+  else if (o.dtype == TT_DTYPE_BF16) static_cast<__nv_bfloat16 *>(o.p)[i] = __float2bfloat16_rn(x);
+  else f16_split(x, static_cast<uint16_t *>(o.p)[i], static_cast<uint16_t *>(o.lo)[i]);
 }
 
 // 16 consecutive elements from element i on; `vec`: the address is a multiple of 16 bytes.
@@ -104,10 +105,22 @@ __device__ __forceinline__ void store_row16(T *p, const float *x) {
     reinterpret_cast<uint4 *>(p)[n] = raw;
   }
 }
-__device__ __forceinline__ void kv_store_row16(int dtype, void *p, int64_t i, const float *x) {
-  if (dtype == TT_DTYPE_F32) store_row16(static_cast<float *>(p) + i, x);
-  else if (dtype == TT_DTYPE_F16) store_row16(static_cast<__half *>(p) + i, x);
-  else store_row16(static_cast<__nv_bfloat16 *>(p) + i, x);
+__device__ __forceinline__ void kv_store_row16(const KvOut &o, int64_t i, const float *x) {
+  if (o.dtype == TT_DTYPE_F32) {
+    store_row16(static_cast<float *>(o.p) + i, x);
+  } else if (o.dtype == TT_DTYPE_F16) {
+    store_row16(static_cast<__half *>(o.p) + i, x);
+  } else if (o.dtype == TT_DTYPE_BF16) {
+    store_row16(static_cast<__nv_bfloat16 *>(o.p) + i, x);
+  } else {
+    uint32_t hi[8], lo[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f16_split2(x[2 * k], x[2 * k + 1], hi[k], lo[k]);
+    uint4 *h = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(o.p) + i);
+    uint4 *l = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(o.lo) + i);
+    h[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]), h[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+    l[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]), l[1] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+  }
 }
 
 }  // namespace tt

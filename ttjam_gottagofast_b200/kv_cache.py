@@ -121,9 +121,9 @@ class KVCache:
         self._status = torch.zeros(2, dtype=torch.int32, device=k.device)
         self._lib = _lib.load()
         self._ws_bytes = {}
-        self._structs = []
-        for i in range(layers):
-            c = _lib.TTKVCache()
+        self._array = (_lib.TTKVCache * layers)()  # one entry a layer
+        self._structs = [ctypes.pointer(c) for c in self._array]
+        for i, c in enumerate(self._array):
             c.k_codes, c.v_codes = k[i].data_ptr(), v[i].data_ptr()
             c.k_scale, c.v_scale = k_scale[i].data_ptr(), v_scale[i].data_ptr()
             c.block_table, c.lengths = block_table.data_ptr(), lengths.data_ptr()
@@ -133,7 +133,6 @@ class KVCache:
             # an empty write makes every check of the shape and touches nothing
             _lib.check(self._lib.tt_kv_write(ctypes.byref(c), 0, None, None, None, None, 0, None,
                                              None), "KVCache", self._lib)
-            self._structs.append(ctypes.pointer(c))
 
     # ---- lengths ------------------------------------------------------------
     def advance(self, tokens: int, new_tokens: Optional[torch.Tensor] = None) -> None:

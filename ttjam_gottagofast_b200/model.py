@@ -31,6 +31,9 @@ Parameters and inputs may be float32, float16 or bfloat16 (the reference's
 share one dtype; the input's may differ; the output has the input's dtype.
 16-bit values widen exactly to fp32 and every schedule computes in fp32
 accuracy; a 16-bit output is that result rounded once to nearest even.
+
+`forward_cached(x, cache)` runs a causal model on new tokens alone, over an
+8-bit key/value cache (`make_cache`, kv_cache.py) of the earlier ones.
 """
 from __future__ import annotations
 
@@ -41,6 +44,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
+from .kv_cache import KVCache
 
 
 class SelfAttention(nn.Module):
@@ -366,6 +370,73 @@ class TTForward:
         inner = b - 2 * edge
         mids = [edge + inner * i // (slices - 2) for i in range(slices - 1)]
         return [0] + mids + [b]
+
+    # ---- token by token ---------------------------------------------------
+    def make_cache(self, batch: int, max_tokens: int, *, fmt: str = "e4m3",
+                   page_size: int = 64, device=None) -> KVCache:
+        """An empty 8-bit key/value cache for this model's layers, on the
+        parameters' device unless told otherwise."""
+        cfg = self.config
+        if device is None:
+            device = next(self.parameters()).device
+        return KVCache(batch, max_tokens, cfg.num_heads, cfg.d_model // cfg.num_heads,
+                       num_layers=cfg.num_layers, page_size=page_size, fmt=fmt, device=device)
+
+    def forward_cached(self, x: torch.Tensor, cache: KVCache,
+                       new_tokens: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The causal forward of new tokens alone: x [B, n, d_model] (float32,
+        float16 or bfloat16) are the next n tokens of every sequence of
+        `cache`, or the next new_tokens[b] <= n ([B] int32 on the device) of
+        sequence b with padding behind them. Adds them to the cache (its
+        lengths, and each layer's keys and values, rounded to 8 bits) and
+        returns y [B, n, d_model] of x's type, zero at the padding. A prompt
+        is one call, or several with pieces of it; a next token a call with
+        n = 1. A call that raises once the arguments were accepted leaves the
+        tokens counted in the cache."""
+        if not x.is_cuda:
+            raise RuntimeError("UserOptimizedTransformer runs on CUDA only (no CPU path)")
+        dname = str(x.dtype).split(".")[-1]
+        if dname not in _lib.DTYPE_CODES:
+            raise ValueError(f"expected a float32, float16 or bfloat16 input, got {x.dtype}")
+        dcode = _lib.DTYPE_CODES[dname]
+        cfg = self.config
+        if x.dim() != 3 or x.shape[0] != cache.batch or x.shape[-1] != cfg.d_model:
+            raise ValueError(f"expected x of shape [{cache.batch}, n, {cfg.d_model}], "
+                             f"got {tuple(x.shape)}")
+        if x.device != cache.device:
+            raise ValueError(f"cache must be on the same device as x, got {cache.device}")
+        if not cfg.causal:
+            raise ValueError("only a causal model runs token by token")
+        if (cache.num_layers != cfg.num_layers or cache.kv_heads != cfg.num_heads
+                or cache.head_dim * cfg.num_heads != cfg.d_model):
+            raise ValueError("cache has other layers, heads or head_dim than the model")
+        if x.device.index != torch.cuda.current_device():
+            with torch.cuda.device(x.device):
+                return self.forward_cached(x, cache, new_tokens)
+        if not x.is_contiguous() or x.data_ptr() % 16:
+            x = x.contiguous().clone() if x.data_ptr() % 16 else x.contiguous()
+        b, n, _ = x.shape
+        counts = cache._counts(new_tokens)
+        image = self._ensure_image(x.device)
+        # a context averages values rounded to codes, which can exceed the
+        # operand bound by 2^-4
+        tight = self.fp16_operand_bound * 1.0625 >= _lib.TT_FP16_MAX
+        ccfg = _lib.make_config(cfg, self._plan if self._plan.startswith("ops") else "auto",
+                                _lib.TT_FLAG_FP32_ONLY if tight else self._flags)
+        lib = self._lib
+        y = torch.empty_like(x)
+        nbytes = lib.tt_cached_workspace_bytes(ctypes.byref(ccfg), dcode, cache._array, b, n)
+        if nbytes == 0 and x.numel():
+            raise ValueError(f"tt_forward_cached: {_lib.last_error(lib)}")
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        cache.advance(n, new_tokens=counts)
+        stream = torch.cuda.current_stream(x.device).cuda_stream
+        rc = lib.tt_forward_cached(ctypes.byref(ccfg), image.data_ptr(), dcode, x.data_ptr(),
+                                   cache._array, None if counts is None else counts.data_ptr(), b, n,
+                                   y.data_ptr(), ws.data_ptr(), nbytes, stream)
+        if rc != 0:
+            _lib.check(rc, "tt_forward_cached", lib)
+        return y
 
     # ---- diagnostics ------------------------------------------------------
     def forward_plan(self, batch: int, seq: int) -> str:
