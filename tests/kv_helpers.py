@@ -61,8 +61,9 @@ def attention_bound(size, total, reach, hd, tokens, dtype):
     at most 2^-22 of the sum of magnitudes: (hd / 16 + 2) 2^-22 reach. The
     exponent's fused multiply-add rounds a number of up to 2^5 where p matters
     (2^-19 of p after ln 2), exp2 and p's split add less than 2^-21 together.
-    Sums of up to `tokens` terms lose at most tokens * 2^-24 in all, /4 because
-    four warps share them. Each relative error of p_j counts once in the sum of
+    The sum of p v takes two additions for 16 tokens, each losing up to 2^-23 of the
+    sum, in runs of at most 1024 tokens, and one of 2^-24 for each run; the sum of p
+    one of 2^-24 for 16 tokens. Each relative error of p_j counts once in the sum of
     p v and once in the sum of p. 16-bit rows may round p to fp16 for its product
     with v (not in the sum): float16's steps are 2^-10 of a power of two, so half
     a step is at most eps / 2 = 2^-11 of p, once.
@@ -74,7 +75,8 @@ def attention_bound(size, total, reach, hd, tokens, dtype):
     The output's own rounding adds half a step of its type: eps / 2 of the value,
     and below the type's smallest normal number, where the steps stay as they are
     there, half of smallest_normal * eps (float16: 2^-14 2^-10 / 2 = 2^-25)."""
-    eps = (hd / 16 + 2) * 2.0 ** -22 * reach + 2.0 ** -18 + tokens * 2.0 ** -26
+    sums = min(tokens, 1024) / 8 * 2.0 ** -23 + (tokens / 1024 + tokens / 16 + 8) * 2.0 ** -24
+    eps = (hd / 16 + 2) * 2.0 ** -22 * reach + 2.0 ** -18 + sums / 2
     info = torch.finfo(dtype)
     once = 2.0 ** -11 if info.bits == 16 else 0.0
     return (2 * eps[..., None] + once) * size + 2.0 ** -31 * total + info.smallest_normal * info.eps / 2, info.eps / 2

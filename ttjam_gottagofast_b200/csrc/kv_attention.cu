@@ -45,6 +45,9 @@ struct RowShape {
   static constexpr int GR = HD <= 64 ? 2 : 1;        // 16-token groups per warp step
   static constexpr int kStep = 16 * GR;              // tokens per warp step
   static constexpr int kUnit = kStep * kWarps;       // tokens per unit
+  // tensor cores add by rounding toward zero: after 1024 tokens the sum moves to
+  // shared memory, so that it does not drift
+  static constexpr int kFlush = 1024 / kStep;
   static constexpr int KW = HD / 16;                 // words of a token's keys per thread
   static constexpr int VW = HD / 32;                 // words of a token's values per thread
   static constexpr int kSlot = kRows * HD + 2 * kRows;  // floats of a partial result
@@ -252,6 +255,22 @@ __global__ void __launch_bounds__(kThreads) kv_attention_rows_kernel(KvAttention
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
 
+    bool flushed = false;
+    float beta = 1.f;  // what the flushed sum is scaled by when read next
+    auto flush = [&] {
+#pragma unroll
+      for (int w = 0; w < VW; ++w)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            float &sum = s_o[warp][gid][out_dim<HD>(w, i, 2 * tig + n)];
+            const float v = o[4 * w + i][n] + o[4 * w + i][2 + n];
+            sum = flushed ? fmaf(sum, beta, v) : v;
+          }
+      flushed = true;
+      beta = 1.f;
+    };
     auto t0_of = [&](int t) { return t * Sh::kUnit + warp * Sh::kStep; };
     auto page_at = [&](int t0) {
       return t0 < any_end ? c.page_of(b, t0 >> c.page_log2) : -1;
@@ -265,6 +284,13 @@ __global__ void __launch_bounds__(kThreads) kv_attention_rows_kernel(KvAttention
     }
     for (int t = t_lo; t < t_hi; ++t) {
       const int t0 = t0_of(t);
+      if (t > t_lo && (t - t_lo) % Sh::kFlush == 0) {
+        flush();
+#pragma unroll
+        for (int i = 0; i < 4 * VW; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+      }
       if (t + 1 < t_hi) {
 #pragma unroll
         for (int g = 0; g < GR; ++g) {
@@ -320,6 +346,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_rows_kernel(KvAttention
           const float alpha = mn == m ? 1.f : exp2_approx(m - mn);  // 0 from -inf
           m = mn;
           l *= alpha;
+          beta *= alpha;
 #pragma unroll
           for (int i = 0; i < 4 * VW; ++i)
 #pragma unroll
@@ -364,13 +391,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_rows_kernel(KvAttention
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     if (tig == 0) s_m[warp][gid] = m, s_l[warp][gid] = l;
-#pragma unroll
-    for (int w = 0; w < VW; ++w)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-          s_o[warp][gid][out_dim<HD>(w, i, 2 * tig + n)] = o[4 * w + i][n] + o[4 * w + i][2 + n];
+    flush();
     __syncthreads();
     const bool whole = t_lo == 0 && t_hi == units;
     const int rows = min(kRows, rows_all - rb * kRows);

@@ -59,6 +59,11 @@ struct TcShape {
   static constexpr uint32_t T_O = 0, T_S = MT * HD, T_Q = MT * (HD + TOK);
   static_assert(T_Q + (QT ? MT * PIECES * HD / 2 : 0) <= 512, "tensor memory");
   static_assert(NS >= 3 && SMEM <= 227 * 1024, "shared memory");
+  // Tensor memory adds a product to O by rounding toward zero, so a long sum drifts
+  // (measured: 7e-6 of the output after 4096 tokens, in proportion to them).
+  // fp32 rows therefore take O out every FLUSH tiles (1024 tokens), into a sum
+  // kept in the row's own place of the output, and start it anew.
+  static constexpr int FLUSH = PIECES == 2 ? 1024 / TOK : INT32_MAX;
   static constexpr int GROUPS = TOK / 16;  // of 16 tokens, each in one page
   static constexpr int NCH = TOK * HD / 16 / kConvThreads;  // 16-code chunks a converter thread
   static constexpr uint32_t IDESC_S =
@@ -333,7 +338,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
             for (int w = 0; w < PIECES; ++w)
               mma_ts(tm + Sh::T_O + (uint32_t)(HD * x),
                      p + 32u * (kk >> 1) + 8u * (kk & 1) + 16u * w, vd, Sh::IDESC_PV,
-                     (j | kk | w) != 0);
+                     ((j % Sh::FLUSH) | kk | w) != 0);
           }
           mma_commit(o_done(x));
           if (j + 1 < nj) {
@@ -492,7 +497,12 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(q_ready);
     }
-    float m = -CUDART_INF_F, l = 0.f;
+    // where this row's sum of flushed O stands: its partial result, or its output
+    const int64_t at = out_row(r < rows_all ? r : 0);
+    const KvOut sum_out = splits > 1 ? KvOut{a.ws, nullptr, TT_DTYPE_F32} : a.out;
+    const int64_t sum_at = splits > 1 ? part(r) * HD : at;
+    const int sum_dims = alive ? (splits > 1 ? HD : c.hd) : 0;
+    float m = -CUDART_INF_F, l = 0.f, beta = 0.f;  // beta: what the sum is scaled by when read next
     for (int j = 0; j < nj; ++j) {
       const int t0 = (j0 + j) * TOK;
       mbar_wait(sc_full(j & 3), (j >> 2) & 1, abort_w, c.status, 0x6500);
@@ -532,7 +542,34 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       const bool raise = top > m + kLazy || (m == -CUDART_INF_F && top > m);
       const float mn = raise ? ceilf(top) : m;
       const float alpha = raise ? exp2_approx(m - mn) : 1.f;  // 0 from -inf
-      if (j > 0 && __any_sync(0xffffffffu, raise && m != -CUDART_INF_F)) {
+      const bool flush = PIECES == 2 && j > 0 && j % Sh::FLUSH == 0;
+      if (flush) {
+        mbar_wait(o_done(x), (j - 1) & 1, abort_w, c.status, 0x6700);
+        fence_after();
+#pragma unroll 1
+        for (int d = 0; d < HD; d += 16) {
+          uint32_t o[16];
+          float v[16];
+          tmem_ld16(t_o + d, o);
+          tmem_wait_ld();
+          if (d < sum_dims) {
+            if (j > Sh::FLUSH) {
+              kv_load_sum16(sum_out, sum_at + d, v);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i] = fmaf(v[i], beta, __uint_as_float(o[i]));
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(o[i]);
+            }
+            kv_store_sum16(sum_out, sum_at + d, v);
+          }
+          __syncwarp();
+        }
+        beta = alpha;
+      } else {
+        beta *= alpha;
+      }
+      if (!flush && j > 0 && __any_sync(0xffffffffu, raise && m != -CUDART_INF_F)) {
         mbar_wait(o_done(x), (j - 1) & 1, abort_w, c.status, 0x6700);
         fence_after();
 #pragma unroll 1
@@ -591,13 +628,17 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
     mbar_wait(o_done(x), (nj - 1) & 1, abort_w, c.status, 0x6800);
     fence_after();
     const float inv = l == 0.f ? 0.f : kCodeUnit<FMT> / l;
-    const int64_t at = out_row(r < rows_all ? r : 0);
 #pragma unroll
     for (int d = 0; d < HD; d += 16) {
       uint32_t o[16];
       tmem_ld16(t_o + d, o);
       tmem_wait_ld();
       float v[16];
+      if (PIECES == 2 && nj > Sh::FLUSH && d < sum_dims) {
+        kv_load_sum16(sum_out, sum_at + d, v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(fmaf(v[i], beta, __uint_as_float(o[i])));
+      }
       if (splits > 1) {
 #pragma unroll
         for (int i = 0; i < 16; i += 4)

@@ -123,4 +123,41 @@ __device__ __forceinline__ void kv_store_row16(const KvOut &o, int64_t i, const 
   }
 }
 
+// 16 fp32 sums kept in an fp32 or split output row until its values are written
+// there: their bits, in the split form as upper and lower halves.
+__device__ __forceinline__ void kv_store_sum16(const KvOut &o, int64_t i, const float *x) {
+  if (o.dtype == TT_DTYPE_F32) {
+    store_row16(static_cast<float *>(o.p) + i, x);
+    return;
+  }
+  uint32_t hi[8], lo[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    hi[k] = __byte_perm(__float_as_uint(x[2 * k]), __float_as_uint(x[2 * k + 1]), 0x7632);
+    lo[k] = __byte_perm(__float_as_uint(x[2 * k]), __float_as_uint(x[2 * k + 1]), 0x5410);
+  }
+  uint4 *h = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(o.p) + i);
+  uint4 *l = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(o.lo) + i);
+  h[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]), h[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+  l[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]), l[1] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+}
+__device__ __forceinline__ void kv_load_sum16(const KvOut &o, int64_t i, float *x) {
+  if (o.dtype == TT_DTYPE_F32) {
+    load_row16(static_cast<const float *>(o.p) + i, true, x);
+    return;
+  }
+  uint4 h[2], l[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    h[k] = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(o.p) + i)[k];
+    l[k] = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(o.lo) + i)[k];
+  }
+  const uint32_t *hw = &h[0].x, *lw = &l[0].x;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    x[2 * k] = __uint_as_float(__byte_perm(lw[k], hw[k], 0x5410));
+    x[2 * k + 1] = __uint_as_float(__byte_perm(lw[k], hw[k], 0x7632));
+  }
+}
+
 }  // namespace tt
