@@ -18,10 +18,14 @@
 // in fp16, are the other operand. Row q is scaled by a power of two to have its
 // largest element in [1, 2), p by 2^14 to stay clear of the fp16 subnormals.
 //
-// A warp takes 16 tokens at a time, straight from global memory into operand
-// registers: the tokens and head dims are numbered within a step so that a
-// thread's operand elements are consecutive bytes (which token or dim stands at
-// which operand index is free as long as both operands agree).
+// A warp takes kStep tokens at a time from a ring of its own in shared memory,
+// which its lanes fill with bulk copies (16 tokens of a page and head are
+// consecutive bytes) up to kStages steps ahead, over the borders of heads and
+// sequences, so that a warp always has its next copies in flight. Bytes go from
+// there straight into operand registers: the tokens and head dims are numbered
+// within a step so that a thread's operand elements are consecutive bytes (which
+// token or dim stands at which operand index is free as long as both operands
+// agree) and so that few of a warp's loads share banks.
 //
 // Work is split into units of kUnit tokens of one (sequence, key head, row block);
 // every CTA takes an equal run of consecutive units, whatever the lengths, and a
@@ -42,9 +46,16 @@ constexpr int kThreads = 32 * kWarps;
 
 template <int HD>
 struct RowShape {
-  static constexpr int GR = HD <= 64 ? 2 : 1;        // 16-token groups per warp step
-  static constexpr int kStep = 16 * GR;              // tokens per warp step
+  static constexpr int kStep = HD == 32 ? 64 : HD == 64 ? 32 : 16;  // tokens per warp step
+  static constexpr int GR = kStep / 16;              // groups of 16 tokens, each in one page
   static constexpr int kUnit = kStep * kWarps;       // tokens per unit
+  static constexpr int kStages = HD == 256 ? 2 : 3;  // steps in a warp's ring
+  static constexpr uint32_t kStage = 2 * kStep * HD;  // bytes: keys, then values
+  // shared memory: the rings, the warps' results, barriers
+  static constexpr uint32_t kO = kWarps * kStages * kStage;
+  static constexpr uint32_t kBars = kO + kWarps * kRows * HD * 4;
+  static constexpr uint32_t kSmem = kBars + 8 * kWarps * kStages;
+  static constexpr int kCtas = HD == 256 ? 2 : 3;    // per SM, as registers and shared memory allow
   // tensor cores add by rounding toward zero: after 1024 tokens the sum moves to
   // shared memory, so that it does not drift
   static constexpr int kFlush = 1024 / kStep;
@@ -53,6 +64,52 @@ struct RowShape {
   static constexpr int kSlot = kRows * HD + 2 * kRows;  // floats of a partial result
 };
 
+__device__ __forceinline__ uint32_t smem_u32(const void *p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// Bounded wait: false after about 2^28 cycles, latching TT_ERR_DEVICE_TIMEOUT.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, DeviceStatus *st) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 31) == 0 && clock64() - t0 > (1LL << 28)) {
+      raise_status(st, TT_ERR_DEVICE_TIMEOUT, 0x6900);
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+template <int BYTES>
+__device__ __forceinline__ void lds(uint32_t addr, uint32_t *r) {
+  if constexpr (BYTES == 16)
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+  else if constexpr (BYTES == 8)
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr));
+  else
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r[0]) : "r"(addr));
+}
 __device__ __forceinline__ void mma16816(float *c, uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -71,75 +128,39 @@ __device__ __forceinline__ int units_of(const KvAttentionArgs &a, int b, int uni
   return count > 0 ? (len + unit - 1) / unit : 1;
 }
 
-// What one warp knows of 16 tokens of its step, loaded ahead.
-template <int HD>
-struct Group {
-  uint32_t k[2][RowShape<HD>::KW];
-  uint32_t v[2][2][RowShape<HD>::VW];  // [operand half][token parity]
-  float ks, vs;
-};
-
-template <int HD>
-__device__ __forceinline__ void load_group(Group<HD> &g, const KvView &c, int pg, int h, int t0,
-                                           int lane) {
-  constexpr int KW = RowShape<HD>::KW, VW = RowShape<HD>::VW;
-  const int gid = lane >> 2, tig = lane & 3;
-  if (pg < 0) {
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-#pragma unroll
-      for (int i = 0; i < KW; ++i) g.k[x][i] = 0;
-#pragma unroll
-      for (int p = 0; p < 2; ++p)
-#pragma unroll
-        for (int i = 0; i < VW; ++i) g.v[x][p][i] = 0;
-    }
-    g.ks = g.vs = 1.f;
-    return;
-  }
-  const int64_t tile = c.tile(pg, h) + (int64_t)(t0 & ((1 << c.page_log2) - 1)) * c.hd;
-  g.ks = c.ks[(int64_t)pg * c.heads + h];
-  g.vs = c.vs[(int64_t)pg * c.heads + h];
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    // operand column n of half x is token 8 x + 4 (n & 1) + (n >> 1) of the group
-    const uint8_t *row = c.k + tile + (8 * x + 4 * (gid & 1) + (gid >> 1)) * c.hd;
-    if constexpr (HD == 32) {
-      uint2 w = make_uint2(0, 0);
-      if (8 * tig < c.hd) w = __ldcs(reinterpret_cast<const uint2 *>(row + 8 * tig));
-      g.k[x][0] = w.x, g.k[x][1] = w.y;
-    } else {
-#pragma unroll
-      for (int j = 0; j < HD / 64; ++j) {
-        const int d = 64 * j + 16 * tig;
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (d < c.hd) w = __ldcs(reinterpret_cast<const uint4 *>(row + d));
-        g.k[x][4 * j] = w.x, g.k[x][4 * j + 1] = w.y;
-        g.k[x][4 * j + 2] = w.z, g.k[x][4 * j + 3] = w.w;
-      }
-    }
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const uint8_t *vrow = c.v + tile + (8 * x + 4 * p + tig) * c.hd;
-      if constexpr (HD == 32) {
-        g.v[x][p][0] = 4 * gid < c.hd ? __ldcs(reinterpret_cast<const uint32_t *>(vrow + 4 * gid)) : 0;
-      } else if constexpr (HD == 64) {
-        uint2 w = make_uint2(0, 0);
-        if (8 * gid < c.hd) w = __ldcs(reinterpret_cast<const uint2 *>(vrow + 8 * gid));
-        g.v[x][p][0] = w.x, g.v[x][p][1] = w.y;
-      } else {
-#pragma unroll
-        for (int j = 0; j < HD / 128; ++j) {
-          const int d = 128 * j + 16 * gid;
-          uint4 w = make_uint4(0, 0, 0, 0);
-          if (d < c.hd) w = __ldcs(reinterpret_cast<const uint4 *>(vrow + d));
-          g.v[x][p][4 * j] = w.x, g.v[x][p][4 * j + 1] = w.y;
-          g.v[x][p][4 * j + 2] = w.z, g.v[x][p][4 * j + 3] = w.w;
-        }
-      }
-    }
-  }
+// Token (0-7) of operand column n of an 8-token half: such that two neighbouring
+// columns are an odd number of rows apart, and four alternate ones two and two.
+__device__ __forceinline__ int half_token(int n) {
+  const int r = ((n >> 1) & 1) + 4 * (n >> 2);
+  return n & 1 ? r ^ 3 : r;
 }
+
+// Where a CTA's run of units stands: unit t of the (sequence, key head, row
+// block) segment [seg_lo, seg_hi) that the run holds of it.
+struct Cursor {
+  int64_t left;   // units of the run from this one on
+  int64_t first;  // units of the sequence before this segment's first
+  int b, len, count, units, pair, t, t_hi;
+
+  __device__ __forceinline__ void segment(int64_t skip) {  // `skip` units of the sequence are behind
+    pair = (int)(skip / units);
+    t = (int)(skip - (int64_t)pair * units);
+    t_hi = (int)min((int64_t)units, t + left);
+  }
+  // to the next segment; false at the end of the run
+  __device__ __forceinline__ bool next_segment(const KvAttentionArgs &a, int unit, int64_t hr) {
+    left -= t_hi - seg_lo;
+    if (left <= 0) return false;
+    if (++pair >= hr) {
+      pair = 0;
+      units = units_of(a, ++b, unit, len, count);
+    }
+    t = seg_lo = 0;
+    t_hi = (int)min((int64_t)units, left);
+    return true;
+  }
+  int seg_lo;
+};
 
 // The head dim of output tile 4 w + i (8 columns), column n.
 template <int HD>
@@ -148,23 +169,30 @@ __device__ __forceinline__ int out_dim(int w, int i, int n) {
   else return 128 * (w / 4) + 16 * n + 4 * (w % 4) + i;
 }
 
-template <int HD, int FMT>
-__global__ void __launch_bounds__(kThreads) kv_attention_rows_kernel(KvAttentionArgs a,
-                                                                     int row_blocks, bool join) {
+template <int HD, int FMT, bool EXACT>
+__global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
+    kv_attention_rows_kernel(KvAttentionArgs a, int row_blocks) {
   using Sh = RowShape<HD>;
-  constexpr int KW = Sh::KW, VW = Sh::VW, GR = Sh::GR;
-  __shared__ float s_o[kWarps][kRows][HD];
+  constexpr int KW = Sh::KW, VW = Sh::VW, GR = Sh::GR, S = Sh::kStages;
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
   __shared__ int64_t s_scan[kThreads];
   pdl_trigger();
-  pdl_wait();
   const KvView &c = a.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int gid = lane >> 2, tig = lane & 3;
+  const int hd = EXACT ? HD : c.hd;
   const int64_t hr = (int64_t)c.heads * row_blocks;  // (key head, row block) pairs
   const int rows_all = a.tokens * a.group;           // query rows of a key head
+  const uint32_t ring = smem_u32(smem) + warp * S * Sh::kStage;
+  const uint32_t bars = smem_u32(smem) + Sh::kBars + 8 * warp * S;
+  float *const s_o = reinterpret_cast<float *>(smem + Sh::kO);  // [kWarps][kRows][HD]
+  if (lane < S)
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bars + 8 * lane), "r"(GR) : "memory");
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  pdl_wait();
 
-  // the CTA's run of units [lo, hi), and the sequence that holds unit lo
+  // the CTA's run of units, and the sequence that holds its first
   const int per_thread = (c.batch + kThreads - 1) / kThreads;
   const int b0 = min(c.batch, tid * per_thread), b1 = min(c.batch, b0 + per_thread);
   int64_t mine = 0;
@@ -172,52 +200,107 @@ __global__ void __launch_bounds__(kThreads) kv_attention_rows_kernel(KvAttention
     int len, count;
     mine += units_of(a, b, Sh::kUnit, len, count);
   }
+  // inclusive sums over the threads
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, mine, o);
+    if (lane >= o) mine += v;
+  }
   s_scan[tid] = mine;
   __syncthreads();
-  for (int o = 1; o < kThreads; o <<= 1) {
-    const int64_t x = tid >= o ? s_scan[tid - o] : 0;
-    __syncthreads();
-    s_scan[tid] += x;
-    __syncthreads();
-  }
+  for (int w = 0; w < warp; ++w) mine += s_scan[32 * w + 31];
+  __syncthreads();
+  s_scan[tid] = mine;
+  __syncthreads();
   const int64_t total = s_scan[kThreads - 1] * hr;
   const int64_t run = (total + gridDim.x - 1) / gridDim.x;
-  const int64_t lo = blockIdx.x * run, hi = min(total, lo + run);
-  if (lo >= hi) return;
-  int b = 0;
-  int64_t first = 0;  // first unit of sequence b
+  const int64_t lo = blockIdx.x * run;
+  if (lo >= total) return;
+  Cursor use;  // what is computed; `fill` below is what is copied, ahead of it
+  use.left = min(run, total - lo);
   {
     int t = 0;
     while (s_scan[t] * hr <= lo) ++t;
-    b = t * per_thread;
-    first = t > 0 ? s_scan[t - 1] * hr : 0;
-  }
-  int len, count;
-  int units = units_of(a, b, Sh::kUnit, len, count);
-  while (first + units * hr <= lo) {
-    first += units * hr;
-    units = units_of(a, ++b, Sh::kUnit, len, count);
-  }
-
-  for (int64_t u = lo; u < hi;) {
-    if (u >= first + units * hr) {
-      first += units * hr;
-      units = units_of(a, ++b, Sh::kUnit, len, count);
+    use.b = t * per_thread;
+    int64_t first = t > 0 ? s_scan[t - 1] * hr : 0;
+    use.units = units_of(a, use.b, Sh::kUnit, use.len, use.count);
+    while (first + use.units * hr <= lo) {
+      first += use.units * hr;
+      use.units = units_of(a, ++use.b, Sh::kUnit, use.len, use.count);
     }
-    const int64_t pair = (u - first) / units;
-    const int h = (int)(pair / row_blocks), rb = (int)(pair % row_blocks);
-    const int64_t seg0 = first + pair * units, seg1 = seg0 + units;
-    const int t_lo = (int)(u - seg0), t_hi = (int)(min(hi, seg1) - seg0);
+    use.segment(lo - first);
+    use.seg_lo = use.t;
+  }
 
+  // tokens that the last live row of the cursor's row block sees
+  auto seen_by_block = [&](const Cursor &u) {
+    const int rb = u.pair % row_blocks;
+    const int r_first = rb * kRows / a.group;
+    const int r_last = min(rb * kRows + kRows - 1, rows_all - 1) / a.group;
+    return r_first < u.count ? u.len - u.count + min(r_last, u.count - 1) + 1 : 0;
+  };
+  auto t0_of = [&](int t) { return t * Sh::kUnit + warp * Sh::kStep; };
+
+  // ---- the copies -----------------------------------------------------------
+  // Lane g < GR copies group g's keys and values; its page is looked up one step
+  // before, its scales wait in the lane's queue for as long as the bytes do in the
+  // ring. A group without a page, or past the last seen token, copies nothing and
+  // has the key scale -1.
+  Cursor fill = use;
+  bool more = true;
+  int fill_end = seen_by_block(fill), fill_stage = 0, pg_next;
+  float q_ks[S], q_vs[S];
+  auto look_up = [&] {
+    const int t0 = t0_of(fill.t) + 16 * lane;
+    pg_next = lane < GR && t0 < fill_end ? c.page_of(fill.b, t0 >> c.page_log2) : -1;
+  };
+  auto issue = [&](float &ks, float &vs) {
+    const uint32_t bar = bars + 8 * fill_stage;
+    ks = -1.f;
+    vs = 1.f;
+    if (lane < GR) {
+      const uint32_t bytes = 16 * hd;
+      mbar_expect(bar, pg_next >= 0 ? 2 * bytes : 0);
+      if (pg_next >= 0) {
+        const int h = fill.pair / row_blocks;
+        const int t0 = t0_of(fill.t) + 16 * lane;
+        const int64_t at = c.tile(pg_next, h) + (int64_t)(t0 & ((1 << c.page_log2) - 1)) * hd;
+        const uint32_t dst = ring + fill_stage * Sh::kStage + lane * bytes;
+        bulk_copy(dst, c.k + at, bytes, bar);
+        bulk_copy(dst + Sh::kStep * hd, c.v + at, bytes, bar);
+        ks = c.ks[(int64_t)pg_next * c.heads + h];
+        vs = c.vs[(int64_t)pg_next * c.heads + h];
+      }
+    }
+    fill_stage = fill_stage + 1 == S ? 0 : fill_stage + 1;
+    if (++fill.t == fill.t_hi) {
+      more = fill.next_segment(a, Sh::kUnit, hr);
+      if (more) fill_end = seen_by_block(fill);
+    }
+    if (more) look_up();
+  };
+  look_up();
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    q_ks[s] = -1.f, q_vs[s] = 1.f;
+    if (more) issue(q_ks[s], q_vs[s]);
+  }
+  int stage = 0;
+  uint32_t phase = 0;
+  bool alive = true;  // false once a wait gave up: the rest of the run computes nothing
+
+  bool going = true;
+  while (going) {
+    const int h = use.pair / row_blocks, rb = use.pair % row_blocks;
+    const int b = use.b, len = use.len, count = use.count;
     // the row of this thread's accumulators, and the tokens it sees
     const int r = rb * kRows + gid;
     const int tok = r / a.group;
     const bool live = r < rows_all && tok < count;
     const int end = live ? len - count + tok + 1 : 0;
     const int r_first = rb * kRows / a.group;
-    const int r_last = min(rb * kRows + kRows - 1, rows_all - 1) / a.group;
-    const int all_end = len - count + min(r_first, count) + 1;      // tokens that every live row sees
-    const int any_end = r_first < count ? len - count + min(r_last, count - 1) + 1 : 0;
+    const int all_end = len - count + min(r_first, count) + 1;  // tokens that every live row sees
+    const int any_end = seen_by_block(use);
 
     // q, scaled to [1, 2) and split
     uint32_t qa[KW][4];
@@ -231,7 +314,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_rows_kernel(KvAttention
         const int d = HD == 32 ? 8 * tig + 4 * w : 64 * (w / 4) + 16 * tig + 4 * (w % 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x[w][i] = live && d < c.hd ? kv_load_in(a.dtype, a.q, off + d + i) : 0.f;
+          x[w][i] = live && d < hd ? kv_load_in(a.dtype, a.q, off + d + i) : 0.f;
           mx = fmaxf(mx, fabsf(x[w][i]));
         }
       }
@@ -245,7 +328,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_rows_kernel(KvAttention
         f16_split2(x[w][0] * f, x[w][1] * f, qa[w][0], qa[w][1]);
         f16_split2(x[w][2] * f, x[w][3] * f, qa[w][2], qa[w][3]);
       }
-      sc = a.scale * 1.4426950408889634f * kCodeUnit<FMT> * kv_pow2(e);
+      sc = a.scale * 1.4426950408889634f * kv_pow2(e);
     }
 
     float m = -CUDART_INF_F, l = 0.f;
@@ -254,7 +337,6 @@ __global__ void __launch_bounds__(kThreads) kv_attention_rows_kernel(KvAttention
     for (int i = 0; i < 4 * VW; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
-
     bool flushed = false;
     float beta = 1.f;  // what the flushed sum is scaled by when read next
     auto flush = [&] {
@@ -264,24 +346,15 @@ __global__ void __launch_bounds__(kThreads) kv_attention_rows_kernel(KvAttention
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
-            float &sum = s_o[warp][gid][out_dim<HD>(w, i, 2 * tig + n)];
+            float &sum = s_o[(warp * kRows + gid) * HD + out_dim<HD>(w, i, 2 * tig + n)];
             const float v = o[4 * w + i][n] + o[4 * w + i][2 + n];
             sum = flushed ? fmaf(sum, beta, v) : v;
           }
       flushed = true;
       beta = 1.f;
     };
-    auto t0_of = [&](int t) { return t * Sh::kUnit + warp * Sh::kStep; };
-    auto page_at = [&](int t0) {
-      return t0 < any_end ? c.page_of(b, t0 >> c.page_log2) : -1;
-    };
-    Group<HD> cur[GR], nxt[GR];
-    int pg[GR], npg[GR];
-#pragma unroll
-    for (int g = 0; g < GR; ++g) {
-      pg[g] = page_at(t0_of(t_lo) + 16 * g);
-      load_group<HD>(cur[g], c, pg[g], h, t0_of(t_lo) + 16 * g, lane);
-    }
+
+    const int t_lo = use.seg_lo, t_hi = use.t_hi;
     for (int t = t_lo; t < t_hi; ++t) {
       const int t0 = t0_of(t);
       if (t > t_lo && (t - t_lo) % Sh::kFlush == 0) {
@@ -291,55 +364,64 @@ __global__ void __launch_bounds__(kThreads) kv_attention_rows_kernel(KvAttention
 #pragma unroll
           for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
       }
-      if (t + 1 < t_hi) {
-#pragma unroll
-        for (int g = 0; g < GR; ++g) {
-          npg[g] = page_at(t0_of(t + 1) + 16 * g);
-          load_group<HD>(nxt[g], c, npg[g], h, t0_of(t + 1) + 16 * g, lane);
-        }
-      }
-      if (t0 < any_end) {  // the same for the whole warp
+      if (alive) alive = __all_sync(0xffffffffu, mbar_wait(bars + 8 * stage, phase, c.status));
+      if (alive && t0 < any_end) {  // the same for the whole warp
+        const uint32_t kb = ring + stage * Sh::kStage, vb = kb + Sh::kStep * hd;
         float s[GR][2][4];
 #pragma unroll
         for (int g = 0; g < GR; ++g)
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
+          for (int x = 0; x < 2; ++x) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[g][x][i] = 0.f;
+            const uint32_t row = kb + (16 * g + 8 * x + half_token(gid)) * hd;
+            constexpr int LB = HD == 32 ? 8 : 16;  // bytes a load
 #pragma unroll
-        for (int w = 0; w < KW; ++w)
+            for (int j = 0; j < KW * 4 / LB; ++j) {
+              uint32_t w[LB / 4] = {};
+              const int d = 4 * LB * j + LB * tig;
+              if (EXACT || d < hd) lds<LB>(row + d, w);
 #pragma unroll
-          for (int g = 0; g < GR; ++g)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              uint32_t k0, k1;
-              codes_along<FMT>(cur[g].k[x][w], k0, k1);
-              mma16816(s[g][x], qa[w][0], qa[w][1], qa[w][2], qa[w][3], k0, k1);
+              for (int i = 0; i < LB / 4; ++i) {
+                uint32_t k0, k1;
+                codes_along<FMT>(w[i], k0, k1);
+                const uint32_t *q = qa[j * (LB / 4) + i];
+                mma16816(s[g][x], q[0], q[1], q[2], q[3], k0, k1);
+              }
             }
-        // scores of this thread: row gid, tokens 8 x + 4 p + tig of group g
+          }
+        // scores of this thread: row gid, tokens 8 x + half_token(2 tig + p) of group g
+        const float ve_lane = q_vs[0] == q_vs[0] ? (float)((__float_as_int(q_vs[0]) >> 23) - 127) : q_vs[0];
         float kc[GR], ve[GR], top = -CUDART_INF_F;
-        bool masked[GR];
+        bool none[GR], masked[GR], dirty[GR];
 #pragma unroll
         for (int g = 0; g < GR; ++g) {
           const int tg = t0 + 16 * g;
-          kc[g] = cur[g].ks * sc;
-          // vs = 2^e; a NaN scale stays NaN
-          ve[g] = cur[g].vs == cur[g].vs ? (float)((__float_as_int(cur[g].vs) >> 23) - 127) : cur[g].vs;
-          masked[g] = pg[g] < 0 || tg + 16 > all_end;
-          float mx = -CUDART_INF_F;
+          const float ks = __shfl_sync(0xffffffffu, q_ks[0], g);
+          ve[g] = __shfl_sync(0xffffffffu, ve_lane, g);
+          none[g] = ks < 0.f;
+          kc[g] = fabsf(ks) * sc;  // never negative: it meets -inf below
+          masked[g] = none[g] || tg + 16 > all_end;
+          dirty[g] = none[g] || tg + 16 > len;
+          if (masked[g]) {
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int p = 0; p < 2; ++p) {
-              float v = s[g][x][p] + s[g][x][2 + p];
-              if (masked[g] && (pg[g] < 0 || tg + 8 * x + 4 * p + tig >= end)) v = -CUDART_INF_F;
-              s[g][x][p] = v;
-              mx = fmaxf(mx, v);
-            }
+              for (int p = 0; p < 2; ++p) {
+                const bool see = !none[g] && tg + 8 * x + half_token(2 * tig + p) < end;
+                s[g][x][p] = see ? s[g][x][p] + s[g][x][2 + p] : -CUDART_INF_F;
+              }
+          } else {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+              for (int p = 0; p < 2; ++p) s[g][x][p] += s[g][x][2 + p];
+          }
+          const float mx = fmaxf(fmax3(s[g][0][0], s[g][0][1], s[g][1][0]), s[g][1][1]);
           top = fmaxf(top, fmaf(mx, kc[g], ve[g]));
         }
         // p stays below 2^15: the reference moves when a score passes it by more than 1
-        if (__any_sync(0xffffffffu, top > m + 1.f || (m == -CUDART_INF_F && top > m))) {
+        if (__any_sync(0xffffffffu, top > m + 1.f)) {
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           const float mn = fmaxf(m, ceilf(top));
@@ -357,34 +439,66 @@ __global__ void __launch_bounds__(kThreads) kv_attention_rows_kernel(KvAttention
         for (int g = 0; g < GR; ++g) {
           const int tg = t0 + 16 * g;
           const float base = ve[g] - ref + 14.f;
-          float p[2][2], sum = 0.f;
+          float p[2][2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) p[x][q] = exp2_approx(fmaf(s[g][x][q], kc[g], base));
+          if (masked[g]) {  // a NaN scale leaves NaN at the tokens behind the mask
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+              for (int q = 0; q < 2; ++q)
+                if (none[g] || tg + 8 * x + half_token(2 * tig + q) >= end) p[x][q] = 0.f;
+          }
+          const float sum = (p[0][0] + p[0][1]) + (p[1][0] + p[1][1]);
+          // 2^-e; a NaN counts only where a token of its page is seen
+          if (sum != 0.f) l = fmaf(sum, exp2_approx(-ve[g]), l);
+          uint32_t pa[4];
+          f16_split2(p[0][0], p[0][1], pa[0], pa[1]);
+          f16_split2(p[1][0], p[1][1], pa[2], pa[3]);
+          uint32_t v[2][2][VW];
 #pragma unroll
           for (int x = 0; x < 2; ++x)
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-              float v = exp2_approx(fmaf(s[g][x][q], kc[g], base));
-              if (masked[g] && (pg[g] < 0 || tg + 8 * x + 4 * q + tig >= end)) v = 0.f;
-              p[x][q] = v;
-              sum += v;
+              const int in_g = 8 * x + half_token(2 * tig + q);
+              const uint32_t row = vb + (16 * g + in_g) * hd;
+              constexpr int LB = VW >= 4 ? 16 : 4 * VW;  // bytes a load
+              const bool clean = !(FMT == TT_KV_E4M3 && dirty[g]) || (!none[g] && tg + in_g < len);
+#pragma unroll
+              for (int j = 0; j < VW * 4 / LB; ++j) {
+                const int d = 8 * LB * j + LB * gid;
+                if (EXACT || d < hd) {
+                  lds<LB>(row + d, &v[x][q][j * (LB / 4)]);
+                } else {
+#pragma unroll
+                  for (int i = 0; i < LB / 4; ++i) v[x][q][j * (LB / 4) + i] = 0;
+                }
+              }
+              if (!clean) {
+#pragma unroll
+                for (int i = 0; i < VW; ++i) v[x][q][i] = 0;
+              }
             }
-          // a NaN scale counts only where a token of its page is seen
-          if (sum != 0.f) l = fmaf(sum, 1.f / cur[g].vs, l);
-          uint32_t pa[4];
-          f16_split2(p[0][0], p[0][1], pa[0], pa[1]);
-          f16_split2(p[1][0], p[1][1], pa[2], pa[3]);
 #pragma unroll
           for (int w = 0; w < VW; ++w) {
             uint32_t v0[4], v1[4];
-            codes_across<FMT>(cur[g].v[0][0][w], cur[g].v[0][1][w], v0);
-            codes_across<FMT>(cur[g].v[1][0][w], cur[g].v[1][1][w], v1);
+            codes_across<FMT>(v[0][0][w], v[0][1][w], v0);
+            codes_across<FMT>(v[1][0][w], v[1][1][w], v1);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               mma16816(o[4 * w + i], pa[0], pa[1], pa[2], pa[3], v0[i], v1[i]);
           }
         }
       }
+      // the step's bytes are in registers: its place in the ring takes the next copies
+      __syncwarp();
+      stage = stage + 1 == S ? 0 : stage + 1;
+      phase ^= stage == 0;
 #pragma unroll
-      for (int g = 0; g < GR; ++g) cur[g] = nxt[g], pg[g] = npg[g];
+      for (int i = 0; i + 1 < S; ++i) q_ks[i] = q_ks[i + 1], q_vs[i] = q_vs[i + 1];
+      if (more && alive) issue(q_ks[S - 1], q_vs[S - 1]);
     }
 
     // the warps' results joined
@@ -393,7 +507,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_rows_kernel(KvAttention
     if (tig == 0) s_m[warp][gid] = m, s_l[warp][gid] = l;
     flush();
     __syncthreads();
-    const bool whole = t_lo == 0 && t_hi == units;
+    const bool whole = t_lo == 0 && t_hi == use.units;
     const int rows = min(kRows, rows_all - rb * kRows);
     float *slot = a.ws + ((int64_t)blockIdx.x * 2 + (t_lo == 0 ? 1 : 0)) * Sh::kSlot;
     for (int i = tid; i < rows * HD; i += kThreads) {
@@ -408,13 +522,13 @@ __global__ void __launch_bounds__(kThreads) kv_attention_rows_kernel(KvAttention
         const float f = s_m[w][rr] == mm ? 1.f : exp2_approx(s_m[w][rr] - mm);
         const float fw = s_l[w][rr] == s_l[w][rr] ? f : 1.f;
         ll = fmaf(s_l[w][rr], fw, ll);
-        oo = fmaf(s_o[w][rr][d], fw, oo);
+        oo = fmaf(s_o[(w * kRows + rr) * HD + d], fw, oo);
       }
       if (whole) {
         const int row = rb * kRows + rr, ti = row / a.group;
-        if (d < c.hd) {
-          const float v = ti >= count || ll == 0.f ? 0.f : oo * kCodeUnit<FMT> / ll;
-          kv_store_out(a.out, (((int64_t)b * a.tokens + ti) * a.heads + h * a.group + row % a.group) * c.hd + d, v);
+        if (d < hd) {
+          const float v = ti >= count || ll == 0.f ? 0.f : oo / ll;
+          kv_store_out(a.out, (((int64_t)b * a.tokens + ti) * a.heads + h * a.group + row % a.group) * hd + d, v);
         }
       } else {
         slot[rr * HD + d] = oo;
@@ -422,13 +536,20 @@ __global__ void __launch_bounds__(kThreads) kv_attention_rows_kernel(KvAttention
       }
     }
     __syncthreads();
-    u += t_hi - t_lo;
+    going = use.next_segment(a, Sh::kUnit, hr);
   }
+  // after a wait that gave up: the copies still in flight, waited for (bounded)
+  if (!alive)
+    for (int s = 0; s < S; ++s) {
+      mbar_wait(bars + 8 * stage, phase, nullptr);
+      stage = stage + 1 == S ? 0 : stage + 1;
+      phase ^= stage == 0;
+    }
 }
 
 // Joins the partial results of the (sequence, key head, row block) runs that
 // several CTAs shared, in the order of the CTAs; the others are done already.
-template <int HD, int FMT>
+template <int HD>
 __global__ void __launch_bounds__(kThreads) kv_attention_join_kernel(KvAttentionArgs a,
                                                                      int row_blocks, int ctas) {
   using Sh = RowShape<HD>;
@@ -480,27 +601,9 @@ __global__ void __launch_bounds__(kThreads) kv_attention_join_kernel(KvAttention
       ll = fmaf(lk, f, ll);
       oo = fmaf(s[rr * HD + d], f, oo);
     }
-    const float v = ti >= count || ll == 0.f ? 0.f : oo * kCodeUnit<FMT> / ll;
+    const float v = ti >= count || ll == 0.f ? 0.f : oo / ll;
     kv_store_out(a.out, (((int64_t)b * a.tokens + ti) * a.heads + h * a.group + row % a.group) * c.hd + d, v);
   }
-}
-
-template <int HD, int FMT>
-int rows_ctas(int *out) {
-  static int cached[64] = {};
-  int dev = 0;
-  TT_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev < 64 && cached[dev] > 0) {
-    *out = cached[dev];
-    return TT_OK;
-  }
-  int sms = 0, per = 0;
-  TT_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  TT_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(
-      &per, kv_attention_rows_kernel<HD, FMT>, kThreads, 0));
-  *out = sms * std::max(per, 1);
-  if (dev < 64) cached[dev] = *out;
-  return TT_OK;
 }
 
 struct RowPlan {
@@ -510,7 +613,7 @@ struct RowPlan {
   size_t ws_bytes;
 };
 
-template <int HD, int FMT>
+template <int HD>
 int rows_plan(const KvView &c, int64_t tokens, int heads, RowPlan *p) {
   using Sh = RowShape<HD>;
   const int64_t rows = tokens * (heads / c.heads);
@@ -518,66 +621,87 @@ int rows_plan(const KvView &c, int64_t tokens, int heads, RowPlan *p) {
   if (rows > INT32_MAX || blocks * c.heads > INT32_MAX || c.batch > 65535)
     return fail(TT_ERR_UNSUPPORTED, "tt_kv_attention: too many rows or sequences");
   p->row_blocks = (int)blocks;
-  int most = 0;
-  const int rc = rows_ctas<HD, FMT>(&most);
+  int sms = 0;
+  const int rc = kv_sm_count(&sms);
   if (rc != TT_OK) return rc;
   const int64_t each = ceil_div((int64_t)c.columns << c.page_log2, Sh::kUnit);
   // no run is split when every sequence is one unit
   p->join = each > 1;
-  p->ctas = (int)std::min<int64_t>(most, each * blocks * c.heads * c.batch);
+  p->ctas = (int)std::min<int64_t>(sms * Sh::kCtas, each * blocks * c.heads * c.batch);
   p->ws_bytes = p->join ? (size_t)p->ctas * 2 * Sh::kSlot * sizeof(float) : 0;
   return TT_OK;
 }
 
-template <int HD, int FMT>
+template <int HD, int FMT, bool EXACT>
 int launch_rows(const KvAttentionArgs &a, cudaStream_t stream) {
+  using Sh = RowShape<HD>;
   RowPlan p;
-  const int rc = rows_plan<HD, FMT>(a.c, a.tokens, a.heads, &p);
+  int rc = rows_plan<HD>(a.c, a.tokens, a.heads, &p);
   if (rc != TT_OK) return rc;
-  TT_CUDA_TRY(launch_kernel(kv_attention_rows_kernel<HD, FMT>, dim3(p.ctas), dim3(kThreads), 0,
-                            stream, 1, a, p.row_blocks, p.join));
+  auto *kern = kv_attention_rows_kernel<HD, FMT, EXACT>;
+  static KvSmemSet set;
+  if ((rc = set.ensure(reinterpret_cast<const void *>(kern), Sh::kSmem)) != TT_OK) return rc;
+  TT_CUDA_TRY(launch_kernel(kern, dim3(p.ctas), dim3(kThreads), Sh::kSmem, stream, 1, a, p.row_blocks));
   if (p.join)
-    TT_CUDA_TRY(launch_kernel(kv_attention_join_kernel<HD, FMT>,
-                              dim3(p.row_blocks * a.c.heads, a.c.batch), dim3(kThreads), 0, stream,
-                              1, a, p.row_blocks, p.ctas));
+    TT_CUDA_TRY(launch_kernel(kv_attention_join_kernel<HD>, dim3(p.row_blocks * a.c.heads, a.c.batch),
+                              dim3(kThreads), 0, stream, 1, a, p.row_blocks, p.ctas));
   return TT_OK;
 }
 
-// The instantiation for a head_dim: the smallest width that holds it.
-template <class F>
-int for_shape(const KvView &c, F &&f) {
-  const bool i8 = c.format == TT_KV_INT8;
-#define TT_KV_SHAPE(HD)                                                        \
-  return i8 ? f(std::integral_constant<int, HD>(), std::integral_constant<int, TT_KV_INT8>()) \
-            : f(std::integral_constant<int, HD>(), std::integral_constant<int, TT_KV_E4M3>())
-  if (c.hd <= 32) TT_KV_SHAPE(32);
-  if (c.hd <= 64) TT_KV_SHAPE(64);
-  if (c.hd <= 128) TT_KV_SHAPE(128);
-  TT_KV_SHAPE(256);
-#undef TT_KV_SHAPE
+template <int HD>
+int launch_rows_of(const KvAttentionArgs &a, cudaStream_t stream) {
+  const bool i8 = a.c.format == TT_KV_INT8;
+  if (a.c.hd == HD)
+    return i8 ? launch_rows<HD, TT_KV_INT8, true>(a, stream) : launch_rows<HD, TT_KV_E4M3, true>(a, stream);
+  return i8 ? launch_rows<HD, TT_KV_INT8, false>(a, stream) : launch_rows<HD, TT_KV_E4M3, false>(a, stream);
+}
+
+// Rows of a key head from which the tile kernel takes over.
+bool use_tiles(const KvView &c, int64_t tokens, int heads) {
+  return tokens * (heads / c.heads) >= 64;
 }
 
 }  // namespace
 
-// Rows of a key head from which the tile kernel takes over.
-static bool use_tiles(const KvView &c, int64_t tokens, int heads) {
-  return tokens * (heads / c.heads) >= 64;
+int kv_sm_count(int *out) {
+  static int cached[64] = {};
+  int dev = 0;
+  TT_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 64 && cached[dev] > 0) {
+    *out = cached[dev];
+    return TT_OK;
+  }
+  TT_CUDA_TRY(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev));
+  if (dev < 64) cached[dev] = *out;
+  return TT_OK;
 }
 
+int KvSmemSet::ensure(const void *kernel, size_t bytes) {
+  int dev = 0;
+  TT_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 64 && done[dev]) return TT_OK;
+  TT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  if (dev < 64) done[dev] = true;
+  return TT_OK;
+}
+
+// The smallest width that holds a head_dim: 32, 64, 128 or 256.
 size_t kv_attention_ws_bytes(const KvView &c, int64_t tokens, int heads) {
   if (use_tiles(c, tokens, heads)) return kv_attention_tiles_ws_bytes(c, tokens, heads);
   RowPlan p{};
-  const int rc = for_shape(c, [&](auto hd, auto fmt) {
-    return rows_plan<decltype(hd)::value, decltype(fmt)::value>(c, tokens, heads, &p);
-  });
+  const int rc = c.hd <= 32    ? rows_plan<32>(c, tokens, heads, &p)
+                 : c.hd <= 64  ? rows_plan<64>(c, tokens, heads, &p)
+                 : c.hd <= 128 ? rows_plan<128>(c, tokens, heads, &p)
+                               : rows_plan<256>(c, tokens, heads, &p);
   return rc == TT_OK ? p.ws_bytes : 0;
 }
 
 int launch_kv_attention(const KvAttentionArgs &a, cudaStream_t stream) {
   if (use_tiles(a.c, a.tokens, a.heads)) return launch_kv_attention_tiles(a, stream);
-  return for_shape(a.c, [&](auto hd, auto fmt) {
-    return launch_rows<decltype(hd)::value, decltype(fmt)::value>(a, stream);
-  });
+  if (a.c.hd <= 32) return launch_rows_of<32>(a, stream);
+  if (a.c.hd <= 64) return launch_rows_of<64>(a, stream);
+  if (a.c.hd <= 128) return launch_rows_of<128>(a, stream);
+  return launch_rows_of<256>(a, stream);
 }
 
 }  // namespace tt

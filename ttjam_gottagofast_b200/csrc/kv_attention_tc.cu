@@ -378,7 +378,8 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
         const int i = u * kConvThreads + ct, t = i / CPR, d = (i % CPR) * 16;
         const int pg = __shfl_sync(0xffffffffu, ids, t >> 4);
         r[u] = make_uint4(0, 0, 0, 0);
-        if (pg >= 0 && d < c.hd) {
+        // nothing behind the last token: such a slot may hold any bits
+        if (pg >= 0 && d < c.hd && (j0 + j) * TOK + t < any_end) {
           const int in_page = ((j0 + j) * TOK + t) & ((1 << c.page_log2) - 1);
           r[u] = *reinterpret_cast<const uint4 *>(pool + c.tile(pg, h) + (int64_t)in_page * c.hd + d);
         }
@@ -490,7 +491,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
           }
         }
       }
-      sc = a.scale * 1.4426950408889634f * kCodeUnit<FMT> * kv_pow2(e);
+      sc = a.scale * 1.4426950408889634f * kv_pow2(e);
       if constexpr (Sh::QT) tmem_wait_st();
       else fence_async();
       fence_before();
@@ -627,7 +628,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
     }
     mbar_wait(o_done(x), (nj - 1) & 1, abort_w, c.status, 0x6800);
     fence_after();
-    const float inv = l == 0.f ? 0.f : kCodeUnit<FMT> / l;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int d = 0; d < HD; d += 16) {
       uint32_t o[16];
@@ -699,7 +700,7 @@ __global__ void __launch_bounds__(256) kv_attention_tiles_join_kernel(KvAttentio
     o[0] = fmaf(v.x, f, o[0]), o[1] = fmaf(v.y, f, o[1]);
     o[2] = fmaf(v.z, f, o[2]), o[3] = fmaf(v.w, f, o[3]);
   }
-  const float inv = l == 0.f ? 0.f : kCodeUnit<FMT> / l;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   const int64_t at = (((int64_t)b * a.tokens + r / a.group) * a.heads + h * a.group + r % a.group) * c.hd + d;
 #pragma unroll
   for (int k = 0; k < 4; ++k) kv_store_out(a.out, at + k, o[k] * inv);
@@ -727,18 +728,11 @@ TilePlan tile_plan(const KvView &c, int64_t tokens, int heads, int sms) {
   return p;
 }
 
-int sm_count(int *out) {
-  int dev = 0;
-  TT_CUDA_TRY(cudaGetDevice(&dev));
-  TT_CUDA_TRY(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev));
-  return TT_OK;
-}
-
 template <int HD, int FMT, int PIECES>
 int launch_tiles(const KvAttentionArgs &a, cudaStream_t stream) {
   using Sh = TcShape<HD, PIECES>;
   int sms = 0;
-  const int rc = sm_count(&sms);
+  const int rc = kv_sm_count(&sms);
   if (rc != TT_OK) return rc;
   if ((int64_t)a.tokens * a.group > INT32_MAX || a.c.batch > 65535 || a.c.heads > 65535)
     return fail(TT_ERR_UNSUPPORTED, "tt_kv_attention: too many rows, heads or sequences");
@@ -746,13 +740,9 @@ int launch_tiles(const KvAttentionArgs &a, cudaStream_t stream) {
   if ((int64_t)p.row_tiles * a.c.heads > INT32_MAX)
     return fail(TT_ERR_UNSUPPORTED, "tt_kv_attention: too many rows");
   auto *kern = kv_attention_tiles_kernel<HD, FMT, PIECES>;
-  static bool set[64] = {};
-  int dev = 0;
-  TT_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev >= 64 || !set[dev]) {
-    TT_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::SMEM));
-    if (dev < 64) set[dev] = true;
-  }
+  static KvSmemSet set;
+  const int set_rc = set.ensure(reinterpret_cast<const void *>(kern), Sh::SMEM);
+  if (set_rc != TT_OK) return set_rc;
   TT_CUDA_TRY(launch_kernel(kern, dim3(p.row_tiles * a.c.heads, a.c.batch, p.splits), dim3(Sh::THREADS),
                             Sh::SMEM, stream, 1, a, p.row_tiles, p.splits));
   if (p.splits > 1)
@@ -787,7 +777,7 @@ int for_tiles(const KvView &c, int dtype, F &&f) {
 
 size_t kv_attention_tiles_ws_bytes(const KvView &c, int64_t tokens, int heads) {
   int sms = 0;
-  if (sm_count(&sms) != TT_OK) return 0;
+  if (kv_sm_count(&sms) != TT_OK) return 0;
   size_t n = 0;
   for_tiles(c, TT_DTYPE_F32, [&](auto hd, auto, auto pieces) {  // the same for every type
     n = tile_plan<decltype(hd)::value, decltype(pieces)::value>(c, tokens, heads, sms).ws_bytes;
