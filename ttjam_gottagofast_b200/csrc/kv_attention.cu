@@ -27,9 +27,12 @@
 // token or dim stands at which operand index is free as long as both operands
 // agree) and so that few of a warp's loads share banks.
 //
-// Work is split into units of kUnit tokens of one (sequence, key head, row block);
-// every CTA takes an equal run of consecutive units, whatever the lengths, and a
-// second kernel joins the (sequence, head) runs that ended up on several CTAs.
+// Work is counted in units: kStep tokens of one (sequence, key head, row block), and
+// kOver units for each such segment, as its start and end cost about that much
+// (without them, warps with many short sequences end last). Every warp takes an
+// equal run of consecutive units, whatever the lengths, and a second kernel joins
+// the segments that ended up on several warps. Where no segment is longer than
+// kWhole steps, warps take whole ones, and nothing is left to join.
 #include <math_constants.h>
 
 #include <algorithm>
@@ -48,7 +51,8 @@ template <int HD>
 struct RowShape {
   static constexpr int kStep = HD == 32 ? 64 : HD == 64 ? 32 : 16;  // tokens per warp step
   static constexpr int GR = kStep / 16;              // groups of 16 tokens, each in one page
-  static constexpr int kUnit = kStep * kWarps;       // tokens per unit
+  static constexpr int kOver = 2;                    // units of a segment besides its steps
+  static constexpr int kWhole = 4;                   // steps of a segment that is never split
   static constexpr int kStages = HD == 256 ? 2 : 3;  // steps in a warp's ring
   static constexpr uint32_t kStage = 2 * kStep * HD;  // bytes: keys, then values
   // shared memory: the rings, the warps' results, barriers
@@ -119,13 +123,14 @@ __device__ __forceinline__ void mma16816(float *c, uint32_t a0, uint32_t a1, uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Units of sequence b for one (key head, row block): at least one, which writes
-// the zeros of a sequence that has no new token.
-__device__ __forceinline__ int units_of(const KvAttentionArgs &a, int b, int unit, int &len,
-                                        int &count) {
+// Units of a segment of sequence b; at least one step, which writes the zeros of
+// a sequence that has no new token.
+template <int HD>
+__device__ __forceinline__ int units_of(const KvAttentionArgs &a, int b, int &len, int &count) {
+  using Sh = RowShape<HD>;
   len = a.c.length(b);
   count = a.c.count(a.counts, b, a.tokens, len);
-  return count > 0 ? (len + unit - 1) / unit : 1;
+  return Sh::kOver + (count > 0 ? (len + Sh::kStep - 1) / Sh::kStep : 1);
 }
 
 // Token (0-7) of operand column n of an 8-token half: such that two neighbouring
@@ -135,31 +140,41 @@ __device__ __forceinline__ int half_token(int n) {
   return n & 1 ? r ^ 3 : r;
 }
 
-// Where a CTA's run of units stands: unit t of the (sequence, key head, row
-// block) segment [seg_lo, seg_hi) that the run holds of it.
+// Where a warp's run of units stands: unit t of the segment whose units [lo, hi)
+// the run holds. The steps are the units from kOver on.
+template <int HD>
 struct Cursor {
-  int64_t left;   // units of the run from this one on
-  int64_t first;  // units of the sequence before this segment's first
-  int b, len, count, units, pair, t, t_hi;
+  int64_t left;  // units of the run from unit lo of this segment on
+  int b, len, count, units, pair, t, lo, hi;
 
-  __device__ __forceinline__ void segment(int64_t skip) {  // `skip` units of the sequence are behind
+  // the segment that holds unit `skip` of the sequence
+  __device__ __forceinline__ void enter(int64_t skip, bool whole) {
     pair = (int)(skip / units);
-    t = (int)(skip - (int64_t)pair * units);
-    t_hi = (int)min((int64_t)units, t + left);
+    lo = (int)(skip - (int64_t)pair * units);
+    bound(whole);
   }
-  // to the next segment; false at the end of the run
-  __device__ __forceinline__ bool next_segment(const KvAttentionArgs &a, int unit, int64_t hr) {
-    left -= t_hi - seg_lo;
+  __device__ __forceinline__ void bound(bool whole) {
+    hi = whole ? units : (int)min((int64_t)units, lo + left);
+    t = max(lo, RowShape<HD>::kOver);
+  }
+  // to the run's next segment; false at its end
+  __device__ __forceinline__ bool next(const KvAttentionArgs &a, int64_t hr, bool whole) {
+    left -= hi - lo;
     if (left <= 0) return false;
     if (++pair >= hr) {
       pair = 0;
-      units = units_of(a, ++b, unit, len, count);
+      units = units_of<HD>(a, ++b, len, count);
     }
-    t = seg_lo = 0;
-    t_hi = (int)min((int64_t)units, left);
+    lo = 0;
+    bound(whole);
     return true;
   }
-  int seg_lo;
+  // past segments of which the run holds no step
+  __device__ __forceinline__ bool to_step(const KvAttentionArgs &a, int64_t hr, bool whole) {
+    while (t >= hi)
+      if (!next(a, hr, whole)) return false;
+    return true;
+  }
 };
 
 // The head dim of output tile 4 w + i (8 columns), column n.
@@ -171,11 +186,10 @@ __device__ __forceinline__ int out_dim(int w, int i, int n) {
 
 template <int HD, int FMT, bool EXACT>
 __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
-    kv_attention_rows_kernel(KvAttentionArgs a, int row_blocks) {
+    kv_attention_rows_kernel(KvAttentionArgs a, int row_blocks, bool whole) {
   using Sh = RowShape<HD>;
   constexpr int KW = Sh::KW, VW = Sh::VW, GR = Sh::GR, S = Sh::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
   __shared__ int64_t s_scan[kThreads];
   pdl_trigger();
   const KvView &c = a.c;
@@ -186,19 +200,19 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
   const int rows_all = a.tokens * a.group;           // query rows of a key head
   const uint32_t ring = smem_u32(smem) + warp * S * Sh::kStage;
   const uint32_t bars = smem_u32(smem) + Sh::kBars + 8 * warp * S;
-  float *const s_o = reinterpret_cast<float *>(smem + Sh::kO);  // [kWarps][kRows][HD]
+  float *const s_o = reinterpret_cast<float *>(smem + Sh::kO) + warp * kRows * HD;  // [kRows][HD]
   if (lane < S)
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bars + 8 * lane), "r"(GR) : "memory");
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   pdl_wait();
 
-  // the CTA's run of units, and the sequence that holds its first
+  // the warp's run of units, and the sequence that holds its first
   const int per_thread = (c.batch + kThreads - 1) / kThreads;
   const int b0 = min(c.batch, tid * per_thread), b1 = min(c.batch, b0 + per_thread);
   int64_t mine = 0;
   for (int b = b0; b < b1; ++b) {
     int len, count;
-    mine += units_of(a, b, Sh::kUnit, len, count);
+    mine += units_of<HD>(a, b, len, count);
   }
   // inclusive sums over the threads
 #pragma unroll
@@ -213,40 +227,45 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
   s_scan[tid] = mine;
   __syncthreads();
   const int64_t total = s_scan[kThreads - 1] * hr;
-  const int64_t run = (total + gridDim.x - 1) / gridDim.x;
-  const int64_t lo = blockIdx.x * run;
+  const int gw = blockIdx.x * kWarps + warp;
+  const int64_t run = (total + gridDim.x * kWarps - 1) / (gridDim.x * kWarps);
+  const int64_t lo = gw * run;
   if (lo >= total) return;
-  Cursor use;  // what is computed; `fill` below is what is copied, ahead of it
+  Cursor<HD> use;  // what is computed; `fill` below is what is copied, ahead of it
   use.left = min(run, total - lo);
   {
-    int t = 0;
-    while (s_scan[t] * hr <= lo) ++t;
+    int t = 0;  // threads whose sequences end at or before lo
+#pragma unroll
+    for (int k = 0; k < kThreads / 32; ++k)
+      t += __popc(__ballot_sync(0xffffffffu, s_scan[32 * k + lane] * hr <= lo));
     use.b = t * per_thread;
     int64_t first = t > 0 ? s_scan[t - 1] * hr : 0;
-    use.units = units_of(a, use.b, Sh::kUnit, use.len, use.count);
+    use.units = units_of<HD>(a, use.b, use.len, use.count);
     while (first + use.units * hr <= lo) {
       first += use.units * hr;
-      use.units = units_of(a, ++use.b, Sh::kUnit, use.len, use.count);
+      use.units = units_of<HD>(a, ++use.b, use.len, use.count);
     }
-    use.segment(lo - first);
-    use.seg_lo = use.t;
+    use.enter(lo - first, whole);
+    // whole segments belong to the run that holds their first unit
+    if (whole && use.lo > 0 && !use.next(a, hr, whole)) return;
+    if (!use.to_step(a, hr, whole)) return;
   }
 
   // tokens that the last live row of the cursor's row block sees
-  auto seen_by_block = [&](const Cursor &u) {
+  auto seen_by_block = [&](const Cursor<HD> &u) {
     const int rb = u.pair % row_blocks;
     const int r_first = rb * kRows / a.group;
     const int r_last = min(rb * kRows + kRows - 1, rows_all - 1) / a.group;
     return r_first < u.count ? u.len - u.count + min(r_last, u.count - 1) + 1 : 0;
   };
-  auto t0_of = [&](int t) { return t * Sh::kUnit + warp * Sh::kStep; };
+  auto t0_of = [&](int t) { return (t - Sh::kOver) * Sh::kStep; };
 
   // ---- the copies -----------------------------------------------------------
   // Lane g < GR copies group g's keys and values; its page is looked up one step
   // before, its scales wait in the lane's queue for as long as the bytes do in the
   // ring. A group without a page, or past the last seen token, copies nothing and
   // has the key scale -1.
-  Cursor fill = use;
+  Cursor<HD> fill = use;
   bool more = true;
   int fill_end = seen_by_block(fill), fill_stage = 0, pg_next;
   float q_ks[S], q_vs[S];
@@ -273,8 +292,8 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
       }
     }
     fill_stage = fill_stage + 1 == S ? 0 : fill_stage + 1;
-    if (++fill.t == fill.t_hi) {
-      more = fill.next_segment(a, Sh::kUnit, hr);
+    if (++fill.t == fill.hi) {
+      more = fill.to_step(a, hr, whole);
       if (more) fill_end = seen_by_block(fill);
     }
     if (more) look_up();
@@ -314,9 +333,14 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
         const int d = HD == 32 ? 8 * tig + 4 * w : 64 * (w / 4) + 16 * tig + 4 * (w % 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x[w][i] = live && d < hd ? kv_load_in(a.dtype, a.q, off + d + i) : 0.f;
-          mx = fmaxf(mx, fabsf(x[w][i]));
+          x[w][i] = 0.f;
         }
+        if (live && d < hd) kv_load_in4(a.dtype, a.q, off + d, a.q_vec, x[w]);
+      }
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fabsf(x[w][i]));
       }
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
@@ -346,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
-            float &sum = s_o[(warp * kRows + gid) * HD + out_dim<HD>(w, i, 2 * tig + n)];
+            float &sum = s_o[gid * HD + out_dim<HD>(w, i, 2 * tig + n)];
             const float v = o[4 * w + i][n] + o[4 * w + i][2 + n];
             sum = flushed ? fmaf(sum, beta, v) : v;
           }
@@ -354,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
       beta = 1.f;
     };
 
-    const int t_lo = use.seg_lo, t_hi = use.t_hi;
+    const int t_lo = use.t, t_hi = use.hi;
     for (int t = t_lo; t < t_hi; ++t) {
       const int t0 = t0_of(t);
       if (t > t_lo && (t - t_lo) % Sh::kFlush == 0) {
@@ -501,42 +525,36 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
       if (more && alive) issue(q_ks[S - 1], q_vs[S - 1]);
     }
 
-    // the warps' results joined
+    // the row's result: its output, or a partial one
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if (tig == 0) s_m[warp][gid] = m, s_l[warp][gid] = l;
-    flush();
-    __syncthreads();
-    const bool whole = t_lo == 0 && t_hi == use.units;
-    const int rows = min(kRows, rows_all - rb * kRows);
-    float *slot = a.ws + ((int64_t)blockIdx.x * 2 + (t_lo == 0 ? 1 : 0)) * Sh::kSlot;
-    for (int i = tid; i < rows * HD; i += kThreads) {
-      const int rr = i / HD, d = i % HD;
-      float mm = -CUDART_INF_F;
+    const bool from_start = t_lo == Sh::kOver, done = from_start && t_hi == use.units;
+    if (r < rows_all) {
+      float *slot = a.ws + ((int64_t)gw * 2 + (from_start ? 1 : 0)) * Sh::kSlot;
+      const float inv = tok >= count || l == 0.f ? 0.f : 1.f / l;
+      const int64_t at = (((int64_t)b * a.tokens + tok) * a.heads + h * a.group + r % a.group) * hd;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w][rr]);
-      float ll = 0.f, oo = 0.f;
+      for (int w = 0; w < VW; ++w)
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        // a warp whose scores are all NaN has m = -inf and a NaN sum
-        const float f = s_m[w][rr] == mm ? 1.f : exp2_approx(s_m[w][rr] - mm);
-        const float fw = s_l[w][rr] == s_l[w][rr] ? f : 1.f;
-        ll = fmaf(s_l[w][rr], fw, ll);
-        oo = fmaf(s_o[(w * kRows + rr) * HD + d], fw, oo);
-      }
-      if (whole) {
-        const int row = rb * kRows + rr, ti = row / a.group;
-        if (d < hd) {
-          const float v = ti >= count || ll == 0.f ? 0.f : oo / ll;
-          kv_store_out(a.out, (((int64_t)b * a.tokens + ti) * a.heads + h * a.group + row % a.group) * hd + d, v);
+        for (int n = 0; n < 2; ++n) {
+          const int d = out_dim<HD>(w, 0, 2 * tig + n);  // and the three after it
+          float v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            v[i] = o[4 * w + i][n] + o[4 * w + i][2 + n];
+            if (flushed) v[i] = fmaf(s_o[gid * HD + d + i], beta, v[i]);
+          }
+          if (!done) {
+            *reinterpret_cast<float4 *>(slot + gid * HD + d) = make_float4(v[0], v[1], v[2], v[3]);
+          } else if (EXACT || d < hd) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = inv == 0.f ? 0.f : v[i] * inv;
+            kv_store_out4(a.out, at + d, v);
+          }
         }
-      } else {
-        slot[rr * HD + d] = oo;
-        if (d == 0) slot[kRows * HD + rr] = mm, slot[kRows * HD + kRows + rr] = ll;
-      }
+      if (!done && tig == 0) slot[kRows * HD + gid] = m, slot[kRows * HD + kRows + gid] = l;
     }
-    __syncthreads();
-    going = use.next_segment(a, Sh::kUnit, hr);
+    going = use.next(a, hr, whole) && use.to_step(a, hr, whole);
   }
   // after a wait that gave up: the copies still in flight, waited for (bounded)
   if (!alive)
@@ -547,11 +565,11 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
     }
 }
 
-// Joins the partial results of the (sequence, key head, row block) runs that
-// several CTAs shared, in the order of the CTAs; the others are done already.
+// Joins the partial results of the segments that several warps shared, in the
+// order of the warps; the others are done already. One thread per 4 dims of a row.
 template <int HD>
-__global__ void __launch_bounds__(kThreads) kv_attention_join_kernel(KvAttentionArgs a,
-                                                                     int row_blocks, int ctas) {
+__global__ void __launch_bounds__(kThreads) kv_attention_join_kernel(KvAttentionArgs a, int row_blocks,
+                                                                     int warps) {
   using Sh = RowShape<HD>;
   __shared__ int64_t s_sum[kWarps][2];
   pdl_trigger();
@@ -563,7 +581,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_join_kernel(KvAttention
   int64_t before = 0, total = 0;
   for (int i = tid; i < c.batch; i += kThreads) {
     int len, count;
-    const int n = units_of(a, i, Sh::kUnit, len, count);
+    const int n = units_of<HD>(a, i, len, count);
     total += n;
     if (i < b) before += n;
   }
@@ -578,38 +596,44 @@ __global__ void __launch_bounds__(kThreads) kv_attention_join_kernel(KvAttention
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) before += s_sum[w][0], total += s_sum[w][1];
   int len, count;
-  const int units = units_of(a, b, Sh::kUnit, len, count);
-  const int64_t run = (total * hr + ctas - 1) / ctas;
+  const int units = units_of<HD>(a, b, len, count);
+  const int64_t run = (total * hr + warps - 1) / warps;
   const int64_t pair = blockIdx.x;
   const int64_t u0 = before * hr + pair * units, u1 = u0 + units;
-  const int64_t c0 = u0 / run, c1 = (u1 - 1) / run;
+  const int64_t c0 = (u0 + Sh::kOver) / run, c1 = (u1 - 1) / run;
   if (c0 == c1) return;
   const int h = (int)(pair / row_blocks), rb = (int)(pair % row_blocks);
   const int rows_all = a.tokens * a.group, rows = min(kRows, rows_all - rb * kRows);
-  auto slot = [&](int64_t cta) { return a.ws + (cta * 2 + (cta == c0 ? 1 : 0)) * Sh::kSlot; };
-  for (int i = tid; i < rows * HD; i += kThreads) {
-    const int rr = i / HD, d = i % HD;
+  const int hd4 = c.hd / 4;
+  for (int i = tid; i < rows * hd4; i += kThreads) {
+    const int rr = i / hd4, d = i % hd4 * 4;
     const int row = rb * kRows + rr, ti = row / a.group;
-    if (d >= c.hd) continue;
+    const float *const base = a.ws + rr * HD + d, *const ml = a.ws + kRows * HD + rr;
+    auto slot = [&](int64_t w) { return (w * 2 + (w == c0 ? 1 : 0)) * Sh::kSlot; };
     float mm = -CUDART_INF_F;
-    for (int64_t k = c0; k <= c1; ++k) mm = fmaxf(mm, slot(k)[kRows * HD + rr]);
-    float ll = 0.f, oo = 0.f;
+    for (int64_t k = c0; k <= c1; ++k) mm = fmaxf(mm, ml[slot(k)]);
+    float ll = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int64_t k = c0; k <= c1; ++k) {
-      const float *s = slot(k);
-      const float mk = s[kRows * HD + rr], lk = s[kRows * HD + kRows + rr];
+      const float mk = ml[slot(k)], lk = ml[slot(k) + kRows];
+      const float4 v = *reinterpret_cast<const float4 *>(base + slot(k));
+      // a warp whose scores are all NaN has m = -inf and a NaN sum
       const float f = mk == mm || !(lk == lk) ? 1.f : exp2_approx(mk - mm);
       ll = fmaf(lk, f, ll);
-      oo = fmaf(s[rr * HD + d], f, oo);
+      o[0] = fmaf(v.x, f, o[0]), o[1] = fmaf(v.y, f, o[1]);
+      o[2] = fmaf(v.z, f, o[2]), o[3] = fmaf(v.w, f, o[3]);
     }
-    const float v = ti >= count || ll == 0.f ? 0.f : oo / ll;
-    kv_store_out(a.out, (((int64_t)b * a.tokens + ti) * a.heads + h * a.group + row % a.group) * c.hd + d, v);
+    const float inv = ti >= count || ll == 0.f ? 0.f : 1.f / ll;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = inv == 0.f ? 0.f : o[k] * inv;
+    kv_store_out4(a.out, (((int64_t)b * a.tokens + ti) * a.heads + h * a.group + row % a.group) * c.hd + d, o);
   }
 }
 
 struct RowPlan {
   int row_blocks;
   int ctas;
-  bool join;
+  bool whole;
   size_t ws_bytes;
 };
 
@@ -624,11 +648,12 @@ int rows_plan(const KvView &c, int64_t tokens, int heads, RowPlan *p) {
   int sms = 0;
   const int rc = kv_sm_count(&sms);
   if (rc != TT_OK) return rc;
-  const int64_t each = ceil_div((int64_t)c.columns << c.page_log2, Sh::kUnit);
-  // no run is split when every sequence is one unit
-  p->join = each > 1;
-  p->ctas = (int)std::min<int64_t>(sms * Sh::kCtas, each * blocks * c.heads * c.batch);
-  p->ws_bytes = p->join ? (size_t)p->ctas * 2 * Sh::kSlot * sizeof(float) : 0;
+  const int64_t steps = ceil_div((int64_t)c.columns << c.page_log2, Sh::kStep);  // of a segment, at most
+  const int64_t segments = blocks * c.heads * c.batch;
+  p->whole = steps <= Sh::kWhole;
+  const int64_t most = p->whole ? segments : steps * segments;  // warps that could have work
+  p->ctas = (int)std::min<int64_t>(sms * Sh::kCtas, ceil_div(most, kWarps));
+  p->ws_bytes = p->whole ? 0 : (size_t)p->ctas * kWarps * 2 * Sh::kSlot * sizeof(float);
   return TT_OK;
 }
 
@@ -641,10 +666,11 @@ int launch_rows(const KvAttentionArgs &a, cudaStream_t stream) {
   auto *kern = kv_attention_rows_kernel<HD, FMT, EXACT>;
   static KvSmemSet set;
   if ((rc = set.ensure(reinterpret_cast<const void *>(kern), Sh::kSmem)) != TT_OK) return rc;
-  TT_CUDA_TRY(launch_kernel(kern, dim3(p.ctas), dim3(kThreads), Sh::kSmem, stream, 1, a, p.row_blocks));
-  if (p.join)
+  TT_CUDA_TRY(launch_kernel(kern, dim3(p.ctas), dim3(kThreads), Sh::kSmem, stream, 1, a, p.row_blocks,
+                            p.whole));
+  if (!p.whole)
     TT_CUDA_TRY(launch_kernel(kv_attention_join_kernel<HD>, dim3(p.row_blocks * a.c.heads, a.c.batch),
-                              dim3(kThreads), 0, stream, 1, a, p.row_blocks, p.ctas));
+                              dim3(kThreads), 0, stream, 1, a, p.row_blocks, p.ctas * kWarps));
   return TT_OK;
 }
 

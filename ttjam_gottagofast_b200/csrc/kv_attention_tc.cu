@@ -703,7 +703,8 @@ __global__ void __launch_bounds__(256) kv_attention_tiles_join_kernel(KvAttentio
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int64_t at = (((int64_t)b * a.tokens + r / a.group) * a.heads + h * a.group + r % a.group) * c.hd + d;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) kv_store_out(a.out, at + k, o[k] * inv);
+  for (int k = 0; k < 4; ++k) o[k] *= inv;
+  kv_store_out4(a.out, at, o);
 }
 
 struct TilePlan {

@@ -278,6 +278,8 @@ int kv_view(const tt_kv_cache *c, const char *what, KvView *v) {
     return no(TT_ERR_UNSUPPORTED, "head_dim must be a multiple of 16, at most 256");
   if (c->kv_heads <= 0 || c->num_pages <= 0 || c->batch < 0 || c->table_columns <= 0)
     return no(TT_ERR_INVALID_ARGUMENT, "kv_heads, num_pages and table_columns must be positive");
+  if ((int64_t)c->num_pages * c->kv_heads > INT32_MAX)
+    return no(TT_ERR_UNSUPPORTED, "num_pages * kv_heads must fit 32 bits");
   if ((int64_t)c->table_columns * c->page_size > INT32_MAX)
     return no(TT_ERR_UNSUPPORTED, "table_columns * page_size must fit 32 bits");
   if (c->batch > 0 && (c->k_codes == nullptr || c->v_codes == nullptr || c->k_scale == nullptr ||

@@ -67,7 +67,8 @@ struct KvView {
   }
   // first code of (page p, head h) in a pool
   __device__ __forceinline__ int64_t tile(int p, int h) const {
-    return ((int64_t)p * heads + h) * ((int64_t)hd << page_log2);
+    // kv_view: num_pages * kv_heads fits 32 bits
+    return (int64_t)((uint64_t)((uint32_t)p * (uint32_t)heads + (uint32_t)h) * (uint32_t)(hd << page_log2));
   }
 };
 

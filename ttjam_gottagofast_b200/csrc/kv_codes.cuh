@@ -52,11 +52,47 @@ __device__ __forceinline__ float kv_load_in(int dtype, const void *p, int64_t i)
   if (dtype == TT_DTYPE_F16) return __half2float(static_cast<const __half *>(p)[i]);
   return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
 }
-__device__ __forceinline__ void kv_store_out(const KvOut &o, int64_t i, float x) {
-  if (o.dtype == TT_DTYPE_F32) static_cast<float *>(o.p)[i] = x;
-  else if (o.dtype == TT_DTYPE_F16) static_cast<__half *>(o.p)[i] = __float2half_rn(x);
-  else if (o.dtype == TT_DTYPE_BF16) static_cast<__nv_bfloat16 *>(o.p)[i] = __float2bfloat16_rn(x);
-  else f16_split(x, static_cast<uint16_t *>(o.p)[i], static_cast<uint16_t *>(o.lo)[i]);
+
+// Four consecutive elements; i is a multiple of 4, `vec` as below.
+__device__ __forceinline__ void kv_load_in4(int dtype, const void *p, int64_t i, bool vec, float *x) {
+  if (!vec) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = kv_load_in(dtype, p, i + k);
+  } else if (dtype == TT_DTYPE_F32) {
+    const float4 v = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + i);
+    if (dtype == TT_DTYPE_F16) {
+      const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&v.x));
+      const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&v.y));
+      x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+    } else {
+      x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u);
+      x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
+    }
+  }
+}
+__device__ __forceinline__ void kv_store_out4(const KvOut &o, int64_t i, const float *x) {
+  if (o.dtype == TT_DTYPE_F32) {
+    *reinterpret_cast<float4 *>(static_cast<float *>(o.p) + i) = make_float4(x[0], x[1], x[2], x[3]);
+  } else if (o.dtype == kKvSplit) {
+    uint2 h, l;
+    f16_split2(x[0], x[1], h.x, l.x);
+    f16_split2(x[2], x[3], h.y, l.y);
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(o.p) + i) = h;
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(o.lo) + i) = l;
+  } else {
+    uint2 v;
+    if (o.dtype == TT_DTYPE_F16) {
+      asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(v.x) : "f"(x[1]), "f"(x[0]));
+      asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(v.y) : "f"(x[3]), "f"(x[2]));
+    } else {
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v.x) : "f"(x[1]), "f"(x[0]));
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v.y) : "f"(x[3]), "f"(x[2]));
+    }
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(o.p) + i) = v;
+  }
 }
 
 // 16 consecutive elements from element i on; `vec`: the address is a multiple of 16 bytes.
