@@ -114,13 +114,18 @@ __device__ __forceinline__ void lds(uint32_t addr, uint32_t *r) {
   else
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r[0]) : "r"(addr));
 }
-__device__ __forceinline__ void mma16816(float *c, uint32_t a0, uint32_t a1, uint32_t a2,
-                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+// c += a b (or c = a b); not volatile, so that independent products are interleaved
+__device__ __forceinline__ void mma16816(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_first(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 // Units of a segment of sequence b; at least one step, which writes the zeros of
@@ -378,6 +383,131 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
       beta = 1.f;
     };
 
+    // one step: scores, running maximum, p, p v
+    auto compute = [&](auto masked_form, int t0, uint32_t absent) {
+      constexpr bool MASKED = decltype(masked_form)::value;
+      const uint32_t kb = ring + stage * Sh::kStage, vb = kb + Sh::kStep * hd;
+      float s[GR][2][4];
+      {
+        constexpr int LB = HD == 32 ? 8 : 16;  // bytes a load
+        uint32_t w[GR][2][KW];
+#pragma unroll
+        for (int g = 0; g < GR; ++g)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const uint32_t row = kb + (16 * g + 8 * x + half_token(gid)) * hd;
+#pragma unroll
+            for (int j = 0; j < KW * 4 / LB; ++j) {
+              const int d = 4 * LB * j + LB * tig;
+              if (EXACT || d < hd) {
+                lds<LB>(row + d, &w[g][x][j * (LB / 4)]);
+              } else {
+#pragma unroll
+                for (int i = 0; i < LB / 4; ++i) w[g][x][j * (LB / 4) + i] = 0;
+              }
+            }
+          }
+#pragma unroll
+        for (int i = 0; i < KW; ++i)
+#pragma unroll
+          for (int g = 0; g < GR; ++g)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              uint32_t k0, k1;
+              codes_along<FMT>(w[g][x][i], k0, k1);
+              if (i == 0) mma16816_first(s[g][x], qa[i], k0, k1);
+              else mma16816(s[g][x], qa[i], k0, k1);
+            }
+      }
+      // scores of this thread: row gid, tokens 8 x + half_token(2 tig + p) of group g
+      const float ve_lane = q_vs[0] == q_vs[0] ? (float)((__float_as_int(q_vs[0]) >> 23) - 127) : q_vs[0];
+      auto sees = [&](int g, int x, int p) {
+        return !((absent >> g) & 1u) && t0 + 16 * g + 8 * x + half_token(2 * tig + p) < end;
+      };
+      float kc[GR], ve[GR], top = -CUDART_INF_F;
+#pragma unroll
+      for (int g = 0; g < GR; ++g) {
+        ve[g] = __shfl_sync(0xffffffffu, ve_lane, g);
+        kc[g] = fabsf(__shfl_sync(0xffffffffu, q_ks[0], g)) * sc;  // never negative: it meets -inf
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            s[g][x][p] += s[g][x][2 + p];
+            if (MASKED && !sees(g, x, p)) s[g][x][p] = -CUDART_INF_F;
+          }
+        const float mx = fmaxf(fmax3(s[g][0][0], s[g][0][1], s[g][1][0]), s[g][1][1]);
+        top = fmaxf(top, fmaf(mx, kc[g], ve[g]));
+      }
+      // p stays below 2^15: the reference moves when a score passes it by more than 1
+      if (__any_sync(0xffffffffu, top > m + 1.f)) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float mn = fmaxf(m, ceilf(top));
+        const float alpha = mn == m ? 1.f : exp2_approx(m - mn);  // 0 from -inf
+        m = mn;
+        l *= alpha;
+        beta *= alpha;
+#pragma unroll
+        for (int i = 0; i < 4 * VW; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[i][j] *= alpha;
+      }
+      const float ref = 14.f - (m == -CUDART_INF_F ? 0.f : m);
+#pragma unroll
+      for (int g = 0; g < GR; ++g) {
+        uint32_t v[2][2][VW];
+        constexpr int LB = VW >= 4 ? 16 : 4 * VW;  // bytes a load
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const int in_g = 8 * x + half_token(2 * tig + q);
+            const uint32_t row = vb + (16 * g + in_g) * hd;
+#pragma unroll
+            for (int j = 0; j < VW * 4 / LB; ++j) {
+              const int d = 8 * LB * j + LB * gid;
+              if (EXACT || d < hd) {
+                lds<LB>(row + d, &v[x][q][j * (LB / 4)]);
+              } else {
+#pragma unroll
+                for (int i = 0; i < LB / 4; ++i) v[x][q][j * (LB / 4) + i] = 0;
+              }
+            }
+            // what stands behind the last token may be any bits, e4m3's NaN among them
+            if (MASKED && FMT == TT_KV_E4M3 && (((absent >> g) & 1u) || t0 + 16 * g + in_g >= len)) {
+#pragma unroll
+              for (int i = 0; i < VW; ++i) v[x][q][i] = 0;
+            }
+          }
+        const float base = ve[g] + ref;
+        float p[2][2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            p[x][q] = exp2_approx(fmaf(s[g][x][q], kc[g], base));
+            // a NaN scale leaves NaN at the tokens behind the mask
+            if (MASKED && !sees(g, x, q)) p[x][q] = 0.f;
+          }
+        const float sum = (p[0][0] + p[0][1]) + (p[1][0] + p[1][1]);
+        // 2^-e; a NaN counts only where a token of its page is seen
+        const float more_l = fmaf(sum, exp2_approx(-ve[g]), l);
+        l = !MASKED || sum != 0.f ? more_l : l;
+        uint32_t pa[4];
+        f16_split2(p[0][0], p[0][1], pa[0], pa[1]);
+        f16_split2(p[1][0], p[1][1], pa[2], pa[3]);
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+          uint32_t v0[4], v1[4];
+          codes_across<FMT>(v[0][0][w], v[0][1][w], v0);
+          codes_across<FMT>(v[1][0][w], v[1][1][w], v1);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mma16816(o[4 * w + i], pa, v0[i], v1[i]);
+        }
+      }
+    };
+
     const int t_lo = use.t, t_hi = use.hi;
     for (int t = t_lo; t < t_hi; ++t) {
       const int t0 = t0_of(t);
@@ -390,131 +520,10 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
       }
       if (alive) alive = __all_sync(0xffffffffu, mbar_wait(bars + 8 * stage, phase, c.status));
       if (alive && t0 < any_end) {  // the same for the whole warp
-        const uint32_t kb = ring + stage * Sh::kStage, vb = kb + Sh::kStep * hd;
-        float s[GR][2][4];
-#pragma unroll
-        for (int g = 0; g < GR; ++g)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[g][x][i] = 0.f;
-            const uint32_t row = kb + (16 * g + 8 * x + half_token(gid)) * hd;
-            constexpr int LB = HD == 32 ? 8 : 16;  // bytes a load
-#pragma unroll
-            for (int j = 0; j < KW * 4 / LB; ++j) {
-              uint32_t w[LB / 4] = {};
-              const int d = 4 * LB * j + LB * tig;
-              if (EXACT || d < hd) lds<LB>(row + d, w);
-#pragma unroll
-              for (int i = 0; i < LB / 4; ++i) {
-                uint32_t k0, k1;
-                codes_along<FMT>(w[i], k0, k1);
-                const uint32_t *q = qa[j * (LB / 4) + i];
-                mma16816(s[g][x], q[0], q[1], q[2], q[3], k0, k1);
-              }
-            }
-          }
-        // scores of this thread: row gid, tokens 8 x + half_token(2 tig + p) of group g
-        const float ve_lane = q_vs[0] == q_vs[0] ? (float)((__float_as_int(q_vs[0]) >> 23) - 127) : q_vs[0];
-        float kc[GR], ve[GR], top = -CUDART_INF_F;
-        bool none[GR], masked[GR], dirty[GR];
-#pragma unroll
-        for (int g = 0; g < GR; ++g) {
-          const int tg = t0 + 16 * g;
-          const float ks = __shfl_sync(0xffffffffu, q_ks[0], g);
-          ve[g] = __shfl_sync(0xffffffffu, ve_lane, g);
-          none[g] = ks < 0.f;
-          kc[g] = fabsf(ks) * sc;  // never negative: it meets -inf below
-          masked[g] = none[g] || tg + 16 > all_end;
-          dirty[g] = none[g] || tg + 16 > len;
-          if (masked[g]) {
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-              for (int p = 0; p < 2; ++p) {
-                const bool see = !none[g] && tg + 8 * x + half_token(2 * tig + p) < end;
-                s[g][x][p] = see ? s[g][x][p] + s[g][x][2 + p] : -CUDART_INF_F;
-              }
-          } else {
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-              for (int p = 0; p < 2; ++p) s[g][x][p] += s[g][x][2 + p];
-          }
-          const float mx = fmaxf(fmax3(s[g][0][0], s[g][0][1], s[g][1][0]), s[g][1][1]);
-          top = fmaxf(top, fmaf(mx, kc[g], ve[g]));
-        }
-        // p stays below 2^15: the reference moves when a score passes it by more than 1
-        if (__any_sync(0xffffffffu, top > m + 1.f)) {
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          const float mn = fmaxf(m, ceilf(top));
-          const float alpha = mn == m ? 1.f : exp2_approx(m - mn);  // 0 from -inf
-          m = mn;
-          l *= alpha;
-          beta *= alpha;
-#pragma unroll
-          for (int i = 0; i < 4 * VW; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[i][j] *= alpha;
-        }
-        const float ref = m == -CUDART_INF_F ? 0.f : m;
-#pragma unroll
-        for (int g = 0; g < GR; ++g) {
-          const int tg = t0 + 16 * g;
-          const float base = ve[g] - ref + 14.f;
-          float p[2][2];
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int q = 0; q < 2; ++q) p[x][q] = exp2_approx(fmaf(s[g][x][q], kc[g], base));
-          if (masked[g]) {  // a NaN scale leaves NaN at the tokens behind the mask
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-              for (int q = 0; q < 2; ++q)
-                if (none[g] || tg + 8 * x + half_token(2 * tig + q) >= end) p[x][q] = 0.f;
-          }
-          const float sum = (p[0][0] + p[0][1]) + (p[1][0] + p[1][1]);
-          // 2^-e; a NaN counts only where a token of its page is seen
-          if (sum != 0.f) l = fmaf(sum, exp2_approx(-ve[g]), l);
-          uint32_t pa[4];
-          f16_split2(p[0][0], p[0][1], pa[0], pa[1]);
-          f16_split2(p[1][0], p[1][1], pa[2], pa[3]);
-          uint32_t v[2][2][VW];
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const int in_g = 8 * x + half_token(2 * tig + q);
-              const uint32_t row = vb + (16 * g + in_g) * hd;
-              constexpr int LB = VW >= 4 ? 16 : 4 * VW;  // bytes a load
-              const bool clean = !(FMT == TT_KV_E4M3 && dirty[g]) || (!none[g] && tg + in_g < len);
-#pragma unroll
-              for (int j = 0; j < VW * 4 / LB; ++j) {
-                const int d = 8 * LB * j + LB * gid;
-                if (EXACT || d < hd) {
-                  lds<LB>(row + d, &v[x][q][j * (LB / 4)]);
-                } else {
-#pragma unroll
-                  for (int i = 0; i < LB / 4; ++i) v[x][q][j * (LB / 4) + i] = 0;
-                }
-              }
-              if (!clean) {
-#pragma unroll
-                for (int i = 0; i < VW; ++i) v[x][q][i] = 0;
-              }
-            }
-#pragma unroll
-          for (int w = 0; w < VW; ++w) {
-            uint32_t v0[4], v1[4];
-            codes_across<FMT>(v[0][0][w], v[0][1][w], v0);
-            codes_across<FMT>(v[1][0][w], v[1][1][w], v1);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              mma16816(o[4 * w + i], pa[0], pa[1], pa[2], pa[3], v0[i], v1[i]);
-          }
-        }
+        // a step whose every token every live row sees takes the form without masks
+        const uint32_t absent = __ballot_sync(0xffffffffu, lane < GR && q_ks[0] < 0.f);
+        if (absent == 0 && t0 + Sh::kStep <= all_end) compute(std::false_type(), t0, absent);
+        else compute(std::true_type(), t0, absent);
       }
       // the step's bytes are in registers: its place in the ring takes the next copies
       __syncwarp();
@@ -565,13 +574,18 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
     }
 }
 
-// Joins the partial results of the segments that several warps shared, in the
-// order of the warps; the others are done already. One thread per 4 dims of a row.
+// Joins the partial results of the segments that several warps shared; the others
+// are done already. A thread takes 4 dims of a row, and every n-th partial result
+// where there are threads to spare; their sums meet in shared memory, always in
+// the same order.
+constexpr int kJoinThreads = 256;
+
 template <int HD>
-__global__ void __launch_bounds__(kThreads) kv_attention_join_kernel(KvAttentionArgs a, int row_blocks,
-                                                                     int warps) {
+__global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(KvAttentionArgs a,
+                                                                         int row_blocks, int warps) {
   using Sh = RowShape<HD>;
-  __shared__ int64_t s_sum[kWarps][2];
+  __shared__ int64_t s_sum[kJoinThreads / 32][2];
+  __shared__ float s_part[kJoinThreads][6];  // m, l, o
   pdl_trigger();
   pdl_wait();
   const KvView &c = a.c;
@@ -579,7 +593,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_join_kernel(KvAttention
   const int b = blockIdx.y;
   const int64_t hr = (int64_t)c.heads * row_blocks;
   int64_t before = 0, total = 0;
-  for (int i = tid; i < c.batch; i += kThreads) {
+  for (int i = tid; i < c.batch; i += kJoinThreads) {
     int len, count;
     const int n = units_of<HD>(a, i, len, count);
     total += n;
@@ -594,39 +608,61 @@ __global__ void __launch_bounds__(kThreads) kv_attention_join_kernel(KvAttention
   __syncthreads();
   before = total = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) before += s_sum[w][0], total += s_sum[w][1];
+  for (int w = 0; w < kJoinThreads / 32; ++w) before += s_sum[w][0], total += s_sum[w][1];
   int len, count;
   const int units = units_of<HD>(a, b, len, count);
   const int64_t run = (total * hr + warps - 1) / warps;
   const int64_t pair = blockIdx.x;
   const int64_t u0 = before * hr + pair * units, u1 = u0 + units;
-  const int64_t c0 = (u0 + Sh::kOver) / run, c1 = (u1 - 1) / run;
+  const int c0 = (int)((u0 + Sh::kOver) / run), c1 = (int)((u1 - 1) / run);
   if (c0 == c1) return;
   const int h = (int)(pair / row_blocks), rb = (int)(pair % row_blocks);
   const int rows_all = a.tokens * a.group, rows = min(kRows, rows_all - rb * kRows);
-  const int hd4 = c.hd / 4;
-  for (int i = tid; i < rows * hd4; i += kThreads) {
-    const int rr = i / hd4, d = i % hd4 * 4;
-    const int row = rb * kRows + rr, ti = row / a.group;
+  const int hd4 = c.hd / 4, items = rows * hd4;
+  // threads on one item: a power of two, so that their sums pair up
+  int team = 1;
+  while (2 * team * items <= kJoinThreads && team < c1 - c0 + 1) team *= 2;
+  for (int first = 0; first < items; first += kJoinThreads / team) {
+    const int i = first + tid / team, part = tid % team;
+    const bool in = i < items && tid < kJoinThreads / team * team;
+    const int rr = in ? i / hd4 : 0, d = in ? i % hd4 * 4 : 0;
     const float *const base = a.ws + rr * HD + d, *const ml = a.ws + kRows * HD + rr;
-    auto slot = [&](int64_t w) { return (w * 2 + (w == c0 ? 1 : 0)) * Sh::kSlot; };
-    float mm = -CUDART_INF_F;
-    for (int64_t k = c0; k <= c1; ++k) mm = fmaxf(mm, ml[slot(k)]);
-    float ll = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    auto slot = [&](int w) { return ((int64_t)w * 2 + (w == c0 ? 1 : 0)) * Sh::kSlot; };
+    float m = -CUDART_INF_F, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    // (m, l, o) += (mk, lk, v); a sum of NaN scores has m = -inf and a NaN l
+    auto add = [&](float mk, float lk, const float4 &v) {
+      const float mn = fmaxf(m, mk);
+      const float fo = m == mn || !(l == l) ? 1.f : exp2_approx(m - mn);
+      const float fk = mk == mn || !(lk == lk) ? 1.f : exp2_approx(mk - mn);
+      m = mn;
+      l = fmaf(l, fo, lk * fk);
+      o[0] = fmaf(o[0], fo, v.x * fk), o[1] = fmaf(o[1], fo, v.y * fk);
+      o[2] = fmaf(o[2], fo, v.z * fk), o[3] = fmaf(o[3], fo, v.w * fk);
+    };
+    if (in) {
 #pragma unroll 4
-    for (int64_t k = c0; k <= c1; ++k) {
-      const float mk = ml[slot(k)], lk = ml[slot(k) + kRows];
-      const float4 v = *reinterpret_cast<const float4 *>(base + slot(k));
-      // a warp whose scores are all NaN has m = -inf and a NaN sum
-      const float f = mk == mm || !(lk == lk) ? 1.f : exp2_approx(mk - mm);
-      ll = fmaf(lk, f, ll);
-      o[0] = fmaf(v.x, f, o[0]), o[1] = fmaf(v.y, f, o[1]);
-      o[2] = fmaf(v.z, f, o[2]), o[3] = fmaf(v.w, f, o[3]);
+      for (int k = c0 + part; k <= c1; k += team)
+        add(ml[slot(k)], ml[slot(k) + kRows], *reinterpret_cast<const float4 *>(base + slot(k)));
     }
-    const float inv = ti >= count || ll == 0.f ? 0.f : 1.f / ll;
+    if (team > 1) {
+      for (int step = team / 2; step > 0; step /= 2) {
+        float *mine = s_part[tid];
+        mine[0] = m, mine[1] = l, mine[2] = o[0], mine[3] = o[1], mine[4] = o[2], mine[5] = o[3];
+        __syncthreads();
+        if (part < step) {
+          const float *s = s_part[tid + step];
+          add(s[0], s[1], make_float4(s[2], s[3], s[4], s[5]));
+        }
+        __syncthreads();
+      }
+    }
+    if (in && part == 0) {
+      const int row = rb * kRows + rr, ti = row / a.group;
+      const float inv = ti >= count || l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) o[k] = inv == 0.f ? 0.f : o[k] * inv;
-    kv_store_out4(a.out, (((int64_t)b * a.tokens + ti) * a.heads + h * a.group + row % a.group) * c.hd + d, o);
+      for (int k = 0; k < 4; ++k) o[k] = inv == 0.f ? 0.f : o[k] * inv;
+      kv_store_out4(a.out, (((int64_t)b * a.tokens + ti) * a.heads + h * a.group + row % a.group) * c.hd + d, o);
+    }
   }
 }
 
@@ -670,7 +706,7 @@ int launch_rows(const KvAttentionArgs &a, cudaStream_t stream) {
                             p.whole));
   if (!p.whole)
     TT_CUDA_TRY(launch_kernel(kv_attention_join_kernel<HD>, dim3(p.row_blocks * a.c.heads, a.c.batch),
-                              dim3(kThreads), 0, stream, 1, a, p.row_blocks, p.ctas * kWarps));
+                              dim3(kJoinThreads), 0, stream, 1, a, p.row_blocks, p.ctas * kWarps));
   return TT_OK;
 }
 
