@@ -49,11 +49,12 @@ constexpr int kThreads = 32 * kWarps;
 
 template <int HD>
 struct RowShape {
-  static constexpr int kStep = HD == 32 ? 64 : HD == 64 ? 32 : 16;  // tokens per warp step
-  static constexpr int GR = kStep / 16;              // groups of 16 tokens, each in one page
-  static constexpr int kOver = 2;                    // units of a segment besides its steps
-  static constexpr int kWhole = 4;                   // steps of a segment that is never split
-  static constexpr int kStages = HD == 256 ? 2 : 3;  // steps in a warp's ring
+  static constexpr int GC = HD == 32 ? 4 : HD == 64 ? 2 : 1;  // groups of 16 tokens computed at once
+  static constexpr int GR = HD <= 64 ? 2 * GC : GC;   // ... and copied at once: a step
+  static constexpr int kStep = 16 * GR;              // tokens
+  static constexpr int kOver = HD <= 64 ? 1 : 2;     // units of a segment besides its steps
+  static constexpr int kWhole = HD <= 64 ? 2 : 4;                   // steps of a segment that is never split
+  static constexpr int kStages = HD == 128 ? 3 : 2;  // steps in a warp's ring
   static constexpr uint32_t kStage = 2 * kStep * HD;  // bytes: keys, then values
   // shared memory: the rings, the warps' results, barriers
   static constexpr uint32_t kO = kWarps * kStages * kStage;
@@ -193,7 +194,7 @@ template <int HD, int FMT, bool EXACT>
 __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
     kv_attention_rows_kernel(KvAttentionArgs a, int row_blocks, bool whole) {
   using Sh = RowShape<HD>;
-  constexpr int KW = Sh::KW, VW = Sh::VW, GR = Sh::GR, S = Sh::kStages;
+  constexpr int KW = Sh::KW, VW = Sh::VW, GR = Sh::GR, GC = Sh::GC, S = Sh::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int64_t s_scan[kThreads];
   pdl_trigger();
@@ -383,16 +384,17 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
       beta = 1.f;
     };
 
-    // one step: scores, running maximum, p, p v
-    auto compute = [&](auto masked_form, int t0, uint32_t absent) {
+    // groups g0 .. g0 + GC - 1 of a step, the first at token t0: scores, running
+    // maximum, p, p v
+    auto compute = [&](auto masked_form, int g0, int t0, uint32_t absent) {
       constexpr bool MASKED = decltype(masked_form)::value;
-      const uint32_t kb = ring + stage * Sh::kStage, vb = kb + Sh::kStep * hd;
-      float s[GR][2][4];
+      const uint32_t kb = ring + stage * Sh::kStage + 16 * g0 * hd, vb = kb + Sh::kStep * hd;
+      float s[GC][2][4];
       {
         constexpr int LB = HD == 32 ? 8 : 16;  // bytes a load
-        uint32_t w[GR][2][KW];
+        uint32_t w[GC][2][KW];
 #pragma unroll
-        for (int g = 0; g < GR; ++g)
+        for (int g = 0; g < GC; ++g)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const uint32_t row = kb + (16 * g + 8 * x + half_token(gid)) * hd;
@@ -410,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
 #pragma unroll
         for (int i = 0; i < KW; ++i)
 #pragma unroll
-          for (int g = 0; g < GR; ++g)
+          for (int g = 0; g < GC; ++g)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               uint32_t k0, k1;
@@ -422,13 +424,13 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
       // scores of this thread: row gid, tokens 8 x + half_token(2 tig + p) of group g
       const float ve_lane = q_vs[0] == q_vs[0] ? (float)((__float_as_int(q_vs[0]) >> 23) - 127) : q_vs[0];
       auto sees = [&](int g, int x, int p) {
-        return !((absent >> g) & 1u) && t0 + 16 * g + 8 * x + half_token(2 * tig + p) < end;
+        return !((absent >> (g0 + g)) & 1u) && t0 + 16 * g + 8 * x + half_token(2 * tig + p) < end;
       };
-      float kc[GR], ve[GR], top = -CUDART_INF_F;
+      float kc[GC], ve[GC], top = -CUDART_INF_F;
 #pragma unroll
-      for (int g = 0; g < GR; ++g) {
-        ve[g] = __shfl_sync(0xffffffffu, ve_lane, g);
-        kc[g] = fabsf(__shfl_sync(0xffffffffu, q_ks[0], g)) * sc;  // never negative: it meets -inf
+      for (int g = 0; g < GC; ++g) {
+        ve[g] = __shfl_sync(0xffffffffu, ve_lane, g0 + g);
+        kc[g] = fabsf(__shfl_sync(0xffffffffu, q_ks[0], g0 + g)) * sc;  // never negative: it meets -inf
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -455,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
       }
       const float ref = 14.f - (m == -CUDART_INF_F ? 0.f : m);
 #pragma unroll
-      for (int g = 0; g < GR; ++g) {
+      for (int g = 0; g < GC; ++g) {
         uint32_t v[2][2][VW];
         constexpr int LB = VW >= 4 ? 16 : 4 * VW;  // bytes a load
 #pragma unroll
@@ -475,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
               }
             }
             // what stands behind the last token may be any bits, e4m3's NaN among them
-            if (MASKED && FMT == TT_KV_E4M3 && (((absent >> g) & 1u) || t0 + 16 * g + in_g >= len)) {
+            if (MASKED && FMT == TT_KV_E4M3 && (((absent >> (g0 + g)) & 1u) || t0 + 16 * g + in_g >= len)) {
 #pragma unroll
               for (int i = 0; i < VW; ++i) v[x][q][i] = 0;
             }
@@ -520,10 +522,15 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
       }
       if (alive) alive = __all_sync(0xffffffffu, mbar_wait(bars + 8 * stage, phase, c.status));
       if (alive && t0 < any_end) {  // the same for the whole warp
-        // a step whose every token every live row sees takes the form without masks
         const uint32_t absent = __ballot_sync(0xffffffffu, lane < GR && q_ks[0] < 0.f);
-        if (absent == 0 && t0 + Sh::kStep <= all_end) compute(std::false_type(), t0, absent);
-        else compute(std::true_type(), t0, absent);
+#pragma unroll 1
+        for (int g0 = 0; g0 < GR; g0 += GC) {
+          const int tg = t0 + 16 * g0;
+          if (tg >= any_end) break;
+          // where every live row sees every token, the form without masks
+          if (absent == 0 && tg + 16 * GC <= all_end) compute(std::false_type(), g0, tg, absent);
+          else compute(std::true_type(), g0, tg, absent);
+        }
       }
       // the step's bytes are in registers: its place in the ring takes the next copies
       __syncwarp();
