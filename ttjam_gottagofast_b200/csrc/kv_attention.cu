@@ -19,13 +19,13 @@
 // largest element in [1, 2), p by 2^14 to stay clear of the fp16 subnormals.
 //
 // A warp takes kStep tokens at a time from a ring of its own in shared memory,
-// which its lanes fill with bulk copies (16 tokens of a page and head are
-// consecutive bytes) up to kStages steps ahead, over the borders of heads and
-// sequences, so that a warp always has its next copies in flight. Bytes go from
-// there straight into operand registers: the tokens and head dims are numbered
-// within a step so that a thread's operand elements are consecutive bytes (which
-// token or dim stands at which operand index is free as long as both operands
-// agree) and so that few of a warp's loads share banks.
+// which its lanes fill with asynchronous 16-byte copies up to kStages steps ahead,
+// over the borders of heads and sequences, so that a warp always has its next
+// copies in flight and never waits for another warp. Bytes go from there straight
+// into operand registers: the tokens and head dims are numbered within a step so
+// that a thread's operand elements are consecutive bytes (which token or dim stands
+// at which operand index is free as long as both operands agree), and 16-byte
+// chunks are exchanged within a row so that a load's rows lie in different banks.
 //
 // Work is counted in units: kStep tokens of one (sequence, key head, row block), and
 // kOver units for each such segment, as its start and end cost about that much
@@ -56,10 +56,9 @@ struct RowShape {
   static constexpr int kWhole = HD <= 64 ? 2 : 4;                   // steps of a segment that is never split
   static constexpr int kStages = HD == 128 ? 3 : 2;  // steps in a warp's ring
   static constexpr uint32_t kStage = 2 * kStep * HD;  // bytes: keys, then values
-  // shared memory: the rings, the warps' results, barriers
+  // shared memory: the rings, the flushed sums
   static constexpr uint32_t kO = kWarps * kStages * kStage;
-  static constexpr uint32_t kBars = kO + kWarps * kRows * HD * 4;
-  static constexpr uint32_t kSmem = kBars + 8 * kWarps * kStages;
+  static constexpr uint32_t kSmem = kO + kWarps * kRows * HD * 4;
   static constexpr int kCtas = HD == 256 ? 2 : 3;    // per SM, as registers and shared memory allow
   // tensor cores add by rounding toward zero: after 1024 tokens the sum moves to
   // shared memory, so that it does not drift
@@ -72,38 +71,13 @@ struct RowShape {
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
-__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return done != 0;
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-// Bounded wait: false after about 2^28 cycles, latching TT_ERR_DEVICE_TIMEOUT.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, DeviceStatus *st) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64();
-  for (uint32_t i = 1;; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 31) == 0 && clock64() - t0 > (1LL << 28)) {
-      raise_status(st, TT_ERR_DEVICE_TIMEOUT, 0x6900);
-      return false;
-    }
-  }
-}
-__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-               : "memory");
-}
-__device__ __forceinline__ void bulk_copy(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-      "l"(src), "r"(bytes), "r"(bar)
-      : "memory");
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 template <int BYTES>
 __device__ __forceinline__ void lds(uint32_t addr, uint32_t *r) {
@@ -139,11 +113,19 @@ __device__ __forceinline__ int units_of(const KvAttentionArgs &a, int b, int &le
   return Sh::kOver + (count > 0 ? (len + Sh::kStep - 1) / Sh::kStep : 1);
 }
 
-// Token (0-7) of operand column n of an 8-token half: such that two neighbouring
-// columns are an odd number of rows apart, and four alternate ones two and two.
+// Token (0-7) of operand column n of an 8-token half, and the swizzle of a row's
+// 16-byte chunks (chunk c of row r stands at c ^ chunk_swizzle(r)): together they
+// put the 8 lanes that load K in one cycle (2 rows, 4 chunks) and those that load
+// V (4 rows, at one or two chunks) into different banks, at every width.
+template <int HD>
 __device__ __forceinline__ int half_token(int n) {
-  const int r = ((n >> 1) & 1) + 4 * (n >> 2);
-  return n & 1 ? r ^ 3 : r;
+  const int t = n >> 1;
+  return n & 1 ? 4 + (t ^ (HD == 64 ? 1 : 2)) : t;
+}
+template <int HD, bool EXACT>
+__device__ __forceinline__ int chunk_swizzle(int row) {
+  if constexpr (!EXACT || HD == 32) return 0;
+  return HD == 64 ? row & 2 : (row & 3) << 1;
 }
 
 // Where a warp's run of units stands: unit t of the segment whose units [lo, hi)
@@ -205,11 +187,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
   const int64_t hr = (int64_t)c.heads * row_blocks;  // (key head, row block) pairs
   const int rows_all = a.tokens * a.group;           // query rows of a key head
   const uint32_t ring = smem_u32(smem) + warp * S * Sh::kStage;
-  const uint32_t bars = smem_u32(smem) + Sh::kBars + 8 * warp * S;
   float *const s_o = reinterpret_cast<float *>(smem + Sh::kO) + warp * kRows * HD;  // [kRows][HD]
-  if (lane < S)
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bars + 8 * lane), "r"(GR) : "memory");
-  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   pdl_wait();
 
   // the warp's run of units, and the sequence that holds its first
@@ -267,10 +245,10 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
   auto t0_of = [&](int t) { return (t - Sh::kOver) * Sh::kStep; };
 
   // ---- the copies -----------------------------------------------------------
-  // Lane g < GR copies group g's keys and values; its page is looked up one step
-  // before, its scales wait in the lane's queue for as long as the bytes do in the
-  // ring. A group without a page, or past the last seen token, copies nothing and
-  // has the key scale -1.
+  // Lane g < GR looks group g's page up one step before its bytes are copied; its
+  // scales wait in the lane's queue for as long as the bytes do in the ring. A
+  // group without a page, or past the last seen token, copies nothing and has the
+  // key scale -1.
   Cursor<HD> fill = use;
   bool more = true;
   int fill_end = seen_by_block(fill), fill_stage = 0, pg_next;
@@ -279,22 +257,38 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
     const int t0 = t0_of(fill.t) + 16 * lane;
     pg_next = lane < GR && t0 < fill_end ? c.page_of(fill.b, t0 >> c.page_log2) : -1;
   };
+  // where this lane's 16 bytes of every 512 of a group go
+  constexpr int kCopies = HD / 32;  // of 512 bytes, in a group of full width
+  uint32_t copy_at[EXACT && HD > 64 ? 2 : 1];
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(copy_at) / 4); ++i) {
+    const int at = 32 * i + lane, row = EXACT ? at / (HD / 16) : 0, ch = EXACT ? at % (HD / 16) : at;
+    copy_at[i] = ring + row * HD + ((ch ^ chunk_swizzle<HD, EXACT>(row)) << 4);
+  }
   auto issue = [&](float &ks, float &vs) {
-    const uint32_t bar = bars + 8 * fill_stage;
     ks = -1.f;
     vs = 1.f;
-    if (lane < GR) {
-      const uint32_t bytes = 16 * hd;
-      mbar_expect(bar, pg_next >= 0 ? 2 * bytes : 0);
-      if (pg_next >= 0) {
-        const int h = fill.pair / row_blocks;
-        const int t0 = t0_of(fill.t) + 16 * lane;
-        const int64_t at = c.tile(pg_next, h) + (int64_t)(t0 & ((1 << c.page_log2) - 1)) * hd;
-        const uint32_t dst = ring + fill_stage * Sh::kStage + lane * bytes;
-        bulk_copy(dst, c.k + at, bytes, bar);
-        bulk_copy(dst + Sh::kStep * hd, c.v + at, bytes, bar);
-        ks = c.ks[(int64_t)pg_next * c.heads + h];
-        vs = c.vs[(int64_t)pg_next * c.heads + h];
+    const int h = fill.pair / row_blocks;
+    if (pg_next >= 0) {  // lanes 0 .. GR - 1
+      const uint32_t at = (uint32_t)pg_next * (uint32_t)c.heads + (uint32_t)h;
+      ks = c.ks[at];
+      vs = c.vs[at];
+    }
+    const int t0 = t0_of(fill.t);
+#pragma unroll
+    for (int g = 0; g < GR; ++g) {
+      const int pg = __shfl_sync(0xffffffffu, pg_next, g);
+      if (pg < 0) continue;
+      const int64_t from = c.tile(pg, h) + ((t0 + 16 * g) & ((1 << c.page_log2) - 1)) * hd + 16 * lane;
+      const uint32_t to = fill_stage * Sh::kStage + 16 * g * hd;
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        // rows of 128 bytes and more: the swizzle of every other copy's rows differs
+        const uint32_t dst = EXACT && HD > 64 ? copy_at[i & 1] + (i >> 1) * 1024 + to : copy_at[0] + i * 512 + to;
+        if (EXACT || 512 * i + 16 * lane < 16 * hd) {
+          copy16(dst, c.k + from + 512 * i);
+          copy16(dst + Sh::kStep * hd, c.v + from + 512 * i);
+        }
       }
     }
     fill_stage = fill_stage + 1 == S ? 0 : fill_stage + 1;
@@ -309,10 +303,9 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
   for (int s = 0; s < S; ++s) {
     q_ks[s] = -1.f, q_vs[s] = 1.f;
     if (more) issue(q_ks[s], q_vs[s]);
+    copies_commit();
   }
   int stage = 0;
-  uint32_t phase = 0;
-  bool alive = true;  // false once a wait gave up: the rest of the run computes nothing
 
   bool going = true;
   while (going) {
@@ -388,7 +381,8 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
     // maximum, p, p v
     auto compute = [&](auto masked_form, int g0, int t0, uint32_t absent) {
       constexpr bool MASKED = decltype(masked_form)::value;
-      const uint32_t kb = ring + stage * Sh::kStage + 16 * g0 * hd, vb = kb + Sh::kStep * hd;
+      const uint32_t kb = ring + stage * Sh::kStage + 16 * g0 * hd;
+      const uint32_t vb = kb + Sh::kStep * hd;
       float s[GC][2][4];
       {
         constexpr int LB = HD == 32 ? 8 : 16;  // bytes a load
@@ -397,12 +391,13 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
         for (int g = 0; g < GC; ++g)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const uint32_t row = kb + (16 * g + 8 * x + half_token(gid)) * hd;
+            const int r8 = half_token<HD>(gid);
+            const uint32_t row = kb + (16 * g + 8 * x + r8) * hd;
 #pragma unroll
             for (int j = 0; j < KW * 4 / LB; ++j) {
               const int d = 4 * LB * j + LB * tig;
               if (EXACT || d < hd) {
-                lds<LB>(row + d, &w[g][x][j * (LB / 4)]);
+                lds<LB>(row + (d ^ (chunk_swizzle<HD, EXACT>(r8) << 4)), &w[g][x][j * (LB / 4)]);
               } else {
 #pragma unroll
                 for (int i = 0; i < LB / 4; ++i) w[g][x][j * (LB / 4) + i] = 0;
@@ -424,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
       // scores of this thread: row gid, tokens 8 x + half_token(2 tig + p) of group g
       const float ve_lane = q_vs[0] == q_vs[0] ? (float)((__float_as_int(q_vs[0]) >> 23) - 127) : q_vs[0];
       auto sees = [&](int g, int x, int p) {
-        return !((absent >> (g0 + g)) & 1u) && t0 + 16 * g + 8 * x + half_token(2 * tig + p) < end;
+        return !((absent >> (g0 + g)) & 1u) && t0 + 16 * g + 8 * x + half_token<HD>(2 * tig + p) < end;
       };
       float kc[GC], ve[GC], top = -CUDART_INF_F;
 #pragma unroll
@@ -464,13 +459,13 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
         for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            const int in_g = 8 * x + half_token(2 * tig + q);
+            const int in_g = 8 * x + half_token<HD>(2 * tig + q);
             const uint32_t row = vb + (16 * g + in_g) * hd;
 #pragma unroll
             for (int j = 0; j < VW * 4 / LB; ++j) {
               const int d = 8 * LB * j + LB * gid;
               if (EXACT || d < hd) {
-                lds<LB>(row + d, &v[x][q][j * (LB / 4)]);
+                lds<LB>(row + (d ^ (chunk_swizzle<HD, EXACT>(in_g & 7) << 4)), &v[x][q][j * (LB / 4)]);
               } else {
 #pragma unroll
                 for (int i = 0; i < LB / 4; ++i) v[x][q][j * (LB / 4) + i] = 0;
@@ -520,8 +515,9 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
 #pragma unroll
           for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
       }
-      if (alive) alive = __all_sync(0xffffffffu, mbar_wait(bars + 8 * stage, phase, c.status));
-      if (alive && t0 < any_end) {  // the same for the whole warp
+      copies_wait<S - 1>();
+      __syncwarp();
+      if (t0 < any_end) {  // the same for the whole warp
         const uint32_t absent = __ballot_sync(0xffffffffu, lane < GR && q_ks[0] < 0.f);
 #pragma unroll 1
         for (int g0 = 0; g0 < GR; g0 += GC) {
@@ -535,10 +531,10 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
       // the step's bytes are in registers: its place in the ring takes the next copies
       __syncwarp();
       stage = stage + 1 == S ? 0 : stage + 1;
-      phase ^= stage == 0;
 #pragma unroll
       for (int i = 0; i + 1 < S; ++i) q_ks[i] = q_ks[i + 1], q_vs[i] = q_vs[i + 1];
-      if (more && alive) issue(q_ks[S - 1], q_vs[S - 1]);
+      if (more) issue(q_ks[S - 1], q_vs[S - 1]);
+      copies_commit();
     }
 
     // the row's result: its output, or a partial one
@@ -572,20 +568,13 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
     }
     going = use.next(a, hr, whole) && use.to_step(a, hr, whole);
   }
-  // after a wait that gave up: the copies still in flight, waited for (bounded)
-  if (!alive)
-    for (int s = 0; s < S; ++s) {
-      mbar_wait(bars + 8 * stage, phase, nullptr);
-      stage = stage + 1 == S ? 0 : stage + 1;
-      phase ^= stage == 0;
-    }
 }
 
 // Joins the partial results of the segments that several warps shared; the others
 // are done already. A thread takes 4 dims of a row, and every n-th partial result
 // where there are threads to spare; their sums meet in shared memory, always in
 // the same order.
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256, kJoinItems = 64;
 
 template <int HD>
 __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(KvAttentionArgs a,
@@ -625,11 +614,14 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(KvAtten
   if (c0 == c1) return;
   const int h = (int)(pair / row_blocks), rb = (int)(pair % row_blocks);
   const int rows_all = a.tokens * a.group, rows = min(kRows, rows_all - rb * kRows);
-  const int hd4 = c.hd / 4, items = rows * hd4;
-  // threads on one item: a power of two, so that their sums pair up
+  // this block's items, and the threads on one: a power of two, so that their sums
+  // pair up
+  const int hd4 = c.hd / 4, begin = blockIdx.z * kJoinItems;
+  const int items = min(rows * hd4, begin + kJoinItems);
+  if (begin >= items) return;
   int team = 1;
-  while (2 * team * items <= kJoinThreads && team < c1 - c0 + 1) team *= 2;
-  for (int first = 0; first < items; first += kJoinThreads / team) {
+  while (2 * team * (items - begin) <= kJoinThreads && team < c1 - c0 + 1) team *= 2;
+  for (int first = begin; first < items; first += kJoinThreads / team) {
     const int i = first + tid / team, part = tid % team;
     const bool in = i < items && tid < kJoinThreads / team * team;
     const int rr = in ? i / hd4 : 0, d = in ? i % hd4 * 4 : 0;
@@ -712,7 +704,9 @@ int launch_rows(const KvAttentionArgs &a, cudaStream_t stream) {
   TT_CUDA_TRY(launch_kernel(kern, dim3(p.ctas), dim3(kThreads), Sh::kSmem, stream, 1, a, p.row_blocks,
                             p.whole));
   if (!p.whole)
-    TT_CUDA_TRY(launch_kernel(kv_attention_join_kernel<HD>, dim3(p.row_blocks * a.c.heads, a.c.batch),
+    TT_CUDA_TRY(launch_kernel(kv_attention_join_kernel<HD>,
+                              dim3(p.row_blocks * a.c.heads, a.c.batch,
+                                   (unsigned)ceil_div(std::min(kRows, a.tokens * a.group) * (a.c.hd / 4), kJoinItems)),
                               dim3(kJoinThreads), 0, stream, 1, a, p.row_blocks, p.ctas * kWarps));
   return TT_OK;
 }
