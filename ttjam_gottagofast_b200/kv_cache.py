@@ -120,7 +120,10 @@ class KVCache:
         self._longest = None  # an upper bound on lengths known to the host, or None
         self._status = torch.zeros(2, dtype=torch.int32, device=k.device)
         self._lib = _lib.load()
-        self._ws_bytes = {}
+        self._c_write, self._c_read = self._lib.tt_kv_write, self._lib.tt_kv_read
+        self._c_attend = self._lib.tt_kv_attention
+        self._index, self._scale = k.device.index, hd ** -0.5
+        self._plans = {}
         self._array = (_lib.TTKVCache * layers)()  # one entry a layer
         self._structs = [ctypes.pointer(c) for c in self._array]
         for i, c in enumerate(self._array):
@@ -163,6 +166,9 @@ class KVCache:
         self._longest = None
 
     # ---- the operators ------------------------------------------------------
+    # What a call's shapes, strides and types decide (its checks, the constant
+    # arguments of the C call) is worked out once and kept under those; a step's
+    # call then costs little more than its launches.
     def write(self, k: torch.Tensor, v: torch.Tensor, new_tokens: Optional[torch.Tensor] = None,
               layer: int = 0) -> None:
         """Quantise the keys and values of new tokens into layer `layer`: k and
@@ -170,16 +176,28 @@ class KVCache:
         (any strides with head_dim contiguous). new_tokens, [batch] int32, says
         how many leading rows of each sequence are new tokens (default: all);
         `lengths` counts them already."""
-        for name, t in (("k", k), ("v", v)):
-            self._check(t, name, self.kv_heads)
-        if k.shape != v.shape or k.dtype != v.dtype:
-            raise ValueError(f"k and v must agree in shape and type, got {tuple(k.shape)} "
-                             f"{k.dtype} and {tuple(v.shape)} {v.dtype}")
-        k, v = self._rows(k), self._rows(v)
-        counts = self._counts(new_tokens)
-        self._call("tt_kv_write", layer, _dtype_code(k, "k"), k.data_ptr(), v.data_ptr(),
-                   _strides(k), _strides(v), k.shape[1],
-                   None if counts is None else counts.data_ptr())
+        key = (layer, k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(), v.dtype,
+               v.get_device())
+        plan = self._plans.get(key)
+        if plan is None:
+            for name, t in (("k", k), ("v", v)):
+                self._check(t, name, self.kv_heads)
+            if k.shape != v.shape or k.dtype != v.dtype:
+                raise ValueError(f"k and v must agree in shape and type, got {tuple(k.shape)} "
+                                 f"{k.dtype} and {tuple(v.shape)} {v.dtype}")
+            if k.stride(3) != 1 or v.stride(3) != 1:
+                return self.write(k.contiguous(), v.contiguous(), new_tokens, layer)
+            plan = self._keep(key, (self._struct(layer), _dtype_code(k, "k"), _strides(k),
+                                    _strides(v), k.shape[1]))
+        struct, dtype, ks, vs, n = plan
+        counts = None if new_tokens is None else self._counts(new_tokens)
+        if _current_device() != self._index:
+            with torch.cuda.device(self.device):
+                return self.write(k, v, new_tokens, layer)
+        rc = self._c_write(struct, dtype, k.data_ptr(), v.data_ptr(), ks, vs, n,
+                           None if counts is None else counts.data_ptr(), _raw_stream(self._index))
+        if rc != 0:
+            _lib.check(rc, "tt_kv_write", self._lib)
 
     def read(self, dtype: torch.dtype = torch.float32, max_tokens: Optional[int] = None,
              layer: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -189,9 +207,17 @@ class KVCache:
         n = self.max_tokens if max_tokens is None else max_tokens
         if n < 0:
             raise ValueError("max_tokens must be >= 0")
+        struct = self._struct(layer)
         shape = (self.batch, n, self.kv_heads, self.head_dim)
-        k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
-        self._call("tt_kv_read", layer, _dtype_code(k, "dtype"), k.data_ptr(), v.data_ptr(), n)
+        k = torch.empty(shape, dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
+        if _current_device() != self._index:
+            with torch.cuda.device(self.device):
+                return self.read(dtype, max_tokens, layer)
+        rc = self._c_read(struct, _dtype_code(k, "dtype"), k.data_ptr(), v.data_ptr(), n,
+                          _raw_stream(self._index))
+        if rc != 0:
+            _lib.check(rc, "tt_kv_read", self._lib)
         return k, v
 
     def attend(self, q: torch.Tensor, new_tokens: Optional[torch.Tensor] = None, layer: int = 0,
@@ -203,29 +229,39 @@ class KVCache:
         position lengths[b] - new_tokens[b] + i and sees the tokens up to its
         own. `scale` (default head_dim ** -0.5) multiplies the scores. Returns
         (or writes to `out`, contiguous) [batch, tokens, heads, head_dim] of
-        q's type, computed to fp32 accuracy; rows behind new_tokens[b] are 0."""
-        if q.dim() != 4 or q.shape[2] % self.kv_heads or q.shape[2] == 0:
-            raise ValueError(f"q must be [batch, tokens, heads, head_dim] with heads a multiple of "
-                             f"{self.kv_heads}, got {tuple(q.shape)}")
-        self._check(q, "q", q.shape[2])
-        q = self._rows(q)
-        n, heads = q.shape[1], q.shape[2]
+        q's type, computed to fp32 accuracy (float16 and bfloat16 prompts may
+        round the probabilities to 11 bits); rows behind new_tokens[b] are 0."""
+        key = (layer, q.shape, q.stride(), q.dtype, q.get_device())
+        plan = self._plans.get(key)
+        if plan is None:
+            if q.dim() != 4 or q.shape[2] % self.kv_heads or q.shape[2] == 0:
+                raise ValueError(f"q must be [batch, tokens, heads, head_dim] with heads a multiple "
+                                 f"of {self.kv_heads}, got {tuple(q.shape)}")
+            self._check(q, "q", q.shape[2])
+            if q.stride(3) != 1:
+                return self.attend(q.contiguous(), new_tokens, layer, scale, out)
+            with torch.cuda.device(self.device):
+                nbytes = self._lib.tt_kv_attention_workspace_bytes(self._structs[0], q.shape[1],
+                                                                   q.shape[2])
+            plan = self._keep(key, (self._struct(layer), _dtype_code(q, "q"), _strides(q),
+                                    q.shape[1], q.shape[2], nbytes))
+        struct, dtype, strides, n, heads, nbytes = plan
+        counts = None if new_tokens is None else self._counts(new_tokens)
+        if _current_device() != self._index:
+            with torch.cuda.device(self.device):
+                return self.attend(q, new_tokens, layer, scale, out)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = q.new_empty(q.shape)
         elif (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device
               or not out.is_contiguous()):
             raise ValueError("out must be a contiguous tensor of q's shape, type and device")
-        counts = self._counts(new_tokens)
-        scale = self.head_dim ** -0.5 if scale is None else float(scale)
-        nbytes = self._ws_bytes.get((n, heads))
-        if nbytes is None:
-            with torch.cuda.device(self.device):
-                nbytes = self._lib.tt_kv_attention_workspace_bytes(self._structs[0], n, heads)
-            self._ws_bytes[(n, heads)] = nbytes
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        self._call("tt_kv_attention", layer, _dtype_code(q, "q"), q.data_ptr(), _strides(q), n,
-                   heads, None if counts is None else counts.data_ptr(), scale, out.data_ptr(),
-                   None if ws is None else ws.data_ptr(), nbytes)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+        rc = self._c_attend(struct, dtype, q.data_ptr(), strides, n, heads,
+                            None if counts is None else counts.data_ptr(),
+                            self._scale if scale is None else scale, out.data_ptr(),
+                            None if ws is None else ws.data_ptr(), nbytes, _raw_stream(self._index))
+        if rc != 0:
+            _lib.check(rc, "tt_kv_attention", self._lib)
         return out
 
     def read_device_status(self) -> Tuple[int, int]:
@@ -249,32 +285,40 @@ class KVCache:
             raise ValueError(f"{name} must be [{self.batch}, tokens, {heads}, {self.head_dim}], "
                              f"got {tuple(t.shape)}")
 
-    @staticmethod
-    def _rows(t: torch.Tensor) -> torch.Tensor:
-        return t if t.stride(3) == 1 else t.contiguous()
+    def _struct(self, layer: int):
+        if not 0 <= layer < self.num_layers:
+            raise ValueError(f"layer must be in [0, {self.num_layers}), got {layer}")
+        return self._structs[layer]
+
+    def _keep(self, key, plan):
+        if len(self._plans) >= 1024:  # prompts of ever new lengths
+            self._plans.clear()
+        self._plans[key] = plan
+        return plan
 
     def _counts(self, new_tokens: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
         if new_tokens is None:
             return None
         if (new_tokens.shape != (self.batch,) or new_tokens.dtype != torch.int32
-                or new_tokens.device != self.device):
+                or new_tokens.get_device() != self._index):
             raise ValueError(f"new_tokens must be an int32 tensor of shape ({self.batch},) on "
                              f"{self.device}, got {new_tokens.dtype} of "
                              f"{tuple(new_tokens.shape)} on {new_tokens.device}")
-        return new_tokens.contiguous()
-
-    def _call(self, name: str, layer: int, *args) -> None:
-        if not 0 <= layer < self.num_layers:
-            raise ValueError(f"layer must be in [0, {self.num_layers}), got {layer}")
-        if self.device.index != torch.cuda.current_device():
-            with torch.cuda.device(self.device):
-                return self._call(name, layer, *args)
-        stream = torch.cuda.current_stream(self.device).cuda_stream
-        rc = getattr(self._lib, name)(self._structs[layer], *args, stream)
-        if rc != 0:
-            _lib.check(rc, name, self._lib)
+        return new_tokens if new_tokens.is_contiguous() else new_tokens.contiguous()
 
 
 def _strides(t: torch.Tensor):
     s = t.stride()
     return (ctypes.c_int64 * 3)(s[0], s[1], s[2])
+
+
+# The current device and stream without the Python objects that torch.cuda makes
+# of them, where this torch has the functions behind it.
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _stream_of(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or _stream_of
