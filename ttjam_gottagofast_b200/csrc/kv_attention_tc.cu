@@ -21,7 +21,7 @@
 //             stored as 128-byte-swizzled rows of 64 dims, K-major for K and, the
 //             same bytes read the other way, MN-major for V; one tile ahead in
 //             registers. The tile's scales go to shared memory.
-//   1 warp    allocates tensor memory; its lane 0 issues the MMAs: S_x = q_x K^T,
+//   1 warp (of a fourth group) allocates tensor memory; its lane 0 issues the MMAs: S_x = q_x K^T,
 //             O_x += P_x V (A = P from tensor memory), the tiles in turn, so that
 //             one's softmax runs under the other's products.
 // K and V tiles share a ring of NS slots (K_0 V_0 K_1 ...). Every wait is bounded;
@@ -54,7 +54,13 @@ struct TcShape {
   static constexpr uint32_t BARS = QBYTES + NS * SLOT;  // barriers, after the operands
   static constexpr size_t SMEM = BARS + 1024 + 1024;    // alignment of the base, barriers
   static constexpr int SOFT_WARPS = 4 * MT;
-  static constexpr int THREADS = 32 * (SOFT_WARPS + kConvWarps + 1);
+  // warpgroups: softmax (MT), conversion, MMA issue (one warp of it). With two
+  // softmax groups the block starts with 128 registers a thread, and they take
+  // 176 (152), which the other two give up: 2 * 176 + 2 * 80 = 4 * 128.
+  static constexpr int THREADS = 32 * (SOFT_WARPS + kConvWarps + 4);
+  static constexpr bool SHIFT_REGS = MT == 2;
+  static constexpr int SOFT_REGS = HD == 64 ? 176 : 152, OTHER_REGS = HD == 64 ? 80 : 104;
+  static_assert(!SHIFT_REGS || 2 * SOFT_REGS + 2 * OTHER_REGS <= 4 * 128, "registers of the block");
   // tensor-memory columns
   static constexpr uint32_t T_O = 0, T_S = MT * HD, T_Q = MT * (HD + TOK);
   static_assert(T_Q + (QT ? MT * PIECES * HD / 2 : 0) <= 512, "tensor memory");
@@ -195,11 +201,27 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
   return r;
 }
-__device__ __forceinline__ float widen_nonneg(uint32_t h16) {
-  // an fp16's bits under the fp32 exponent are its value * 2^-112 (subnormals too)
-  float r;
-  asm("mul.rn.f32 %0, %1, 0f77800000;" : "=f"(r) : "f"(__uint_as_float(h16 << 13)));
-  return r;
+// Pairs of fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+// The upper 11 significant bits, exact in fp16 from 2^-14 on; below that, rounded
+// there to a multiple of 2^-24.
+__device__ __forceinline__ float upper11(float x) {
+  return __uint_as_float(__float_as_uint(x) & 0xffffe000u);
 }
 
 template <int HD, int FMT, int PIECES>
@@ -282,7 +304,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
     *abort_w = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  constexpr int kMmaWarp = Sh::SOFT_WARPS + kConvWarps;
+  constexpr int kMmaWarp = Sh::SOFT_WARPS + kConvWarps;  // the rest of its group only waits
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tmem_slot)
                  : "memory");
@@ -292,9 +314,15 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
   __syncthreads();
   fence_after();
   const uint32_t tm = *tmem_slot_p;
+  if constexpr (Sh::SHIFT_REGS) {
+    if (warp < Sh::SOFT_WARPS)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Sh::SOFT_REGS));
+    else
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::OTHER_REGS));
+  }
 
-  if (warp == kMmaWarp) {
-    if (lane == 0) {
+  if (warp >= kMmaWarp) {
+    if (warp == kMmaWarp && lane == 0) {
       // ---- MMA issuer ------------------------------------------------------
       auto slot_addr = [&](int i) { return base + Sh::QBYTES + (uint32_t)(i % NS) * Sh::SLOT; };
       auto wait_slot = [&](int i) {
@@ -364,7 +392,11 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
     __syncwarp();
   } else if (warp >= Sh::SOFT_WARPS) {
     // ---- conversion of the codes -------------------------------------------
-    constexpr int NCH = Sh::NCH, CPR = HD / 16;  // chunks per thread, per token
+    // chunk i: four of 16 codes in a row's 64 dims, then the next token, then the
+    // next box, so that eight lanes' stores of 16 bytes meet different banks
+    constexpr int NCH = Sh::NCH;
+    auto chunk_token = [&](int i) { return (i / 4) % TOK; };
+    auto chunk_dim = [&](int i) { return i / (4 * TOK) * 64 + (i % 4) * 16; };
     const int ct = threadIdx.x - 32 * Sh::SOFT_WARPS;
     const int cw = warp - Sh::SOFT_WARPS;
     auto pages_of = [&](int j) {  // lane g < GROUPS: the page of group g
@@ -375,7 +407,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
     auto load = [&](const uint8_t *pool, int ids, int j, uint4 *r) {
 #pragma unroll
       for (int u = 0; u < NCH; ++u) {
-        const int i = u * kConvThreads + ct, t = i / CPR, d = (i % CPR) * 16;
+        const int i = u * kConvThreads + ct, t = chunk_token(i), d = chunk_dim(i);
         const int pg = __shfl_sync(0xffffffffu, ids, t >> 4);
         r[u] = make_uint4(0, 0, 0, 0);
         // nothing behind the last token: such a slot may hold any bits
@@ -389,7 +421,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       uint8_t *dst = smem + Sh::QBYTES + (uint32_t)(i_slot % NS) * Sh::SLOT;
 #pragma unroll
       for (int u = 0; u < NCH; ++u) {
-        const int i = u * kConvThreads + ct, t = i / CPR, ch = i % CPR;
+        const int i = u * kConvThreads + ct, t = chunk_token(i), ch = chunk_dim(i) / 16;
         uint32_t f[8];
         codes_along<FMT>(r[u].x, f[0], f[1]);
         codes_along<FMT>(r[u].y, f[2], f[3]);
@@ -518,25 +550,43 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
         const uint32_t mask = n >= 16 ? 0xffffu : n <= 0 ? 0u : (1u << n) - 1u;
         return (okm >> g) & 1u ? mask : 0u;
       };
+      // first pass: the largest s' + e. Each load of 32 scores is under way while the
+      // one before it is worked on.
       float top = -CUDART_INF_F;
-#pragma unroll
-      for (int q = 0; q < TOK / 32; ++q) {
-        float s[32];
-        tmem_ld32(t_s + 32u * q, s);
-        tmem_wait_ld();
+      auto largest = [&](auto masked, const float *s, int q) {
 #pragma unroll
         for (int g2 = 0; g2 < 2; ++g2) {
           const int g = 2 * q + g2;
-          float *sg = s + 16 * g2;
-          if (!open) {
-            const uint32_t mk = seen(g);
+          float v[16];
+          const uint32_t mk = masked.value ? seen(g) : 0u;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sg[i] = (mk >> i) & 1u ? sg[i] : -CUDART_INF_F;
-          }
-          float mx = fmaxf(fmax3(sg[0], sg[1], sg[2]), sg[3]);
+          for (int i = 0; i < 16; ++i)
+            v[i] = !masked.value || ((mk >> i) & 1u) ? s[16 * g2 + i] : -CUDART_INF_F;
+          float a0 = fmax3(v[0], v[1], v[2]), a1 = fmax3(v[3], v[4], v[5]);
+          a0 = fmax3(a0, v[6], v[7]), a1 = fmax3(a1, v[8], v[9]);
+          a0 = fmax3(a0, v[10], v[11]), a1 = fmax3(a1, v[12], v[13]);
+          top = fmaxf(top, fmaf(fmax3(fmaxf(a0, a1), v[14], v[15]), ks[g] * sc, ve[g]));
+        }
+      };
+      if (open) {
+        float s0[32], s1[32];
+        tmem_ld32(t_s, s0);
 #pragma unroll
-          for (int i = 4; i < 16; i += 2) mx = fmax3(mx, sg[i], sg[i + 1]);
-          top = fmaxf(top, fmaf(mx, ks[g] * sc, ve[g]));
+        for (int q = 0; q < TOK / 32; q += 2) {
+          tmem_wait_ld();
+          tmem_ld32(t_s + 32u * (q + 1), s1);
+          largest(std::false_type(), s0, q);
+          tmem_wait_ld();
+          if (q + 2 < TOK / 32) tmem_ld32(t_s + 32u * (q + 2), s0);
+          largest(std::false_type(), s1, q + 1);
+        }
+      } else {
+#pragma unroll 1
+        for (int q = 0; q < TOK / 32; ++q) {
+          float s[32];
+          tmem_ld32(t_s + 32u * q, s);
+          tmem_wait_ld();
+          largest(std::true_type(), s, q);
         }
       }
       constexpr float kLazy = 8.f;
@@ -585,41 +635,62 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       }
       l *= alpha;
       m = mn;
-      const float ref = m == -CUDART_INF_F ? 0.f : m;
-#pragma unroll
-      for (int q = 0; q < TOK / 32; ++q) {
-        float s[32];
-        tmem_ld32(t_s + 32u * q, s);
-        tmem_wait_ld();
+      const float ref = 7.f - (m == -CUDART_INF_F ? 0.f : m);
+      // second pass: p, its sum, and its pieces over the scores
+      auto exponentials = [&](auto masked, const float *s, int q) {
         uint32_t w[32];
 #pragma unroll
         for (int g2 = 0; g2 < 2; ++g2) {
           const int g = 2 * q + g2;
-          const float kc = ks[g] * sc, bs = ve[g] - ref + 7.f;
-          const uint32_t mk = open ? 0xffffu : seen(g);
-          float sum[2] = {0.f, 0.f};
+          const float kc = ks[g] * sc, bs = ve[g] + ref;
+          const uint32_t mk = masked.value ? seen(g) : 0u;
+          float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            float p0 = exp2_approx(fmaf(s[16 * g2 + 2 * i], kc, bs));
-            float p1 = exp2_approx(fmaf(s[16 * g2 + 2 * i + 1], kc, bs));
-            if (!open) {
-              p0 = (mk >> (2 * i)) & 1u ? p0 : 0.f;
-              p1 = (mk >> (2 * i + 1)) & 1u ? p1 : 0.f;
+            const float2 y = fma_pair(make_float2(s[16 * g2 + 2 * i], s[16 * g2 + 2 * i + 1]),
+                                      make_float2(kc, kc), make_float2(bs, bs));
+            float2 p = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+            if (masked.value) {
+              p.x = (mk >> (2 * i)) & 1u ? p.x : 0.f;
+              p.y = (mk >> (2 * i + 1)) & 1u ? p.y : 0.f;
             }
-            sum[0] += p0;
-            sum[1] += p1;
-            const uint32_t hp = pack_f16(p0, p1);
-            w[8 * g2 + i] = hp;
-            if constexpr (PIECES == 2)
-              w[16 + 8 * g2 + i] = pack_f16(__fsub_rn(p0, widen_nonneg(hp & 0xffffu)),
-                                            __fsub_rn(p1, widen_nonneg(hp >> 16)));
+            sum = add_pair(sum, p);
+            if constexpr (PIECES == 2) {
+              const float2 h = make_float2(upper11(p.x), upper11(p.y));
+              const float2 r = fma_pair(h, make_float2(-1.f, -1.f), p);
+              w[8 * g2 + i] = pack_f16(h.x, h.y);
+              w[16 + 8 * g2 + i] = pack_f16(r.x, r.y);
+            } else {
+              w[8 * g2 + i] = pack_f16(p.x, p.y);
+            }
           }
           // 2^-e from the exponent; a NaN counts only where a token of it is seen
-          const float both = sum[0] + sum[1];
-          if (both != 0.f) l = fmaf(both, exp2_approx(-ve[g]), l);
+          const float both = sum.x + sum.y, more = fmaf(both, exp2_approx(-ve[g]), l);
+          l = !masked.value || both != 0.f ? more : l;
         }
         tmem_st16(t_s + 32u * q, w);
         if constexpr (PIECES == 2) tmem_st16(t_s + 32u * q + 16u, w + 16);
+      };
+      if (open) {
+        float s0[32], s1[32];
+        tmem_ld32(t_s, s0);
+#pragma unroll
+        for (int q = 0; q < TOK / 32; q += 2) {
+          tmem_wait_ld();
+          tmem_ld32(t_s + 32u * (q + 1), s1);
+          exponentials(std::false_type(), s0, q);
+          tmem_wait_ld();
+          if (q + 2 < TOK / 32) tmem_ld32(t_s + 32u * (q + 2), s0);
+          exponentials(std::false_type(), s1, q + 1);
+        }
+      } else {
+#pragma unroll 1
+        for (int q = 0; q < TOK / 32; ++q) {
+          float s[32];
+          tmem_ld32(t_s + 32u * q, s);
+          tmem_wait_ld();
+          exponentials(std::true_type(), s, q);
+        }
       }
       tmem_wait_st();
       fence_before();
