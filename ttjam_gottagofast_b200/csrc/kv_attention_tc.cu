@@ -12,21 +12,24 @@
 // before that rounding, in fp32.
 //
 // CTA = (row tile, key head, sequence, split of the tokens): MT tiles of 128 query
-// rows (row = token * group + head of the group) against tiles of TOK tokens.
-//   warps 0 .. 4 MT - 1   softmax: tensor-memory lane t of tile x is one thread's
-//             row. Two passes over the TOK scores (the row maximum, then p, which
-//             replaces the scores 32 columns at a time); O is rescaled in tensor
-//             memory only when the maximum grows by more than 2^8.
-//   4 warps   conversion: 16 codes a load, eight fp16 pairs by integer operations,
-//             stored as 128-byte-swizzled rows of 64 dims, K-major for K and, the
-//             same bytes read the other way, MN-major for V; one tile ahead in
-//             registers. The tile's scales go to shared memory.
-//   1 warp (of a fourth group) allocates tensor memory; its lane 0 issues the MMAs: S_x = q_x K^T,
-//             O_x += P_x V (A = P from tensor memory), the tiles in turn, so that
-//             one's softmax runs under the other's products.
-// K and V tiles share a ring of NS slots (K_0 V_0 K_1 ...). Every wait is bounded;
-// one that gives up latches TT_ERR_DEVICE_TIMEOUT in the cache's status word, and
-// the kernel frees its tensor memory and returns.
+// rows (row = token * group + head of the group) against tiles of 64 tokens.
+//   softmax   MT warpgroups: tensor-memory lane t of tile x is one thread's row. It
+//             reads the 64 scores of a token tile into registers, takes their
+//             maximum and writes p over them. O is rescaled in tensor memory only
+//             when the maximum grows by more than 2^8.
+//   conversion  a warpgroup: 16 codes a load, eight fp16 pairs, stored as
+//             128-byte-swizzled rows of 64 dims, K-major for K and, the same bytes
+//             read the other way, MN-major for V; one tile ahead in registers. The
+//             tile's scales go to shared memory.
+//   MMA       one warp of a last group allocates tensor memory; its lane 0 issues the
+//             products: S_x = q_x K^T into the tile's two score buffers in turn, two
+//             token tiles ahead of the softmax, and O_x += P_x V (A = P from tensor
+//             memory). (With one score buffer a row tile and 128 tokens a tile, a
+//             softmax group waited for its own products: 355 us against ... for
+//             4 x 2048 fp32 rows behind 2048, 16 heads of 64.)
+// K and V tiles have a ring each. Every wait is bounded; one that gives up latches
+// TT_ERR_DEVICE_TIMEOUT in the cache's status word, and the kernel frees its tensor
+// memory and returns.
 #include <math_constants.h>
 
 #include <algorithm>
@@ -43,28 +46,34 @@ template <int HD_, int PIECES>
 struct TcShape {
   static constexpr int HD = HD_;
   static constexpr int MT = HD <= 128 ? 2 : 1;    // 128-row tiles per CTA
-  static constexpr int TOK = HD <= 128 ? 128 : 64;  // tokens per tile
+  static constexpr int TOK = 64;                  // tokens per tile
   static constexpr bool QT = HD == 64;            // q in tensor memory (else shared memory)
   static constexpr int BOXES = HD / 64;           // 64-dim boxes of an operand tile
   static constexpr uint32_t BOX = TOK * 128;      // bytes
   static constexpr uint32_t SLOT = BOXES * BOX;
   static constexpr uint32_t QBOX = 128 * 128;
   static constexpr uint32_t QBYTES = QT ? 0 : MT * PIECES * BOXES * QBOX;
-  static constexpr int NS = (int)std::min<uint32_t>(6, (224 * 1024 - QBYTES) / SLOT);
-  static constexpr uint32_t BARS = QBYTES + NS * SLOT;  // barriers, after the operands
-  static constexpr size_t SMEM = BARS + 1024 + 1024;    // alignment of the base, barriers
+  static constexpr int SLOTS = (int)std::min<uint32_t>(8, (224 * 1024 - QBYTES) / SLOT);
+  static constexpr int NK = SLOTS / 2, NV = SLOTS - NK;  // ring of K tiles, of V tiles
+  static constexpr uint32_t V0 = QBYTES + NK * SLOT;     // first V slot
+  static constexpr uint32_t BARS = QBYTES + SLOTS * SLOT;  // barriers, after the operands
+  static constexpr size_t SMEM = BARS + 1024 + 1024;       // alignment of the base, barriers
   static constexpr int SOFT_WARPS = 4 * MT;
   // warpgroups: softmax (MT), conversion, MMA issue (one warp of it). With two
   // softmax groups the block starts with 128 registers a thread, and they take
-  // 176 (152), which the other two give up: 2 * 176 + 2 * 80 = 4 * 128.
+  // 152, which the other two give up: 2 * 152 + 2 * 104 = 4 * 128.
   static constexpr int THREADS = 32 * (SOFT_WARPS + kConvWarps + 4);
   static constexpr bool SHIFT_REGS = MT == 2;
-  static constexpr int SOFT_REGS = HD == 64 ? 176 : 152, OTHER_REGS = HD == 64 ? 80 : 104;
+  static constexpr int SOFT_REGS = 152, OTHER_REGS = 104;
   static_assert(!SHIFT_REGS || 2 * SOFT_REGS + 2 * OTHER_REGS <= 4 * 128, "registers of the block");
-  // tensor-memory columns
-  static constexpr uint32_t T_O = 0, T_S = MT * HD, T_Q = MT * (HD + TOK);
+  // tensor-memory columns: O, two score buffers a row tile, q
+  static constexpr uint32_t T_O = 0, T_S = MT * HD, T_Q = MT * (HD + 2 * TOK);
   static_assert(T_Q + (QT ? MT * PIECES * HD / 2 : 0) <= 512, "tensor memory");
-  static_assert(NS >= 3 && SMEM <= 227 * 1024, "shared memory");
+  static_assert(NK >= 1 && NV >= 2 && SMEM <= 227 * 1024, "shared memory");
+  // Tile j's scales stand in place j % 8; they are written once V tile j - 1 has a
+  // slot, that is, once the softmax of tile j - 1 - NV is done.
+  static constexpr int SCALES = 8;
+  static_assert(NV + 1 <= SCALES, "scales");
   // Tensor memory adds a product to O by rounding toward zero, so a long sum drifts
   // (measured: 7e-6 of the output after 4096 tokens, in proportion to them).
   // fp32 rows therefore take O out every FLUSH tiles (1024 tokens), into a sum
@@ -228,23 +237,29 @@ template <int HD, int FMT, int PIECES>
 __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
     kv_attention_tiles_kernel(KvAttentionArgs a, int row_tiles, int splits) {
   using Sh = TcShape<HD, PIECES>;
-  constexpr int MT = Sh::MT, TOK = Sh::TOK, NS = Sh::NS, GROUPS = Sh::GROUPS;
+  constexpr int MT = Sh::MT, TOK = Sh::TOK, NK = Sh::NK, NV = Sh::NV, GROUPS = Sh::GROUPS;
+  constexpr int SCALES = Sh::SCALES;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ float s_ks[4][GROUPS], s_ve[4][GROUPS];  // of tile j in [j & 3]
-  __shared__ uint32_t s_ok[4];                        // groups whose page exists
+  __shared__ float s_ks[SCALES][GROUPS], s_ve[SCALES][GROUPS];
+  __shared__ uint32_t s_ok[SCALES];  // groups whose page exists
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t *const smem = smem_raw + (base - raw);
   const uint32_t bars = base + Sh::BARS;
-  auto slot_full = [&](int s) { return bars + 8u * s; };
-  auto slot_empty = [&](int s) { return bars + 8u * (NS + s); };
-  auto s_full = [&](int x) { return bars + 8u * (2 * NS + x); };
-  auto p_full = [&](int x) { return bars + 8u * (2 * NS + MT + x); };
-  auto o_done = [&](int x) { return bars + 8u * (2 * NS + 2 * MT + x); };
-  constexpr uint32_t XB = 2 * NS + 3 * MT;
+  auto k_full = [&](int i) { return bars + 8u * i; };
+  auto k_empty = [&](int i) { return bars + 8u * (NK + i); };
+  auto v_full = [&](int i) { return bars + 8u * (2 * NK + i); };
+  auto v_empty = [&](int i) { return bars + 8u * (2 * NK + NV + i); };
+  constexpr uint32_t XS = 2 * NK + 2 * NV;
+  auto s_full = [&](int x, int buf) { return bars + 8u * (XS + 2 * x + buf); };
+  auto p_full = [&](int x, int buf) { return bars + 8u * (XS + 2 * MT + 2 * x + buf); };
+  auto o_done = [&](int x) { return bars + 8u * (XS + 4 * MT + x); };
+  auto o_final = [&](int x) { return bars + 8u * (XS + 5 * MT + x); };
+  constexpr uint32_t XB = XS + 6 * MT;
   auto sc_full = [&](int i) { return bars + 8u * (XB + i); };
-  const uint32_t q_ready = bars + 8u * (XB + 4), drain_bar = bars + 8u * (XB + 5);
-  const uint32_t tmem_slot = bars + 8u * (XB + 6);
+  const uint32_t q_ready = bars + 8u * (XB + SCALES), drain_bar = bars + 8u * (XB + SCALES + 1);
+  const uint32_t tmem_slot = bars + 8u * (XB + SCALES + 2);
+  static_assert(8 * (XB + SCALES + 3) <= 1024, "barriers");
   volatile uint32_t *tmem_slot_p = reinterpret_cast<volatile uint32_t *>(smem + (tmem_slot - base));
   volatile int *abort_w = reinterpret_cast<volatile int *>(smem + (tmem_slot + 4 - base));
 
@@ -289,16 +304,13 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
   }
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < NS; ++s) {
-      mbar_init(slot_full(s), kConvWarps);
-      mbar_init(slot_empty(s), 1);
-    }
+    for (int i = 0; i < NK; ++i) mbar_init(k_full(i), kConvWarps), mbar_init(k_empty(i), 1);
+    for (int i = 0; i < NV; ++i) mbar_init(v_full(i), kConvWarps), mbar_init(v_empty(i), 1);
     for (int x = 0; x < MT; ++x) {
-      mbar_init(s_full(x), 1);
-      mbar_init(p_full(x), 4);
-      mbar_init(o_done(x), 1);
+      for (int buf = 0; buf < 2; ++buf) mbar_init(s_full(x, buf), 1), mbar_init(p_full(x, buf), 4);
+      mbar_init(o_done(x), 1), mbar_init(o_final(x), 1);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(sc_full(i), 1);
+    for (int i = 0; i < SCALES; ++i) mbar_init(sc_full(i), 1);
     mbar_init(q_ready, 4 * active);
     mbar_init(drain_bar, 1);
     *abort_w = 0;
@@ -324,60 +336,62 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
   if (warp >= kMmaWarp) {
     if (warp == kMmaWarp && lane == 0) {
       // ---- MMA issuer ------------------------------------------------------
-      auto slot_addr = [&](int i) { return base + Sh::QBYTES + (uint32_t)(i % NS) * Sh::SLOT; };
-      auto wait_slot = [&](int i) {
-        return mbar_wait(slot_full(i % NS), (i / NS) & 1, abort_w, c.status, 0x6100);
+      auto wait_k = [&](int j) {
+        return mbar_wait(k_full(j % NK), (j / NK) & 1, abort_w, c.status, 0x6100);
       };
-      auto issue_s = [&](int x, int i) {
-        const uint32_t k = slot_addr(i), d = tm + Sh::T_S + (uint32_t)(TOK * x);
+      auto issue_s = [&](int x, int j) {
+        const uint32_t k = base + Sh::QBYTES + (uint32_t)(j % NK) * Sh::SLOT;
+        const uint32_t d = tm + Sh::T_S + (uint32_t)(TOK * (2 * x + (j & 1)));
+        const uint64_t kd0 = sdesc(k, 16);
+        const uint64_t qd0 = sdesc(base + (uint32_t)(x * PIECES * Sh::BOXES) * Sh::QBOX, 16);
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint64_t kd = sdesc(k + (kk / 4) * Sh::BOX, 16) + 2 * (kk % 4);
+          const uint64_t kd = kd0 + (kk / 4) * (Sh::BOX >> 4) + 2 * (kk % 4);
 #pragma unroll
           for (int w = 0; w < PIECES; ++w) {
             if constexpr (Sh::QT) {
               mma_ts(d, tm + Sh::T_Q + (uint32_t)((x * PIECES + w) * (HD / 2) + 8 * kk), kd,
                      Sh::IDESC_S, (kk | w) != 0);
             } else {
-              const uint32_t q = base + (uint32_t)((x * PIECES + w) * Sh::BOXES + kk / 4) * Sh::QBOX;
-              mma_ss(d, sdesc(q, 16) + 2 * (kk % 4), kd, Sh::IDESC_S, (kk | w) != 0);
+              mma_ss(d, qd0 + (w * Sh::BOXES + kk / 4) * (Sh::QBOX >> 4) + 2 * (kk % 4), kd,
+                     Sh::IDESC_S, (kk | w) != 0);
             }
           }
         }
-        mma_commit(s_full(x));
+        mma_commit(s_full(x, j & 1));
       };
-      bool ok = mbar_wait(q_ready, 0, abort_w, c.status, 0x6000) && wait_slot(0);
-      fence_after();
-      if (ok) {
-        for (int x = 0; x < active; ++x) issue_s(x, 0);
-        mma_commit(slot_empty(0));
+      bool ok = mbar_wait(q_ready, 0, abort_w, c.status, 0x6000);
+      for (int j = 0; ok && j < 2 && j < nj; ++j) {
+        if (!(ok = wait_k(j))) break;
+        fence_after();
+        for (int x = 0; x < active; ++x) issue_s(x, j);
+        mma_commit(k_empty(j % NK));
       }
       for (int j = 0; ok && j < nj; ++j) {
-        const int vi = 2 * j + 1, ki = 2 * j + 2;
-        ok = wait_slot(vi);
+        ok = mbar_wait(v_full(j % NV), (j / NV) & 1, abort_w, c.status, 0x6110);
+        const uint32_t v = base + Sh::V0 + (uint32_t)(j % NV) * Sh::SLOT;
         for (int x = 0; ok && x < active; ++x) {
-          if (!(ok = mbar_wait(p_full(x), j & 1, abort_w, c.status, 0x6200))) break;
+          if (!(ok = mbar_wait(p_full(x, j & 1), (j >> 1) & 1, abort_w, c.status, 0x6200))) break;
           fence_after();
-          const uint32_t v = slot_addr(vi), p = tm + Sh::T_S + (uint32_t)(TOK * x);
+          const uint32_t p = tm + Sh::T_S + (uint32_t)(TOK * (2 * x + (j & 1)));
+          const uint64_t vd0 = sdesc(v, Sh::BOX);
 #pragma unroll
-          for (int kk = 0; kk < TOK / 16; ++kk) {
-            const uint64_t vd = sdesc(v, Sh::BOX) + 128 * kk;
+          for (int kk = 0; kk < TOK / 16; ++kk)
 #pragma unroll
             for (int w = 0; w < PIECES; ++w)
               mma_ts(tm + Sh::T_O + (uint32_t)(HD * x),
-                     p + 32u * (kk >> 1) + 8u * (kk & 1) + 16u * w, vd, Sh::IDESC_PV,
+                     p + 32u * (kk >> 1) + 8u * (kk & 1) + 16u * w, vd0 + 128 * kk, Sh::IDESC_PV,
                      ((j % Sh::FLUSH) | kk | w) != 0);
-          }
-          mma_commit(o_done(x));
-          if (j + 1 < nj) {
-            if (x == 0 && !(ok = wait_slot(ki))) break;
+          mma_commit(j + 1 < nj ? o_done(x) : o_final(x));
+          if (j + 2 < nj) {  // into the buffer that this product has read
+            if (x == 0 && !(ok = wait_k(j + 2))) break;
             fence_after();
-            issue_s(x, ki);
+            issue_s(x, j + 2);
           }
         }
         if (ok) {
-          mma_commit(slot_empty(vi % NS));
-          if (j + 1 < nj) mma_commit(slot_empty(ki % NS));
+          mma_commit(v_empty(j % NV));
+          if (j + 2 < nj) mma_commit(k_empty((j + 2) % NK));
         }
       }
       // every MMA issued above has completed before the tensor memory is freed
@@ -417,8 +431,8 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
         }
       }
     };
-    auto store = [&](int i_slot, const uint4 *r) {
-      uint8_t *dst = smem + Sh::QBYTES + (uint32_t)(i_slot % NS) * Sh::SLOT;
+    auto store = [&](uint32_t slot, uint32_t full, const uint4 *r) {
+      uint8_t *dst = smem + slot;
 #pragma unroll
       for (int u = 0; u < NCH; ++u) {
         const int i = u * kConvThreads + ct, t = chunk_token(i), ch = chunk_dim(i) / 16;
@@ -434,7 +448,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       }
       fence_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(slot_full(i_slot % NS));
+      if (lane == 0) mbar_arrive(full);
     };
     int ids = pages_of(0), ids_next = pages_of(1);
     load(c.k, ids, 0, raw_k);
@@ -442,25 +456,22 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
     bool ok = true;
     for (int j = 0; ok && j < nj; ++j) {
       if (cw == 0) {
-        // scales of the tile's groups; tile j - 4's were read before slot V_{j-2}
-        // was handed back, which this warp has waited for
         if (lane < GROUPS) {
           const int64_t at = (int64_t)(ids < 0 ? 0 : ids) * c.heads + h;
           const float ks = c.ks[at], vs = c.vs[at];
-          s_ks[j & 3][lane] = ids < 0 ? 1.f : ks;
-          s_ve[j & 3][lane] = ids < 0 ? 0.f : vs == vs ? (float)((__float_as_int(vs) >> 23) - 127) : vs;
+          s_ks[j % SCALES][lane] = ids < 0 ? 1.f : ks;
+          s_ve[j % SCALES][lane] = ids < 0 ? 0.f : vs == vs ? (float)((__float_as_int(vs) >> 23) - 127) : vs;
         }
         const uint32_t okm = __ballot_sync(0xffffffffu, lane < GROUPS && ids >= 0);
-        if (lane == 0) s_ok[j & 3] = okm;
+        if (lane == 0) s_ok[j % SCALES] = okm;
         __syncwarp();
-        if (lane == 0) mbar_arrive(sc_full(j & 3));
+        if (lane == 0) mbar_arrive(sc_full(j % SCALES));
       }
-      const int ki = 2 * j, vi = 2 * j + 1;
-      if (ki >= NS && !mbar_wait(slot_empty(ki % NS), (ki / NS - 1) & 1, abort_w, c.status, 0x6300)) break;
-      store(ki, raw_k);
+      if (j >= NK && !mbar_wait(k_empty(j % NK), (j / NK - 1) & 1, abort_w, c.status, 0x6300)) break;
+      store(Sh::QBYTES + (uint32_t)(j % NK) * Sh::SLOT, k_full(j % NK), raw_k);
       if (j + 1 < nj) load(c.k, ids_next, j + 1, raw_k);
-      if (vi >= NS && !mbar_wait(slot_empty(vi % NS), (vi / NS - 1) & 1, abort_w, c.status, 0x6400)) break;
-      store(vi, raw_v);
+      if (j >= NV && !mbar_wait(v_empty(j % NV), (j / NV - 1) & 1, abort_w, c.status, 0x6400)) break;
+      store(Sh::V0 + (uint32_t)(j % NV) * Sh::SLOT, v_full(j % NV), raw_v);
       if (j + 1 < nj) load(c.v, ids_next, j + 1, raw_v);
       ids = ids_next;
       ids_next = pages_of(j + 2);
@@ -475,7 +486,6 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
     const int first = row0 + 128 * x;
     const int all_end = len - count + first / a.group + 1;  // tokens that every live row sees
     const uint32_t lane_base = tm + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t t_s = lane_base + Sh::T_S + (uint32_t)(TOK * x);
     const uint32_t t_o = lane_base + Sh::T_O + (uint32_t)(HD * x);
     float sc;
     {
@@ -536,168 +546,140 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
     const int64_t sum_at = splits > 1 ? part(r) * HD : at;
     const int sum_dims = alive ? (splits > 1 ? HD : c.hd) : 0;
     float m = -CUDART_INF_F, l = 0.f, beta = 0.f;  // beta: what the sum is scaled by when read next
-    for (int j = 0; j < nj; ++j) {
-      const int t0 = (j0 + j) * TOK;
-      mbar_wait(sc_full(j & 3), (j >> 2) & 1, abort_w, c.status, 0x6500);
-      const uint32_t okm = s_ok[j & 3];
-      const bool open = t0 + TOK <= all_end && okm == (1u << GROUPS) - 1u;  // the same for the warp
-      const float *ks = s_ks[j & 3], *ve = s_ve[j & 3];
-      mbar_wait(s_full(x), j & 1, abort_w, c.status, 0x6600);
+    // O_x holds the products up to tile j - 1's, while tile j's scores are there but
+    // not yet its p: tile j - 2's product came before those scores, so one parity is
+    // enough.
+    auto wait_o_before = [&](int j) {
+      mbar_wait(o_done(x), (j - 1) & 1, abort_w, c.status, 0x6700);
       fence_after();
-      // bits of the columns this row sees, in its 16-token group g
-      auto seen = [&](int g) -> uint32_t {
-        const int n = end - t0 - 16 * g;
-        const uint32_t mask = n >= 16 ? 0xffffu : n <= 0 ? 0u : (1u << n) - 1u;
-        return (okm >> g) & 1u ? mask : 0u;
-      };
-      // first pass: the largest s' + e. Each load of 32 scores is under way while the
-      // one before it is worked on.
-      float top = -CUDART_INF_F;
-      auto largest = [&](auto masked, const float *s, int q) {
+    };
+    // tile j's scores s[0 .. 63] to p, in the buffer that they came from
+    auto softmax = [&](auto masked, int j, float *s, uint32_t t_s) {
+      constexpr bool MASKED = decltype(masked)::value;
+      const int t0 = (j0 + j) * TOK;
+      uint32_t see[2] = {0u, 0u};  // the columns that this row sees
+      if (MASKED) {
+        const uint32_t okm = s_ok[j % SCALES];
 #pragma unroll
-        for (int g2 = 0; g2 < 2; ++g2) {
-          const int g = 2 * q + g2;
-          float v[16];
-          const uint32_t mk = masked.value ? seen(g) : 0u;
+        for (int g = 0; g < GROUPS; ++g) {
+          const int n = end - t0 - 16 * g;
+          const uint32_t mask = n >= 16 ? 0xffffu : n <= 0 ? 0u : (1u << n) - 1u;
+          if ((okm >> g) & 1u) see[g >> 1] |= mask << (16 * (g & 1));
+        }
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            v[i] = !masked.value || ((mk >> i) & 1u) ? s[16 * g2 + i] : -CUDART_INF_F;
-          float a0 = fmax3(v[0], v[1], v[2]), a1 = fmax3(v[3], v[4], v[5]);
-          a0 = fmax3(a0, v[6], v[7]), a1 = fmax3(a1, v[8], v[9]);
-          a0 = fmax3(a0, v[10], v[11]), a1 = fmax3(a1, v[12], v[13]);
-          top = fmaxf(top, fmaf(fmax3(fmaxf(a0, a1), v[14], v[15]), ks[g] * sc, ve[g]));
-        }
-      };
-      if (open) {
-        float s0[32], s1[32];
-        tmem_ld32(t_s, s0);
+        for (int i = 0; i < TOK; ++i) s[i] = (see[i >> 5] >> (i & 31)) & 1u ? s[i] : -CUDART_INF_F;
+      }
+      float kc[GROUPS], ve[GROUPS], top = -CUDART_INF_F;
 #pragma unroll
-        for (int q = 0; q < TOK / 32; q += 2) {
-          tmem_wait_ld();
-          tmem_ld32(t_s + 32u * (q + 1), s1);
-          largest(std::false_type(), s0, q);
-          tmem_wait_ld();
-          if (q + 2 < TOK / 32) tmem_ld32(t_s + 32u * (q + 2), s0);
-          largest(std::false_type(), s1, q + 1);
-        }
-      } else {
-#pragma unroll 1
-        for (int q = 0; q < TOK / 32; ++q) {
-          float s[32];
-          tmem_ld32(t_s + 32u * q, s);
-          tmem_wait_ld();
-          largest(std::true_type(), s, q);
-        }
+      for (int g = 0; g < GROUPS; ++g) {
+        kc[g] = s_ks[j % SCALES][g] * sc;
+        ve[g] = s_ve[j % SCALES][g];
+        const float *v = s + 16 * g;
+        float a0 = fmax3(v[0], v[1], v[2]), a1 = fmax3(v[3], v[4], v[5]);
+        a0 = fmax3(a0, v[6], v[7]), a1 = fmax3(a1, v[8], v[9]);
+        a0 = fmax3(a0, v[10], v[11]), a1 = fmax3(a1, v[12], v[13]);
+        top = fmaxf(top, fmaf(fmax3(fmaxf(a0, a1), v[14], v[15]), kc[g], ve[g]));
       }
       constexpr float kLazy = 8.f;
       const bool raise = top > m + kLazy || (m == -CUDART_INF_F && top > m);
-      const float mn = raise ? ceilf(top) : m;
-      const float alpha = raise ? exp2_approx(m - mn) : 1.f;  // 0 from -inf
-      const bool flush = PIECES == 2 && j > 0 && j % Sh::FLUSH == 0;
-      if (flush) {
-        mbar_wait(o_done(x), (j - 1) & 1, abort_w, c.status, 0x6700);
-        fence_after();
+      if (__any_sync(0xffffffffu, raise)) {
+        const float mn = raise ? ceilf(top) : m;
+        const float alpha = raise ? exp2_approx(m - mn) : 1.f;  // 0 from -inf
+        if (j % Sh::FLUSH != 0 && __any_sync(0xffffffffu, raise && m != -CUDART_INF_F)) {
+          wait_o_before(j);
 #pragma unroll 1
-        for (int d = 0; d < HD; d += 16) {
-          uint32_t o[16];
-          float v[16];
-          tmem_ld16(t_o + d, o);
-          tmem_wait_ld();
-          if (d < sum_dims) {
-            if (j > Sh::FLUSH) {
-              kv_load_sum16(sum_out, sum_at + d, v);
+          for (int d = 0; d < HD; d += 16) {
+            uint32_t o[16];
+            tmem_ld16(t_o + d, o);
+            tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) v[i] = fmaf(v[i], beta, __uint_as_float(o[i]));
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(o[i]);
-            }
-            kv_store_sum16(sum_out, sum_at + d, v);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st16(t_o + d, o);
           }
-          __syncwarp();
         }
-        beta = alpha;
-      } else {
         beta *= alpha;
+        l *= alpha;
+        m = mn;
       }
-      if (!flush && j > 0 && __any_sync(0xffffffffu, raise && m != -CUDART_INF_F)) {
-        mbar_wait(o_done(x), (j - 1) & 1, abort_w, c.status, 0x6700);
-        fence_after();
-#pragma unroll 1
-        for (int d = 0; d < HD; d += 16) {
-          uint32_t o[16];
-          tmem_ld16(t_o + d, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-          tmem_st16(t_o + d, o);
-        }
-      }
-      l *= alpha;
-      m = mn;
       const float ref = 7.f - (m == -CUDART_INF_F ? 0.f : m);
-      // second pass: p, its sum, and its pieces over the scores
-      auto exponentials = [&](auto masked, const float *s, int q) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
         uint32_t w[32];
 #pragma unroll
         for (int g2 = 0; g2 < 2; ++g2) {
-          const int g = 2 * q + g2;
-          const float kc = ks[g] * sc, bs = ve[g] + ref;
-          const uint32_t mk = masked.value ? seen(g) : 0u;
+          const int g = 2 * half + g2;
+          const float bs = ve[g] + ref;
           float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float2 y = fma_pair(make_float2(s[16 * g2 + 2 * i], s[16 * g2 + 2 * i + 1]),
-                                      make_float2(kc, kc), make_float2(bs, bs));
+            const int col = 16 * g + 2 * i;
+            const float2 y = fma_pair(make_float2(s[col], s[col + 1]), make_float2(kc[g], kc[g]),
+                                      make_float2(bs, bs));
             float2 p = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-            if (masked.value) {
-              p.x = (mk >> (2 * i)) & 1u ? p.x : 0.f;
-              p.y = (mk >> (2 * i + 1)) & 1u ? p.y : 0.f;
+            if (MASKED) {  // a NaN scale leaves NaN behind the mask
+              p.x = (see[half] >> (col & 31)) & 1u ? p.x : 0.f;
+              p.y = (see[half] >> ((col & 31) + 1)) & 1u ? p.y : 0.f;
             }
             sum = add_pair(sum, p);
             if constexpr (PIECES == 2) {
-              const float2 h = make_float2(upper11(p.x), upper11(p.y));
-              const float2 r = fma_pair(h, make_float2(-1.f, -1.f), p);
-              w[8 * g2 + i] = pack_f16(h.x, h.y);
-              w[16 + 8 * g2 + i] = pack_f16(r.x, r.y);
+              const float2 hi = make_float2(upper11(p.x), upper11(p.y));
+              const float2 lo = fma_pair(hi, make_float2(-1.f, -1.f), p);
+              w[8 * g2 + i] = pack_f16(hi.x, hi.y);
+              w[16 + 8 * g2 + i] = pack_f16(lo.x, lo.y);
             } else {
               w[8 * g2 + i] = pack_f16(p.x, p.y);
             }
           }
           // 2^-e from the exponent; a NaN counts only where a token of it is seen
           const float both = sum.x + sum.y, more = fmaf(both, exp2_approx(-ve[g]), l);
-          l = !masked.value || both != 0.f ? more : l;
+          l = !MASKED || both != 0.f ? more : l;
         }
-        tmem_st16(t_s + 32u * q, w);
-        if constexpr (PIECES == 2) tmem_st16(t_s + 32u * q + 16u, w + 16);
-      };
-      if (open) {
-        float s0[32], s1[32];
-        tmem_ld32(t_s, s0);
-#pragma unroll
-        for (int q = 0; q < TOK / 32; q += 2) {
-          tmem_wait_ld();
-          tmem_ld32(t_s + 32u * (q + 1), s1);
-          exponentials(std::false_type(), s0, q);
-          tmem_wait_ld();
-          if (q + 2 < TOK / 32) tmem_ld32(t_s + 32u * (q + 2), s0);
-          exponentials(std::false_type(), s1, q + 1);
-        }
-      } else {
-#pragma unroll 1
-        for (int q = 0; q < TOK / 32; ++q) {
-          float s[32];
-          tmem_ld32(t_s + 32u * q, s);
-          tmem_wait_ld();
-          exponentials(std::true_type(), s, q);
-        }
+        tmem_st16(t_s + 32u * half, w);
+        if constexpr (PIECES == 2) tmem_st16(t_s + 32u * half + 16u, w + 16);
       }
+    };
+    for (int j = 0; j < nj; ++j) {
+      const int t0 = (j0 + j) * TOK, buf = j & 1;
+      mbar_wait(sc_full(j % SCALES), (j / SCALES) & 1, abort_w, c.status, 0x6500);
+      // whether every live row sees every token (the same for the warp)
+      const bool open = t0 + TOK <= all_end && s_ok[j % SCALES] == (1u << GROUPS) - 1u;
+      mbar_wait(s_full(x, buf), (j >> 1) & 1, abort_w, c.status, 0x6600);
+      fence_after();
+      if (PIECES == 2 && j > 0 && j % Sh::FLUSH == 0) {
+        wait_o_before(j);
+#pragma unroll 1
+        for (int d = 0; d < HD; d += 32) {
+          float o[32], v[32];
+          const bool mine = d < sum_dims, both = d + 16 < sum_dims;
+          if (j > Sh::FLUSH) {
+            if (mine) kv_load_sum16(sum_out, sum_at + d, v);
+            if (both) kv_load_sum16(sum_out, sum_at + d + 16, v + 16);
+          }
+          __syncwarp();
+          tmem_ld32(t_o + d, o);
+          tmem_wait_ld();
+          if (j > Sh::FLUSH) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = fmaf(v[i], beta, o[i]);
+          }
+          if (mine) kv_store_sum16(sum_out, sum_at + d, o);
+          if (both) kv_store_sum16(sum_out, sum_at + d + 16, o + 16);
+        }
+        beta = 1.f;
+      }
+      const uint32_t t_s = lane_base + Sh::T_S + (uint32_t)(TOK * (2 * x + buf));
+      float s[TOK];
+      tmem_ld32(t_s, s);
+      tmem_ld32(t_s + 32u, s + 32);
+      tmem_wait_ld();
+      if (open) softmax(std::false_type(), j, s, t_s);
+      else softmax(std::true_type(), j, s, t_s);
       tmem_wait_st();
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full(x));
+      if (lane == 0) mbar_arrive(p_full(x, buf));
     }
-    mbar_wait(o_done(x), (nj - 1) & 1, abort_w, c.status, 0x6800);
+    mbar_wait(o_final(x), 0, abort_w, c.status, 0x6800);
     fence_after();
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
