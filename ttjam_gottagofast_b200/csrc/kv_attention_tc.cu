@@ -53,10 +53,12 @@ struct TcShape {
   static constexpr uint32_t SLOT = BOXES * BOX;
   static constexpr uint32_t QBOX = 128 * 128;
   static constexpr uint32_t QBYTES = QT ? 0 : MT * PIECES * BOXES * QBOX;
-  static constexpr int SLOTS = (int)std::min<uint32_t>(8, (224 * 1024 - QBYTES) / SLOT);
+  static constexpr uint32_t SUMS = PIECES == 2 && HD == 64 ? MT * 128 * HD * 4 : 0;  // see FLUSH
+  static constexpr int SLOTS = (int)std::min<uint32_t>(8, (224 * 1024 - QBYTES - SUMS) / SLOT);
   static constexpr int NK = SLOTS / 2, NV = SLOTS - NK;  // ring of K tiles, of V tiles
   static constexpr uint32_t V0 = QBYTES + NK * SLOT;     // first V slot
-  static constexpr uint32_t BARS = QBYTES + SLOTS * SLOT;  // barriers, after the operands
+  static constexpr uint32_t SUM0 = QBYTES + SLOTS * SLOT;  // flushed sums
+  static constexpr uint32_t BARS = SUM0 + SUMS;            // barriers, after all those
   static constexpr size_t SMEM = BARS + 1024 + 1024;       // alignment of the base, barriers
   static constexpr int SOFT_WARPS = 4 * MT;
   // warpgroups: softmax (MT), conversion, MMA issue (one warp of it). With two
@@ -76,9 +78,11 @@ struct TcShape {
   static_assert(NV + 1 <= SCALES, "scales");
   // Tensor memory adds a product to O by rounding toward zero, so a long sum drifts
   // (measured: 7e-6 of the output after 4096 tokens, in proportion to them).
-  // fp32 rows therefore take O out every FLUSH tiles (1024 tokens), into a sum
-  // kept in the row's own place of the output, and start it anew.
-  static constexpr int FLUSH = PIECES == 2 ? 1024 / TOK : INT32_MAX;
+  // fp32 rows therefore take O out every FLUSH tiles (512 tokens; 1024 where shared
+  // memory has no room for the sums and they are kept in the rows' own places of the
+  // output) and start it anew.
+  static constexpr bool SUM_SMEM = PIECES == 2 && HD == 64;
+  static constexpr int FLUSH = PIECES == 2 ? (SUM_SMEM ? 512 : 1024) / TOK : INT32_MAX;
   static constexpr int GROUPS = TOK / 16;  // of 16 tokens, each in one page
   static constexpr int NCH = TOK * HD / 16 / kConvThreads;  // 16-code chunks a converter thread
   static constexpr uint32_t IDESC_S =
@@ -136,25 +140,29 @@ __device__ __forceinline__ uint64_t sdesc(uint32_t saddr, uint32_t lead) {
   d |= (uint64_t)2 << 61;
   return d;
 }
+// The MMA warp stays converged, so that descriptors live in uniform registers; one
+// elected lane issues.
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
                                        uint32_t accum) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
       "r"(a), "l"(b), "r"(idesc), "r"(accum)
       : "memory");
 }
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                        uint32_t accum) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(accum)
       : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-               : "memory");
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
+      : "memory");
 }
 __device__ __forceinline__ void fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -264,7 +272,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
   volatile int *abort_w = reinterpret_cast<volatile int *>(smem + (tmem_slot + 4 - base));
 
   const KvView &c = a.c;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   pdl_trigger();
   pdl_wait();
   // latest row tiles (the longest, causally) first
@@ -325,7 +333,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tm = *tmem_slot_p;
+  const uint32_t tm = __shfl_sync(0xffffffffu, *tmem_slot_p, 0);
   if constexpr (Sh::SHIFT_REGS) {
     if (warp < Sh::SOFT_WARPS)
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Sh::SOFT_REGS));
@@ -334,10 +342,13 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
   }
 
   if (warp >= kMmaWarp) {
-    if (warp == kMmaWarp && lane == 0) {
+    if (warp == kMmaWarp) {
       // ---- MMA issuer ------------------------------------------------------
+      auto warp_wait = [&](uint32_t bar, uint32_t parity, int detail) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_w, c.status, detail)) != 0;
+      };
       auto wait_k = [&](int j) {
-        return mbar_wait(k_full(j % NK), (j / NK) & 1, abort_w, c.status, 0x6100);
+        return warp_wait(k_full(j % NK), (j / NK) & 1, 0x6100);
       };
       auto issue_s = [&](int x, int j) {
         const uint32_t k = base + Sh::QBYTES + (uint32_t)(j % NK) * Sh::SLOT;
@@ -360,7 +371,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
         }
         mma_commit(s_full(x, j & 1));
       };
-      bool ok = mbar_wait(q_ready, 0, abort_w, c.status, 0x6000);
+      bool ok = warp_wait(q_ready, 0, 0x6000);
       for (int j = 0; ok && j < 2 && j < nj; ++j) {
         if (!(ok = wait_k(j))) break;
         fence_after();
@@ -368,10 +379,10 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
         mma_commit(k_empty(j % NK));
       }
       for (int j = 0; ok && j < nj; ++j) {
-        ok = mbar_wait(v_full(j % NV), (j / NV) & 1, abort_w, c.status, 0x6110);
+        ok = warp_wait(v_full(j % NV), (j / NV) & 1, 0x6110);
         const uint32_t v = base + Sh::V0 + (uint32_t)(j % NV) * Sh::SLOT;
         for (int x = 0; ok && x < active; ++x) {
-          if (!(ok = mbar_wait(p_full(x, j & 1), (j >> 1) & 1, abort_w, c.status, 0x6200))) break;
+          if (!(ok = warp_wait(p_full(x, j & 1), (j >> 1) & 1, 0x6200))) break;
           fence_after();
           const uint32_t p = tm + Sh::T_S + (uint32_t)(TOK * (2 * x + (j & 1)));
           const uint64_t vd0 = sdesc(v, Sh::BOX);
@@ -545,6 +556,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
     const KvOut sum_out = splits > 1 ? KvOut{a.ws, nullptr, TT_DTYPE_F32} : a.out;
     const int64_t sum_at = splits > 1 ? part(r) * HD : at;
     const int sum_dims = alive ? (splits > 1 ? HD : c.hd) : 0;
+    float4 *const sums = reinterpret_cast<float4 *>(smem + Sh::SUM0) + x * 128 * (HD / 4) + t;
     float m = -CUDART_INF_F, l = 0.f, beta = 0.f;  // beta: what the sum is scaled by when read next
     // O_x holds the products up to tile j - 1's, while tile j's scores are there but
     // not yet its p: tile j - 2's product came before those scores, so one parity is
@@ -647,23 +659,42 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       fence_after();
       if (PIECES == 2 && j > 0 && j % Sh::FLUSH == 0) {
         wait_o_before(j);
-#pragma unroll 1
-        for (int d = 0; d < HD; d += 32) {
-          float o[32], v[32];
-          const bool mine = d < sum_dims, both = d + 16 < sum_dims;
-          if (j > Sh::FLUSH) {
-            if (mine) kv_load_sum16(sum_out, sum_at + d, v);
-            if (both) kv_load_sum16(sum_out, sum_at + d + 16, v + 16);
-          }
-          __syncwarp();
-          tmem_ld32(t_o + d, o);
-          tmem_wait_ld();
-          if (j > Sh::FLUSH) {
+        if constexpr (Sh::SUM_SMEM) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = fmaf(v[i], beta, o[i]);
+          for (int d = 0; d < HD; d += 32) {
+            float o[32];
+            tmem_ld32(t_o + d, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              float4 v = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+              if (j > Sh::FLUSH) {
+                const float4 w = sums[(d + i) / 4 * 128];
+                v.x = fmaf(w.x, beta, v.x), v.y = fmaf(w.y, beta, v.y);
+                v.z = fmaf(w.z, beta, v.z), v.w = fmaf(w.w, beta, v.w);
+              }
+              sums[(d + i) / 4 * 128] = v;
+            }
           }
-          if (mine) kv_store_sum16(sum_out, sum_at + d, o);
-          if (both) kv_store_sum16(sum_out, sum_at + d + 16, o + 16);
+        } else {
+#pragma unroll 1
+          for (int d = 0; d < HD; d += 32) {
+            float o[32], v[32];
+            const bool mine = d < sum_dims, both = d + 16 < sum_dims;
+            if (j > Sh::FLUSH) {
+              if (mine) kv_load_sum16(sum_out, sum_at + d, v);
+              if (both) kv_load_sum16(sum_out, sum_at + d + 16, v + 16);
+            }
+            __syncwarp();
+            tmem_ld32(t_o + d, o);
+            tmem_wait_ld();
+            if (j > Sh::FLUSH) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = fmaf(v[i], beta, o[i]);
+            }
+            if (mine) kv_store_sum16(sum_out, sum_at + d, o);
+            if (both) kv_store_sum16(sum_out, sum_at + d + 16, o + 16);
+          }
         }
         beta = 1.f;
       }
@@ -688,8 +719,16 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       tmem_ld16(t_o + d, o);
       tmem_wait_ld();
       float v[16];
-      if (PIECES == 2 && nj > Sh::FLUSH && d < sum_dims) {
-        kv_load_sum16(sum_out, sum_at + d, v);
+      if (PIECES == 2 && nj > Sh::FLUSH && (Sh::SUM_SMEM || d < sum_dims)) {
+        if constexpr (Sh::SUM_SMEM) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const float4 w = sums[(d + i) / 4 * 128];
+            v[i] = w.x, v[i + 1] = w.y, v[i + 2] = w.z, v[i + 3] = w.w;
+          }
+        } else {
+          kv_load_sum16(sum_out, sum_at + d, v);
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(fmaf(v[i], beta, __uint_as_float(o[i])));
       }
