@@ -85,6 +85,7 @@ struct TcShape {
   static constexpr int FLUSH = PIECES == 2 ? (SUM_SMEM ? 512 : 1024) / TOK : INT32_MAX;
   static constexpr int GROUPS = TOK / 16;  // of 16 tokens, each in one page
   static constexpr int NCH = TOK * HD / 16 / kConvThreads;  // 16-code chunks a converter thread
+  static constexpr int AHEAD = HD <= 128 ? 2 : 1;  // tiles whose codes it has in registers
   static constexpr uint32_t IDESC_S =
       (1u << 4) | ((uint32_t)(TOK >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
   static constexpr uint32_t IDESC_PV =  // B is MN-major
@@ -424,16 +425,27 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
     auto chunk_dim = [&](int i) { return i / (4 * TOK) * 64 + (i % 4) * 16; };
     const int ct = threadIdx.x - 32 * Sh::SOFT_WARPS;
     const int cw = warp - Sh::SOFT_WARPS;
-    auto pages_of = [&](int j) {  // lane g < GROUPS: the page of group g
+    // Lane g < GROUPS looks up group g's page: the table entry a tile before its
+    // check, which comes a tile or two (AHEAD) before the codes that it leads to.
+    constexpr int AHEAD = Sh::AHEAD;
+    auto entry_of = [&](int j) {
       const int t = (j0 + j) * TOK + 16 * lane;
-      return j < nj && lane < GROUPS && t < any_end ? c.page_of(b, t >> c.page_log2) : -1;
+      return j < nj && lane < GROUPS && t < any_end ? c.table[(int64_t)b * c.columns + (t >> c.page_log2)]
+                                                    : INT32_MIN;
     };
-    uint4 raw_k[NCH], raw_v[NCH];
-    auto load = [&](const uint8_t *pool, int ids, int j, uint4 *r) {
+    auto page_of = [&](int entry) {
+      if ((unsigned)entry < (unsigned)c.pages) return entry;
+      if (entry != INT32_MIN) raise_status(c.status, TT_ERR_DEVICE_FAULT, kKvBadPage);
+      return -1;
+    };
+    uint4 raw_k[AHEAD][NCH], raw_v[AHEAD][NCH];
+    int ids[AHEAD];
+    float ks[AHEAD], vs[AHEAD];
+    auto load = [&](const uint8_t *pool, int id, int j, uint4 *r) {
 #pragma unroll
       for (int u = 0; u < NCH; ++u) {
         const int i = u * kConvThreads + ct, t = chunk_token(i), d = chunk_dim(i);
-        const int pg = __shfl_sync(0xffffffffu, ids, t >> 4);
+        const int pg = __shfl_sync(0xffffffffu, id, t >> 4);
         r[u] = make_uint4(0, 0, 0, 0);
         // nothing behind the last token: such a slot may hold any bits
         if (pg >= 0 && d < c.hd && (j0 + j) * TOK + t < any_end) {
@@ -461,31 +473,51 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(full);
     };
-    int ids = pages_of(0), ids_next = pages_of(1);
-    load(c.k, ids, 0, raw_k);
-    load(c.v, ids, 0, raw_v);
-    bool ok = true;
-    for (int j = 0; ok && j < nj; ++j) {
+    auto scales = [&](int id, float &k, float &v) {
+      k = 1.f, v = 1.f;
+      if (cw == 0 && id >= 0) {
+        const uint32_t at = (uint32_t)id * (uint32_t)c.heads + (uint32_t)h;
+        k = c.ks[at], v = c.vs[at];
+      }
+    };
+#pragma unroll
+    for (int a2 = 0; a2 < AHEAD; ++a2) {
+      ids[a2] = page_of(entry_of(a2));
+      load(c.k, ids[a2], a2, raw_k[a2]);
+      load(c.v, ids[a2], a2, raw_v[a2]);
+      scales(ids[a2], ks[a2], vs[a2]);
+    }
+    int entry = entry_of(AHEAD);
+    // tile j from register set `at`, and the loads of tile j + AHEAD into it
+    auto tile = [&](int j, auto at_c) -> bool {
+      constexpr int at = decltype(at_c)::value;
       if (cw == 0) {
         if (lane < GROUPS) {
-          const int64_t at = (int64_t)(ids < 0 ? 0 : ids) * c.heads + h;
-          const float ks = c.ks[at], vs = c.vs[at];
-          s_ks[j % SCALES][lane] = ids < 0 ? 1.f : ks;
-          s_ve[j % SCALES][lane] = ids < 0 ? 0.f : vs == vs ? (float)((__float_as_int(vs) >> 23) - 127) : vs;
+          const float v = vs[at];
+          s_ks[j % SCALES][lane] = ks[at];
+          s_ve[j % SCALES][lane] = v == v ? (float)((__float_as_int(v) >> 23) - 127) : v;
         }
-        const uint32_t okm = __ballot_sync(0xffffffffu, lane < GROUPS && ids >= 0);
+        const uint32_t okm = __ballot_sync(0xffffffffu, lane < GROUPS && ids[at] >= 0);
         if (lane == 0) s_ok[j % SCALES] = okm;
         __syncwarp();
         if (lane == 0) mbar_arrive(sc_full(j % SCALES));
       }
-      if (j >= NK && !mbar_wait(k_empty(j % NK), (j / NK - 1) & 1, abort_w, c.status, 0x6300)) break;
-      store(Sh::QBYTES + (uint32_t)(j % NK) * Sh::SLOT, k_full(j % NK), raw_k);
-      if (j + 1 < nj) load(c.k, ids_next, j + 1, raw_k);
-      if (j >= NV && !mbar_wait(v_empty(j % NV), (j / NV - 1) & 1, abort_w, c.status, 0x6400)) break;
-      store(Sh::V0 + (uint32_t)(j % NV) * Sh::SLOT, v_full(j % NV), raw_v);
-      if (j + 1 < nj) load(c.v, ids_next, j + 1, raw_v);
-      ids = ids_next;
-      ids_next = pages_of(j + 2);
+      if (j >= NK && !mbar_wait(k_empty(j % NK), (j / NK - 1) & 1, abort_w, c.status, 0x6300)) return false;
+      store(Sh::QBYTES + (uint32_t)(j % NK) * Sh::SLOT, k_full(j % NK), raw_k[at]);
+      const int id = page_of(entry);
+      entry = entry_of(j + AHEAD + 1);
+      load(c.k, id, j + AHEAD, raw_k[at]);
+      scales(id, ks[at], vs[at]);
+      ids[at] = id;
+      if (j >= NV && !mbar_wait(v_empty(j % NV), (j / NV - 1) & 1, abort_w, c.status, 0x6400)) return false;
+      store(Sh::V0 + (uint32_t)(j % NV) * Sh::SLOT, v_full(j % NV), raw_v[at]);
+      load(c.v, id, j + AHEAD, raw_v[at]);
+      return true;
+    };
+    for (int j = 0; j < nj; j += AHEAD) {
+      if (!tile(j, std::integral_constant<int, 0>())) break;
+      if constexpr (AHEAD == 2)
+        if (j + 1 < nj && !tile(j + 1, std::integral_constant<int, 1>())) break;
     }
   } else if (warp / 4 < active) {
     // ---- softmax -----------------------------------------------------------
