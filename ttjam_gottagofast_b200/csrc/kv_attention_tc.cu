@@ -418,13 +418,13 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
     __syncwarp();
   } else if (warp >= Sh::SOFT_WARPS) {
     // ---- conversion of the codes -------------------------------------------
-    // chunk i: four of 16 codes in a row's 64 dims, then the next token, then the
-    // next box, so that eight lanes' stores of 16 bytes meet different banks
+    // Chunk u of a thread: 16 codes, dims 64 (u / 2) + 16 (ct % 4) of token ct / 4 +
+    // 32 (u % 2): eight lanes' stores of 16 bytes meet different banks.
     constexpr int NCH = Sh::NCH;
-    auto chunk_token = [&](int i) { return (i / 4) % TOK; };
-    auto chunk_dim = [&](int i) { return i / (4 * TOK) * 64 + (i % 4) * 16; };
-    const int ct = threadIdx.x - 32 * Sh::SOFT_WARPS;
+    static_assert(TOK * 4 == 2 * kConvThreads, "two tokens a thread");
+    const int ct = threadIdx.x - 32 * Sh::SOFT_WARPS, row = ct >> 2;
     const int cw = warp - Sh::SOFT_WARPS;
+    const uint32_t put = row * 128 + (((2 * (ct & 3)) ^ (row & 7)) << 4);
     // Lane g < GROUPS looks up group g's page: the table entry a tile before its
     // check, which comes a tile or two (AHEAD) before the codes that it leads to.
     constexpr int AHEAD = Sh::AHEAD;
@@ -441,33 +441,39 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
     uint4 raw_k[AHEAD][NCH], raw_v[AHEAD][NCH];
     int ids[AHEAD];
     float ks[AHEAD], vs[AHEAD];
-    auto load = [&](const uint8_t *pool, int id, int j, uint4 *r) {
+    // where this thread's two tokens of tile j lie in the pools; -1: nowhere (behind
+    // the last token too: such a slot may hold any bits)
+    auto places = [&](int id, int j, int64_t *at) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int t = row + 32 * r, pg = __shfl_sync(0xffffffffu, id, t >> 4);
+        const int tok = (j0 + j) * TOK + t;
+        at[r] = pg >= 0 && tok < any_end
+                    ? c.tile(pg, h) + (tok & ((1 << c.page_log2) - 1)) * c.hd + 16 * (ct & 3)
+                    : -1;
+      }
+    };
+    auto load = [&](const uint8_t *pool, const int64_t *at, uint4 *r) {
 #pragma unroll
       for (int u = 0; u < NCH; ++u) {
-        const int i = u * kConvThreads + ct, t = chunk_token(i), d = chunk_dim(i);
-        const int pg = __shfl_sync(0xffffffffu, id, t >> 4);
         r[u] = make_uint4(0, 0, 0, 0);
-        // nothing behind the last token: such a slot may hold any bits
-        if (pg >= 0 && d < c.hd && (j0 + j) * TOK + t < any_end) {
-          const int in_page = ((j0 + j) * TOK + t) & ((1 << c.page_log2) - 1);
-          r[u] = *reinterpret_cast<const uint4 *>(pool + c.tile(pg, h) + (int64_t)in_page * c.hd + d);
-        }
+        if (at[u & 1] >= 0 && 64 * (u >> 1) + 16 * (ct & 3) < c.hd)
+          r[u] = *reinterpret_cast<const uint4 *>(pool + at[u & 1] + 64 * (u >> 1));
       }
     };
     auto store = [&](uint32_t slot, uint32_t full, const uint4 *r) {
-      uint8_t *dst = smem + slot;
+      uint8_t *const dst = smem + slot;
 #pragma unroll
       for (int u = 0; u < NCH; ++u) {
-        const int i = u * kConvThreads + ct, t = chunk_token(i), ch = chunk_dim(i) / 16;
         uint32_t f[8];
         codes_along<FMT>(r[u].x, f[0], f[1]);
         codes_along<FMT>(r[u].y, f[2], f[3]);
         codes_along<FMT>(r[u].z, f[4], f[5]);
         codes_along<FMT>(r[u].w, f[6], f[7]);
-        uint8_t *row = dst + (ch / 4) * Sh::BOX + t * 128;
-        const int c0 = (2 * ch) % 8;
-        *reinterpret_cast<uint4 *>(row + ((c0 ^ (t & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
-        *reinterpret_cast<uint4 *>(row + (((c0 + 1) ^ (t & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
+        constexpr uint32_t kHalf = 32 * 128;
+        uint8_t *const at = dst + (u >> 1) * Sh::BOX + (u & 1) * kHalf;
+        *reinterpret_cast<uint4 *>(at + put) = make_uint4(f[0], f[1], f[2], f[3]);
+        *reinterpret_cast<uint4 *>(at + (put ^ 16)) = make_uint4(f[4], f[5], f[6], f[7]);
       }
       fence_async();
       __syncwarp();
@@ -483,8 +489,10 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
 #pragma unroll
     for (int a2 = 0; a2 < AHEAD; ++a2) {
       ids[a2] = page_of(entry_of(a2));
-      load(c.k, ids[a2], a2, raw_k[a2]);
-      load(c.v, ids[a2], a2, raw_v[a2]);
+      int64_t at[2];
+      places(ids[a2], a2, at);
+      load(c.k, at, raw_k[a2]);
+      load(c.v, at, raw_v[a2]);
       scales(ids[a2], ks[a2], vs[a2]);
     }
     int entry = entry_of(AHEAD);
@@ -506,12 +514,14 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       store(Sh::QBYTES + (uint32_t)(j % NK) * Sh::SLOT, k_full(j % NK), raw_k[at]);
       const int id = page_of(entry);
       entry = entry_of(j + AHEAD + 1);
-      load(c.k, id, j + AHEAD, raw_k[at]);
+      int64_t from[2];
+      places(id, j + AHEAD, from);
+      load(c.k, from, raw_k[at]);
       scales(id, ks[at], vs[at]);
       ids[at] = id;
       if (j >= NV && !mbar_wait(v_empty(j % NV), (j / NV - 1) & 1, abort_w, c.status, 0x6400)) return false;
       store(Sh::V0 + (uint32_t)(j % NV) * Sh::SLOT, v_full(j % NV), raw_v[at]);
-      load(c.v, id, j + AHEAD, raw_v[at]);
+      load(c.v, from, raw_v[at]);
       return true;
     };
     for (int j = 0; j < nj; j += AHEAD) {
@@ -684,10 +694,10 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
     };
     for (int j = 0; j < nj; ++j) {
       const int t0 = (j0 + j) * TOK, buf = j & 1;
+      mbar_wait(s_full(x, buf), (j >> 1) & 1, abort_w, c.status, 0x6600);
       mbar_wait(sc_full(j % SCALES), (j / SCALES) & 1, abort_w, c.status, 0x6500);
       // whether every live row sees every token (the same for the warp)
       const bool open = t0 + TOK <= all_end && s_ok[j % SCALES] == (1u << GROUPS) - 1u;
-      mbar_wait(s_full(x, buf), (j >> 1) & 1, abort_w, c.status, 0x6600);
       fence_after();
       if (PIECES == 2 && j > 0 && j % Sh::FLUSH == 0) {
         wait_o_before(j);
