@@ -441,27 +441,34 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
     uint4 raw_k[AHEAD][NCH], raw_v[AHEAD][NCH];
     int ids[AHEAD];
     float ks[AHEAD], vs[AHEAD];
-    // where this thread's two tokens of tile j lie in the pools; -1: nowhere (behind
-    // the last token too: such a slot may hold any bits)
-    auto places = [&](int id, int j, int64_t *at) {
+    // where this thread's two tokens of tile j lie in the pools; bit r of `none` where
+    // token r lies nowhere, or behind the last one (such a slot may hold any bits):
+    // something else is read then, and zeros are stored
+    auto places = [&](int id, int j, int64_t *at) -> uint32_t {
+      uint32_t none = 0;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const int t = row + 32 * r, pg = __shfl_sync(0xffffffffu, id, t >> 4);
         const int tok = (j0 + j) * TOK + t;
-        at[r] = pg >= 0 && tok < any_end
-                    ? c.tile(pg, h) + (tok & ((1 << c.page_log2) - 1)) * c.hd + 16 * (ct & 3)
-                    : -1;
+        const bool there = pg >= 0 && tok < any_end;
+        at[r] = there ? c.tile(pg, h) + (tok & ((1 << c.page_log2) - 1)) * c.hd + 16 * (ct & 3) : 0;
+        none |= there ? 0u : 1u << r;
       }
+      return none;
     };
     auto load = [&](const uint8_t *pool, const int64_t *at, uint4 *r) {
 #pragma unroll
-      for (int u = 0; u < NCH; ++u) {
-        r[u] = make_uint4(0, 0, 0, 0);
-        if (at[u & 1] >= 0 && 64 * (u >> 1) + 16 * (ct & 3) < c.hd)
+      for (int u = 0; u < NCH; ++u)
+        if (64 * (u >> 1) + 16 * (ct & 3) < c.hd)
           r[u] = *reinterpret_cast<const uint4 *>(pool + at[u & 1] + 64 * (u >> 1));
-      }
     };
-    auto store = [&](uint32_t slot, uint32_t full, const uint4 *r) {
+    const bool narrow = c.hd != HD;  // dims past head_dim are zero
+    auto store = [&](uint32_t slot, uint32_t full, uint32_t none, uint4 *r) {
+      if (__any_sync(0xffffffffu, none != 0) || narrow) {
+#pragma unroll
+        for (int u = 0; u < NCH; ++u)
+          if ((none >> (u & 1)) & 1u || 64 * (u >> 1) + 16 * (ct & 3) >= c.hd) r[u] = make_uint4(0, 0, 0, 0);
+      }
       uint8_t *const dst = smem + slot;
 #pragma unroll
       for (int u = 0; u < NCH; ++u) {
@@ -479,6 +486,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(full);
     };
+    uint32_t none[AHEAD];
     auto scales = [&](int id, float &k, float &v) {
       k = 1.f, v = 1.f;
       if (cw == 0 && id >= 0) {
@@ -490,7 +498,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
     for (int a2 = 0; a2 < AHEAD; ++a2) {
       ids[a2] = page_of(entry_of(a2));
       int64_t at[2];
-      places(ids[a2], a2, at);
+      none[a2] = places(ids[a2], a2, at);
       load(c.k, at, raw_k[a2]);
       load(c.v, at, raw_v[a2]);
       scales(ids[a2], ks[a2], vs[a2]);
@@ -511,16 +519,17 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
         if (lane == 0) mbar_arrive(sc_full(j % SCALES));
       }
       if (j >= NK && !mbar_wait(k_empty(j % NK), (j / NK - 1) & 1, abort_w, c.status, 0x6300)) return false;
-      store(Sh::QBYTES + (uint32_t)(j % NK) * Sh::SLOT, k_full(j % NK), raw_k[at]);
+      store(Sh::QBYTES + (uint32_t)(j % NK) * Sh::SLOT, k_full(j % NK), none[at], raw_k[at]);
       const int id = page_of(entry);
       entry = entry_of(j + AHEAD + 1);
       int64_t from[2];
-      places(id, j + AHEAD, from);
+      const uint32_t none_ahead = places(id, j + AHEAD, from);
       load(c.k, from, raw_k[at]);
       scales(id, ks[at], vs[at]);
       ids[at] = id;
       if (j >= NV && !mbar_wait(v_empty(j % NV), (j / NV - 1) & 1, abort_w, c.status, 0x6400)) return false;
-      store(Sh::V0 + (uint32_t)(j % NV) * Sh::SLOT, v_full(j % NV), raw_v[at]);
+      store(Sh::V0 + (uint32_t)(j % NV) * Sh::SLOT, v_full(j % NV), none[at], raw_v[at]);
+      none[at] = none_ahead;
       load(c.v, from, raw_v[at]);
       return true;
     };
@@ -608,26 +617,27 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       fence_after();
     };
     // tile j's scores s[0 .. 63] to p, in the buffer that they came from
-    auto softmax = [&](auto masked, int j, float *s, uint32_t t_s) {
-      constexpr bool MASKED = decltype(masked)::value;
-      const int t0 = (j0 + j) * TOK;
-      uint32_t see[2] = {0u, 0u};  // the columns that this row sees
-      if (MASKED) {
-        const uint32_t okm = s_ok[j % SCALES];
-#pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-          const int n = end - t0 - 16 * g;
-          const uint32_t mask = n >= 16 ? 0xffffu : n <= 0 ? 0u : (1u << n) - 1u;
-          if ((okm >> g) & 1u) see[g >> 1] |= mask << (16 * (g & 1));
-        }
-#pragma unroll
-        for (int i = 0; i < TOK; ++i) s[i] = (see[i >> 5] >> (i & 31)) & 1u ? s[i] : -CUDART_INF_F;
-      }
+    auto softmax = [&](int j, bool open, float *s, uint32_t t_s) {
       float kc[GROUPS], ve[GROUPS], top = -CUDART_INF_F;
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) {
         kc[g] = s_ks[j % SCALES][g] * sc;
         ve[g] = s_ve[j % SCALES][g];
+      }
+      if (!open) {  // the same for the warp
+        const int left = end - (j0 + j) * TOK;  // tokens of the tile that this row sees
+        const uint32_t okm = s_ok[j % SCALES];
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+          const int n = (okm >> g) & 1u ? left - 16 * g : 0;
+          // a group that the row sees nothing of: its scales, NaN perhaps, do not count
+          if (n <= 0) kc[g] = 1.f, ve[g] = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[16 * g + i] = i < n ? s[16 * g + i] : -CUDART_INF_F;
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
         const float *v = s + 16 * g;
         float a0 = fmax3(v[0], v[1], v[2]), a1 = fmax3(v[3], v[4], v[5]);
         a0 = fmax3(a0, v[6], v[7]), a1 = fmax3(a1, v[8], v[9]);
@@ -669,11 +679,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
             const int col = 16 * g + 2 * i;
             const float2 y = fma_pair(make_float2(s[col], s[col + 1]), make_float2(kc[g], kc[g]),
                                       make_float2(bs, bs));
-            float2 p = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-            if (MASKED) {  // a NaN scale leaves NaN behind the mask
-              p.x = (see[half] >> (col & 31)) & 1u ? p.x : 0.f;
-              p.y = (see[half] >> ((col & 31) + 1)) & 1u ? p.y : 0.f;
-            }
+            const float2 p = make_float2(exp2_approx(y.x), exp2_approx(y.y));
             sum = add_pair(sum, p);
             if constexpr (PIECES == 2) {
               const float2 hi = make_float2(upper11(p.x), upper11(p.y));
@@ -684,9 +690,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
               w[8 * g2 + i] = pack_f16(p.x, p.y);
             }
           }
-          // 2^-e from the exponent; a NaN counts only where a token of it is seen
-          const float both = sum.x + sum.y, more = fmaf(both, exp2_approx(-ve[g]), l);
-          l = !MASKED || both != 0.f ? more : l;
+          l = fmaf(sum.x + sum.y, exp2_approx(-ve[g]), l);
         }
         tmem_st16(t_s + 32u * half, w);
         if constexpr (PIECES == 2) tmem_st16(t_s + 32u * half + 16u, w + 16);
@@ -745,8 +749,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       tmem_ld32(t_s, s);
       tmem_ld32(t_s + 32u, s + 32);
       tmem_wait_ld();
-      if (open) softmax(std::false_type(), j, s, t_s);
-      else softmax(std::true_type(), j, s, t_s);
+      softmax(j, open, s, t_s);
       tmem_wait_st();
       fence_before();
       __syncwarp();
