@@ -54,19 +54,28 @@ struct TcShape {
   static constexpr uint32_t QBOX = 128 * 128;
   static constexpr uint32_t QBYTES = QT ? 0 : MT * PIECES * BOXES * QBOX;
   static constexpr uint32_t SUMS = PIECES == 2 && HD == 64 ? MT * 128 * HD * 4 : 0;  // see FLUSH
-  static constexpr int SLOTS = (int)std::min<uint32_t>(8, (224 * 1024 - QBYTES - SUMS) / SLOT);
+  // Codes on their way: AHEAD tiles in shared memory, every thread's own chunks, copied
+  // asynchronously. (In registers the loads shared the few scoreboards, and a wait
+  // for a page's number was one for the codes behind it: 480 us against ... for
+  // prompt grouped.) At head_dim 256 there is room for neither more than one tile.
+  static constexpr bool STAGED = HD <= 128;
+  static constexpr int AHEAD = STAGED ? 2 : 1;
+  static constexpr uint32_t STAGE = STAGED ? 2 * TOK * HD : 0;  // bytes of a tile's codes
+  static constexpr int SLOTS =
+      (int)std::min<uint32_t>(8, (224 * 1024 - QBYTES - SUMS - AHEAD * STAGE) / SLOT);
   static constexpr int NK = SLOTS / 2, NV = SLOTS - NK;  // ring of K tiles, of V tiles
   static constexpr uint32_t V0 = QBYTES + NK * SLOT;     // first V slot
   static constexpr uint32_t SUM0 = QBYTES + SLOTS * SLOT;  // flushed sums
-  static constexpr uint32_t BARS = SUM0 + SUMS;            // barriers, after all those
+  static constexpr uint32_t STAGE0 = SUM0 + SUMS;          // codes on their way
+  static constexpr uint32_t BARS = STAGE0 + AHEAD * STAGE;  // barriers, after all those
   static constexpr size_t SMEM = BARS + 1024 + 1024;       // alignment of the base, barriers
   static constexpr int SOFT_WARPS = 4 * MT;
   // warpgroups: softmax (MT), conversion, MMA issue (one warp of it). With two
   // softmax groups the block starts with 128 registers a thread, and they take
-  // 152, which the other two give up: 2 * 152 + 2 * 104 = 4 * 128.
+  // 176, which the other two give up: 2 * 176 + 2 * 80 = 4 * 128.
   static constexpr int THREADS = 32 * (SOFT_WARPS + kConvWarps + 4);
   static constexpr bool SHIFT_REGS = MT == 2;
-  static constexpr int SOFT_REGS = 152, OTHER_REGS = 104;
+  static constexpr int SOFT_REGS = 176, OTHER_REGS = 80;
   static_assert(!SHIFT_REGS || 2 * SOFT_REGS + 2 * OTHER_REGS <= 4 * 128, "registers of the block");
   // tensor-memory columns: O, two score buffers a row tile, q
   static constexpr uint32_t T_O = 0, T_S = MT * HD, T_Q = MT * (HD + 2 * TOK);
@@ -85,7 +94,6 @@ struct TcShape {
   static constexpr int FLUSH = PIECES == 2 ? (SUM_SMEM ? 512 : 1024) / TOK : INT32_MAX;
   static constexpr int GROUPS = TOK / 16;  // of 16 tokens, each in one page
   static constexpr int NCH = TOK * HD / 16 / kConvThreads;  // 16-code chunks a converter thread
-  static constexpr int AHEAD = HD <= 128 ? 2 : 1;  // tiles whose codes it has in registers
   static constexpr uint32_t IDESC_S =
       (1u << 4) | ((uint32_t)(TOK >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
   static constexpr uint32_t IDESC_PV =  // B is MN-major
@@ -438,7 +446,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       if (entry != INT32_MIN) raise_status(c.status, TT_ERR_DEVICE_FAULT, kKvBadPage);
       return -1;
     };
-    uint4 raw_k[AHEAD][NCH], raw_v[AHEAD][NCH];
+    uint4 raw_k[Sh::STAGED ? 1 : NCH], raw_v[Sh::STAGED ? 1 : NCH];
     int ids[AHEAD];
     float ks[AHEAD], vs[AHEAD];
     // where this thread's two tokens of tile j lie in the pools; bit r of `none` where
@@ -456,27 +464,40 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       }
       return none;
     };
+    auto in_head = [&](int u) { return 64 * (u >> 1) + 16 * (ct & 3) < c.hd; };
     auto load = [&](const uint8_t *pool, const int64_t *at, uint4 *r) {
 #pragma unroll
       for (int u = 0; u < NCH; ++u)
-        if (64 * (u >> 1) + 16 * (ct & 3) < c.hd)
-          r[u] = *reinterpret_cast<const uint4 *>(pool + at[u & 1] + 64 * (u >> 1));
+        if (in_head(u)) r[u] = *reinterpret_cast<const uint4 *>(pool + at[u & 1] + 64 * (u >> 1));
     };
-    const bool narrow = c.hd != HD;  // dims past head_dim are zero
-    auto store = [&](uint32_t slot, uint32_t full, uint32_t none, uint4 *r) {
-      if (__any_sync(0xffffffffu, none != 0) || narrow) {
+    // place n of the staged codes; chunk u of this thread's keys (kv 0) or values (1)
+    auto staged = [&](int n, int kv, int u) {
+      return Sh::STAGE0 + n * Sh::STAGE + (uint32_t)((kv * NCH + u) * kConvThreads + ct) * 16;
+    };
+    auto copy = [&](int n, const int64_t *at) {
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv)
 #pragma unroll
         for (int u = 0; u < NCH; ++u)
-          if ((none >> (u & 1)) & 1u || 64 * (u >> 1) + 16 * (ct & 3) >= c.hd) r[u] = make_uint4(0, 0, 0, 0);
-      }
+          if (in_head(u))
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + staged(n, kv, u)),
+                         "l"((kv ? c.v : c.k) + at[u & 1] + 64 * (u >> 1))
+                         : "memory");
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    const bool narrow = c.hd != HD;  // dims past head_dim are zero
+    auto store = [&](uint32_t slot, uint32_t full, uint32_t none, auto &&chunk) {
+      const bool clear = __any_sync(0xffffffffu, none != 0) || narrow;
       uint8_t *const dst = smem + slot;
 #pragma unroll
       for (int u = 0; u < NCH; ++u) {
+        uint4 r = chunk(u);
+        if (clear && (((none >> (u & 1)) & 1u) || !in_head(u))) r = make_uint4(0, 0, 0, 0);
         uint32_t f[8];
-        codes_along<FMT>(r[u].x, f[0], f[1]);
-        codes_along<FMT>(r[u].y, f[2], f[3]);
-        codes_along<FMT>(r[u].z, f[4], f[5]);
-        codes_along<FMT>(r[u].w, f[6], f[7]);
+        codes_along<FMT>(r.x, f[0], f[1]);
+        codes_along<FMT>(r.y, f[2], f[3]);
+        codes_along<FMT>(r.z, f[4], f[5]);
+        codes_along<FMT>(r.w, f[6], f[7]);
         constexpr uint32_t kHalf = 32 * 128;
         uint8_t *const at = dst + (u >> 1) * Sh::BOX + (u & 1) * kHalf;
         *reinterpret_cast<uint4 *>(at + put) = make_uint4(f[0], f[1], f[2], f[3]);
@@ -495,42 +516,53 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       }
     };
 #pragma unroll
-    for (int a2 = 0; a2 < AHEAD; ++a2) {
-      ids[a2] = page_of(entry_of(a2));
+    for (int n = 0; n < AHEAD; ++n) {
+      ids[n] = page_of(entry_of(n));
       int64_t at[2];
-      none[a2] = places(ids[a2], a2, at);
-      load(c.k, at, raw_k[a2]);
-      load(c.v, at, raw_v[a2]);
-      scales(ids[a2], ks[a2], vs[a2]);
+      none[n] = places(ids[n], n, at);
+      if constexpr (Sh::STAGED) {
+        copy(n, at);
+      } else {
+        load(c.k, at, raw_k);
+        load(c.v, at, raw_v);
+      }
+      scales(ids[n], ks[n], vs[n]);
     }
     int entry = entry_of(AHEAD);
-    // tile j from register set `at`, and the loads of tile j + AHEAD into it
-    auto tile = [&](int j, auto at_c) -> bool {
-      constexpr int at = decltype(at_c)::value;
+    // tile j, whose codes are in place n, and then those of tile j + AHEAD into it
+    auto tile = [&](int j, auto n_c) -> bool {
+      constexpr int n = decltype(n_c)::value;
       if (cw == 0) {
         if (lane < GROUPS) {
-          const float v = vs[at];
-          s_ks[j % SCALES][lane] = ks[at];
+          const float v = vs[n];
+          s_ks[j % SCALES][lane] = ks[n];
           s_ve[j % SCALES][lane] = v == v ? (float)((__float_as_int(v) >> 23) - 127) : v;
         }
-        const uint32_t okm = __ballot_sync(0xffffffffu, lane < GROUPS && ids[at] >= 0);
+        const uint32_t okm = __ballot_sync(0xffffffffu, lane < GROUPS && ids[n] >= 0);
         if (lane == 0) s_ok[j % SCALES] = okm;
         __syncwarp();
         if (lane == 0) mbar_arrive(sc_full(j % SCALES));
       }
-      if (j >= NK && !mbar_wait(k_empty(j % NK), (j / NK - 1) & 1, abort_w, c.status, 0x6300)) return false;
-      store(Sh::QBYTES + (uint32_t)(j % NK) * Sh::SLOT, k_full(j % NK), none[at], raw_k[at]);
-      const int id = page_of(entry);
+      ids[n] = page_of(entry);
       entry = entry_of(j + AHEAD + 1);
+      scales(ids[n], ks[n], vs[n]);
       int64_t from[2];
-      const uint32_t none_ahead = places(id, j + AHEAD, from);
-      load(c.k, from, raw_k[at]);
-      scales(id, ks[at], vs[at]);
-      ids[at] = id;
+      const uint32_t none_next = places(ids[n], j + AHEAD, from);
+      if constexpr (Sh::STAGED) asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
+      if (j >= NK && !mbar_wait(k_empty(j % NK), (j / NK - 1) & 1, abort_w, c.status, 0x6300)) return false;
+      store(Sh::QBYTES + (uint32_t)(j % NK) * Sh::SLOT, k_full(j % NK), none[n], [&](int u) {
+        if constexpr (Sh::STAGED) return *reinterpret_cast<const uint4 *>(smem + staged(n, 0, u));
+        else return raw_k[u];
+      });
+      if constexpr (!Sh::STAGED) load(c.k, from, raw_k);
       if (j >= NV && !mbar_wait(v_empty(j % NV), (j / NV - 1) & 1, abort_w, c.status, 0x6400)) return false;
-      store(Sh::V0 + (uint32_t)(j % NV) * Sh::SLOT, v_full(j % NV), none[at], raw_v[at]);
-      none[at] = none_ahead;
-      load(c.v, from, raw_v[at]);
+      store(Sh::V0 + (uint32_t)(j % NV) * Sh::SLOT, v_full(j % NV), none[n], [&](int u) {
+        if constexpr (Sh::STAGED) return *reinterpret_cast<const uint4 *>(smem + staged(n, 1, u));
+        else return raw_v[u];
+      });
+      if constexpr (Sh::STAGED) copy(n, from);
+      else load(c.v, from, raw_v);
+      none[n] = none_next;
       return true;
     };
     for (int j = 0; j < nj; j += AHEAD) {
@@ -538,6 +570,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       if constexpr (AHEAD == 2)
         if (j + 1 < nj && !tile(j + 1, std::integral_constant<int, 1>())) break;
     }
+    if constexpr (Sh::STAGED) asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else if (warp / 4 < active) {
     // ---- softmax -----------------------------------------------------------
     const int x = warp / 4, t = threadIdx.x & 127;
@@ -554,23 +587,32 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       // q: the row's largest magnitude, then scaled and split
       const int64_t off = b * a.qs.batch + (int64_t)tok * a.qs.token +
                           (int64_t)(h * a.group + r % a.group) * a.qs.head;
-      float mx = 0.f, v[16];
-      for (int d = 0; d < c.hd; d += 16) {
-        if (alive) kv_load_row16(a.dtype, a.q, off + d, a.q_vec, v);
+      // (64 dims' loads under way at once; the second time they come from the cache)
+      float mx = 0.f, v64[64];
+      auto fetch = [&](int d0) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, alive ? fabsf(v[i]) : 0.f);
+        for (int d = 0; d < 64; d += 16) {
+          if (alive && d0 + d < c.hd) {
+            kv_load_row16(a.dtype, a.q, off + d0 + d, a.q_vec, v64 + d);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v64[d + i] = 0.f;
+          }
+        }
+      };
+#pragma unroll
+      for (int d0 = 0; d0 < HD; d0 += 64) {
+        fetch(d0);
+#pragma unroll
+        for (int i = 0; i < 64; ++i) mx = fmaxf(mx, fabsf(v64[i]));
       }
       int e = (__float_as_int(mx) >> 23) - 127;
       e = mx > 0.f ? min(max(e, -126), 126) : 0;
       const float f = kv_pow2(-e);
 #pragma unroll
       for (int d = 0; d < HD; d += 16) {
-        if (alive && d < c.hd) {
-          kv_load_row16(a.dtype, a.q, off + d, a.q_vec, v);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = 0.f;
-        }
+        if (HD > 64 && d % 64 == 0) fetch(d);
+        const float *v = v64 + d % 64;
         uint32_t hi[8], lo[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
