@@ -54,12 +54,13 @@ struct TcShape {
   static constexpr uint32_t QBOX = 128 * 128;
   static constexpr uint32_t QBYTES = QT ? 0 : MT * PIECES * BOXES * QBOX;
   static constexpr uint32_t SUMS = PIECES == 2 && HD == 64 ? MT * 128 * HD * 4 : 0;  // see FLUSH
-  // Codes on their way: AHEAD tiles in shared memory, every thread's own chunks, copied
-  // asynchronously. (In registers the loads shared the few scoreboards, and a wait
-  // for a page's number was one for the codes behind it: 480 us against ... for
-  // prompt grouped.) At head_dim 256 there is room for neither more than one tile.
-  static constexpr bool STAGED = HD <= 128;
-  static constexpr int AHEAD = STAGED ? 2 : 1;
+  // Codes on their way, AHEAD tiles: up to head_dim 64 in shared memory, every thread's
+  // own chunks, copied asynchronously (in registers, loads share the few scoreboards,
+  // and a wait for a page's number is one for the codes behind it: prompt 265 us, in
+  // shared memory 258). Wider heads keep shared memory's bandwidth for the products
+  // (prompt grouped 564 us staged, 480 in registers).
+  static constexpr bool STAGED = HD <= 64;
+  static constexpr int AHEAD = HD <= 128 ? 2 : 1;
   static constexpr uint32_t STAGE = STAGED ? 2 * TOK * HD : 0;  // bytes of a tile's codes
   static constexpr int SLOTS =
       (int)std::min<uint32_t>(8, (224 * 1024 - QBYTES - SUMS - AHEAD * STAGE) / SLOT);
@@ -72,10 +73,10 @@ struct TcShape {
   static constexpr int SOFT_WARPS = 4 * MT;
   // warpgroups: softmax (MT), conversion, MMA issue (one warp of it). With two
   // softmax groups the block starts with 128 registers a thread, and they take
-  // 176, which the other two give up: 2 * 176 + 2 * 80 = 4 * 128.
+  // 176 (152), which the other two give up: 2 * 176 + 2 * 80 = 4 * 128.
   static constexpr int THREADS = 32 * (SOFT_WARPS + kConvWarps + 4);
   static constexpr bool SHIFT_REGS = MT == 2;
-  static constexpr int SOFT_REGS = 176, OTHER_REGS = 80;
+  static constexpr int SOFT_REGS = HD == 64 ? 176 : 152, OTHER_REGS = HD == 64 ? 80 : 104;
   static_assert(!SHIFT_REGS || 2 * SOFT_REGS + 2 * OTHER_REGS <= 4 * 128, "registers of the block");
   // tensor-memory columns: O, two score buffers a row tile, q
   static constexpr uint32_t T_O = 0, T_S = MT * HD, T_Q = MT * (HD + 2 * TOK);
@@ -446,7 +447,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       if (entry != INT32_MIN) raise_status(c.status, TT_ERR_DEVICE_FAULT, kKvBadPage);
       return -1;
     };
-    uint4 raw_k[Sh::STAGED ? 1 : NCH], raw_v[Sh::STAGED ? 1 : NCH];
+    uint4 raw_k[AHEAD][NCH], raw_v[AHEAD][NCH];  // (unless staged)
     int ids[AHEAD];
     float ks[AHEAD], vs[AHEAD];
     // where this thread's two tokens of tile j lie in the pools; bit r of `none` where
@@ -523,8 +524,8 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       if constexpr (Sh::STAGED) {
         copy(n, at);
       } else {
-        load(c.k, at, raw_k);
-        load(c.v, at, raw_v);
+        load(c.k, at, raw_k[n]);
+        load(c.v, at, raw_v[n]);
       }
       scales(ids[n], ks[n], vs[n]);
     }
@@ -552,16 +553,16 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       if (j >= NK && !mbar_wait(k_empty(j % NK), (j / NK - 1) & 1, abort_w, c.status, 0x6300)) return false;
       store(Sh::QBYTES + (uint32_t)(j % NK) * Sh::SLOT, k_full(j % NK), none[n], [&](int u) {
         if constexpr (Sh::STAGED) return *reinterpret_cast<const uint4 *>(smem + staged(n, 0, u));
-        else return raw_k[u];
+        else return raw_k[n][u];
       });
-      if constexpr (!Sh::STAGED) load(c.k, from, raw_k);
+      if constexpr (!Sh::STAGED) load(c.k, from, raw_k[n]);
       if (j >= NV && !mbar_wait(v_empty(j % NV), (j / NV - 1) & 1, abort_w, c.status, 0x6400)) return false;
       store(Sh::V0 + (uint32_t)(j % NV) * Sh::SLOT, v_full(j % NV), none[n], [&](int u) {
         if constexpr (Sh::STAGED) return *reinterpret_cast<const uint4 *>(smem + staged(n, 1, u));
-        else return raw_v[u];
+        else return raw_v[n][u];
       });
       if constexpr (Sh::STAGED) copy(n, from);
-      else load(c.v, from, raw_v);
+      else load(c.v, from, raw_v[n]);
       none[n] = none_next;
       return true;
     };
