@@ -8,86 +8,92 @@
 namespace tt {
 namespace {
 
-// 16 consecutive elements as fp32: four 16-byte loads (fp32) or two (16-bit).
-template <typename T, bool VEC>
-__device__ __forceinline__ void load16(const T *p, float *x) {
-  if constexpr (VEC) {
-    constexpr int N = 16 * sizeof(T) / 16, E = 16 / sizeof(T);
-    uint4 raw[N];
+// 16 bytes of input: 4 fp32 or 8 16-bit elements, as fp32 bits.
+template <typename T>
+constexpr int kPiece = 16 / sizeof(T);
+
+template <typename T>
+__device__ __forceinline__ void widen(const uint4 &raw, float *x) {
+  const T *e = reinterpret_cast<const T *>(&raw);
 #pragma unroll
-    for (int i = 0; i < N; ++i) raw[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const T *e = reinterpret_cast<const T *>(&raw[i]);
-#pragma unroll
-      for (int j = 0; j < E; ++j) x[i * E + j] = kv_to_float(e[j]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = kv_to_float(p[i]);
-  }
+  for (int i = 0; i < kPiece<T>; ++i) x[i] = kv_to_float(e[i]);
 }
 
-// One block per (sequence, page that new tokens of it land in, head, keys or
-// values): the block's chunks of 16 elements stay in registers between the
-// maximum and the rounding, so each new element is read once. The maximum is
-// taken on the bits of |x| (ordered like the values; infinities and NaN on
-// top), so it does not hang on the order of the reduction.
-template <typename T, int FMT, int THREADS, int NC, bool VEC>
-__global__ void __launch_bounds__(THREADS) kv_write_kernel(KvView c, const T *k, const T *v,
-                                                           KvStrides kst, KvStrides vst,
-                                                           int tokens, const int32_t *counts,
-                                                           int touched) {
-  __shared__ uint32_t s_max[THREADS / 32];
+// NW warps for each item: (sequence, page that new tokens of it land in, head, keys
+// or values). The item's pieces of 16 bytes stay in registers between the maximum
+// and the rounding, so each new element is read once, every load of a warp is 512
+// consecutive bytes, and an item of one warp meets no barrier. (One block of 256
+// threads an item, with 32 bytes a thread: 65 us for 16 prompts of 2048 tokens, 16
+// heads of 64, bf16.) The maximum is taken on the bits of |x| (ordered like the
+// values; infinities and NaN on top), so it does not hang on the order of the
+// reduction. Bound by memory for prompts, by its dependent loads (length, page,
+// scale) for a step.
+constexpr int block_warps(int nw) { return nw < 4 ? 4 : nw; }
+
+template <typename T, int FMT, int NW, int NC>
+__global__ void __launch_bounds__(32 * block_warps(NW))
+    kv_write_kernel(KvView c, const T *k, const T *v, KvStrides kst, KvStrides vst, int tokens,
+                    const int32_t *counts, int touched, unsigned items, bool vec) {
+  constexpr int E = kPiece<T>, LANES = 32 * NW;
+  __shared__ uint32_t s_max[block_warps(NW)];
   pdl_trigger();
-  int item = blockIdx.x;
-  const bool is_v = item & 1;
-  item >>= 1;
+  const int warp = threadIdx.x >> 5, lane = NW == 1 ? threadIdx.x & 31 : threadIdx.x % LANES;
+  unsigned item = blockIdx.x * (block_warps(NW) / NW) + warp / NW;
+  const bool any = item < items;
+  if (NW == 1 && !any) return;
+  if (!any) item = items - 1;  // to the barrier with the others, and nothing written
   const int h = item % c.heads;
   item /= c.heads;
+  const bool is_v = item & 1;
+  item >>= 1;
   const int b = item / touched, j = item % touched;
   pdl_wait();
   const int len = c.length(b), count = c.count(counts, b, tokens, len);
   const int start = len - count, page = 1 << c.page_log2;
   const int col = (start >> c.page_log2) + j;
   const int lo = max(start, col << c.page_log2), hi = min(len, (col + 1) << c.page_log2);
-  if (lo >= hi) return;  // no new token of this sequence in that page
-  const int pg = c.page_of(b, col);
-  if (pg < 0) return;  // tokens of a page that does not exist are dropped
-  const T *src = is_v ? v : k;
+  // no new token of this sequence in that page, or a page that does not exist
+  const int pg = any && lo < hi ? c.page_of(b, col) : -1;
+  if (NW == 1 && pg < 0) return;
   const KvStrides st = is_v ? vst : kst;
-  src += b * st.batch + h * st.head;
-  uint8_t *dst = (is_v ? c.v : c.k) + c.tile(pg, h);
-  float *scale_p = (is_v ? c.vs : c.ks) + (int64_t)pg * c.heads + h;
-  const int slot = lo & (page - 1);  // tokens the page held before
-  const float old = slot > 0 ? *scale_p : 0.f;
-  const int hd16 = c.hd >> 4, chunks = (hi - lo) * hd16;
+  const T *src = (is_v ? v : k) + b * st.batch + h * st.head + (int64_t)(lo - start) * st.token;
+  const int row = c.hd / E, pieces = pg >= 0 ? (hi - lo) * row : 0;  // pieces of a token, in all
 
-  float x[NC][16];
+  uint4 raw[NC];
+#pragma unroll
+  for (int u = 0; u < NC; ++u) {
+    const int i = u * LANES + lane;
+    raw[u] = make_uint4(0, 0, 0, 0);
+    if (i < pieces) {
+      const int t = i / row, d = (i - t * row) * E;
+      const T *p = src + t * st.token + d;
+      if (vec) {
+        raw[u] = __ldcs(reinterpret_cast<const uint4 *>(p));
+      } else {
+        T *e = reinterpret_cast<T *>(&raw[u]);
+#pragma unroll
+        for (int q = 0; q < E; ++q) e[q] = p[q];
+      }
+    }
+  }
+  const int slot = lo & (page - 1);  // tokens the page held before
+  float *scale_p = (is_v ? c.vs : c.ks) + (int64_t)max(pg, 0) * c.heads + h;
+  const float old = pg >= 0 && slot > 0 ? *scale_p : 0.f;
   uint32_t mx = 0;
 #pragma unroll
   for (int u = 0; u < NC; ++u) {
-    const int i = threadIdx.x + u * THREADS;
-    if (i < chunks) {
-      const int t = i / hd16, d = (i - t * hd16) << 4;
-      load16<T, VEC>(src + (int64_t)(lo - start + t) * st.token + d, x[u]);
-    } else {
+    float x[E];
+    widen<T>(raw[u], x);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[u][e] = 0.f;
-    }
+    for (int e = 0; e < E; ++e) mx = max(mx, __float_as_uint(x[e]) & 0x7fffffffu);
   }
-#pragma unroll
-  for (int u = 0; u < NC; ++u)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) mx = max(mx, __float_as_uint(x[u][e]) & 0x7fffffffu);
   mx = __reduce_max_sync(0xffffffffu, mx);
-  if constexpr (THREADS > 32) {
-    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = mx;
+  if constexpr (NW > 1) {
+    if ((threadIdx.x & 31) == 0) s_max[warp] = mx;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) mx = max(mx, s_max[w]);
-  } else {
-    __syncwarp();
+    for (int w = 0; w < NW; ++w) mx = max(mx, s_max[warp / NW * NW + w]);
+    if (pg < 0) return;
   }
   // the exponent: |x| = 1.m * 2^e; 448 = 1.75 * 2^8, 127 = 1.984375 * 2^6
   constexpr int TOP_E = FMT == TT_KV_INT8 ? 6 : 8;
@@ -97,12 +103,13 @@ __global__ void __launch_bounds__(THREADS) kv_write_kernel(KvView c, const T *k,
   e = max(e, kKvLeastExponent);
   float scale = kv_pow2(bad ? 0 : e);
   if (!bad) scale = fmaxf(scale, old);
-  const float inv = bad ? 0.f : 1.f / scale;  // a power of two: exact
-  if (threadIdx.x == 0) *scale_p = bad ? __int_as_float(0x7fc00000) : scale;
+  const float inv = 1.f / scale;  // a power of two: exact
+  uint8_t *dst = (is_v ? c.v : c.k) + c.tile(pg, h);
+  if (lane == 0) *scale_p = bad ? __int_as_float(0x7fc00000) : scale;
   if (slot > 0 && !bad && scale != old) {
     // the page's scale grew: its old codes move to the new one
     const float ratio = old * inv;
-    for (int i = threadIdx.x; i < slot * hd16; i += THREADS) {
+    for (int i = lane; i < slot * (c.hd >> 4); i += LANES) {
       uint4 w = reinterpret_cast<uint4 *>(dst)[i];
       uint32_t *ww = &w.x;
 #pragma unroll
@@ -116,61 +123,73 @@ __global__ void __launch_bounds__(THREADS) kv_write_kernel(KvView c, const T *k,
       reinterpret_cast<uint4 *>(dst)[i] = w;
     }
   }
-  uint4 *out = reinterpret_cast<uint4 *>(dst + slot * c.hd);
+  uint32_t *out = reinterpret_cast<uint32_t *>(dst + slot * c.hd);
 #pragma unroll
   for (int u = 0; u < NC; ++u) {
-    const int i = threadIdx.x + u * THREADS;
-    if (i >= chunks) break;
-    uint32_t w[4];
+    const int i = u * LANES + lane;
+    if (i >= pieces) break;
+    float x[E];
+    widen<T>(raw[u], x);
+    uint32_t w[E / 4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < E / 4; ++q) {
       float y[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) y[r] = bad ? 0.f : x[u][4 * q + r] * inv;
+      for (int r = 0; r < 4; ++r) y[r] = bad ? 0.f : x[4 * q + r] * inv;
       w[q] = kv_encode4<FMT>(y);
     }
-    out[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    if constexpr (E == 8) reinterpret_cast<uint2 *>(out)[i] = make_uint2(w[0], w[1]);
+    else out[i] = w[0];
   }
 }
 
-// One thread per 16 codes of (keys or values, sequence, token, head); rows
-// behind a sequence's end, and of pages that do not exist, are zero.
+// A thread takes 16 bytes of output in each of kReadRows rows ((token, head) pairs),
+// whose loads it has under way at once; x runs along a row, so every store of a warp
+// covers consecutive bytes. Rows behind a sequence's end, and of pages that do not
+// exist, are zero.
+constexpr int kReadRows = 4;
+
 template <typename T, int FMT>
-__global__ void __launch_bounds__(256) kv_read_kernel(KvView c, T *k, T *v, uint32_t per_seq) {
+__global__ void __launch_bounds__(256) kv_read_kernel(KvView c, T *k, T *v, uint32_t rows) {
+  constexpr int E = kPiece<T>;
   pdl_trigger();
   pdl_wait();
-  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
-  if (i >= per_seq) return;
-  const int b = blockIdx.y;
-  const uint32_t hd16 = c.hd >> 4;
-  const uint32_t d16 = i % hd16, r = i / hd16;
-  const int h = r % c.heads, t = r / c.heads;
-  float x[16];
+  const int b = blockIdx.y, d = threadIdx.x * E;
+  const uint32_t r0 = (blockIdx.x * kReadRows) * blockDim.y + threadIdx.y;
+  const int len = c.length(b);
+  const uint8_t *pool = blockIdx.z ? c.v : c.k;
+  const float *scales = blockIdx.z ? c.vs : c.ks;
+  uint2 w[kReadRows];
+  float s[kReadRows];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) x[e] = 0.f;
-  if (t < c.length(b)) {
-    const int pg = c.page_of(b, t >> c.page_log2);
-    if (pg >= 0) {
-      const int64_t off = c.tile(pg, h) + (int64_t)(t & ((1 << c.page_log2) - 1)) * c.hd + 16 * d16;
-      const uint4 w = *reinterpret_cast<const uint4 *>((blockIdx.z ? c.v : c.k) + off);
-      const float s = (blockIdx.z ? c.vs : c.ks)[(int64_t)pg * c.heads + h];
-      kv_decode4<FMT>(w.x, x);
-      kv_decode4<FMT>(w.y, x + 4);
-      kv_decode4<FMT>(w.z, x + 8);
-      kv_decode4<FMT>(w.w, x + 12);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] *= s;
+  for (int u = 0; u < kReadRows; ++u) {
+    const uint32_t r = r0 + u * blockDim.y;
+    const int t = r / c.heads, h = r - t * c.heads;
+    w[u] = make_uint2(0, 0);
+    s[u] = 0.f;
+    if (r < rows && t < len) {
+      const int pg = c.page_of(b, t >> c.page_log2);
+      if (pg >= 0) {
+        const uint8_t *p = pool + c.tile(pg, h) + (t & ((1 << c.page_log2) - 1)) * c.hd + d;
+        if constexpr (E == 8) w[u] = __ldcs(reinterpret_cast<const uint2 *>(p));
+        else w[u].x = __ldcs(reinterpret_cast<const uint32_t *>(p));
+        s[u] = scales[(int64_t)pg * c.heads + h];
+      }
     }
   }
-  T *out = (blockIdx.z ? v : k) + ((int64_t)b * per_seq + i) * 16;
-  constexpr int N = 16 * sizeof(T) / 16, E = 16 / sizeof(T);
+  T *out = (blockIdx.z ? v : k) + (int64_t)b * rows * c.hd + d;
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
+  for (int u = 0; u < kReadRows; ++u) {
+    const uint32_t r = r0 + u * blockDim.y;
+    if (r >= rows) break;
+    float x[8];
+    kv_decode4<FMT>(w[u].x, x);
+    if constexpr (E == 8) kv_decode4<FMT>(w[u].y, x + 4);
     uint4 raw;
     T *e = reinterpret_cast<T *>(&raw);
 #pragma unroll
-    for (int q = 0; q < E; ++q) kv_store(e + q, x[n * E + q]);
-    __stcs(reinterpret_cast<uint4 *>(out) + n, raw);
+    for (int q = 0; q < E; ++q) kv_store(e + q, x[q] * s[u]);
+    __stcs(reinterpret_cast<uint4 *>(out + (int64_t)r * c.hd), raw);
   }
 }
 
@@ -188,16 +207,15 @@ bool vec_ok(const void *p, const KvStrides &s, int size) {
          (s.token * size) % 16 == 0 && (s.head * size) % 16 == 0;
 }
 
-template <typename T, int FMT, int THREADS, int NC>
+template <typename T, int FMT, int NW, int NC>
 int write_nc(const KvView &c, const void *k, const void *v, KvStrides ks, KvStrides vs,
              int tokens, const int32_t *counts, int touched, unsigned items,
              cudaStream_t stream) {
   const bool vec = vec_ok(k, ks, sizeof(T)) && vec_ok(v, vs, sizeof(T));
-  auto *kern = vec ? kv_write_kernel<T, FMT, THREADS, NC, true>
-                   : kv_write_kernel<T, FMT, THREADS, NC, false>;
-  TT_CUDA_TRY(launch_kernel(kern, dim3(items), dim3(THREADS), 0, stream, 1, c,
-                            static_cast<const T *>(k), static_cast<const T *>(v), ks, vs, tokens,
-                            counts, touched));
+  constexpr int per_block = block_warps(NW) / NW;
+  TT_CUDA_TRY(launch_kernel(kv_write_kernel<T, FMT, NW, NC>, dim3((items + per_block - 1) / per_block),
+                            dim3(32 * block_warps(NW)), 0, stream, 1, c, static_cast<const T *>(k),
+                            static_cast<const T *>(v), ks, vs, tokens, counts, touched, items, vec));
   return TT_OK;
 }
 
@@ -208,14 +226,16 @@ int write_typed(const KvView &c, const void *k, const void *v, KvStrides ks, KvS
   const int touched = (tokens + page - 2) / page + 1;  // pages that `tokens` in a row can touch
   const int64_t items = (int64_t)2 * c.heads * touched * c.batch;
   if (items > INT32_MAX) return fail(TT_ERR_UNSUPPORTED, "tt_kv_write: too many tokens");
-  const int chunks = std::min(tokens, page) * (c.hd >> 4);  // of 16 elements, in one page
-#define TT_KV_WRITE(THREADS, NC) \
-  return write_nc<T, FMT, THREADS, NC>(c, k, v, ks, vs, tokens, counts, touched, (unsigned)items, stream)
-  if (chunks <= 32) TT_KV_WRITE(32, 1);
-  if (chunks <= 256) TT_KV_WRITE(256, 1);
-  if (chunks <= 512) TT_KV_WRITE(256, 2);
-  if (chunks <= 1024) TT_KV_WRITE(256, 4);
-  TT_KV_WRITE(256, 8);  // 128 tokens of 256 elements, the largest page
+  const int pieces = std::min(tokens, page) * (c.hd / kPiece<T>);  // of 16 bytes, in one page
+#define TT_KV_WRITE(NW, NC) \
+  return write_nc<T, FMT, NW, NC>(c, k, v, ks, vs, tokens, counts, touched, (unsigned)items, stream)
+  if (pieces <= 32) TT_KV_WRITE(1, 1);
+  if (pieces <= 128) TT_KV_WRITE(1, 4);
+  if (pieces <= 512) TT_KV_WRITE(1, 16);
+  if (pieces <= 1024) TT_KV_WRITE(2, 16);
+  if (pieces <= 2048) TT_KV_WRITE(4, 16);
+  if (pieces <= 4096) TT_KV_WRITE(8, 16);
+  TT_KV_WRITE(16, 16);  // 128 tokens of 256 fp32 elements, the largest page
 #undef TT_KV_WRITE
 }
 
@@ -247,13 +267,13 @@ int launch_kv_mask(const KvView &c, const int32_t *counts, int64_t tokens, uint8
 
 template <typename T>
 static int read_typed(const KvView &c, void *k, void *v, int64_t max_tokens, cudaStream_t stream) {
-  const int64_t per_seq = max_tokens * c.heads * (c.hd >> 4);
-  if (per_seq > UINT32_MAX - 256 || c.batch > 65535)
+  const int64_t rows = max_tokens * c.heads;
+  if (rows > INT32_MAX || c.batch > 65535)
     return fail(TT_ERR_UNSUPPORTED, "tt_kv_read: too many tokens or sequences");
   auto *kern = c.format == TT_KV_INT8 ? kv_read_kernel<T, TT_KV_INT8> : kv_read_kernel<T, TT_KV_E4M3>;
-  TT_CUDA_TRY(launch_kernel(kern, dim3((unsigned)ceil_div(per_seq, 256), c.batch, 2), dim3(256), 0,
-                            stream, 1, c, static_cast<T *>(k), static_cast<T *>(v),
-                            (uint32_t)per_seq));
+  const unsigned x = c.hd / kPiece<T>, y = 256 / x;
+  TT_CUDA_TRY(launch_kernel(kern, dim3((unsigned)ceil_div(rows, y * kReadRows), c.batch, 2), dim3(x, y), 0,
+                            stream, 1, c, static_cast<T *>(k), static_cast<T *>(v), (uint32_t)rows));
   return TT_OK;
 }
 
