@@ -19,6 +19,24 @@ __device__ __forceinline__ void widen(const uint4 &raw, float *x) {
   for (int i = 0; i < kPiece<T>; ++i) x[i] = kv_to_float(e[i]);
 }
 
+// The larger of the magnitudes in `mx` and those of 16 bytes, on their bits: fp32
+// words, or two 16-bit halves a word (integers order like the values; infinities
+// and NaN come on top); and the bits of that maximum as fp32.
+template <typename T>
+__device__ __forceinline__ uint32_t magnitude(uint32_t mx, const uint4 &raw) {
+  const uint32_t *w = &raw.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    mx = sizeof(T) == 4 ? max(mx, w[i] & 0x7fffffffu) : __vmaxu2(mx, w[i] & 0x7fff7fffu);
+  return mx;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t magnitude_bits(uint32_t mx) {
+  if constexpr (sizeof(T) == 4) return mx;
+  const uint16_t h = (uint16_t)max(mx & 0xffffu, mx >> 16);
+  return __float_as_uint(kv_to_float(*reinterpret_cast<const T *>(&h))) & 0x7fffffffu;
+}
+
 // NW warps for each item: (sequence, page that new tokens of it land in, head, keys
 // or values). The item's pieces of 16 bytes stay in registers between the maximum
 // and the rounding, so each new element is read once, every load of a warp is 512
@@ -81,13 +99,8 @@ __global__ void __launch_bounds__(32 * block_warps(NW))
   const float old = pg >= 0 && slot > 0 ? *scale_p : 0.f;
   uint32_t mx = 0;
 #pragma unroll
-  for (int u = 0; u < NC; ++u) {
-    float x[E];
-    widen<T>(raw[u], x);
-#pragma unroll
-    for (int e = 0; e < E; ++e) mx = max(mx, __float_as_uint(x[e]) & 0x7fffffffu);
-  }
-  mx = __reduce_max_sync(0xffffffffu, mx);
+  for (int u = 0; u < NC; ++u) mx = magnitude<T>(mx, raw[u]);
+  mx = __reduce_max_sync(0xffffffffu, magnitude_bits<T>(mx));
   if constexpr (NW > 1) {
     if ((threadIdx.x & 31) == 0) s_max[warp] = mx;
     __syncthreads();
