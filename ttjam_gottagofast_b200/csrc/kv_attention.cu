@@ -10,13 +10,20 @@
 // with M the running maximum of s' + e rounded up to a whole number, so that
 // e - M and every rescaling by 2^(M_old - M_new) are exact.
 //
-// A block of 8 query rows of one key head is one m16n8k16 tensor-core operand:
-// q and p are split into two fp16 pieces (22 significant bits, as the forward's
-// split-precision schedule), the high pieces in operand rows 0-7, the low ones
-// in rows 8-15, whose products meet in one thread's accumulators. So a step of
-// one token has fp32 accuracy at the cost of one product, and the codes, exact
-// in fp16, are the other operand. Row q is scaled by a power of two to have its
-// largest element in [1, 2), p by 2^14 to stay clear of the fp16 subnormals.
+// Tensor cores, m16n8k16: 16 tokens' codes, exact in fp16, are the 16-row operand of
+// both products (S^T = K q^T, O^T = V^T p^T), a block of 8 query rows of one key head
+// the 8 columns of the other. q and p are split into two fp16 pieces (22 significant
+// bits, as the forward's split-precision schedule), both added into the same sums,
+// so a step of one token has fp32 accuracy. p leaves the first product with the token
+// along the rows and enters the second along them too; a transposition of 8 x 8
+// fp16 values between registers (movmatrix) lies in between. Row q is scaled by a
+// power of two to have its largest element in [1, 2), p by 2^14 to stay clear of the
+// fp16 subnormals.
+//
+// Where a key head has a single query row (ONE: a step of one token without grouped
+// heads), the 8 columns hold the two pieces for each of 4 groups of 16 tokens instead:
+// every lane then works on 2 tokens of 64 rather than every eighth on one, and the
+// sums of a group's columns meet at the end.
 //
 // A warp takes kStep tokens at a time from a ring of its own in shared memory,
 // which its lanes fill with asynchronous 16-byte copies up to kStages steps ahead,
@@ -47,17 +54,19 @@ constexpr int kRows = 8;     // query rows per block
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 
-template <int HD>
+template <int HD, bool ONE>
 struct RowShape {
-  static constexpr int GC = HD == 32 ? 4 : HD == 64 ? 2 : 1;  // groups of 16 tokens computed at once
-  static constexpr int GR = HD <= 64 ? 2 * GC : GC;   // ... and copied at once: a step
+  // groups of 16 tokens computed at once
+  static constexpr int GC = HD == 32 ? 4 : HD == 64 ? (ONE ? 4 : 2) : HD == 128 && ONE ? 2 : 1;
+  // ... and copied at once: a step
+  static constexpr int GR = HD == 32 ? 8 : HD == 64 ? 4 : GC;
   static constexpr int kStep = 16 * GR;              // tokens
-  static constexpr int kOver = HD <= 64 ? 1 : 2;     // units of a segment besides its steps
-  static constexpr int kWhole = HD <= 64 ? 2 : 4;                   // steps of a segment that is never split
-  static constexpr int kStages = HD == 128 ? 3 : 2;  // steps in a warp's ring
+  static constexpr int kOver = GR >= 4 ? 1 : 2;      // units of a segment besides its steps
+  static constexpr int kWhole = GR >= 4 ? 2 : 4;                   // steps of a segment that is never split
+  static constexpr int kStages = HD == 128 && !ONE ? 3 : 2;  // steps in a warp's ring
   static constexpr uint32_t kStage = 2 * kStep * HD;  // bytes: keys, then values
   static constexpr uint32_t kSmem = kWarps * kStages * kStage;
-  static constexpr int kCtas = HD == 256 ? 2 : 3;    // per SM, as registers and shared memory allow
+  static constexpr int kCtas = HD == 256 && !ONE ? 2 : 3;                    // per SM, as registers and shared memory allow
   // tensor cores add by rounding toward zero: after 1024 tokens the sum moves to the
   // place of the warp's partial result, so that it does not drift
   static constexpr int kFlush = 1024 / kStep;
@@ -88,6 +97,13 @@ __device__ __forceinline__ void lds(uint32_t addr, uint32_t *r) {
   else
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r[0]) : "r"(addr));
 }
+// An 8 x 8 matrix of 16-bit values, row lane / 4, columns 2 (lane % 4) and the next:
+// transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 // c += a b (or c = a b); not volatile, so that independent products are interleaved
 __device__ __forceinline__ void mma16816(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
@@ -104,9 +120,9 @@ __device__ __forceinline__ void mma16816_first(float *c, const uint32_t *a, uint
 
 // Units of a segment of sequence b; at least one step, which writes the zeros of
 // a sequence that has no new token.
-template <int HD>
+template <int HD, bool ONE>
 __device__ __forceinline__ int units_of(const KvAttentionArgs &a, int b, int &len, int &count) {
-  using Sh = RowShape<HD>;
+  using Sh = RowShape<HD, ONE>;
   len = a.c.length(b);
   count = a.c.count(a.counts, b, a.tokens, len);
   return Sh::kOver + (count > 0 ? (len + Sh::kStep - 1) / Sh::kStep : 1);
@@ -129,7 +145,7 @@ __device__ __forceinline__ int chunk_swizzle(int row) {
 
 // Where a warp's run of units stands: unit t of the segment whose units [lo, hi)
 // the run holds. The steps are the units from kOver on.
-template <int HD>
+template <int HD, bool ONE>
 struct Cursor {
   int64_t left;  // units of the run from unit lo of this segment on
   int b, len, count, units, pair, t, lo, hi;
@@ -142,7 +158,7 @@ struct Cursor {
   }
   __device__ __forceinline__ void bound(bool whole) {
     hi = whole ? units : (int)min((int64_t)units, lo + left);
-    t = max(lo, RowShape<HD>::kOver);
+    t = max(lo, RowShape<HD, ONE>::kOver);
   }
   // to the run's next segment; false at its end
   __device__ __forceinline__ bool next(const KvAttentionArgs &a, int64_t hr, bool whole) {
@@ -150,7 +166,7 @@ struct Cursor {
     if (left <= 0) return false;
     if (++pair >= hr) {
       pair = 0;
-      units = units_of<HD>(a, ++b, len, count);
+      units = units_of<HD, ONE>(a, ++b, len, count);
     }
     lo = 0;
     bound(whole);
@@ -171,11 +187,12 @@ __device__ __forceinline__ int out_dim(int w, int i, int n) {
   else return 128 * (w / 4) + 16 * n + 4 * (w % 4) + i;
 }
 
-template <int HD, int FMT, bool EXACT>
-__global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
+template <int HD, int FMT, bool EXACT, bool ONE>
+__global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
     kv_attention_rows_kernel(KvAttentionArgs a, int row_blocks, bool whole) {
-  using Sh = RowShape<HD>;
+  using Sh = RowShape<HD, ONE>;
   constexpr int KW = Sh::KW, VW = Sh::VW, GR = Sh::GR, GC = Sh::GC, S = Sh::kStages;
+  constexpr int NR = ONE ? 1 : 2;  // rows of a lane's results
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int64_t s_scan[kThreads];
   const KvView &c = a.c;
@@ -193,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
   int64_t mine = 0;
   for (int b = b0; b < b1; ++b) {
     int len, count;
-    mine += units_of<HD>(a, b, len, count);
+    mine += units_of<HD, ONE>(a, b, len, count);
   }
   // inclusive sums over the threads
 #pragma unroll
@@ -212,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
   const int64_t run = (total + gridDim.x * kWarps - 1) / (gridDim.x * kWarps);
   const int64_t lo = gw * run;
   if (lo >= total) return;
-  Cursor<HD> use;  // what is computed; `fill` below is what is copied, ahead of it
+  Cursor<HD, ONE> use;  // what is computed; `fill` below is what is copied, ahead of it
   use.left = min(run, total - lo);
   {
     int t = 0;  // threads whose sequences end at or before lo
@@ -221,10 +238,10 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
       t += __popc(__ballot_sync(0xffffffffu, s_scan[32 * k + lane] * hr <= lo));
     use.b = t * per_thread;
     int64_t first = t > 0 ? s_scan[t - 1] * hr : 0;
-    use.units = units_of<HD>(a, use.b, use.len, use.count);
+    use.units = units_of<HD, ONE>(a, use.b, use.len, use.count);
     while (first + use.units * hr <= lo) {
       first += use.units * hr;
-      use.units = units_of<HD>(a, ++use.b, use.len, use.count);
+      use.units = units_of<HD, ONE>(a, ++use.b, use.len, use.count);
     }
     use.enter(lo - first, whole);
     // whole segments belong to the run that holds their first unit
@@ -233,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
   }
 
   // tokens that the last live row of the cursor's row block sees
-  auto seen_by_block = [&](const Cursor<HD> &u) {
+  auto seen_by_block = [&](const Cursor<HD, ONE> &u) {
     const int rb = u.pair % row_blocks;
     const int r_first = rb * kRows / a.group;
     const int r_last = min(rb * kRows + kRows - 1, rows_all - 1) / a.group;
@@ -246,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
   // scales wait in the lane's queue for as long as the bytes do in the ring. A
   // group without a page, or past the last seen token, copies nothing and has the
   // key scale -1.
-  Cursor<HD> fill = use;
+  Cursor<HD, ONE> fill = use;
   bool more = true;
   int fill_end = seen_by_block(fill), fill_stage = 0, pg_next;
   float q_ks[S], q_vs[S];
@@ -308,29 +325,30 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
   while (going) {
     const int h = use.pair / row_blocks, rb = use.pair % row_blocks;
     const int b = use.b, len = use.len, count = use.count;
-    // the row of this thread's accumulators, and the tokens it sees
-    const int r = rb * kRows + gid;
-    const int tok = r / a.group;
-    const bool live = r < rows_all && tok < count;
-    const int end = live ? len - count + tok + 1 : 0;
     const int r_first = rb * kRows / a.group;
     const int all_end = len - count + min(r_first, count) + 1;  // tokens that every live row sees
     const int any_end = seen_by_block(use);
+    // the block's row that column n stands for, its token and how many tokens that sees
+    auto row_of = [&](int n) { return rb * kRows + (ONE ? 0 : n); };
+    auto end_of = [&](int r) {
+      const int tok = r / a.group;
+      return r < rows_all && tok < count ? len - count + tok + 1 : 0;
+    };
 
-    // q, scaled to [1, 2) and split
-    uint32_t qa[KW][4];
-    float sc;
+    // q of column gid, scaled to [1, 2) and split
+    uint32_t qb[KW][ONE ? 2 : 4];
+    float sc[NR];
     {
       float x[KW][4];
       float mx = 0.f;
+      const int r = row_of(gid), tok = r / a.group;
+      const bool live = end_of(r) > 0;
       const int64_t off = b * a.qs.batch + tok * a.qs.token + (h * a.group + r % a.group) * a.qs.head;
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
         const int d = HD == 32 ? 8 * tig + 4 * w : 64 * (w / 4) + 16 * tig + 4 * (w % 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[w][i] = 0.f;
-        }
+        for (int i = 0; i < 4; ++i) x[w][i] = 0.f;
         if (live && d < hd) kv_load_in4(a.dtype, a.q, off + d, a.q_vec, x[w]);
       }
 #pragma unroll
@@ -345,32 +363,58 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
       const float f = kv_pow2(-e);
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
-        f16_split2(x[w][0] * f, x[w][1] * f, qa[w][0], qa[w][1]);
-        f16_split2(x[w][2] * f, x[w][3] * f, qa[w][2], qa[w][3]);
+        uint32_t hi[2], lo[2];
+        f16_split2(x[w][0] * f, x[w][1] * f, hi[0], lo[0]);
+        f16_split2(x[w][2] * f, x[w][3] * f, hi[1], lo[1]);
+        if constexpr (ONE) {  // even columns the high pieces, odd ones the low ones
+          qb[w][0] = gid & 1 ? lo[0] : hi[0];
+          qb[w][1] = gid & 1 ? lo[1] : hi[1];
+        } else {
+          qb[w][0] = hi[0], qb[w][1] = hi[1], qb[w][2] = lo[0], qb[w][3] = lo[1];
+        }
       }
-      sc = a.scale * 1.4426950408889634f * kv_pow2(e);
+      const float scale = a.scale * 1.4426950408889634f * kv_pow2(e);
+#pragma unroll
+      for (int j = 0; j < NR; ++j) sc[j] = __shfl_sync(0xffffffffu, scale, 4 * (2 * tig + j));
     }
 
-    float m = -CUDART_INF_F, l = 0.f;
-    float o[4 * VW][4];
+    // rows of this lane's results: columns 2 tig + j
+    int end[NR];
+    float m[NR], l[NR];
 #pragma unroll
-    for (int i = 0; i < 4 * VW; ++i)
+    for (int j = 0; j < NR; ++j) {
+      end[j] = end_of(row_of(2 * tig + j));
+      m[j] = -CUDART_INF_F, l[j] = 0.f;
+    }
+    float o[2 * VW][4];  // dims out_dim(w, 0, gid) + 0 .. 3 in tiles 2 w and 2 w + 1
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+    for (int i = 0; i < 2 * VW; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
     const int t_lo = use.t, t_hi = use.hi;
     const bool from_start = t_lo == Sh::kOver, done = from_start && t_hi == use.units;
     float *const slot = a.ws + ((int64_t)gw * 2 + (from_start ? 1 : 0)) * Sh::kSlot;
     bool flushed = false;
-    float beta = 1.f;  // what the flushed sum is scaled by when read next
-    // the sums of this thread's dims out_dim(w, 0, 2 tig + n) and the three after it
-    auto sums = [&](int w, int n, float *v) {
-      float4 *at = reinterpret_cast<float4 *>(slot + gid * HD + out_dim<HD>(w, 0, 2 * tig + n));
+    float beta[NR];  // what the flushed sums are scaled by when read next
+    // the sums of row j, dims out_dim(w, 0, gid) and the three after it. (ONE: the
+    // columns' sums meet in every lane of a quad; one of them keeps them.)
+    auto sums = [&](int w, int j, float *v) {
+      float4 *at = reinterpret_cast<float4 *>(slot + (ONE ? 0 : 2 * tig + j) * HD + out_dim<HD>(w, 0, gid));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = o[4 * w + i][n] + o[4 * w + i][2 + n];
-      if (flushed) {
+      for (int i = 0; i < 4; ++i) {
+        const float *c4 = o[2 * w + i / 2] + 2 * (i % 2);
+        if constexpr (ONE) {
+          v[i] = c4[0] + c4[1];
+          v[i] += __shfl_xor_sync(0xffffffffu, v[i], 1);
+          v[i] += __shfl_xor_sync(0xffffffffu, v[i], 2);
+        } else {
+          v[i] = c4[j];
+        }
+      }
+      if (flushed && (!ONE || tig == 0)) {
         const float4 f = *at;
-        v[0] = fmaf(f.x, beta, v[0]), v[1] = fmaf(f.y, beta, v[1]);
-        v[2] = fmaf(f.z, beta, v[2]), v[3] = fmaf(f.w, beta, v[3]);
+        v[0] = fmaf(f.x, beta[j], v[0]), v[1] = fmaf(f.y, beta[j], v[1]);
+        v[2] = fmaf(f.z, beta[j], v[2]), v[3] = fmaf(f.w, beta[j], v[3]);
       }
       return at;
     };
@@ -378,88 +422,157 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
 #pragma unroll
       for (int w = 0; w < VW; ++w)
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
+        for (int j = 0; j < NR; ++j) {
           float v[4];
-          float4 *at = sums(w, n, v);
-          *at = make_float4(v[0], v[1], v[2], v[3]);
+          float4 *at = sums(w, j, v);
+          if (!ONE || tig == 0) *at = make_float4(v[0], v[1], v[2], v[3]);
         }
       flushed = true;
-      beta = 1.f;
+#pragma unroll
+      for (int j = 0; j < NR; ++j) beta[j] = 1.f;
+#pragma unroll
+      for (int i = 0; i < 2 * VW; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
     };
     // groups g0 .. g0 + GC - 1 of a step, the first at token t0: scores, running
-    // maximum, p, p v
+    // maximum, p, p v. A lane's scores: rows j, tokens 8 x + half_token(gid) of group g;
+    // ONE: of group tig alone.
+    constexpr int GS = ONE ? 1 : GC;
     auto compute = [&](auto masked_form, int g0, int t0, uint32_t absent) {
       constexpr bool MASKED = decltype(masked_form)::value;
       const uint32_t kb = ring + stage * Sh::kStage + 16 * g0 * hd;
       const uint32_t vb = kb + Sh::kStep * hd;
-      float s[GC][2][4];
+      float s[GS][2][NR];
       {
         constexpr int LB = HD == 32 ? 8 : 16;  // bytes a load
-        uint32_t w[GC][2][KW];
+        float acc[GC][4];
 #pragma unroll
-        for (int g = 0; g < GC; ++g)
+        for (int g = 0; g < GC; ++g) {
+          uint32_t w[2][KW];
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const int r8 = half_token<HD>(gid);
             const uint32_t row = kb + (16 * g + 8 * x + r8) * hd;
 #pragma unroll
-            for (int j = 0; j < KW * 4 / LB; ++j) {
-              const int d = 4 * LB * j + LB * tig;
+            for (int i = 0; i < KW * 4 / LB; ++i) {
+              const int d = 4 * LB * i + LB * tig;
               if (EXACT || d < hd) {
-                lds<LB>(row + (d ^ (chunk_swizzle<HD, EXACT>(r8) << 4)), &w[g][x][j * (LB / 4)]);
+                lds<LB>(row + (d ^ (chunk_swizzle<HD, EXACT>(r8) << 4)), &w[x][i * (LB / 4)]);
               } else {
 #pragma unroll
-                for (int i = 0; i < LB / 4; ++i) w[g][x][j * (LB / 4) + i] = 0;
+                for (int k = 0; k < LB / 4; ++k) w[x][i * (LB / 4) + k] = 0;
               }
             }
           }
+          float low[4];  // the low pieces' sums, apart: two chains of products
 #pragma unroll
-        for (int i = 0; i < KW; ++i)
-#pragma unroll
-          for (int g = 0; g < GC; ++g)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              uint32_t k0, k1;
-              codes_along<FMT>(w[g][x][i], k0, k1);
-              if (i == 0) mma16816_first(s[g][x], qa[i], k0, k1);
-              else mma16816(s[g][x], qa[i], k0, k1);
+          for (int i = 0; i < KW; ++i) {
+            uint32_t k4[4];
+            codes_along<FMT>(w[0][i], k4[0], k4[2]);
+            codes_along<FMT>(w[1][i], k4[1], k4[3]);
+            if (i == 0) mma16816_first(acc[g], k4, qb[i][0], qb[i][1]);
+            else mma16816(acc[g], k4, qb[i][0], qb[i][1]);
+            if constexpr (!ONE) {
+              if (i == 0) mma16816_first(low, k4, qb[i][2], qb[i][3]);
+              else mma16816(low, k4, qb[i][2], qb[i][3]);
             }
-      }
-      // scores of this thread: row gid, tokens 8 x + half_token(2 tig + p) of group g
-      const float ve_lane = q_vs[0] == q_vs[0] ? (float)((__float_as_int(q_vs[0]) >> 23) - 127) : q_vs[0];
-      auto sees = [&](int g, int x, int p) {
-        return !((absent >> (g0 + g)) & 1u) && t0 + 16 * g + 8 * x + half_token<HD>(2 * tig + p) < end;
-      };
-      float kc[GC], ve[GC], top = -CUDART_INF_F;
-#pragma unroll
-      for (int g = 0; g < GC; ++g) {
-        ve[g] = __shfl_sync(0xffffffffu, ve_lane, g0 + g);
-        kc[g] = fabsf(__shfl_sync(0xffffffffu, q_ks[0], g0 + g)) * sc;  // never negative: it meets -inf
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            s[g][x][p] += s[g][x][2 + p];
-            if (MASKED && !sees(g, x, p)) s[g][x][p] = -CUDART_INF_F;
           }
-        const float mx = fmaxf(fmax3(s[g][0][0], s[g][0][1], s[g][1][0]), s[g][1][1]);
-        top = fmaxf(top, fmaf(mx, kc[g], ve[g]));
-      }
-      // p stays below 2^15: the reference moves when a score passes it by more than 1
-      if (__any_sync(0xffffffffu, top > m + 1.f)) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float mn = fmaxf(m, ceilf(top));
-        const float alpha = mn == m ? 1.f : exp2_approx(m - mn);  // 0 from -inf
-        m = mn;
-        l *= alpha;
-        beta *= alpha;
+          if constexpr (!ONE) {
 #pragma unroll
-        for (int i = 0; i < 4 * VW; ++i)
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) o[i][j] *= alpha;
+              for (int j = 0; j < NR; ++j) s[g][x][j] = acc[g][2 * x + j] + low[2 * x + j];
+          }
+        }
+        if constexpr (ONE) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float hi = acc[0][2 * x], lo = acc[0][2 * x + 1];
+#pragma unroll
+            for (int g = 1; g < GC; ++g) {
+              hi = tig == g ? acc[g][2 * x] : hi;
+              lo = tig == g ? acc[g][2 * x + 1] : lo;
+            }
+            s[0][x][0] = hi + lo;
+          }
+        }
       }
-      const float ref = 14.f - (m == -CUDART_INF_F ? 0.f : m);
+      const float ve_lane = q_vs[0] == q_vs[0] ? (float)((__float_as_int(q_vs[0]) >> 23) - 127) : q_vs[0];
+      auto group = [&](int g) { return ONE ? tig : g; };
+      auto sees = [&](int g, int x, int j) {
+        return !((absent >> (g0 + group(g))) & 1u) &&
+               t0 + 16 * group(g) + 8 * x + half_token<HD>(gid) < end[j];
+      };
+      float ks[GS], ve[GS], top[NR];
+#pragma unroll
+      for (int j = 0; j < NR; ++j) top[j] = -CUDART_INF_F;
+#pragma unroll
+      for (int g = 0; g < GS; ++g) {
+        ve[g] = __shfl_sync(0xffffffffu, ve_lane, g0 + group(g));
+        ks[g] = fabsf(__shfl_sync(0xffffffffu, q_ks[0], g0 + group(g)));  // never negative: it meets -inf
+#pragma unroll
+        for (int j = 0; j < NR; ++j) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            if ((MASKED && !sees(g, x, j)) || (ONE && GC < 4 && tig >= GC)) s[g][x][j] = -CUDART_INF_F;
+          top[j] = fmaxf(top[j], fmaf(fmaxf(s[g][0][j], s[g][1][j]), ks[g] * sc[j], ve[g]));
+        }
+      }
+      // p stays below 2^15: a row's reference moves when a score passes it by more than 1
+      bool moves = false;
+#pragma unroll
+      for (int j = 0; j < NR; ++j) moves |= top[j] > m[j] + 1.f;
+      if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+        for (int j = 0; j < NR; ++j) {
+#pragma unroll
+          for (int k = ONE ? 1 : 4; k < 32; k *= 2) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], k));
+          const float mn = fmaxf(m[j], ceilf(top[j]));
+          const float alpha = mn == m[j] ? 1.f : exp2_approx(m[j] - mn);  // 0 from -inf
+          m[j] = mn;
+          l[j] *= alpha;
+          beta[j] *= alpha;
+#pragma unroll
+          for (int i = 0; i < 2 * VW; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (ONE || (k & 1) == j) o[i][k] *= alpha;
+        }
+      }
+      float ref[NR];
+#pragma unroll
+      for (int j = 0; j < NR; ++j) ref[j] = 14.f - (m[j] == -CUDART_INF_F ? 0.f : m[j]);
+      uint32_t pb[2][2];  // p of a group as the second product's columns: [piece][half]
+      auto probabilities = [&](int g) {
+        float p[2][NR];
+#pragma unroll
+        for (int j = 0; j < NR; ++j) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            p[x][j] = exp2_approx(fmaf(s[g][x][j], ks[g] * sc[j], ve[g] + ref[j]));
+            // a NaN scale leaves NaN at the tokens behind the mask
+            if ((MASKED && !sees(g, x, j)) || (ONE && GC < 4 && tig >= GC)) p[x][j] = 0.f;
+          }
+          // 2^-e; a NaN counts only where a token of its page is seen
+          const float sum = p[0][j] + p[1][j], more_l = fmaf(sum, exp2_approx(-ve[g]), l[j]);
+          l[j] = !(MASKED || (ONE && GC < 4)) || sum != 0.f ? more_l : l[j];
+        }
+        uint32_t hi[2], lo[2];
+        if constexpr (ONE) {  // (high, low) of each token: the columns of group tig
+          f16_split2(p[0][0], p[1][0], hi[0], lo[0]);
+          pb[0][0] = transpose8(__byte_perm(hi[0], lo[0], 0x5410));
+          pb[0][1] = transpose8(__byte_perm(hi[0], lo[0], 0x7632));
+        } else {  // (row 2 tig, row 2 tig + 1) of each token
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            f16_split2(p[x][0], p[x][NR - 1], hi[x], lo[x]);
+            pb[0][x] = transpose8(hi[x]);
+            pb[1][x] = transpose8(lo[x]);
+          }
+        }
+      };
+      if constexpr (ONE) probabilities(0);
 #pragma unroll
       for (int g = 0; g < GC; ++g) {
         uint32_t v[2][2][VW];
@@ -471,13 +584,13 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
             const int in_g = 8 * x + half_token<HD>(2 * tig + q);
             const uint32_t row = vb + (16 * g + in_g) * hd;
 #pragma unroll
-            for (int j = 0; j < VW * 4 / LB; ++j) {
-              const int d = 8 * LB * j + LB * gid;
+            for (int i = 0; i < VW * 4 / LB; ++i) {
+              const int d = 8 * LB * i + LB * gid;
               if (EXACT || d < hd) {
-                lds<LB>(row + (d ^ (chunk_swizzle<HD, EXACT>(in_g & 7) << 4)), &v[x][q][j * (LB / 4)]);
+                lds<LB>(row + (d ^ (chunk_swizzle<HD, EXACT>(in_g & 7) << 4)), &v[x][q][i * (LB / 4)]);
               } else {
 #pragma unroll
-                for (int i = 0; i < LB / 4; ++i) v[x][q][j * (LB / 4) + i] = 0;
+                for (int k = 0; k < LB / 4; ++k) v[x][q][i * (LB / 4) + k] = 0;
               }
             }
             // what stands behind the last token may be any bits, e4m3's NaN among them
@@ -486,30 +599,27 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
               for (int i = 0; i < VW; ++i) v[x][q][i] = 0;
             }
           }
-        const float base = ve[g] + ref;
-        float p[2][2];
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            p[x][q] = exp2_approx(fmaf(s[g][x][q], kc[g], base));
-            // a NaN scale leaves NaN at the tokens behind the mask
-            if (MASKED && !sees(g, x, q)) p[x][q] = 0.f;
-          }
-        const float sum = (p[0][0] + p[0][1]) + (p[1][0] + p[1][1]);
-        // 2^-e; a NaN counts only where a token of its page is seen
-        const float more_l = fmaf(sum, exp2_approx(-ve[g]), l);
-        l = !MASKED || sum != 0.f ? more_l : l;
-        uint32_t pa[4];
-        f16_split2(p[0][0], p[0][1], pa[0], pa[1]);
-        f16_split2(p[1][0], p[1][1], pa[2], pa[3]);
+        uint32_t b4[2][2];
+        if constexpr (ONE) {  // only the columns of this group
+          b4[0][0] = gid >> 1 == g ? pb[0][0] : 0u;
+          b4[0][1] = gid >> 1 == g ? pb[0][1] : 0u;
+        } else {
+          probabilities(g);
+          b4[0][0] = pb[0][0], b4[0][1] = pb[0][1], b4[1][0] = pb[1][0], b4[1][1] = pb[1][1];
+        }
+        uint32_t va[VW][2][4];
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
           uint32_t v0[4], v1[4];
           codes_across<FMT>(v[0][0][w], v[0][1][w], v0);
           codes_across<FMT>(v[1][0][w], v[1][1][w], v1);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mma16816(o[4 * w + i], pa, v0[i], v1[i]);
+          for (int i = 0; i < 2; ++i) {
+            va[w][i][0] = v0[2 * i], va[w][i][1] = v0[2 * i + 1];
+            va[w][i][2] = v1[2 * i], va[w][i][3] = v1[2 * i + 1];
+            mma16816(o[2 * w + i], va[w][i], b4[0][0], b4[0][1]);
+            if constexpr (!ONE) mma16816(o[2 * w + i], va[w][i], b4[1][0], b4[1][1]);
+          }
         }
       }
     };
@@ -518,10 +628,6 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
       const int t0 = t0_of(t);
       if (t > t_lo && (t - t_lo) % Sh::kFlush == 0) {
         flush();
-#pragma unroll
-        for (int i = 0; i < 4 * VW; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
       }
       copies_wait<S - 1>();
       __syncwarp();
@@ -545,28 +651,30 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
       copies_commit();
     }
 
-    // the row's result: its output, or a partial one
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if (r < rows_all) {
-      const float inv = tok >= count || l == 0.f ? 0.f : 1.f / l;
+    // the rows' results: their output, or a partial one
+#pragma unroll
+    for (int j = 0; j < NR; ++j) {
+#pragma unroll
+      for (int k = ONE ? 1 : 4; k < 32; k *= 2) l[j] += __shfl_xor_sync(0xffffffffu, l[j], k);
+      const int n = ONE ? 0 : 2 * tig + j, r = row_of(n), tok = r / a.group;
+      const bool mine = r < rows_all && (!ONE || tig == 0);
+      const float inv = tok >= count || l[j] == 0.f ? 0.f : 1.f / l[j];
       const int64_t at = (((int64_t)b * a.tokens + tok) * a.heads + h * a.group + r % a.group) * hd;
 #pragma unroll
-      for (int w = 0; w < VW; ++w)
+      for (int w = 0; w < VW; ++w) {
+        const int d = out_dim<HD>(w, 0, gid);
+        float v[4];
+        float4 *part = sums(w, j, v);
+        if (!mine) continue;
+        if (!done) {
+          *part = make_float4(v[0], v[1], v[2], v[3]);
+        } else if (EXACT || d < hd) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const int d = out_dim<HD>(w, 0, 2 * tig + n);
-          float v[4];
-          float4 *part = sums(w, n, v);
-          if (!done) {
-            *part = make_float4(v[0], v[1], v[2], v[3]);
-          } else if (EXACT || d < hd) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = inv == 0.f ? 0.f : v[i] * inv;
-            kv_store_out4(a.out, at + d, v);
-          }
+          for (int i = 0; i < 4; ++i) v[i] = inv == 0.f ? 0.f : v[i] * inv;
+          kv_store_out4(a.out, at + d, v);
         }
-      if (!done && tig == 0) slot[kRows * HD + gid] = m, slot[kRows * HD + kRows + gid] = l;
+      }
+      if (mine && !done && gid == 0) slot[kRows * HD + n] = m[j], slot[kRows * HD + kRows + n] = l[j];
     }
     going = use.next(a, hr, whole) && use.to_step(a, hr, whole);
     // only now: the next kernel's CTAs would take this one's places on the SMs and
@@ -581,10 +689,10 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD>::kCtas)
 // the same order.
 constexpr int kJoinThreads = 256, kJoinItems = 64;
 
-template <int HD>
+template <int HD, bool ONE>
 __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(KvAttentionArgs a,
                                                                          int row_blocks, int warps) {
-  using Sh = RowShape<HD>;
+  using Sh = RowShape<HD, ONE>;
   __shared__ int64_t s_sum[kJoinThreads / 32][2];
   __shared__ float s_part[kJoinThreads][6];  // m, l, o
   pdl_wait();
@@ -595,7 +703,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(KvAtten
   int64_t before = 0, total = 0;
   for (int i = tid; i < c.batch; i += kJoinThreads) {
     int len, count;
-    const int n = units_of<HD>(a, i, len, count);
+    const int n = units_of<HD, ONE>(a, i, len, count);
     total += n;
     if (i < b) before += n;
   }
@@ -610,7 +718,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(KvAtten
 #pragma unroll
   for (int w = 0; w < kJoinThreads / 32; ++w) before += s_sum[w][0], total += s_sum[w][1];
   int len, count;
-  const int units = units_of<HD>(a, b, len, count);
+  const int units = units_of<HD, ONE>(a, b, len, count);
   const int64_t run = (total * hr + warps - 1) / warps;
   const int64_t pair = blockIdx.x;
   const int64_t u0 = before * hr + pair * units, u1 = u0 + units;
@@ -676,9 +784,9 @@ struct RowPlan {
   size_t ws_bytes;
 };
 
-template <int HD>
+template <int HD, bool ONE>
 int rows_plan(const KvView &c, int64_t tokens, int heads, RowPlan *p) {
-  using Sh = RowShape<HD>;
+  using Sh = RowShape<HD, ONE>;
   const int64_t rows = tokens * (heads / c.heads);
   const int64_t blocks = ceil_div(rows, kRows);
   if (rows > INT32_MAX || blocks * c.heads > INT32_MAX || c.batch > 65535)
@@ -696,31 +804,47 @@ int rows_plan(const KvView &c, int64_t tokens, int heads, RowPlan *p) {
   return TT_OK;
 }
 
-template <int HD, int FMT, bool EXACT>
+template <int HD, int FMT, bool EXACT, bool ONE>
 int launch_rows(const KvAttentionArgs &a, cudaStream_t stream) {
-  using Sh = RowShape<HD>;
+  using Sh = RowShape<HD, ONE>;
   RowPlan p;
-  int rc = rows_plan<HD>(a.c, a.tokens, a.heads, &p);
+  int rc = rows_plan<HD, ONE>(a.c, a.tokens, a.heads, &p);
   if (rc != TT_OK) return rc;
-  auto *kern = kv_attention_rows_kernel<HD, FMT, EXACT>;
+  auto *kern = kv_attention_rows_kernel<HD, FMT, EXACT, ONE>;
   static KvSmemSet set;
   if ((rc = set.ensure(reinterpret_cast<const void *>(kern), Sh::kSmem)) != TT_OK) return rc;
   TT_CUDA_TRY(launch_kernel(kern, dim3(p.ctas), dim3(kThreads), Sh::kSmem, stream, 1, a, p.row_blocks,
                             p.whole));
   if (!p.whole)
-    TT_CUDA_TRY(launch_kernel(kv_attention_join_kernel<HD>,
+    TT_CUDA_TRY(launch_kernel(kv_attention_join_kernel<HD, ONE>,
                               dim3(p.row_blocks * a.c.heads, a.c.batch,
                                    (unsigned)ceil_div(std::min(kRows, a.tokens * a.group) * (a.c.hd / 4), kJoinItems)),
                               dim3(kJoinThreads), 0, stream, 1, a, p.row_blocks, p.ctas * kWarps));
   return TT_OK;
 }
 
-template <int HD>
+template <int HD, bool ONE>
 int launch_rows_of(const KvAttentionArgs &a, cudaStream_t stream) {
   const bool i8 = a.c.format == TT_KV_INT8;
   if (a.c.hd == HD)
-    return i8 ? launch_rows<HD, TT_KV_INT8, true>(a, stream) : launch_rows<HD, TT_KV_E4M3, true>(a, stream);
-  return i8 ? launch_rows<HD, TT_KV_INT8, false>(a, stream) : launch_rows<HD, TT_KV_E4M3, false>(a, stream);
+    return i8 ? launch_rows<HD, TT_KV_INT8, true, ONE>(a, stream)
+              : launch_rows<HD, TT_KV_E4M3, true, ONE>(a, stream);
+  return i8 ? launch_rows<HD, TT_KV_INT8, false, ONE>(a, stream)
+            : launch_rows<HD, TT_KV_E4M3, false, ONE>(a, stream);
+}
+
+// The smallest width that holds a head_dim, 32, 64, 128 or 256, and whether a key
+// head has a single query row.
+template <class F>
+int for_rows(const KvView &c, int64_t rows, F &&f) {
+  using std::integral_constant;
+  auto width = [&](auto one) {
+    if (c.hd <= 32) return f(integral_constant<int, 32>(), one);
+    if (c.hd <= 64) return f(integral_constant<int, 64>(), one);
+    if (c.hd <= 128) return f(integral_constant<int, 128>(), one);
+    return f(integral_constant<int, 256>(), one);
+  };
+  return rows == 1 ? width(std::true_type()) : width(std::false_type());
 }
 
 // Rows of a key head from which the tile kernel takes over: it takes up to 128 rows in
@@ -756,23 +880,20 @@ int KvSmemSet::ensure(const void *kernel, size_t bytes) {
   return TT_OK;
 }
 
-// The smallest width that holds a head_dim: 32, 64, 128 or 256.
 size_t kv_attention_ws_bytes(const KvView &c, int64_t tokens, int heads) {
   if (use_tiles(c, tokens, heads)) return kv_attention_tiles_ws_bytes(c, tokens, heads);
   RowPlan p{};
-  const int rc = c.hd <= 32    ? rows_plan<32>(c, tokens, heads, &p)
-                 : c.hd <= 64  ? rows_plan<64>(c, tokens, heads, &p)
-                 : c.hd <= 128 ? rows_plan<128>(c, tokens, heads, &p)
-                               : rows_plan<256>(c, tokens, heads, &p);
+  const int rc = for_rows(c, tokens * (heads / c.heads), [&](auto hd, auto one) {
+    return rows_plan<decltype(hd)::value, decltype(one)::value>(c, tokens, heads, &p);
+  });
   return rc == TT_OK ? p.ws_bytes : 0;
 }
 
 int launch_kv_attention(const KvAttentionArgs &a, cudaStream_t stream) {
   if (use_tiles(a.c, a.tokens, a.heads)) return launch_kv_attention_tiles(a, stream);
-  if (a.c.hd <= 32) return launch_rows_of<32>(a, stream);
-  if (a.c.hd <= 64) return launch_rows_of<64>(a, stream);
-  if (a.c.hd <= 128) return launch_rows_of<128>(a, stream);
-  return launch_rows_of<256>(a, stream);
+  return for_rows(a.c, (int64_t)a.tokens * a.group, [&](auto hd, auto one) {
+    return launch_rows_of<decltype(hd)::value, decltype(one)::value>(a, stream);
+  });
 }
 
 }  // namespace tt
