@@ -693,38 +693,48 @@ template <int HD, bool ONE>
 __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(KvAttentionArgs a,
                                                                          int row_blocks, int warps) {
   using Sh = RowShape<HD, ONE>;
-  __shared__ int64_t s_sum[kJoinThreads / 32][2];
+  __shared__ int s_c[3];             // first and last warp of the segment, count
   __shared__ float s_part[kJoinThreads][6];  // m, l, o
   pdl_wait();
   const KvView &c = a.c;
   const int tid = threadIdx.x;
-  const int b = blockIdx.y;
-  const int64_t hr = (int64_t)c.heads * row_blocks;
-  int64_t before = 0, total = 0;
-  for (int i = tid; i < c.batch; i += kJoinThreads) {
-    int len, count;
-    const int n = units_of<HD, ONE>(a, i, len, count);
-    total += n;
-    if (i < b) before += n;
-  }
+  const int b = blockIdx.y, pair = blockIdx.x;
+  if (tid < 32) {
+    const int64_t hr = (int64_t)c.heads * row_blocks;
+    int64_t before = 0, total = 0;
+    int units = 0, mine = 0;
+    for (int i = tid; i < c.batch; i += 32) {
+      int len, count;
+      const int n = units_of<HD, ONE>(a, i, len, count);
+      total += n;
+      if (i < b) before += n;
+      if (i == b) units = n, mine = count;
+    }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-    total += __shfl_xor_sync(0xffffffffu, total, o);
+    for (int o = 16; o > 0; o >>= 1) {
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+    units = __shfl_sync(0xffffffffu, units, b & 31);
+    mine = __shfl_sync(0xffffffffu, mine, b & 31);
+    if (tid == 0) {
+      const int64_t run = (total * hr + warps - 1) / warps;
+      const int64_t u0 = before * hr + (int64_t)pair * units, u1 = u0 + units;
+      // 64-bit divisions are long; few caches need them
+      if (u1 <= INT32_MAX && run <= INT32_MAX) {
+        s_c[0] = ((int)u0 + Sh::kOver) / (int)run;
+        s_c[1] = ((int)u1 - 1) / (int)run;
+      } else {
+        s_c[0] = (int)((u0 + Sh::kOver) / run);
+        s_c[1] = (int)((u1 - 1) / run);
+      }
+      s_c[2] = mine;
+    }
   }
-  if ((tid & 31) == 0) s_sum[tid >> 5][0] = before, s_sum[tid >> 5][1] = total;
   __syncthreads();
-  before = total = 0;
-#pragma unroll
-  for (int w = 0; w < kJoinThreads / 32; ++w) before += s_sum[w][0], total += s_sum[w][1];
-  int len, count;
-  const int units = units_of<HD, ONE>(a, b, len, count);
-  const int64_t run = (total * hr + warps - 1) / warps;
-  const int64_t pair = blockIdx.x;
-  const int64_t u0 = before * hr + pair * units, u1 = u0 + units;
-  const int c0 = (int)((u0 + Sh::kOver) / run), c1 = (int)((u1 - 1) / run);
+  const int c0 = s_c[0], c1 = s_c[1], count = s_c[2];
   if (c0 == c1) return;
-  const int h = (int)(pair / row_blocks), rb = (int)(pair % row_blocks);
+  const int h = pair / row_blocks, rb = pair % row_blocks;
   const int rows_all = a.tokens * a.group, rows = min(kRows, rows_all - rb * kRows);
   // this block's items, and the threads on one: a power of two, so that their sums
   // pair up
