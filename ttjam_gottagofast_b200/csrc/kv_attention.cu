@@ -881,10 +881,17 @@ int kv_sm_count(int *out) {
   return TT_OK;
 }
 
-int KvSmemSet::ensure(const void *kernel, size_t bytes) {
+int KvSmemSet::ensure(const void *kernel, size_t bytes, int regs) {
   int dev = 0;
   TT_CUDA_TRY(cudaGetDevice(&dev));
   if (dev < 64 && done[dev]) return TT_OK;
+  if (regs > 0) {
+    cudaFuncAttributes at{};
+    TT_CUDA_TRY(cudaFuncGetAttributes(&at, kernel));
+    if (at.numRegs != regs)
+      return fail(TT_ERR_UNSUPPORTED, "kernel built with " + std::to_string(at.numRegs) +
+                                          " registers a thread, not " + std::to_string(regs));
+  }
   TT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
   if (dev < 64) done[dev] = true;
   return TT_OK;

@@ -25,8 +25,9 @@
 //             products: S_x = q_x K^T into the tile's two score buffers in turn, two
 //             token tiles ahead of the softmax, and O_x += P_x V (A = P from tensor
 //             memory). (With one score buffer a row tile and 128 tokens a tile, a
-//             softmax group waited for its own products: 355 us against ... for
-//             4 x 2048 fp32 rows behind 2048, 16 heads of 64.)
+//             softmax group waited for its own products: 355 us against 257 for
+//             4 x 2048 fp32 rows behind 2048, 16 heads of 64. Two threads a row
+//             instead of one: 279 us, the same work in more instructions.)
 // K and V tiles have a ring each. Every wait is bounded; one that gives up latches
 // TT_ERR_DEVICE_TIMEOUT in the cache's status word, and the kernel frees its tensor
 // memory and returns.
@@ -76,8 +77,9 @@ struct TcShape {
   // 176 (152), which the other two give up: 2 * 176 + 2 * 80 = 4 * 128.
   static constexpr int THREADS = 32 * (SOFT_WARPS + kConvWarps + 4);
   static constexpr bool SHIFT_REGS = MT == 2;
+  static constexpr int START_REGS = 128;
   static constexpr int SOFT_REGS = HD == 64 ? 176 : 152, OTHER_REGS = HD == 64 ? 80 : 104;
-  static_assert(!SHIFT_REGS || 2 * SOFT_REGS + 2 * OTHER_REGS <= 4 * 128, "registers of the block");
+  static_assert(!SHIFT_REGS || 2 * SOFT_REGS + 2 * OTHER_REGS <= 4 * START_REGS, "registers of the block");
   // tensor-memory columns: O, two score buffers a row tile, q
   static constexpr uint32_t T_O = 0, T_S = MT * HD, T_Q = MT * (HD + 2 * TOK);
   static_assert(T_Q + (QT ? MT * PIECES * HD / 2 : 0) <= 512, "tensor memory");
@@ -922,7 +924,9 @@ int launch_tiles(const KvAttentionArgs &a, cudaStream_t stream) {
     return fail(TT_ERR_UNSUPPORTED, "tt_kv_attention: too many rows");
   auto *kern = kv_attention_tiles_kernel<HD, FMT, PIECES>;
   static KvSmemSet set;
-  const int set_rc = set.ensure(reinterpret_cast<const void *>(kern), Sh::SMEM);
+  // (a block that started with fewer registers than its warps take over would wait for good)
+  const int set_rc = set.ensure(reinterpret_cast<const void *>(kern), Sh::SMEM,
+                                Sh::SHIFT_REGS ? Sh::START_REGS : 0);
   if (set_rc != TT_OK) return set_rc;
   TT_CUDA_TRY(launch_kernel(kern, dim3(p.row_tiles * a.c.heads, a.c.batch, p.splits), dim3(Sh::THREADS),
                             Sh::SMEM, stream, 1, a, p.row_tiles, p.splits));

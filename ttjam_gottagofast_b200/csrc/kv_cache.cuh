@@ -159,10 +159,11 @@ struct KvAttentionArgs {
 // kv_attention.cu
 // The current device's number of SMs, looked up once per device.
 int kv_sm_count(int *out);
-// Sets a kernel's dynamic shared memory limit once per device.
+// Sets a kernel's dynamic shared memory limit once per device, and checks that it
+// was built with `regs` registers a thread (0: any number).
 struct KvSmemSet {
   bool done[64] = {};
-  int ensure(const void *kernel, size_t bytes);
+  int ensure(const void *kernel, size_t bytes, int regs = 0);
 };
 size_t kv_attention_ws_bytes(const KvView &c, int64_t tokens, int heads);
 int launch_kv_attention(const KvAttentionArgs &a, cudaStream_t stream);
