@@ -169,3 +169,19 @@ def test_oracle_attention_is_softmax_over_the_seen_tokens():
         attn_mask=torch.arange(20)[None] <= torch.tensor([[18], [19]]), scale=0.25)
     assert torch.allclose(out[0, :2].transpose(0, 1), want, rtol=0, atol=1e-12)
     assert not out[0, 2].any()
+
+
+def test_sizes_beyond_32_bit_positions_are_refused(lib):
+    """Positions, and rows padded to a tile, stay in 32 bits."""
+    unsupported = _lib.TT_ERR_UNSUPPORTED
+    for columns, page in ((1 << 24, 128), ((1 << 23) + 1, 128), ((1 << 26) + 1, 16)):
+        c = _cache(table_columns=columns, page_size=page)
+        assert _write(lib, c) == unsupported and _attend(lib, c) == unsupported
+        assert lib.tt_kv_read(ctypes.byref(c), 0, FAKE, FAKE, 1, None) == unsupported
+    c = _cache(num_pages=(1 << 30) + 1)
+    assert _write(lib, c) == unsupported and _attend(lib, c) == unsupported
+    c = _cache()
+    assert lib.tt_kv_read(ctypes.byref(c), 0, FAKE, FAKE, (1 << 30) + 1, None) == _lib.TT_ERR_INVALID_ARGUMENT
+    assert _attend(lib, c, tokens=(1 << 30) + 1) == unsupported
+    assert _attend(lib, c, tokens=(1 << 29) + 1, heads=4) == unsupported
+    assert lib.tt_kv_attention_workspace_bytes(ctypes.byref(c), (1 << 30) + 1, 2) == 0

@@ -811,7 +811,11 @@ static int cached_layout(const tt_config *cfg, int dtype, const tt_kv_cache *cac
   if (caches == nullptr) return fail(TT_ERR_INVALID_ARGUMENT, "tt_forward_cached: caches is NULL");
   if (cfg->plan == TT_PLAN_CLUSTER || cfg->plan == TT_PLAN_TILE)
     return fail(TT_ERR_UNSUPPORTED, "tt_forward_cached runs the per-op schedules");
-  views->resize(cfg->num_layers);
+  try {
+    views->resize(cfg->num_layers);
+  } catch (const std::exception &) {
+    return fail(TT_ERR_UNSUPPORTED, "tt_forward_cached: too many layers");
+  }
   for (int l = 0; l < cfg->num_layers; ++l) {
     KvView &v = (*views)[l];
     if ((rc = kv_view(&caches[l], "tt_forward_cached", &v)) != TT_OK) return rc;

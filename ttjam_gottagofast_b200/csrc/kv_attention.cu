@@ -43,6 +43,7 @@
 #include <math_constants.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "kv_cache.cuh"
 #include "kv_codes.cuh"
@@ -62,11 +63,11 @@ struct RowShape {
   static constexpr int GR = HD == 32 ? 8 : HD == 64 ? 4 : GC;
   static constexpr int kStep = 16 * GR;              // tokens
   static constexpr int kOver = GR >= 4 ? 1 : 2;      // units of a segment besides its steps
-  static constexpr int kWhole = GR >= 4 ? 2 : 4;                   // steps of a segment that is never split
+  static constexpr int kWhole = GR >= 4 ? 2 : 4;     // steps of a segment that is never split
   static constexpr int kStages = HD == 128 && !ONE ? 3 : 2;  // steps in a warp's ring
   static constexpr uint32_t kStage = 2 * kStep * HD;  // bytes: keys, then values
   static constexpr uint32_t kSmem = kWarps * kStages * kStage;
-  static constexpr int kCtas = HD == 256 && !ONE ? 2 : 3;                    // per SM, as registers and shared memory allow
+  static constexpr int kCtas = HD == 256 && !ONE ? 2 : 3;  // per SM, as registers and shared memory allow
   // tensor cores add by rounding toward zero: after 1024 tokens the sum moves to the
   // place of the warp's partial result, so that it does not drift
   static constexpr int kFlush = 1024 / kStep;
@@ -799,7 +800,7 @@ int rows_plan(const KvView &c, int64_t tokens, int heads, RowPlan *p) {
   using Sh = RowShape<HD, ONE>;
   const int64_t rows = tokens * (heads / c.heads);
   const int64_t blocks = ceil_div(rows, kRows);
-  if (rows > INT32_MAX || blocks * c.heads > INT32_MAX || c.batch > 65535)
+  if (rows > kKvMost || blocks * c.heads > INT32_MAX || c.batch > 65535)
     return fail(TT_ERR_UNSUPPORTED, "tt_kv_attention: too many rows or sequences");
   p->row_blocks = (int)blocks;
   int sms = 0;
@@ -859,9 +860,11 @@ int for_rows(const KvView &c, int64_t rows, F &&f) {
 
 // Rows of a key head from which the tile kernel takes over: it takes up to 128 rows in
 // the time of one, this file's kernel goes over the codes once for every 8. Measured,
-// e4m3, fp32 rows, this kernel / the tiles: 16 sequences of 2000 tokens, 16 heads of
-// 64: 48 rows 86 / 93 us, 64 rows 113 / 94; 32 heads of 128 on 4: 32 rows 45 / 39 us;
-// 4 of 20000: 48 rows 173 / 159 us; 32 rows 78 / 85 and 48 rows 118 / 85 us.
+// e4m3, fp32 rows, this kernel / the tiles, us. 16 heads of 64: 16 sequences of 2000
+// tokens, 48 rows 89 / 94, 64 rows 113 / 93; 4 of 20000, 48 rows 179 / 160, 32 rows
+// 127 / 161. 32 heads of 128 on 4: 16 of 2000, 24 rows 37 / 39, 32 rows 45 / 39; 4 of
+// 20000, 32 rows 83 / 86, 48 rows 114 / 86. (One short sequence costs 15 to 25 us
+// either way.)
 bool use_tiles(const KvView &c, int64_t tokens, int heads) {
   return tokens * (heads / c.heads) >= (c.hd <= 64 ? 56 : 40);
 }
@@ -869,13 +872,10 @@ bool use_tiles(const KvView &c, int64_t tokens, int heads) {
 }  // namespace
 
 int kv_sm_count(int *out) {
-  static int cached[64] = {};
+  static std::atomic<int> cached[64] = {};
   int dev = 0;
   TT_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev < 64 && cached[dev] > 0) {
-    *out = cached[dev];
-    return TT_OK;
-  }
+  if (dev < 64 && (*out = cached[dev]) > 0) return TT_OK;
   TT_CUDA_TRY(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev));
   if (dev < 64) cached[dev] = *out;
   return TT_OK;

@@ -19,9 +19,9 @@
 //             when the maximum grows by more than 2^8.
 //   conversion  a warpgroup: 16 codes a load, eight fp16 pairs, stored as
 //             128-byte-swizzled rows of 64 dims, K-major for K and, the same bytes
-//             read the other way, MN-major for V; one tile ahead in registers. The
-//             tile's scales go to shared memory.
-//   MMA       one warp of a last group allocates tensor memory; its lane 0 issues the
+//             read the other way, MN-major for V; the next tiles' codes are on their
+//             way meanwhile. The tile's scales go to shared memory.
+//   MMA       one warp of a last group allocates tensor memory; an elected lane issues the
 //             products: S_x = q_x K^T into the tile's two score buffers in turn, two
 //             token tiles ahead of the softmax, and O_x += P_x V (A = P from tensor
 //             memory). (With one score buffer a row tile and 128 tokens a tile, a
@@ -917,7 +917,7 @@ int launch_tiles(const KvAttentionArgs &a, cudaStream_t stream) {
   int sms = 0;
   const int rc = kv_sm_count(&sms);
   if (rc != TT_OK) return rc;
-  if ((int64_t)a.tokens * a.group > INT32_MAX || a.c.batch > 65535 || a.c.heads > 65535)
+  if ((int64_t)a.tokens * a.group > kKvMost || a.c.batch > 65535 || a.c.heads > 65535)
     return fail(TT_ERR_UNSUPPORTED, "tt_kv_attention: too many rows, heads or sequences");
   const TilePlan p = tile_plan<HD, PIECES>(a.c, a.tokens, a.heads, sms);
   if ((int64_t)p.row_tiles * a.c.heads > INT32_MAX)

@@ -313,8 +313,8 @@ int kv_view(const tt_kv_cache *c, const char *what, KvView *v) {
     return no(TT_ERR_INVALID_ARGUMENT, "kv_heads, num_pages and table_columns must be positive");
   if ((int64_t)c->num_pages * c->kv_heads > INT32_MAX)
     return no(TT_ERR_UNSUPPORTED, "num_pages * kv_heads must fit 32 bits");
-  if ((int64_t)c->table_columns * c->page_size > INT32_MAX)
-    return no(TT_ERR_UNSUPPORTED, "table_columns * page_size must fit 32 bits");
+  if ((int64_t)c->table_columns * c->page_size > kKvMost)
+    return no(TT_ERR_UNSUPPORTED, "table_columns * page_size must be at most 2^30");
   if (c->batch > 0 && (c->k_codes == nullptr || c->v_codes == nullptr || c->k_scale == nullptr ||
                        c->v_scale == nullptr || c->block_table == nullptr || c->lengths == nullptr))
     return no(TT_ERR_INVALID_ARGUMENT, "a cache pointer is NULL");
@@ -379,8 +379,8 @@ int tt_kv_read(const tt_kv_cache *cache, int dtype, void *k, void *v, int64_t ma
   if (rc != TT_OK) return rc;
   if (!dtype_ok(dtype))
     return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_read: dtype must be a TT_DTYPE_* value");
-  if (max_tokens < 0 || max_tokens > INT32_MAX)
-    return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_read: max_tokens must be >= 0 and fit 32 bits");
+  if (max_tokens < 0 || max_tokens > kKvMost)
+    return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_read: max_tokens must be >= 0 and at most 2^30");
   if (max_tokens == 0 || c.batch == 0) return TT_OK;
   if (k == nullptr || v == nullptr)
     return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_read: NULL k or v");
@@ -392,7 +392,8 @@ int tt_kv_read(const tt_kv_cache *cache, int dtype, void *k, void *v, int64_t ma
 size_t tt_kv_attention_workspace_bytes(const tt_kv_cache *cache, int64_t tokens, int32_t heads) {
   KvView c;
   if (kv_view(cache, "tt_kv_attention_workspace_bytes", &c) != TT_OK) return 0;
-  if (tokens <= 0 || tokens > INT32_MAX || c.batch == 0 || heads <= 0 || heads % c.heads != 0)
+  if (tokens <= 0 || tokens > INT32_MAX || c.batch == 0 || heads <= 0 || heads % c.heads != 0 ||
+      tokens * (heads / c.heads) > kKvMost)
     return 0;
   return kv_attention_ws_bytes(c, tokens, heads);
 }
@@ -409,6 +410,8 @@ int tt_kv_attention(const tt_kv_cache *cache, int dtype, const void *q, const in
     return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_attention: tokens must be >= 0 and fit 32 bits");
   if (heads <= 0 || heads % c.heads != 0)
     return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_attention: heads must be a multiple of kv_heads");
+  if (tokens * (heads / c.heads) > kKvMost)
+    return fail(TT_ERR_UNSUPPORTED, "tt_kv_attention: more than 2^30 rows a key head");
   if (!(scale > 0.f) || !std::isfinite(scale))
     return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_attention: scale must be positive and finite");
   if (tokens == 0 || c.batch == 0) return TT_OK;

@@ -18,6 +18,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "tt_common.cuh"
 
 namespace tt {
@@ -158,11 +160,14 @@ struct KvAttentionArgs {
 
 // kv_attention.cu
 // The current device's number of SMs, looked up once per device.
+// Tokens of a sequence, and query rows of a key head, at most: sums of a position and
+// a tile's width stay in 32 bits.
+constexpr int64_t kKvMost = 1 << 30;
 int kv_sm_count(int *out);
 // Sets a kernel's dynamic shared memory limit once per device, and checks that it
 // was built with `regs` registers a thread (0: any number).
 struct KvSmemSet {
-  bool done[64] = {};
+  std::atomic<bool> done[64] = {};
   int ensure(const void *kernel, size_t bytes, int regs = 0);
 };
 size_t kv_attention_ws_bytes(const KvView &c, int64_t tokens, int heads);

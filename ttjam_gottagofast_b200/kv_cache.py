@@ -139,10 +139,11 @@ class KVCache:
 
     # ---- lengths ------------------------------------------------------------
     def advance(self, tokens: int, new_tokens: Optional[torch.Tensor] = None) -> None:
-        """Add `tokens` new tokens to every sequence, or new_tokens[b] of at most
-        `tokens` to sequence b. Refuses what `max_tokens` has no room for. (While
-        a CUDA graph is captured, and in its replays, the host cannot know the
-        lengths; a length beyond the room is then latched on the device.)"""
+        """Add `tokens` new tokens to every sequence, or new_tokens[b], at most
+        `tokens` and not negative, to sequence b. Refuses what `max_tokens` has
+        no room for. (While a CUDA graph is captured, and in its replays, the
+        host cannot know the lengths; a length beyond the room is then latched
+        on the device.)"""
         if tokens < 0:
             raise ValueError("tokens must be >= 0")
         new_tokens = self._counts(new_tokens)
@@ -228,9 +229,10 @@ class KVCache:
         reads key head h // (heads // kv_heads). Row i < new_tokens[b] stands at
         position lengths[b] - new_tokens[b] + i and sees the tokens up to its
         own. `scale` (default head_dim ** -0.5) multiplies the scores. Returns
-        (or writes to `out`, contiguous) [batch, tokens, heads, head_dim] of
-        q's type, computed to fp32 accuracy (float16 and bfloat16 prompts may
-        round the probabilities to 11 bits); rows behind new_tokens[b] are 0."""
+        (or writes to `out`, contiguous, sharing no memory with q) [batch,
+        tokens, heads, head_dim] of q's type, computed to fp32 accuracy
+        (float16 and bfloat16 prompts may round the probabilities to 11 bits);
+        rows behind new_tokens[b] are 0."""
         key = (layer, q.shape, q.stride(), q.dtype, q.get_device())
         plan = self._plans.get(key)
         if plan is None:
