@@ -276,6 +276,87 @@ def test_attend_long_contexts_do_not_drift(tokens, heads, hd):
     assert cache.read_device_status() == (0, 0)
 
 
+@pytest.mark.parametrize("tokens", [1, 3, 70])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_attend_unaligned_and_expanded_queries(dtype, tokens):
+    """Rows that start anywhere, and one query for a whole batch (stride 0)."""
+    cache, want = kh.make(71, "int8", 3, 8, 2, 48, 32, [200, 90, 133])
+    raw = torch.randn((tokens, 5, 49), generator=torch.Generator().manual_seed(9)).to(DTYPES[dtype]).cuda()
+    q = raw[:, 1:, 1:].expand(3, tokens, 4, 48)
+    got = cache.attend(q)
+    exact, size, total, reach = ref.attend(want, q.cpu(), [tokens] * 3, 48 ** -0.5)
+    bound, half_step = kh.attention_bound(size, total, reach, 48, 200, q.dtype)
+    assert not torch.isnan(got).any() and kh.worst(got, exact, bound, half_step) <= 1
+    assert kh.same_bits(cache.attend(q.contiguous()), got)
+
+
+@pytest.mark.parametrize("tokens,heads,hd", [(1, 2, 64), (3, 2, 128), (70, 2, 64), (130, 1, 128), (60, 1, 256)])
+def test_attend_moving_references_give_the_same_bits_every_time(tokens, heads, hd):
+    """Scores that grow along the sequence, so that the running reference moves
+    and sums are rescaled all the way: right, and the same bits in 20 calls."""
+    length = 1100
+    cache, _ = kh.make(72, "int8", 2, 20, heads, hd, 64, [length, 700])
+    order = torch.arange(20).float()
+    for b in range(2):
+        cache.k_scale[0, cache.block_table[b].long()] = torch.exp2(torch.floor(order / 3) - 6)[:, None].cuda()
+    want = kh.mirror(cache)
+    q = torch.randn((2, tokens, heads, hd), generator=torch.Generator().manual_seed(3)).cuda()
+    got = cache.attend(q)
+    for _ in range(19):
+        assert kh.same_bits(cache.attend(q), got)
+    exact, size, total, reach = ref.attend(want, q[:, -1:].cpu(), [1, 1], hd ** -0.5)
+    bound, half_step = kh.attention_bound(size, total, reach, hd, length, torch.float32)
+    assert kh.worst(got[:, -1:], exact, bound, half_step) <= 1
+    assert cache.read_device_status() == (0, 0)
+
+
+def test_two_graphs_at_once():
+    """Two captured calls, each with a workspace of its own, replayed on two
+    streams at the same time. 100 new tokens are more than the sequence of 64
+    holds: that is latched as a count beyond the length (0x5200), and the rows
+    are the same in every call all the same."""
+    work = []
+    for seed, tokens in ((1, 1), (2, 100)):
+        cache, _ = kh.make(73 + seed, "e4m3", 4, 40, 2, 64, 64, [2500, 1800, 64, 900])
+        q = torch.randn((4, tokens, 2, 64), generator=torch.Generator().manual_seed(seed)).cuda()
+        want = cache.attend(q)
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.graph(graph, stream=stream):
+            out = cache.attend(q)
+        work.append((cache, stream, graph, out, want))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for _, stream, graph, _, _ in work:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for (cache, _, _, out, want), status in zip(work, ((0, 0), (-7, 0x5200))):
+        assert kh.same_bits(out, want)
+        assert cache.read_device_status() == status
+
+
+def test_shared_pages_and_padded_width_beyond_the_room():
+    """Two sequences over the same pages, read only; and a batch padded to more
+    rows than a sequence has room for."""
+    cache, _ = kh.make(75, "e4m3", 2, 2, 1, 32, 16, [32, 20])
+    own = cache.block_table[1].clone()
+    cache.block_table[1] = cache.block_table[0]
+    want = kh.mirror(cache)
+    q = torch.randn((2, 40, 3, 32), generator=torch.Generator().manual_seed(4)).cuda()
+    counts = [2, 1]
+    got = cache.attend(q, new_tokens=_counts(counts))
+    exact, size, total, reach = ref.attend(want, q.cpu(), counts, 32 ** -0.5)
+    bound, half_step = kh.attention_bound(size, total, reach, 32, 32, torch.float32)
+    assert kh.worst(got, exact, bound, half_step) <= 1 and not got[0, 2:].any() and not got[1, 1:].any()
+    x = torch.ones((2, 40, 1, 32), device="cuda")
+    cache.block_table[1] = own
+    cache.write(x, x, new_tokens=_counts(counts))
+    k, _ = cache.read()
+    assert torch.equal(k[0, 30:], x[0, :2]) and torch.equal(k[1, 19:20], x[0, :1])
+    assert cache.read_device_status() == (0, 0)
+
+
 def test_device_checks_of_lengths_and_counts():
     """A length beyond the room or below zero and a count beyond the length
     are latched and clamped; nothing outside the cache's pages is touched."""
