@@ -458,3 +458,59 @@ def test_lengths_advance_and_refusals():
     assert cache.attend(x[:, :0]).shape == (2, 0, 2, 32)
     cache.write(x[:, :0], x[:, :0])
     assert cache.read(max_tokens=0)[0].shape == (2, 0, 2, 32)
+
+
+def test_advance_knows_of_lengths_that_others_wrote():
+    """The caller's own writes into lengths, a graph's replays, and caches made
+    or used in inference mode: what has no room is still refused."""
+    from ttjam_gottagofast_b200 import KVCache
+
+    cache = KVCache(2, 64, 1, 16, page_size=16)
+    cache.advance(4)
+    cache.lengths.copy_(_counts([60, 1]))
+    with pytest.raises(ValueError, match="full"):
+        cache.advance(5)
+    cache.reset()
+    cache.advance(1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.advance(10)
+    for _ in range(6):
+        graph.replay()
+    with pytest.raises(ValueError, match="full"):
+        cache.advance(4)
+    cache.advance(3)
+    graph.replay()
+    assert cache.lengths.tolist() == [74, 74]
+    with pytest.raises(ValueError, match="full"):
+        cache.advance(0)
+    with torch.inference_mode():
+        for make in (lambda: KVCache(2, 64, 1, 16, page_size=16),
+                     lambda: KVCache.from_tensors(*_empty(2, 4, 1, 16, 16))):
+            cache = make()
+            cache.advance(60)
+            cache.lengths.add_(2)
+            with pytest.raises(ValueError, match="full"):
+                cache.advance(3)
+            cache.advance(2)
+            assert cache.lengths.tolist() == [64, 64]
+
+
+def _empty(batch, columns, heads, hd, page):
+    pages = batch * columns
+    codes = [torch.zeros((1, pages, heads, page, hd), dtype=torch.int8, device="cuda") for _ in range(2)]
+    scales = [torch.zeros((1, pages, heads), device="cuda") for _ in range(2)]
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").view(batch, columns)
+    return [*codes, *scales, table, torch.zeros(batch, dtype=torch.int32, device="cuda")]
+
+
+def test_a_batch_of_none():
+    from ttjam_gottagofast_b200 import KVCache
+
+    k, v, ks, vs, table, lengths = _empty(1, 2, 1, 16, 16)
+    cache = KVCache.from_tensors(k, v, ks, vs, table[:0], lengths[:0])
+    x = torch.ones((0, 3, 1, 16), device="cuda")
+    cache.advance(3)
+    cache.write(x, x)
+    assert cache.attend(x).shape == x.shape and cache.read()[0].shape == (0, 32, 1, 16)
+    assert cache.read_device_status() == (0, 0)

@@ -72,9 +72,10 @@ class KVCache:
                  for _ in range(2)]
         scales = [torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)]
         table = torch.arange(pages, dtype=torch.int32, device=device).view(batch, columns)
-        self._setup(*codes, *scales, table,
-                    torch.zeros(batch, dtype=torch.int32, device=device), max_tokens)
-        self._longest = 0
+        with torch.inference_mode(False):  # so that torch counts the writes into it
+            lengths = torch.zeros(batch, dtype=torch.int32, device=device)
+        self._setup(*codes, *scales, table, lengths, max_tokens)
+        self._longest, self._seen = 0, lengths._version
 
     @classmethod
     def from_tensors(cls, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor,
@@ -117,7 +118,9 @@ class KVCache:
         self.num_layers, self.num_pages = layers, pages
         self.kv_heads, self.page_size, self.head_dim = heads, page, hd
         self.batch, self.max_tokens = batch, max_tokens
-        self._longest = None  # an upper bound on lengths known to the host, or None
+        # An upper bound on lengths, which holds while nothing else has written into
+        # them: torch's count of the writes is still _seen, and no graph advances them.
+        self._longest, self._seen, self._captured = 0, None, False
         self._status = torch.zeros(2, dtype=torch.int32, device=k.device)
         self._lib = _lib.load()
         self._c_write, self._c_read = self._lib.tt_kv_write, self._lib.tt_kv_read
@@ -141,16 +144,20 @@ class KVCache:
     def advance(self, tokens: int, new_tokens: Optional[torch.Tensor] = None) -> None:
         """Add `tokens` new tokens to every sequence, or new_tokens[b], at most
         `tokens` and not negative, to sequence b. Refuses what `max_tokens` has
-        no room for. (While a CUDA graph is captured, and in its replays, the
-        host cannot know the lengths; a length beyond the room is then latched
-        on the device.)"""
+        no room for. The host keeps a bound on the lengths, and reads them from
+        the device only when that does not settle it: near `max_tokens`, after
+        the caller wrote into `lengths`, and in a cache whose advance was
+        captured. (While a CUDA graph is captured, and in its replays, the host
+        cannot know the lengths; one beyond the room is then latched on the
+        device.)"""
         if tokens < 0:
             raise ValueError("tokens must be >= 0")
         new_tokens = self._counts(new_tokens)
         if not torch.cuda.is_current_stream_capturing():
-            if self._longest is None or self._longest + tokens > self.max_tokens:
+            known = self._seen is not None and self._seen == self._writes() and not self._captured
+            if not known or self._longest + tokens > self.max_tokens:
                 grown = self.lengths + (tokens if new_tokens is None else new_tokens)
-                longest = int(grown.max())
+                longest = int(grown.max()) if self.batch else 0
                 if longest > self.max_tokens:
                     raise ValueError(f"cache is full: a sequence would hold {longest} tokens of "
                                      f"at most {self.max_tokens}")
@@ -158,13 +165,17 @@ class KVCache:
             else:
                 self._longest += tokens
         else:
-            self._longest = None
+            self._captured = True
         self.lengths.add_(tokens if new_tokens is None else new_tokens)
+        self._seen = self._writes()
 
     def reset(self) -> None:
         """Forget every token (lengths 0); the pages stay where they are."""
         self.lengths.zero_()
-        self._longest = None
+        self._longest, self._seen = 0, self._writes()
+
+    def _writes(self) -> Optional[int]:
+        return None if self.lengths.is_inference() else self.lengths._version
 
     # ---- the operators ------------------------------------------------------
     # What a call's shapes, strides and types decide (its checks, the constant
@@ -228,7 +239,7 @@ class KVCache:
         (strides as in `write`), heads a multiple of kv_heads: query head h
         reads key head h // (heads // kv_heads). Row i < new_tokens[b] stands at
         position lengths[b] - new_tokens[b] + i and sees the tokens up to its
-        own. `scale` (default head_dim ** -0.5) multiplies the scores. Returns
+        own. `scale` (default head_dim ** -0.5; positive) multiplies the scores. Returns
         (or writes to `out`, contiguous, sharing no memory with q) [batch,
         tokens, heads, head_dim] of q's type, computed to fp32 accuracy
         (float16 and bfloat16 prompts may round the probabilities to 11 bits);
@@ -267,7 +278,7 @@ class KVCache:
         return out
 
     def read_device_status(self) -> Tuple[int, int]:
-        """Synchronise and return (code, detail) latched by the kernels' checks
+        """Synchronise, return and clear (code, detail) latched by the kernels' checks
         of lengths, counts and block-table entries; (0, 0) when all were in range."""
         code, detail = ctypes.c_int32(0), ctypes.c_int32(0)
         stream = torch.cuda.current_stream(self.device).cuda_stream
