@@ -162,3 +162,15 @@ def test_refusals():
             bad()
     assert cache.lengths.tolist() == [0, 0]
     assert model.forward_cached(x[:, :0], cache).shape == (2, 0, 128)
+
+
+def test_a_batch_padded_beyond_the_room_is_refused_before_it_counts():
+    _, _, model = _model(64, 2, 64, 1)
+    cache = model.make_cache(2, 32, page_size=16)
+    x = torch.zeros((2, 33, 64), device="cuda")
+    counts = torch.tensor([1, 2], dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="room"):
+        model.forward_cached(x, cache, new_tokens=counts)
+    assert cache.lengths.tolist() == [0, 0]
+    model.forward_cached(x[:, :32], cache, new_tokens=counts)
+    assert cache.lengths.tolist() == [1, 2]

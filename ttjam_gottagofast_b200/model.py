@@ -416,6 +416,9 @@ class TTForward:
         if not x.is_contiguous() or x.data_ptr() % 16:
             x = x.contiguous().clone() if x.data_ptr() % 16 else x.contiguous()
         b, n, _ = x.shape
+        room = cache.block_table.shape[1] * cache.page_size
+        if n > room:
+            raise ValueError(f"{n} rows are more than a sequence has room for ({room} tokens)")
         counts = cache._counts(new_tokens)
         image = self._ensure_image(x.device)
         # a context averages values rounded to codes, which can exceed the
