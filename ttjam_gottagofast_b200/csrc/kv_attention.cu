@@ -40,6 +40,13 @@
 // equal run of consecutive units, whatever the lengths, and a second kernel joins
 // the segments that ended up on several warps. Where no segment is longer than
 // kWhole steps, warps take whole ones, and nothing is left to join.
+//
+// Measured, one new token a sequence: 2 sequences of 100000, 16 heads of 64, int8, 78
+// to 80 us with the join, its first kernel at 5.5 TB/s of codes (0.84 of a plain
+// copy's rate), bound by memory and by instructions (0.54 of the issue slots); 64 of
+// up to 2048, e4m3, 37 us; 32 of up to 8192, 32 query heads on 4 of 128, e4m3, 48.5 us,
+// bound by the latency between dependent instructions, as registers leave 12 warps an
+// SM. One short sequence: 8 us, a chain of loads (length, page, scale, codes).
 #include <math_constants.h>
 
 #include <algorithm>

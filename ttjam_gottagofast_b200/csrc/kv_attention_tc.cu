@@ -28,6 +28,10 @@
 //             softmax group waited for its own products: 355 us against 257 for
 //             4 x 2048 fp32 rows behind 2048, 16 heads of 64. Two threads a row
 //             instead of one: 279 us, the same work in more instructions.)
+// Bound by the softmax groups' instructions, exp2 and reads of tensor memory at
+// head_dim 64 (fp32, 4 x 2048 rows behind 2048, 16 heads: 103 GFLOP counted once, 257
+// us), by shared memory's rate under the products of 64 columns and the converters'
+// stores at 128 (bf16, 3 x 4096 rows, 32 heads on 4: 347 GFLOP, 448 us, 0.77 PFLOP/s).
 // K and V tiles have a ring each. Every wait is bounded; one that gives up latches
 // TT_ERR_DEVICE_TIMEOUT in the cache's status word, and the kernel frees its tensor
 // memory and returns.

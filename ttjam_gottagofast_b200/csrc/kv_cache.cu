@@ -42,7 +42,8 @@ __device__ __forceinline__ uint32_t magnitude_bits(uint32_t mx) {
 // and the rounding, so each new element is read once, every load of a warp is 512
 // consecutive bytes, and an item of one warp meets no barrier. (One block of 256
 // threads an item, with 32 bytes a thread: 65 us for 16 prompts of 2048 tokens, 16
-// heads of 64, bf16.) The maximum is taken on the bits of |x| (ordered like the
+// heads of 64, bf16; this form 43.5 us, of which the bytes need 30.7 at the rate of a
+// plain copy.) The maximum is taken on the bits of |x| (ordered like the
 // values; infinities and NaN on top), so it does not hang on the order of the
 // reduction. Bound by memory for prompts, by its dependent loads (length, page,
 // scale) for a step.
@@ -159,7 +160,8 @@ __global__ void __launch_bounds__(32 * block_warps(NW))
 // A thread takes 16 bytes of output in each of kReadRows rows ((token, head) pairs),
 // whose loads it has under way at once; x runs along a row, so every store of a warp
 // covers consecutive bytes. Rows behind a sequence's end, and of pages that do not
-// exist, are zero.
+// exist, are zero. Bound by memory: one sequence of 100000 tokens, 16 heads of 64, to
+// bf16, 96 to 102 us, 6.0 to 6.4 TB/s (one row a thread: 119 us).
 constexpr int kReadRows = 4;
 
 template <typename T, int FMT>
