@@ -195,12 +195,13 @@ __device__ __forceinline__ int out_dim(int w, int i, int n) {
   else return 128 * (w / 4) + 16 * n + 4 * (w % 4) + i;
 }
 
-template <int HD, int FMT, bool EXACT, bool ONE>
+template <int HD, int FMT, bool EXACT, bool ONE, bool TWO>
 __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
     kv_attention_rows_kernel(KvAttentionArgs a, int row_blocks, bool whole) {
   using Sh = RowShape<HD, ONE>;
   constexpr int KW = Sh::KW, VW = Sh::VW, GR = Sh::GR, GC = Sh::GC, S = Sh::kStages;
   constexpr int NR = ONE ? 1 : 2;  // rows of a lane's results
+  static_assert(TWO || !ONE, "the columns of a single row are there for both pieces");
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int64_t s_scan[kThreads];
   const KvView &c = a.c;
@@ -344,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
     };
 
     // q of column gid, scaled to [1, 2) and split
-    uint32_t qb[KW][ONE ? 2 : 4];
+    uint32_t qb[KW][TWO && !ONE ? 4 : 2];
     float sc[NR];
     {
       float x[KW][4];
@@ -378,7 +379,8 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
           qb[w][0] = gid & 1 ? lo[0] : hi[0];
           qb[w][1] = gid & 1 ? lo[1] : hi[1];
         } else {
-          qb[w][0] = hi[0], qb[w][1] = hi[1], qb[w][2] = lo[0], qb[w][3] = lo[1];
+          qb[w][0] = hi[0], qb[w][1] = hi[1];
+          if constexpr (TWO) qb[w][2] = lo[0], qb[w][3] = lo[1];
         }
       }
       const float scale = a.scale * 1.4426950408889634f * kv_pow2(e);
@@ -481,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
             codes_along<FMT>(w[1][i], k4[1], k4[3]);
             if (i == 0) mma16816_first(acc[g], k4, qb[i][0], qb[i][1]);
             else mma16816(acc[g], k4, qb[i][0], qb[i][1]);
-            if constexpr (!ONE) {
+            if constexpr (TWO && !ONE) {
               if (i == 0) mma16816_first(low, k4, qb[i][2], qb[i][3]);
               else mma16816(low, k4, qb[i][2], qb[i][3]);
             }
@@ -490,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
-              for (int j = 0; j < NR; ++j) s[g][x][j] = acc[g][2 * x + j] + low[2 * x + j];
+              for (int j = 0; j < NR; ++j) s[g][x][j] = acc[g][2 * x + j] + (TWO ? low[2 * x + j] : 0.f);
           }
         }
         if constexpr (ONE) {
@@ -576,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
           for (int x = 0; x < 2; ++x) {
             f16_split2(p[x][0], p[x][NR - 1], hi[x], lo[x]);
             pb[0][x] = transpose8(hi[x]);
-            pb[1][x] = transpose8(lo[x]);
+            if constexpr (TWO) pb[1][x] = transpose8(lo[x]);
           }
         }
       };
@@ -613,7 +615,8 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
           b4[0][1] = gid >> 1 == g ? pb[0][1] : 0u;
         } else {
           probabilities(g);
-          b4[0][0] = pb[0][0], b4[0][1] = pb[0][1], b4[1][0] = pb[1][0], b4[1][1] = pb[1][1];
+          b4[0][0] = pb[0][0], b4[0][1] = pb[0][1];
+          if constexpr (TWO) b4[1][0] = pb[1][0], b4[1][1] = pb[1][1];
         }
         uint32_t va[VW][2][4];
 #pragma unroll
@@ -626,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
             va[w][i][0] = v0[2 * i], va[w][i][1] = v0[2 * i + 1];
             va[w][i][2] = v1[2 * i], va[w][i][3] = v1[2 * i + 1];
             mma16816(o[2 * w + i], va[w][i], b4[0][0], b4[0][1]);
-            if constexpr (!ONE) mma16816(o[2 * w + i], va[w][i], b4[1][0], b4[1][1]);
+            if constexpr (TWO && !ONE) mma16816(o[2 * w + i], va[w][i], b4[1][0], b4[1][1]);
           }
         }
       }
@@ -822,13 +825,13 @@ int rows_plan(const KvView &c, int64_t tokens, int heads, RowPlan *p) {
   return TT_OK;
 }
 
-template <int HD, int FMT, bool EXACT, bool ONE>
+template <int HD, int FMT, bool EXACT, bool ONE, bool TWO>
 int launch_rows(const KvAttentionArgs &a, cudaStream_t stream) {
   using Sh = RowShape<HD, ONE>;
   RowPlan p;
   int rc = rows_plan<HD, ONE>(a.c, a.tokens, a.heads, &p);
   if (rc != TT_OK) return rc;
-  auto *kern = kv_attention_rows_kernel<HD, FMT, EXACT, ONE>;
+  auto *kern = kv_attention_rows_kernel<HD, FMT, EXACT, ONE, TWO>;
   static KvSmemSet set;
   if ((rc = set.ensure(reinterpret_cast<const void *>(kern), Sh::kSmem)) != TT_OK) return rc;
   TT_CUDA_TRY(launch_kernel(kern, dim3(p.ctas), dim3(kThreads), Sh::kSmem, stream, 1, a, p.row_blocks,
@@ -841,14 +844,14 @@ int launch_rows(const KvAttentionArgs &a, cudaStream_t stream) {
   return TT_OK;
 }
 
-template <int HD, bool ONE>
+template <int HD, int FMT, bool ONE>
 int launch_rows_of(const KvAttentionArgs &a, cudaStream_t stream) {
-  const bool i8 = a.c.format == TT_KV_INT8;
+  const bool two = ONE || a.dtype == TT_DTYPE_F32;
   if (a.c.hd == HD)
-    return i8 ? launch_rows<HD, TT_KV_INT8, true, ONE>(a, stream)
-              : launch_rows<HD, TT_KV_E4M3, true, ONE>(a, stream);
-  return i8 ? launch_rows<HD, TT_KV_INT8, false, ONE>(a, stream)
-            : launch_rows<HD, TT_KV_E4M3, false, ONE>(a, stream);
+    return two ? launch_rows<HD, FMT, true, ONE, true>(a, stream)
+               : launch_rows<HD, FMT, true, ONE, ONE>(a, stream);
+  return two ? launch_rows<HD, FMT, false, ONE, true>(a, stream)
+             : launch_rows<HD, FMT, false, ONE, ONE>(a, stream);
 }
 
 // The smallest width that holds a head_dim, 32, 64, 128 or 256, and whether a key
@@ -916,7 +919,10 @@ size_t kv_attention_ws_bytes(const KvView &c, int64_t tokens, int heads) {
 int launch_kv_attention(const KvAttentionArgs &a, cudaStream_t stream) {
   if (use_tiles(a.c, a.tokens, a.heads)) return launch_kv_attention_tiles(a, stream);
   return for_rows(a.c, (int64_t)a.tokens * a.group, [&](auto hd, auto one) {
-    return launch_rows_of<decltype(hd)::value, decltype(one)::value>(a, stream);
+    constexpr int HD = decltype(hd)::value;
+    constexpr bool ONE = decltype(one)::value;
+    return a.c.format == TT_KV_INT8 ? launch_rows_of<HD, TT_KV_INT8, ONE>(a, stream)
+                                    : launch_rows_of<HD, TT_KV_E4M3, ONE>(a, stream);
   });
 }
 
