@@ -64,14 +64,16 @@ constexpr int kThreads = 32 * kWarps;
 
 template <int HD, bool ONE>
 struct RowShape {
-  // groups of 16 tokens computed at once
-  static constexpr int GC = HD == 32 ? 4 : HD == 64 ? (ONE ? 4 : 2) : HD == 128 && ONE ? 2 : 1;
+  // groups of 16 tokens computed at once: as many as registers hold, since a group is
+  // one chain of dependent instructions. (head_dim 128, one group against two, fp32 rows:
+  // 8 rows 43 / 39 us and 32 rows 83 / 68 us, 4 sequences of 20000; one of 1500 23 / 17.)
+  static constexpr int GC = HD == 32 ? 4 : HD == 64 ? (ONE ? 4 : 2) : HD == 128 ? 2 : 1;
   // ... and copied at once: a step
   static constexpr int GR = HD == 32 ? 8 : HD == 64 ? 4 : GC;
   static constexpr int kStep = 16 * GR;              // tokens
   static constexpr int kOver = GR >= 4 ? 1 : 2;      // units of a segment besides its steps
   static constexpr int kWhole = GR >= 4 ? 2 : 4;     // steps of a segment that is never split
-  static constexpr int kStages = HD == 128 && !ONE ? 3 : 2;  // steps in a warp's ring
+  static constexpr int kStages = 2;  // steps in a warp's ring
   static constexpr uint32_t kStage = 2 * kStep * HD;  // bytes: keys, then values
   static constexpr uint32_t kSmem = kWarps * kStages * kStage;
   static constexpr int kCtas = HD == 256 && !ONE ? 2 : 3;  // per SM, as registers and shared memory allow
