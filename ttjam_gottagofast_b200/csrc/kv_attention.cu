@@ -12,9 +12,14 @@
 //
 // Tensor cores, m16n8k16: 16 tokens' codes, exact in fp16, are the 16-row operand of
 // both products (S^T = K q^T, O^T = V^T p^T), a block of 8 query rows of one key head
-// the 8 columns of the other. q and p are split into two fp16 pieces (22 significant
-// bits, as the forward's split-precision schedule), both added into the same sums,
-// so a step of one token has fp32 accuracy. p leaves the first product with the token
+// the 8 columns of the other. q and p of fp32 rows are split into two fp16 pieces (22
+// significant bits, as the forward's split-precision schedule; TWO), both added into
+// the same sums, so a step of one token has fp32 accuracy. 16-bit rows take one piece,
+// as in the tile kernel: q is exact in it, and p's rounding to 11 bits, at most half a
+// step of float16 and averaged over the tokens, adds to the output's own rounding (a
+// relative error of 2.9e-4 against 2.1e-4 for float16, none to be seen for bfloat16)
+// and saves half of the products (48.5 / 45.4 us for the grouped step below). A single
+// row (ONE) takes both pieces whatever its type, as its columns are there anyhow. p leaves the first product with the token
 // along the rows and enters the second along them too; a transposition of 8 x 8
 // fp16 values between registers (movmatrix) lies in between. Row q is scaled by a
 // power of two to have its largest element in [1, 2), p by 2^14 to stay clear of the
@@ -44,8 +49,8 @@
 // Measured, one new token a sequence: 2 sequences of 100000, 16 heads of 64, int8, 78
 // to 80 us with the join, its first kernel at 5.5 TB/s of codes (0.84 of a plain
 // copy's rate), bound by memory and by instructions (0.54 of the issue slots); 64 of
-// up to 2048, e4m3, 37 us; 32 of up to 8192, 32 query heads on 4 of 128, e4m3, 48.5 us,
-// bound by the latency between dependent instructions, as registers leave 12 warps an
+// up to 2048, e4m3, fp32, 37 us; 32 of up to 8192, 32 query heads on 4 of 128, fp16 on
+// e4m3, 43 us, bound by the latency between dependent instructions, as registers leave 12 warps an
 // SM. One short sequence: 8 us, a chain of loads (length, page, scale, codes).
 #include <math_constants.h>
 
@@ -66,8 +71,9 @@ template <int HD, bool ONE>
 struct RowShape {
   // groups of 16 tokens computed at once: as many as registers hold, since a group is
   // one chain of dependent instructions. (head_dim 128, one group against two, fp32 rows:
-  // 8 rows 43 / 39 us and 32 rows 83 / 68 us, 4 sequences of 20000; one of 1500 23 / 17.)
-  static constexpr int GC = HD == 32 ? 4 : HD == 64 ? (ONE ? 4 : 2) : HD == 128 ? 2 : 1;
+  // 8 rows 43 / 39 us and 32 rows 83 / 68 us, 4 sequences of 20000; one of 1500 23 / 17. head_dim 64,
+  // two against four: 32 rows 126 / 119 us, 8 rows 47.9 / 47.3.)
+  static constexpr int GC = HD == 32 ? 4 : HD == 64 ? 4 : HD == 128 ? 2 : 1;
   // ... and copied at once: a step
   static constexpr int GR = HD == 32 ? 8 : HD == 64 ? 4 : GC;
   static constexpr int kStep = 16 * GR;              // tokens
@@ -873,9 +879,9 @@ int for_rows(const KvView &c, int64_t rows, F &&f) {
 // Rows of a key head from which the tile kernel takes over: it takes up to 128 rows in
 // the time of one, this file's kernel goes over the codes once for every 8. Measured,
 // e4m3, fp32 rows, this kernel / the tiles, us. 16 heads of 64: 16 sequences of 2000
-// tokens, 48 rows 89 / 94, 64 rows 113 / 93; 4 of 20000, 48 rows 179 / 160, 32 rows
-// 127 / 161. 32 heads of 128 on 4: 16 of 2000, 24 rows 37 / 39, 32 rows 45 / 39; 4 of
-// 20000, 32 rows 83 / 86, 48 rows 114 / 86. (One short sequence costs 15 to 25 us
+// tokens, 48 rows 85 / 94; 4 of 20000, 48 rows 167 / 160, 32 rows 119 / 161. 32 heads
+// of 128 on 4: 16 of 2000, 24 rows 33 / 39, 32 rows 39 / 39; 4 of 20000, 32 rows
+// 68 / 86, and 8 to 11 more for every 8 rows. (One short sequence costs 15 to 25 us
 // either way.)
 bool use_tiles(const KvView &c, int64_t tokens, int heads) {
   return tokens * (heads / c.heads) >= (c.hd <= 64 ? 56 : 40);

@@ -242,7 +242,8 @@ class KVCache:
         own. `scale` (default head_dim ** -0.5; positive) multiplies the scores. Returns
         (or writes to `out`, contiguous, sharing no memory with q) [batch,
         tokens, heads, head_dim] of q's type, computed to fp32 accuracy
-        (float16 and bfloat16 prompts may round the probabilities to 11 bits);
+        (float16 and bfloat16 rows, where a key head has several, round the
+        probabilities to 11 bits);
         rows behind new_tokens[b] are 0."""
         key = (layer, q.shape, q.stride(), q.dtype, q.get_device())
         plan = self._plans.get(key)
