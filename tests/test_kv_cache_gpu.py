@@ -310,6 +310,27 @@ def test_attend_moving_references_give_the_same_bits_every_time(tokens, heads, h
     assert cache.read_device_status() == (0, 0)
 
 
+@pytest.mark.parametrize("tokens,hd", [(1, 64), (4, 32), (4, 128), (70, 64), (70, 128), (70, 256)])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_attend_infinite_queries_give_nan(dtype, tokens, hd):
+    """All scores of a row with an infinity are infinite or NaN, and its softmax
+    is NaN, also where every one of them is minus infinity (the keys' first
+    element is negative throughout). Other rows, and rows that see no token, do
+    not know of it."""
+    cache, _ = kh.make(76, "int8", 3, 3, 1, hd, 64, [150, tokens, tokens])
+    cache.k[:, :, :, :, 0] = -5
+    cache.block_table[2, :] = -1
+    q = torch.randn((3, tokens, 1, hd), generator=torch.Generator().manual_seed(6)).to(DTYPES[dtype]).cuda()
+    want = cache.attend(q)
+    q[:, tokens - 1, 0, 0] = float("inf")
+    got = cache.attend(q)
+    assert torch.isnan(got[:2, -1]).all() and not got[2].any()
+    assert kh.same_bits(got[:, :-1], want[:, :-1]) and not torch.isnan(want).any()
+    q[:, tokens - 1, 0, 0] = float("nan")
+    got = cache.attend(q)
+    assert torch.isnan(got[:2, -1]).all() and not got[2].any()
+
+
 def test_two_graphs_at_once():
     """Two captured calls, each with a workspace of its own, replayed on two
     streams at the same time. 100 new tokens are more than the sequence of 64

@@ -391,7 +391,8 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
           if constexpr (TWO) qb[w][2] = lo[0], qb[w][3] = lo[1];
         }
       }
-      const float scale = a.scale * 1.4426950408889634f * kv_pow2(e);
+      float scale = a.scale * 1.4426950408889634f * kv_pow2(e);
+      if (mx == CUDART_INF_F) scale = CUDART_NAN_F;  // also where all its scores are -inf
 #pragma unroll
       for (int j = 0; j < NR; ++j) sc[j] = __shfl_sync(0xffffffffu, scale, 4 * (2 * tig + j));
     }

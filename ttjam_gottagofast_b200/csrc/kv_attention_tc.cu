@@ -645,6 +645,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
         }
       }
       sc = a.scale * 1.4426950408889634f * kv_pow2(e);
+      if (mx == CUDART_INF_F) sc = CUDART_NAN_F;  // also where all its scores are -inf
       if constexpr (Sh::QT) tmem_wait_st();
       else fence_async();
       fence_before();
