@@ -12,15 +12,13 @@
 //
 // Tensor cores, m16n8k16: 16 tokens' codes, exact in fp16, are the 16-row operand of
 // both products (S^T = K q^T, O^T = V^T p^T), a block of 8 query rows of one key head
-// the 8 columns of the other. q and p of fp32 rows are split into two fp16 pieces (22
-// significant bits, as the forward's split-precision schedule; TWO), both added into
-// the same sums, so a step of one token has fp32 accuracy. 16-bit rows take one piece,
-// as in the tile kernel: q is exact in it, and p's rounding to 11 bits, at most half a
-// step of float16 and averaged over the tokens, adds to the output's own rounding (a
-// relative error of 2.9e-4 against 2.1e-4 for float16, none to be seen for bfloat16)
-// and saves half of the products (48.5 / 45.4 us for the grouped step below). A single
-// row (ONE) takes both pieces whatever its type, as its columns are there anyhow. p leaves the first product with the token
-// along the rows and enters the second along them too; a transposition of 8 x 8
+// the 8 columns of the other. p, and q of fp32 rows (TWO), are split into two fp16
+// pieces (22 significant bits, as the forward's split-precision schedule), both added
+// into the same sums, so a row has fp32 accuracy before its one rounding to its own type.
+// q of 16-bit rows needs one piece (scaled as below, a bfloat16 element below 2^-15 of the
+// row's largest loses at most 2^-25 of that). With one piece of p, a float16 output was
+// 2.9e-4 off against 2.1e-4 for its own rounding. p leaves the first product with the
+// token along the rows and enters the second along them too; a transposition of 8 x 8
 // fp16 values between registers (movmatrix) lies in between. Row q is scaled by a
 // power of two to have its largest element in [1, 2), p by 2^14 to stay clear of the
 // fp16 subnormals.
@@ -587,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
           for (int x = 0; x < 2; ++x) {
             f16_split2(p[x][0], p[x][NR - 1], hi[x], lo[x]);
             pb[0][x] = transpose8(hi[x]);
-            if constexpr (TWO) pb[1][x] = transpose8(lo[x]);
+            pb[1][x] = transpose8(lo[x]);
           }
         }
       };
@@ -625,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
         } else {
           probabilities(g);
           b4[0][0] = pb[0][0], b4[0][1] = pb[0][1];
-          if constexpr (TWO) b4[1][0] = pb[1][0], b4[1][1] = pb[1][1];
+          b4[1][0] = pb[1][0], b4[1][1] = pb[1][1];
         }
         uint32_t va[VW][2][4];
 #pragma unroll
@@ -638,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
             va[w][i][0] = v0[2 * i], va[w][i][1] = v0[2 * i + 1];
             va[w][i][2] = v1[2 * i], va[w][i][3] = v1[2 * i + 1];
             mma16816(o[2 * w + i], va[w][i], b4[0][0], b4[0][1]);
-            if constexpr (TWO && !ONE) mma16816(o[2 * w + i], va[w][i], b4[1][0], b4[1][1]);
+            if constexpr (!ONE) mma16816(o[2 * w + i], va[w][i], b4[1][0], b4[1][1]);
           }
         }
       }

@@ -4,12 +4,13 @@
 // joins the exponent, p = 2^(s' + e - M + 7) with a whole-number reference M,
 // out = sum p code / sum p 2^-e; the codes, exact in fp16, are the B operands.
 //
-// PIECES: how many fp16 pieces q and p are split into. fp32 rows take two (22
-// significant bits). 16-bit rows take one: q, scaled by a power of two to have
-// its largest element in [1, 2), is exact in it (bf16 elements below 2^-17 of the
-// row's largest lose at most 2^-25 of that), and rounding p to 11 bits moves the
-// output by less than rounding it to its own type does; the sum of p is taken
-// before that rounding, in fp32.
+// PIECES: how many fp16 pieces q is split into. fp32 rows take two (22 significant
+// bits). 16-bit rows take one: q, scaled by a power of two to have its largest element
+// in [1, 2), is exact in it (bf16 elements below 2^-15 of the row's largest lose at
+// most 2^-25 of that). p takes two whatever the rows' type, so that a row has fp32
+// accuracy before its one rounding (the grouped prompt below takes 520 us; with one
+// piece of p 449, and outputs up to 2^-11 of their largest terms off); the sum of p is
+// taken before p is split, in fp32.
 //
 // CTA = (row tile, key head, sequence, split of the tokens): MT tiles of 128 query
 // rows (row = token * group + head of the group) against tiles of 64 tokens.
@@ -31,7 +32,7 @@
 // Bound by the softmax groups' instructions, exp2 and reads of tensor memory at
 // head_dim 64 (fp32, 4 x 2048 rows behind 2048, 16 heads: 103 GFLOP counted once, 257
 // us), by shared memory's rate under the products of 64 columns and the converters'
-// stores at 128 (bf16, 3 x 4096 rows, 32 heads on 4: 347 GFLOP, 448 us, 0.77 PFLOP/s).
+// stores at 128 (bf16, 3 x 4096 rows, 32 heads on 4: 347 GFLOP, 520 us, 0.67 PFLOP/s).
 // K and V tiles have a ring each. Every wait is bounded; one that gives up latches
 // TT_ERR_DEVICE_TIMEOUT in the cache's status word, and the kernel frees its tensor
 // memory and returns.
@@ -405,7 +406,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
 #pragma unroll
           for (int kk = 0; kk < TOK / 16; ++kk)
 #pragma unroll
-            for (int w = 0; w < PIECES; ++w)
+            for (int w = 0; w < 2; ++w)  // p's pieces
               mma_ts(tm + Sh::T_O + (uint32_t)(HD * x),
                      p + 32u * (kk >> 1) + 8u * (kk & 1) + 16u * w, vd0 + 128 * kk, Sh::IDESC_PV,
                      ((j % Sh::FLUSH) | kk | w) != 0);
@@ -731,19 +732,15 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
                                       make_float2(bs, bs));
             const float2 p = make_float2(exp2_approx(y.x), exp2_approx(y.y));
             sum = add_pair(sum, p);
-            if constexpr (PIECES == 2) {
-              const float2 hi = make_float2(upper11(p.x), upper11(p.y));
-              const float2 lo = fma_pair(hi, make_float2(-1.f, -1.f), p);
-              w[8 * g2 + i] = pack_f16(hi.x, hi.y);
-              w[16 + 8 * g2 + i] = pack_f16(lo.x, lo.y);
-            } else {
-              w[8 * g2 + i] = pack_f16(p.x, p.y);
-            }
+            const float2 hi = make_float2(upper11(p.x), upper11(p.y));
+            const float2 lo = fma_pair(hi, make_float2(-1.f, -1.f), p);
+            w[8 * g2 + i] = pack_f16(hi.x, hi.y);
+            w[16 + 8 * g2 + i] = pack_f16(lo.x, lo.y);
           }
           l = fmaf(sum.x + sum.y, exp2_approx(-ve[g]), l);
         }
         tmem_st16(t_s + 32u * half, w);
-        if constexpr (PIECES == 2) tmem_st16(t_s + 32u * half + 16u, w + 16);
+        tmem_st16(t_s + 32u * half + 16u, w + 16);
       }
     };
     for (int j = 0; j < nj; ++j) {

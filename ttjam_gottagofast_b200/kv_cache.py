@@ -241,10 +241,8 @@ class KVCache:
         position lengths[b] - new_tokens[b] + i and sees the tokens up to its
         own. `scale` (default head_dim ** -0.5; positive) multiplies the scores. Returns
         (or writes to `out`, contiguous, sharing no memory with q) [batch,
-        tokens, heads, head_dim] of q's type, computed to fp32 accuracy
-        (float16 and bfloat16 rows, where a key head has several, round the
-        probabilities to 11 bits);
-        rows behind new_tokens[b] are 0."""
+        tokens, heads, head_dim] of q's type, computed to fp32 accuracy and
+        rounded once; rows behind new_tokens[b] are 0."""
         key = (layer, q.shape, q.stride(), q.dtype, q.get_device())
         plan = self._plans.get(key)
         if plan is None:
