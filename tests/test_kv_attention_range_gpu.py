@@ -1,0 +1,53 @@
+"""Attention over the 8-bit cache at the ends of its range."""
+import pytest
+import torch
+
+import kv_helpers as kh
+from oracle import kv_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def _worst(got, exact, bound, half_step=2.0 ** -24):
+    """kh.worst, where a NaN on one side alone is as far off as can be."""
+    got = got.double().cpu()
+    off = (got - exact).abs()
+    share = torch.where(off == 0, 0.0, off / (bound + half_step * (exact.abs() + bound)))
+    return float(share.masked_fill(torch.isnan(got) & torch.isnan(exact), 0.0).nan_to_num(float("inf")).max())
+
+
+def _large_beside_small(seed, fmt, length, hd, heads, large, exponent, small):
+    """One page of 16 tokens with the value scale 2^exponent, the others with the least
+    one (codes 0 where `small` is "zero")."""
+    cache, _ = kh.make(seed, fmt, 1, -(-length // 16), heads, hd, 16, [length])
+    page = int(cache.block_table[0, large])
+    if small == "zero":
+        keep = cache.v[0, page].clone()
+        cache.v.view(torch.uint8).zero_()
+        cache.v[0, page] = keep
+    cache.v_scale.fill_(2.0 ** -64)
+    cache.v_scale[0, page] = 2.0 ** exponent
+    return cache, kh.mirror(cache)
+
+
+@pytest.mark.parametrize("small", ["zero", "least"])
+@pytest.mark.parametrize("exponent", [45, 63])
+@pytest.mark.parametrize("first", [True, False])
+@pytest.mark.parametrize("tokens,heads,kv_heads,hd,length,fmt", [
+    (1, 1, 1, 64, 100, "e4m3"), (1, 2, 2, 64, 9000, "int8"),  # a single row: whole segments, and joined ones
+    (1, 8, 1, 128, 100, "int8"), (1, 8, 1, 128, 9000, "e4m3"),
+    (4, 2, 1, 32, 5000, "int8"),
+    (150, 1, 1, 64, 300, "int8"), (150, 1, 1, 64, 6000, "e4m3"),  # tiles: one run of tokens, and shared out
+    (60, 1, 1, 128, 3000, "e4m3"), (60, 1, 1, 256, 2000, "int8")])
+def test_value_scales_far_apart(tokens, heads, kv_heads, hd, length, fmt, first, exponent, small):
+    """The largest values beside pages of zeros (scale 2^-64) or of the smallest values:
+    every token's weight counts in the denominator, whichever page comes first."""
+    large = 0 if first else (length - tokens) // 16 - (tokens == 1)
+    cache, want = _large_beside_small(300, fmt, length, hd, kv_heads, large, exponent, small)
+    q = torch.randn((1, tokens, heads, hd), generator=torch.Generator().manual_seed(7)).cuda()
+    got = cache.attend(q)
+    exact, size, total, reach = ref.attend(want, q.cpu(), [tokens], hd ** -0.5)
+    bound, _ = kh.attention_bound(size, total, reach, hd, length, torch.float32)
+    assert _worst(got, exact, bound) <= 1
+    assert float(exact[0, -1].abs().max()) > 2.0 ** (exponent - 12)
+    assert cache.read_device_status() == (0, 0)

@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
     // ONE: of group tig alone.
     constexpr int GS = ONE ? 1 : GC;
     auto compute = [&](auto masked_form, int g0, int t0, uint32_t absent) {
-      constexpr bool MASKED = decltype(masked_form)::value;
+      constexpr bool MASKED = decltype(masked_form)::value;  // or with value scales below kFarScale
       const uint32_t kb = ring + stage * Sh::kStage + 16 * g0 * hd;
       const uint32_t vb = kb + Sh::kStep * hd;
       float s[GS][2][NR];
@@ -547,8 +547,8 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
           for (int k = ONE ? 1 : 4; k < 32; k *= 2) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], k));
           const float mn = fmaxf(m[j], ceilf(top[j]));
           const float alpha = mn == m[j] ? 1.f : exp2_approx(m[j] - mn);  // 0 from -inf
+          l[j] = rescale(l[j], m[j] - mn, alpha);
           m[j] = mn;
-          l[j] *= alpha;
           beta[j] *= alpha;
 #pragma unroll
           for (int i = 0; i < 2 * VW; ++i)
@@ -565,15 +565,25 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
         float p[2][NR];
 #pragma unroll
         for (int j = 0; j < NR; ++j) {
+          auto powers = [&](float e, float *r) {
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            p[x][j] = exp2_approx(fmaf(s[g][x][j], ks[g] * sc[j], ve[g] + ref[j]));
-            // a NaN scale leaves NaN at the tokens behind the mask
-            if ((MASKED && !sees(g, x, j)) || (ONE && GC < 4 && tig >= GC)) p[x][j] = 0.f;
+            for (int x = 0; x < 2; ++x) {
+              r[x] = exp2_approx(fmaf(s[g][x][j], ks[g] * sc[j], e + ref[j]));
+              // a NaN scale leaves NaN at the tokens behind the mask
+              if ((MASKED && !sees(g, x, j)) || (ONE && GC < 4 && tig >= GC)) r[x] = 0.f;
+            }
+          };
+          float r[2];
+          powers(ve[g], r);
+          p[0][j] = r[0], p[1][j] = r[1];
+          if (MASKED && ve[g] < kFarScale) {
+            powers(0.f, r);
+            l[j] += r[0] + r[1];
+          } else {
+            // 2^-e; a NaN counts only where a token of its page is seen
+            const float sum = p[0][j] + p[1][j], more_l = fmaf(sum, exp2_approx(-ve[g]), l[j]);
+            l[j] = !(MASKED || (ONE && GC < 4)) || sum != 0.f ? more_l : l[j];
           }
-          // 2^-e; a NaN counts only where a token of its page is seen
-          const float sum = p[0][j] + p[1][j], more_l = fmaf(sum, exp2_approx(-ve[g]), l[j]);
-          l[j] = !(MASKED || (ONE && GC < 4)) || sum != 0.f ? more_l : l[j];
         }
         uint32_t hi[2], lo[2];
         if constexpr (ONE) {  // (high, low) of each token: the columns of group tig
@@ -651,12 +661,13 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
       __syncwarp();
       if (t0 < any_end) {  // the same for the whole warp
         const uint32_t absent = __ballot_sync(0xffffffffu, lane < GR && q_ks[0] < 0.f);
+        const bool far = __any_sync(0xffffffffu, lane < GR && q_vs[0] < kv_pow2((int)kFarScale));
 #pragma unroll 1
         for (int g0 = 0; g0 < GR; g0 += GC) {
           const int tg = t0 + 16 * g0;
           if (tg >= any_end) break;
           // where every live row sees every token, the form without masks
-          if (absent == 0 && tg + 16 * GC <= all_end) compute(std::false_type(), g0, tg, absent);
+          if (absent == 0 && !far && tg + 16 * GC <= all_end) compute(std::false_type(), g0, tg, absent);
           else compute(std::true_type(), g0, tg, absent);
         }
       }
@@ -678,6 +689,8 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
       const bool mine = r < rows_all && (!ONE || tig == 0);
       const float inv = tok >= count || l[j] == 0.f ? 0.f : 1.f / l[j];
       const int64_t at = (((int64_t)b * a.tokens + tok) * a.heads + h * a.group + r % a.group) * hd;
+      // a partial result's reference is made even: the join takes half of a difference
+      const float even = floorf(0.5f * m[j]) == 0.5f * m[j] ? 1.f : 0.5f;
 #pragma unroll
       for (int w = 0; w < VW; ++w) {
         const int d = out_dim<HD>(w, 0, gid);
@@ -685,14 +698,15 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
         float4 *part = sums(w, j, v);
         if (!mine) continue;
         if (!done) {
-          *part = make_float4(v[0], v[1], v[2], v[3]);
+          *part = make_float4(v[0] * even, v[1] * even, v[2] * even, v[3] * even);
         } else if (EXACT || d < hd) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) v[i] = inv == 0.f ? 0.f : v[i] * inv;
           kv_store_out4(a.out, at + d, v);
         }
       }
-      if (mine && !done && gid == 0) slot[kRows * HD + n] = m[j], slot[kRows * HD + kRows + n] = l[j];
+      if (mine && !done && gid == 0)
+        slot[kRows * HD + n] = even == 1.f ? m[j] : m[j] + 1.f, slot[kRows * HD + kRows + n] = l[j] * even;
     }
     going = use.next(a, hr, whole) && use.to_step(a, hr, whole);
     // only now: the next kernel's CTAs would take this one's places on the SMs and
@@ -768,13 +782,14 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(KvAtten
     const float *const base = a.ws + rr * HD + d, *const ml = a.ws + kRows * HD + rr;
     auto slot = [&](int w) { return ((int64_t)w * 2 + (w == c0 ? 1 : 0)) * Sh::kSlot; };
     float m = -CUDART_INF_F, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    // (m, l, o) += (mk, lk, v); a sum of NaN scores has m = -inf and a NaN l
+    // (m, l, o) += (mk, lk, v); a sum of NaN scores has m = -inf and a NaN l. The factors
+    // 2^(m - mn) are squares, as l may need one below 2^-126 (rescale in kv_codes.cuh).
     auto add = [&](float mk, float lk, const float4 &v) {
       const float mn = fmaxf(m, mk);
-      const float fo = m == mn || !(l == l) ? 1.f : exp2_approx(m - mn);
-      const float fk = mk == mn || !(lk == lk) ? 1.f : exp2_approx(mk - mn);
+      const float ro = m == mn || !(l == l) ? 1.f : exp2_approx(0.5f * (m - mn)), fo = ro * ro;
+      const float rk = mk == mn || !(lk == lk) ? 1.f : exp2_approx(0.5f * (mk - mn)), fk = rk * rk;
       m = mn;
-      l = fmaf(l, fo, lk * fk);
+      l = fmaf(l * ro, ro, lk * rk * rk);
       o[0] = fmaf(o[0], fo, v.x * fk), o[1] = fmaf(o[1], fo, v.y * fk);
       o[2] = fmaf(o[2], fo, v.z * fk), o[3] = fmaf(o[3], fo, v.w * fk);
     };

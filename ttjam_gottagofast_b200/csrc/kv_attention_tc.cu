@@ -266,7 +266,8 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
   constexpr int SCALES = Sh::SCALES;
   extern __shared__ uint8_t smem_raw[];
   __shared__ float s_ks[SCALES][GROUPS], s_ve[SCALES][GROUPS];
-  __shared__ uint32_t s_ok[SCALES];  // groups whose page exists
+  __shared__ float s_we[SCALES][GROUPS];  // 2^-ve, a weight over its p; 0 below kFarScale
+  __shared__ uint32_t s_ok[SCALES];       // groups whose page exists; above them, whether one is below kFarScale
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t *const smem = smem_raw + (base - raw);
@@ -544,10 +545,13 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
         if (lane < GROUPS) {
           const float v = vs[n];
           s_ks[j % SCALES][lane] = ks[n];
-          s_ve[j % SCALES][lane] = v == v ? (float)((__float_as_int(v) >> 23) - 127) : v;
+          const float e = v == v ? (float)((__float_as_int(v) >> 23) - 127) : v;
+          s_ve[j % SCALES][lane] = e;
+          s_we[j % SCALES][lane] = e < kFarScale ? 0.f : exp2_approx(-e);
         }
         const uint32_t okm = __ballot_sync(0xffffffffu, lane < GROUPS && ids[n] >= 0);
-        if (lane == 0) s_ok[j % SCALES] = okm;
+        const bool far = __any_sync(0xffffffffu, lane < GROUPS && vs[n] < kv_pow2((int)kFarScale));
+        if (lane == 0) s_ok[j % SCALES] = okm | (far ? 1u << GROUPS : 0u);
         __syncwarp();
         if (lane == 0) mbar_arrive(sc_full(j % SCALES));
       }
@@ -669,11 +673,12 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
     };
     // tile j's scores s[0 .. 63] to p, in the buffer that they came from
     auto softmax = [&](int j, bool open, float *s, uint32_t t_s) {
-      float kc[GROUPS], ve[GROUPS], top = -CUDART_INF_F;
+      float kc[GROUPS], ve[GROUPS], we[GROUPS], top = -CUDART_INF_F;
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) {
         kc[g] = s_ks[j % SCALES][g] * sc;
         ve[g] = s_ve[j % SCALES][g];
+        we[g] = s_we[j % SCALES][g];
       }
       if (!open) {  // the same for the warp
         const int left = end - (j0 + j) * TOK;  // tokens of the tile that this row sees
@@ -682,7 +687,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
         for (int g = 0; g < GROUPS; ++g) {
           const int n = (okm >> g) & 1u ? left - 16 * g : 0;
           // a group that the row sees nothing of: its scales, NaN perhaps, do not count
-          if (n <= 0) kc[g] = 1.f, ve[g] = 0.f;
+          if (n <= 0) kc[g] = 1.f, ve[g] = 0.f, we[g] = 0.f;
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[16 * g + i] = i < n ? s[16 * g + i] : -CUDART_INF_F;
         }
@@ -713,10 +718,20 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
           }
         }
         beta *= alpha;
-        l *= alpha;
+        l = rescale(l, m - mn, alpha);
         m = mn;
       }
       const float ref = 7.f - (m == -CUDART_INF_F ? 0.f : m);
+      if (!open && s_ok[j % SCALES] >> GROUPS) {  // weights that p may not stand for
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+          if (!(ve[g] < kFarScale)) continue;
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum += exp2_approx(fmaf(s[16 * g + i], kc[g], ref));
+          l += sum;
+        }
+      }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t w[32];
@@ -737,7 +752,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
             w[8 * g2 + i] = pack_f16(hi.x, hi.y);
             w[16 + 8 * g2 + i] = pack_f16(lo.x, lo.y);
           }
-          l = fmaf(sum.x + sum.y, exp2_approx(-ve[g]), l);
+          l = fmaf(sum.x + sum.y, we[g], l);
         }
         tmem_st16(t_s + 32u * half, w);
         tmem_st16(t_s + 32u * half + 16u, w + 16);
@@ -880,7 +895,7 @@ __global__ void __launch_bounds__(256) kv_attention_tiles_join_kernel(KvAttentio
     if (ls == 0.f) continue;  // a split that the row sees nothing of (its O may not exist)
     const float f = ms == m || !(ls == ls) ? 1.f : exp2_approx(ms - m);
     const float4 v = *reinterpret_cast<const float4 *>(a.ws + part(s) * HD + d);
-    l = fmaf(ls, f, l);
+    l += rescale(ls, ms - m, f);
     o[0] = fmaf(v.x, f, o[0]), o[1] = fmaf(v.y, f, o[1]);
     o[2] = fmaf(v.z, f, o[2]), o[3] = fmaf(v.w, f, o[3]);
   }

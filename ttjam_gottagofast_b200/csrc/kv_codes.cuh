@@ -47,6 +47,22 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// A token's p is 2^(s' + e - M + c), its weight in the sum of p 2^(s' - M + c), which is
+// p 2^-e as long as p is not flushed to 0 (below 2^-126). Where the value scale's exponent e
+// is at least kFarScale, a flushed p has a weight below 2^(-126 + 22), and the largest
+// weight is 2^(c - 64) >= 2^-57 at least (M is at most 64 above the largest s'): 2^23
+// such tokens together do not reach 2^-24 of the sum. Below kFarScale (a page of zeros, or of
+// magnitudes below 2^-14) the weights are computed by themselves.
+constexpr float kFarScale = -22.f;
+
+// x * 2^d for a sum of weights x, which may be 2^64 and more, and a whole number d <= 0,
+// minus infinity too; f is exp2_approx(d), which is flushed to 0 below 2^-126.
+__device__ __forceinline__ float rescale(float x, float d, float f) {
+  if (f != 0.f) return x * f;
+  const int n = (int)fmaxf(d, -252.f), h = n >> 1;
+  return x * kv_pow2(h) * kv_pow2(n - h);
+}
+
 __device__ __forceinline__ float kv_load_in(int dtype, const void *p, int64_t i) {
   if (dtype == TT_DTYPE_F32) return static_cast<const float *>(p)[i];
   if (dtype == TT_DTYPE_F16) return __half2float(static_cast<const __half *>(p)[i]);
