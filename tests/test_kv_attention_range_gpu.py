@@ -51,3 +51,35 @@ def test_value_scales_far_apart(tokens, heads, kv_heads, hd, length, fmt, first,
     assert _worst(got, exact, bound) <= 1
     assert float(exact[0, -1].abs().max()) > 2.0 ** (exponent - 12)
     assert cache.read_device_status() == (0, 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tokens,hd,size", [(3, 64, 1e-27), (70, 64, 1e-27), (70, 64, 1e-36), (70, 128, 1e-30),
+                                            (60, 256, 1e-33)])
+def test_keys_of_zero_under_queries_near_zero(tokens, hd, size, dtype):
+    """Scores of exactly 0, also where the factor of the scores underflows: the
+    output is the mean of the values seen."""
+    cache, _ = kh.make(310, "int8", 2, 8, 1, hd, 16, [tokens, tokens + 21])
+    cache.k.zero_()
+    cache.k_scale.fill_(2.0 ** -64)
+    want = kh.mirror(cache)
+    q = (torch.randn((2, tokens, 1, hd), generator=torch.Generator().manual_seed(3)) * size).to(dtype).cuda()
+    for scale in (None, 1e-30):
+        got = cache.attend(q, scale=scale)
+        exact, s, total, reach = ref.attend(want, q.cpu(), [tokens] * 2, scale or hd ** -0.5)
+        bound, half_step = kh.attention_bound(s, total, reach, hd, tokens + 21, dtype)
+        assert _worst(got, exact, bound, half_step) <= 1
+
+
+@pytest.mark.parametrize("tokens,hd", [(1, 64), (3, 64), (3, 128), (70, 64), (70, 128), (60, 256)])
+def test_pages_never_written_read_as_zeros(tokens, hd):
+    """A new cache whose lengths were advanced, nothing written."""
+    from ttjam_gottagofast_b200 import KVCache
+
+    cache = KVCache(2, 128, 1, hd, page_size=32)
+    cache.advance(tokens + 30)
+    q = torch.randn((2, tokens, 1, hd), generator=torch.Generator().manual_seed(3)).cuda()
+    for k in (q, q * 1e-30):
+        assert torch.equal(cache.attend(k), torch.zeros_like(q))
+    assert not cache.read()[0].any()
+    assert cache.read_device_status() == (0, 0)

@@ -39,6 +39,7 @@
 #include <math_constants.h>
 
 #include <algorithm>
+#include <cfloat>
 
 #include "kv_cache.cuh"
 #include "kv_codes.cuh"
@@ -688,6 +689,8 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
           const int n = (okm >> g) & 1u ? left - 16 * g : 0;
           // a group that the row sees nothing of: its scales, NaN perhaps, do not count
           if (n <= 0) kc[g] = 1.f, ve[g] = 0.f, we[g] = 0.f;
+          // a factor that underflowed would make NaN of a masked score
+          if (kc[g] < FLT_MIN) kc[g] = FLT_MIN;
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[16 * g + i] = i < n ? s[16 * g + i] : -CUDART_INF_F;
         }
