@@ -395,7 +395,9 @@ size_t tt_kv_attention_workspace_bytes(const tt_kv_cache *cache, int64_t tokens,
  * reads key head h / (heads / kv_heads). Row i < counts[b] of sequence b stands at
  * position lengths[b] - counts[b] + i and sees the tokens up to its own:
  * out = softmax(scale * q k^T) v, computed to fp32 accuracy and rounded once to
- * `dtype`. out is
+ * `dtype`: an element of q counts to 2^-22 of itself or 2^-39 of its row's largest, a
+ * probability to 2^-22 of itself or 2^-31 of the largest product of a probability and a
+ * value's scale. out is
  * [batch, tokens, heads, head_dim], contiguous, 16-byte aligned, and may not share
  * memory with q; it is written in full: rows at or behind counts[b], and rows that
  * see no token, are 0. The workspace needs no initial value and holds nothing after the call;

@@ -83,3 +83,26 @@ def test_pages_never_written_read_as_zeros(tokens, hd):
         assert torch.equal(cache.attend(k), torch.zeros_like(q))
     assert not cache.read()[0].any()
     assert cache.read_device_status() == (0, 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("tokens,hd", [(1, 64), (3, 64), (3, 128), (70, 64), (70, 128), (60, 256)])
+def test_one_channel_of_a_query_far_above_the_others(tokens, hd, dtype):
+    """q's first channel is 2^13 times the others, and the keys are 0 there: the others
+    count with all of their bits. A score is off by (hd / 16 + 2) 2^-22 of the sum of
+    magnitudes (attention_bound), and the pieces of q lose 2^-22 of an element or 2^-39 of
+    the row's largest."""
+    length = tokens + 200
+    cache, _ = kh.make(320, "int8", 1, 20, 1, hd, 16, [length])
+    cache.k[..., 0] = 0
+    want = kh.mirror(cache)
+    q = torch.randn((1, tokens, 1, hd), generator=torch.Generator().manual_seed(3))
+    q[..., 0] = 2.0 ** 13
+    q = q.to(dtype).cuda()
+    got = cache.attend(q)
+    exact, size, total, _ = ref.attend(want, q.cpu(), [tokens], hd ** -0.5)
+    k = ref.read(want, "k", 0)[0][:, 0].abs()
+    qq = q[0, :, 0].double().abs().cpu()
+    reach = hd ** -0.5 * ((qq + qq.amax(-1, keepdim=True) * 2.0 ** -17) @ k.T).amax(-1)[None, :, None]
+    bound, half_step = kh.attention_bound(size, total, reach, hd, length, dtype)
+    assert _worst(got, exact, bound, half_step) <= 1

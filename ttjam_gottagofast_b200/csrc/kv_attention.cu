@@ -15,13 +15,13 @@
 // the 8 columns of the other. p, and q of fp32 rows (TWO), are split into two fp16
 // pieces (22 significant bits, as the forward's split-precision schedule), both added
 // into the same sums, so a row has fp32 accuracy before its one rounding to its own type.
-// q of 16-bit rows needs one piece (scaled as below, a bfloat16 element below 2^-15 of the
-// row's largest loses at most 2^-25 of that). With one piece of p, a float16 output was
+// q of 16-bit rows needs one piece (scaled as below, a bfloat16 element below 2^-28 of the
+// row's largest loses at most 2^-39 of that). With one piece of p, a float16 output was
 // 2.9e-4 off against 2.1e-4 for its own rounding. p leaves the first product with the
 // token along the rows and enters the second along them too; a transposition of 8 x 8
 // fp16 values between registers (movmatrix) lies in between. Row q is scaled by a
-// power of two to have its largest element in [1, 2), p by 2^14 to stay clear of the
-// fp16 subnormals.
+// power of two to have its largest element in [2^14, 2^15), p by 2^14, to stay clear of
+// the fp16 subnormals.
 //
 // Where a key head has a single query row (ONE: a step of one token without grouped
 // heads), the 8 columns hold the two pieces for each of 4 groups of 16 tokens instead:
@@ -373,8 +373,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
       }
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      int e = (__float_as_int(mx) >> 23) - 127;
-      e = mx > 0.f ? min(max(e, -126), 126) : 0;
+      const int e = q_exponent(mx);
       const float f = kv_pow2(-e);
 #pragma unroll
       for (int w = 0; w < KW; ++w) {

@@ -6,8 +6,8 @@
 //
 // PIECES: how many fp16 pieces q is split into. fp32 rows take two (22 significant
 // bits). 16-bit rows take one: q, scaled by a power of two to have its largest element
-// in [1, 2), is exact in it (bf16 elements below 2^-15 of the row's largest lose at
-// most 2^-25 of that). p takes two whatever the rows' type, so that a row has fp32
+// in [2^14, 2^15), is exact in it (bf16 elements below 2^-28 of the row's largest lose at
+// most 2^-39 of that). p takes two whatever the rows' type, so that a row has fp32
 // accuracy before its one rounding (the grouped prompt below takes 520 us; with one
 // piece of p 449, and outputs up to 2^-11 of their largest terms off); the sum of p is
 // taken before p is split, in fp32.
@@ -619,8 +619,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
 #pragma unroll
         for (int i = 0; i < 64; ++i) mx = fmaxf(mx, fabsf(v64[i]));
       }
-      int e = (__float_as_int(mx) >> 23) - 127;
-      e = mx > 0.f ? min(max(e, -126), 126) : 0;
+      const int e = q_exponent(mx);
       const float f = kv_pow2(-e);
 #pragma unroll
       for (int d = 0; d < HD; d += 16) {

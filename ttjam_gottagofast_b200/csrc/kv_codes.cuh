@@ -63,6 +63,14 @@ __device__ __forceinline__ float rescale(float x, float d, float f) {
   return x * kv_pow2(h) * kv_pow2(n - h);
 }
 
+// The exponent by which a row q with the largest magnitude mx is divided before its split
+// into fp16 pieces: that element comes to lie in [2^14, 2^15), so that a piece's least step,
+// 2^-24, is 2^-38 of it at most and one large channel takes no bits from the others.
+__device__ __forceinline__ int q_exponent(float mx) {
+  const int e = (__float_as_int(mx) >> 23) - 127;
+  return mx > 0.f ? min(max(e, -112), 127) - 14 : 0;
+}
+
 __device__ __forceinline__ float kv_load_in(int dtype, const void *p, int64_t i) {
   if (dtype == TT_DTYPE_F32) return static_cast<const float *>(p)[i];
   if (dtype == TT_DTYPE_F16) return __half2float(static_cast<const __half *>(p)[i]);
