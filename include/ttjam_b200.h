@@ -345,7 +345,10 @@ int tt_test_gelu(const float *x, float *y, int64_t n, void *stream);
  * latched as TT_ERR_DEVICE_FAULT in *status (detail 0x5100, 0x5200 or 0x5300)
  * and never followed: lengths and counts are clamped, tokens of a page that
  * does not exist are dropped when written, zero when read and unseen by the
- * attention.
+ * attention. A scale that tt_kv_write does not make (no power of two from 2^-64
+ * to 2^63, NaN, or the 0 of a page never written) is latched too (0x5400), by the
+ * attention and where tokens are appended to its page, and counts as NaN there;
+ * tt_kv_read multiplies by it as it is.
  * ------------------------------------------------------------------------ */
 
 #define TT_KV_E4M3 0 /* float8 e4m3 (torch.float8_e4m3fn) */

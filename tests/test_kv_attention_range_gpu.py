@@ -106,3 +106,40 @@ def test_one_channel_of_a_query_far_above_the_others(tokens, hd, dtype):
     reach = hd ** -0.5 * ((qq + qq.amax(-1, keepdim=True) * 2.0 ** -17) @ k.T).amax(-1)[None, :, None]
     bound, half_step = kh.attention_bound(size, total, reach, hd, length, dtype)
     assert _worst(got, exact, bound, half_step) <= 1
+
+
+@pytest.mark.parametrize("tokens,hd", [(1, 64), (3, 128), (70, 64), (70, 128), (60, 256)])
+@pytest.mark.parametrize("bad", [0.3, -1.0, 2.0 ** 70, 2.0 ** -70, float("inf")])
+@pytest.mark.parametrize("name", ["k_scale", "v_scale"])
+def test_scales_that_no_write_makes_are_latched(name, bad, tokens, hd):
+    """Attention takes a value scale by its exponent, so one that is no power of two, or out
+    of the format's range, would be wrong without a word: it counts as NaN and is latched.
+    Other heads and sequences do not know of it."""
+    cache, _ = kh.make(330, "int8", 2, 12, 2, hd, 16, [tokens + 90, tokens + 40])
+    q = torch.randn((2, tokens, 2, hd), generator=torch.Generator().manual_seed(3)).cuda()
+    want = cache.attend(q)
+    getattr(cache, name)[0, int(cache.block_table[0, 2]), 1] = bad
+    got = cache.attend(q)
+    assert cache.read_device_status() == (-7, 0x5400)
+    assert torch.isnan(got[0, :, 1]).all()
+    assert kh.same_bits(got[0, :, 0], want[0, :, 0]) and kh.same_bits(got[1], want[1])
+
+
+@pytest.mark.parametrize("bad", [0.3, -1.0, 2.0 ** 70, float("inf")])
+def test_appending_to_a_page_with_such_a_scale(bad):
+    """The page's older codes cannot be moved exactly: its scale becomes NaN, latched."""
+    cache, _ = kh.make(331, "int8", 2, 2, 1, 16, 16, [5, 16])
+    pages = cache.block_table[:, 0].tolist()
+    cache.k_scale[0, pages] = bad
+    cache.lengths.add_(torch.tensor([1, 0], dtype=torch.int32, device="cuda"))
+    x = torch.ones((2, 1, 1, 16), device="cuda")
+    cache.write(x, x, new_tokens=torch.tensor([1, 0], dtype=torch.int32, device="cuda"))
+    assert cache.read_device_status() == (-7, 0x5400)
+    assert torch.isnan(cache.k_scale[0, pages[0]]).all()
+    assert float(cache.k_scale[0, pages[1]]) == pytest.approx(bad)  # no new token there
+    cache.lengths.copy_(torch.tensor([6, 0], dtype=torch.int32, device="cuda"))
+    assert torch.isnan(cache.read(max_tokens=6)[0][0]).all()
+    # started anew, the page is as any other
+    cache.lengths.fill_(1)
+    cache.write(x, x)
+    assert torch.equal(cache.read(max_tokens=1)[0], x) and cache.read_device_status() == (0, 0)

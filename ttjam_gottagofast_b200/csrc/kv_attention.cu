@@ -277,10 +277,11 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
   // Lane g < GR looks group g's page up one step before its bytes are copied; its
   // scales wait in the lane's queue for as long as the bytes do in the ring. A
   // group without a page, or past the last seen token, copies nothing and has the
-  // key scale -1.
+  // key scale -1 and the value scale kNoPage.
   Cursor<HD, ONE> fill = use;
   bool more = true;
   int fill_end = seen_by_block(fill), fill_stage = 0, pg_next;
+  const float kNoPage = __int_as_float(1);  // no scale that a write makes
   float q_ks[S], q_vs[S];
   auto look_up = [&] {
     const int t0 = t0_of(fill.t) + 16 * lane;
@@ -296,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
   }
   auto issue = [&](float &ks, float &vs) {
     ks = -1.f;
-    vs = 1.f;
+    vs = kNoPage;
     const int h = fill.pair / row_blocks;
     if (pg_next >= 0) {  // lanes 0 .. GR - 1
       const uint32_t at = (uint32_t)pg_next * (uint32_t)c.heads + (uint32_t)h;
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
   look_up();
 #pragma unroll
   for (int s = 0; s < S; ++s) {
-    q_ks[s] = -1.f, q_vs[s] = 1.f;
+    q_ks[s] = -1.f, q_vs[s] = kNoPage;
     if (more) issue(q_ks[s], q_vs[s]);
     copies_commit();
   }
@@ -659,14 +660,20 @@ __global__ void __launch_bounds__(kThreads, RowShape<HD, ONE>::kCtas)
       copies_wait<S - 1>();
       __syncwarp();
       if (t0 < any_end) {  // the same for the whole warp
-        const uint32_t absent = __ballot_sync(0xffffffffu, lane < GR && q_ks[0] < 0.f);
-        const bool far = __any_sync(0xffffffffu, lane < GR && q_vs[0] < kv_pow2((int)kFarScale));
+        uint32_t absent = 0;
+        const bool odd = __any_sync(0xffffffffu, lane < GR && !usual_scales(q_ks[0], q_vs[0]));
+        if (odd) {
+          const bool none = q_ks[0] < 0.f && __float_as_uint(q_vs[0]) == __float_as_uint(kNoPage);
+          if (none) q_vs[0] = 1.f;
+          else if (lane < GR) q_ks[0] = kv_scale(q_ks[0], c.status), q_vs[0] = kv_scale(q_vs[0], c.status);
+          absent = __ballot_sync(0xffffffffu, lane < GR && none);
+        }
 #pragma unroll 1
         for (int g0 = 0; g0 < GR; g0 += GC) {
           const int tg = t0 + 16 * g0;
           if (tg >= any_end) break;
           // where every live row sees every token, the form without masks
-          if (absent == 0 && !far && tg + 16 * GC <= all_end) compute(std::false_type(), g0, tg, absent);
+          if (!odd && tg + 16 * GC <= all_end) compute(std::false_type(), g0, tg, absent);
           else compute(std::true_type(), g0, tg, absent);
         }
       }

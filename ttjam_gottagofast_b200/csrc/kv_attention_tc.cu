@@ -543,16 +543,18 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
     auto tile = [&](int j, auto n_c) -> bool {
       constexpr int n = decltype(n_c)::value;
       if (cw == 0) {
-        if (lane < GROUPS) {
-          const float v = vs[n];
-          s_ks[j % SCALES][lane] = ks[n];
-          const float e = v == v ? (float)((__float_as_int(v) >> 23) - 127) : v;
-          s_ve[j % SCALES][lane] = e;
-          s_we[j % SCALES][lane] = e < kFarScale ? 0.f : exp2_approx(-e);
+        float k = ks[n], e = (float)((__float_as_int(vs[n]) >> 23) - 127);
+        float w = __int_as_float((254 << 23) - __float_as_int(vs[n]));  // 2^-e
+        uint32_t okm = __ballot_sync(0xffffffffu, lane < GROUPS && ids[n] >= 0);
+        if (__any_sync(0xffffffffu, !usual_scales(ks[n], vs[n]))) {
+          const float v = kv_scale(vs[n], c.status);
+          k = kv_scale(ks[n], c.status);
+          e = v == v ? (float)((__float_as_int(v) >> 23) - 127) : v;
+          w = v == v ? (e < kFarScale ? 0.f : exp2_approx(-e)) : v;
+          if (__any_sync(0xffffffffu, e < kFarScale)) okm |= 1u << GROUPS;
         }
-        const uint32_t okm = __ballot_sync(0xffffffffu, lane < GROUPS && ids[n] >= 0);
-        const bool far = __any_sync(0xffffffffu, lane < GROUPS && vs[n] < kv_pow2((int)kFarScale));
-        if (lane == 0) s_ok[j % SCALES] = okm | (far ? 1u << GROUPS : 0u);
+        if (lane < GROUPS) s_ks[j % SCALES][lane] = k, s_ve[j % SCALES][lane] = e, s_we[j % SCALES][lane] = w;
+        if (lane == 0) s_ok[j % SCALES] = okm;
         __syncwarp();
         if (lane == 0) mbar_arrive(sc_full(j % SCALES));
       }

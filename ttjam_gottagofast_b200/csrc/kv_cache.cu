@@ -113,7 +113,9 @@ __global__ void __launch_bounds__(32 * block_warps(NW))
   constexpr int TOP_E = FMT == TT_KV_INT8 ? 6 : 8;
   constexpr uint32_t TOP_M = FMT == TT_KV_INT8 ? 0x7e0000u : 0x600000u;
   int e = (int)(mx >> 23) - 127 - TOP_E + ((mx & 0x7fffffu) > TOP_M);
-  const bool bad = mx >= 0x7f800000u || e > kKvMostExponent || !(old == old);
+  const bool odd = !kv_scale_ok(old);  // its codes cannot be moved exactly
+  if (odd && lane == 0) raise_status(c.status, TT_ERR_DEVICE_FAULT, kKvBadScale);
+  const bool bad = mx >= 0x7f800000u || e > kKvMostExponent || !(old == old) || odd;
   e = max(e, kKvLeastExponent);
   float scale = kv_pow2(bad ? 0 : e);
   if (!bad) scale = fmaxf(scale, old);

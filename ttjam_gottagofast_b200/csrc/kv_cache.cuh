@@ -31,6 +31,7 @@ constexpr int kKvMostExponent = 63;
 constexpr int kKvBadLength = 0x5100;  // lengths[b] outside [0, table_columns * page_size]
 constexpr int kKvBadCount = 0x5200;   // counts[b] outside [0, min(tokens, lengths[b])]
 constexpr int kKvBadPage = 0x5300;    // a block-table entry outside [0, num_pages)
+constexpr int kKvBadScale = 0x5400;   // a scale that no write makes
 
 struct KvView {
   uint8_t *k, *v;
@@ -89,6 +90,23 @@ __device__ __forceinline__ float kv_to_float(__nv_bfloat16 x) { return __bfloat1
 __device__ __forceinline__ void kv_store(float *p, float x) { *p = x; }
 __device__ __forceinline__ void kv_store(__half *p, float x) { *p = __float2half_rn(x); }
 __device__ __forceinline__ void kv_store(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
+
+// Whether s is a scale that a write makes: a power of two within the range, or NaN; or
+// the 0 of a page never written.
+__device__ __forceinline__ bool kv_scale_ok(float s) {
+  const uint32_t u = __float_as_uint(s), lo = (uint32_t)(kKvLeastExponent + 127) << 23,
+                 hi = (uint32_t)(kKvMostExponent + 127) << 23;
+  return ((u & 0x807fffffu) == 0 && u >= lo && u <= hi) || u == 0 || s != s;
+}
+// A scale as attention takes it, whose arithmetic needs a power of two: NaN, latched,
+// in place of any that is none; the least one for a page never written.
+__device__ __forceinline__ float kv_scale(float s, DeviceStatus *status) {
+  if (!kv_scale_ok(s)) {
+    raise_status(status, TT_ERR_DEVICE_FAULT, kKvBadScale);
+    return __int_as_float(0x7fc00000);
+  }
+  return s == 0.f ? kv_pow2(kKvLeastExponent) : s;
+}
 
 // Four codes to fp32 values (exact).
 template <int FMT>

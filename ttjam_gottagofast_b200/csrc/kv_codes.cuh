@@ -55,6 +55,15 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // magnitudes below 2^-14) the weights are computed by themselves.
 constexpr float kFarScale = -22.f;
 
+// Whether both scales of a page are as nearly all are: powers of two of the format's
+// range, the values' from kFarScale on.
+__device__ __forceinline__ bool usual_scales(float ks, float vs) {
+  constexpr uint32_t kLow = (uint32_t)(kKvLeastExponent + 127) << 23, kTop = (uint32_t)(kKvMostExponent + 127) << 23,
+                     kFar = (uint32_t)((int)kFarScale + 127) << 23;
+  const uint32_t k = __float_as_uint(ks), v = __float_as_uint(vs);
+  return ((k | v) & 0x807fffffu) == 0 && k - kLow <= kTop - kLow && v - kFar <= kTop - kFar;
+}
+
 // x * 2^d for a sum of weights x, which may be 2^64 and more, and a whole number d <= 0,
 // minus infinity too; f is exp2_approx(d), which is flushed to 0 below 2^-126.
 __device__ __forceinline__ float rescale(float x, float d, float f) {

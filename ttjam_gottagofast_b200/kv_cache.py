@@ -83,7 +83,8 @@ class KVCache:
                      lengths: torch.Tensor) -> "KVCache":
         """A cache over the caller's tensors, of the shapes and types the class
         names (all contiguous, on one device). Scales are powers of two: those
-        that `write` made, or a copy of them."""
+        that `write` made, or a copy of them; others count as NaN in `attend`,
+        and in `write` to the middle of their page (`read_device_status`)."""
         self = cls.__new__(cls)
         if block_table.dim() != 2 or k.dim() != 5:
             raise ValueError("k must be [layers, pages, kv_heads, page_size, head_dim] and "
@@ -278,7 +279,7 @@ class KVCache:
 
     def read_device_status(self) -> Tuple[int, int]:
         """Synchronise, return and clear (code, detail) latched by the kernels' checks
-        of lengths, counts and block-table entries; (0, 0) when all were in range."""
+        of lengths, counts, block-table entries and scales; (0, 0) when all were in range."""
         code, detail = ctypes.c_int32(0), ctypes.c_int32(0)
         stream = torch.cuda.current_stream(self.device).cuda_stream
         _lib.check(self._lib.tt_kv_read_status(self._structs[0], ctypes.byref(code),
