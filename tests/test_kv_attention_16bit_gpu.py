@@ -1,6 +1,6 @@
 """Attention over the 8-bit cache for float16 and bfloat16 rows: fp32 accuracy
 before the one rounding to the rows' type, whether a row is alone or has
-neighbours."""
+neighbours, and over long contexts."""
 import pytest
 import torch
 
@@ -58,3 +58,53 @@ def test_a_row_is_the_same_alone_and_with_neighbours(dtype):
     for n in (1, 9, 80):
         got = cache.attend(q[:, -n:])[:, -1:]
         assert not torch.isnan(got).any() and kh.worst(got, exact, bound, half_step) <= 1, n
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("hd,rows,batch", [(64, 70, 160), (128, 48, 160), (256, 40, 160), (128, 48, 30), (256, 40, 30)])
+def test_long_contexts_do_not_drift(hd, rows, batch, dtype):
+    """400000 tokens a sequence, in 160 sequences (over the same pages, read only), so
+    many that no sequence's tokens are shared out, or 30, whose tokens are. Tensor cores
+    add by rounding toward zero, which moves every sum the same way: the mean error along
+    the output's sign shows it. Sums are taken out after 4096 tokens (bfloat16: 8192), so a
+    run is at most 512 (1024) additions, two pieces for 16 tokens, each of which cuts the 16
+    products and the sum so far: below 2^-22 of that sum, 2^-13 (2^-12) of the output, and in
+    the mean, as the sum so far is half of the run's on average, half of that. All
+    else rounds both ways and is within attention_bound (whose runs are of 1024
+    tokens). The output's rounding is half a step, eps / 2, at most; the mean over
+    rows * hd * 2 elements, whose roundings fall anyhow, is below five times
+    eps / 4 / sqrt(rows * hd * 2)."""
+    length, page = 400000, 128
+    run = (4096 if dtype == "fp16" else 8192) / 8 * 2.0 ** -22
+    g = torch.Generator().manual_seed(5)
+    columns = length // page
+    ramp = torch.linspace(-1, 1, columns).view(-1, 1, 1, 1)
+    base = torch.linspace(20, 120, hd)[torch.randperm(hd, generator=g)]
+    k = torch.randint(-60, 61, (columns, 1, page, hd), generator=g).float()
+    k[..., :1] = ramp * 100
+    v = base * (0.6 + 0.4 * ramp) * (0.8 + 0.2 * torch.rand((columns, 1, page, hd), generator=g))
+    k, v = (x.round().to(torch.int8)[None].cuda() for x in (k, v))
+    from ttjam_gottagofast_b200 import KVCache
+
+    scales = [torch.full((1, columns, 1), 2.0 ** -6, device="cuda") for _ in range(2)]
+    table = torch.arange(columns, dtype=torch.int32, device="cuda").expand(batch, columns).contiguous()
+    cache = KVCache.from_tensors(k, v, *scales, table,
+                                 torch.full((batch,), length, dtype=torch.int32, device="cuda"))
+    q = torch.randn((batch, rows, 1, hd), generator=g) * 0.3
+    q[..., 0] = 2.0 * torch.randn((batch, rows, 1), generator=g)  # each row leans to a part of the context
+    q = q.to(DTYPES[dtype]).cuda()
+    got = cache.attend(q, scale=1.0)
+    assert cache.read_device_status() == (0, 0)
+    kk, vv = (x.double().view(length, hd) / 64 for x in (k, v))
+    hidden = torch.arange(length, device="cuda") > torch.arange(length - rows, length, device="cuda")[:, None]
+    bias, eps = 0.0, torch.finfo(q.dtype).eps
+    for b in (0, batch - 1):
+        qq = q[b, :, 0].double()
+        exact = torch.softmax((qq @ kk.T).masked_fill_(hidden, float("-inf")), -1) @ vv
+        reach = ((qq.abs() + qq.abs().amax(-1, keepdim=True) / 8) @ kk.abs().T).amax(-1)
+        bound, half_step = _bound(exact, vv.sum(0), reach, hd, length, q.dtype)  # every value is positive
+        off = got[b, :, 0].double() - exact
+        bound = bound + run * exact
+        assert bool((off.abs() <= bound + half_step * (exact + bound)).all())
+        bias += float((off / exact).mean()) / 2
+    assert abs(bias) <= run / 2 + 5 * eps / 4 / (rows * hd * 2) ** 0.5

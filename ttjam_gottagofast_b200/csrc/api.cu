@@ -836,7 +836,7 @@ static int cached_layout(const tt_config *cfg, int dtype, const tt_kv_cache *cac
   C->w = 2 * C->io;
   C->mask = C->w + WorkspaceLayout(C->ops, batch, tokens, true).total;
   C->attention = C->mask + align_up(T, 256);
-  C->total = C->attention + (T > 0 ? kv_attention_ws_bytes((*views)[0], tokens, cfg->num_heads) : 0);
+  C->total = C->attention + (T > 0 ? kv_attention_ws_bytes((*views)[0], TT_DTYPE_F32, tokens, cfg->num_heads) : 0);
   return TT_OK;
 }
 

@@ -935,8 +935,8 @@ int KvSmemSet::ensure(const void *kernel, size_t bytes, int regs) {
   return TT_OK;
 }
 
-size_t kv_attention_ws_bytes(const KvView &c, int64_t tokens, int heads) {
-  if (use_tiles(c, tokens, heads)) return kv_attention_tiles_ws_bytes(c, tokens, heads);
+size_t kv_attention_ws_bytes(const KvView &c, int dtype, int64_t tokens, int heads) {
+  if (use_tiles(c, tokens, heads)) return kv_attention_tiles_ws_bytes(c, dtype, tokens, heads);
   RowPlan p{};
   const int rc = for_rows(c, tokens * (heads / c.heads), [&](auto hd, auto one) {
     return rows_plan<decltype(hd)::value, decltype(one)::value>(c, tokens, heads, &p);

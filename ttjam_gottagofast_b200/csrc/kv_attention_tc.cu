@@ -60,7 +60,8 @@ struct TcShape {
   static constexpr uint32_t SLOT = BOXES * BOX;
   static constexpr uint32_t QBOX = 128 * 128;
   static constexpr uint32_t QBYTES = QT ? 0 : MT * PIECES * BOXES * QBOX;
-  static constexpr uint32_t SUMS = PIECES == 2 && HD == 64 ? MT * 128 * HD * 4 : 0;  // see FLUSH
+  static constexpr bool SUM_SMEM = HD == 64;  // see FLUSH
+  static constexpr uint32_t SUMS = SUM_SMEM ? MT * 128 * HD * 4 : 0;
   // Codes on their way, AHEAD tiles: up to head_dim 64 in shared memory, every thread's
   // own chunks, copied asynchronously (in registers, loads share the few scoreboards,
   // and a wait for a page's number is one for the codes behind it: prompt 265 us, in
@@ -94,13 +95,18 @@ struct TcShape {
   // slot, that is, once the softmax of tile j - 1 - NV is done.
   static constexpr int SCALES = 8;
   static_assert(NV + 1 <= SCALES, "scales");
-  // Tensor memory adds a product to O by rounding toward zero, so a long sum drifts
-  // (measured: 7e-6 of the output after 4096 tokens, in proportion to them).
-  // fp32 rows therefore take O out every FLUSH tiles (512 tokens; 1024 where shared
-  // memory has no room for the sums and they are kept in the rows' own places of the
-  // output) and start it anew.
-  static constexpr bool SUM_SMEM = PIECES == 2 && HD == 64;
-  static constexpr int FLUSH = PIECES == 2 ? (SUM_SMEM ? 512 : 1024) / TOK : INT32_MAX;
+  // Tensor memory adds a product to O by rounding toward zero, so a long sum drifts:
+  // 8.6e-9 of the output a token where the values have one sign. The softmax warps
+  // therefore take O out every flush() tiles and start it anew. The sum stands in shared
+  // memory at head_dim 64 (512 tokens); at wider heads in an fp32 row's partial result or
+  // its own place of the output (1024 tokens), or for 16-bit rows in the workspace, the 128
+  // rows of a tile side by side: float16 every 4096 tokens (3.5e-5, 1/14 of its half step),
+  // bfloat16 every 8192 (7e-5, 1/56).
+  static constexpr bool SUM_WS = PIECES == 1 && !SUM_SMEM;
+  static constexpr int MIN_FLUSH = (SUM_SMEM ? 512 : SUM_WS ? 4096 : 1024) / TOK;
+  __host__ __device__ static constexpr int flush(int dtype) {
+    return SUM_WS && dtype == TT_DTYPE_BF16 ? 2 * MIN_FLUSH : MIN_FLUSH;  // a power of two
+  }
   static constexpr int GROUPS = TOK / 16;  // of 16 tokens, each in one page
   static constexpr int NCH = TOK * HD / 16 / kConvThreads;  // 16-code chunks a converter thread
   static constexpr uint32_t IDESC_S =
@@ -307,6 +313,8 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
   const int nj = (int)((int64_t)tiles * (split + 1) / splits) - j0;
   const int active = min(MT, (live + 127) / 128);
 
+  const int flush = Sh::flush(a.dtype);  // tiles between two flushes of O
+
   // results of this thread's row, written where they belong
   const int64_t rows_padded = (int64_t)row_tiles * 128 * MT;
   auto part = [&](int r) {  // partial result of row r
@@ -411,7 +419,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
             for (int w = 0; w < 2; ++w)  // p's pieces
               mma_ts(tm + Sh::T_O + (uint32_t)(HD * x),
                      p + 32u * (kk >> 1) + 8u * (kk & 1) + 16u * w, vd0 + 128 * kk, Sh::IDESC_PV,
-                     ((j % Sh::FLUSH) | kk | w) != 0);
+                     ((j & (flush - 1)) | kk | w) != 0);
           mma_commit(j + 1 < nj ? o_done(x) : o_final(x));
           if (j + 2 < nj) {  // into the buffer that this product has read
             if (x == 0 && !(ok = wait_k(j + 2))) break;
@@ -664,7 +672,9 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
     const KvOut sum_out = splits > 1 ? KvOut{a.ws, nullptr, TT_DTYPE_F32} : a.out;
     const int64_t sum_at = splits > 1 ? part(r) * HD : at;
     const int sum_dims = alive ? (splits > 1 ? HD : c.hd) : 0;
-    float4 *const sums = reinterpret_cast<float4 *>(smem + Sh::SUM0) + x * 128 * (HD / 4) + t;
+    // ... or, a row tile at a time with 4 dims of its rows side by side
+    float4 *const sums = Sh::SUM_WS ? reinterpret_cast<float4 *>(a.ws + part(first) * HD) + t
+                                    : reinterpret_cast<float4 *>(smem + Sh::SUM0) + x * 128 * (HD / 4) + t;
     float m = -CUDART_INF_F, l = 0.f, beta = 0.f;  // beta: what the sum is scaled by when read next
     // O_x holds the products up to tile j - 1's, while tile j's scores are there but
     // not yet its p: tile j - 2's product came before those scores, so one parity is
@@ -709,7 +719,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       if (__any_sync(0xffffffffu, raise)) {
         const float mn = raise ? ceilf(top) : m;
         const float alpha = raise ? exp2_approx(m - mn) : 1.f;  // 0 from -inf
-        if (j % Sh::FLUSH != 0 && __any_sync(0xffffffffu, raise && m != -CUDART_INF_F)) {
+        if ((j & (flush - 1)) != 0 && __any_sync(0xffffffffu, raise && m != -CUDART_INF_F)) {
           wait_o_before(j);
 #pragma unroll 1
           for (int d = 0; d < HD; d += 16) {
@@ -762,6 +772,18 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
         tmem_st16(t_s + 32u * half + 16u, w + 16);
       }
     };
+    // o += beta times the flushed sums of dims d .. d + 15
+    auto add_sums = [&](int d, bool any, uint32_t *o) {
+      if (!any) return;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 v = sums[(d / 4 + i) * 128];
+        o[4 * i] = __float_as_uint(fmaf(v.x, beta, __uint_as_float(o[4 * i])));
+        o[4 * i + 1] = __float_as_uint(fmaf(v.y, beta, __uint_as_float(o[4 * i + 1])));
+        o[4 * i + 2] = __float_as_uint(fmaf(v.z, beta, __uint_as_float(o[4 * i + 2])));
+        o[4 * i + 3] = __float_as_uint(fmaf(v.w, beta, __uint_as_float(o[4 * i + 3])));
+      }
+    };
     for (int j = 0; j < nj; ++j) {
       const int t0 = (j0 + j) * TOK, buf = j & 1;
       mbar_wait(s_full(x, buf), (j >> 1) & 1, abort_w, c.status, 0x6600);
@@ -769,9 +791,21 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       // whether every live row sees every token (the same for the warp)
       const bool open = t0 + TOK <= all_end && s_ok[j % SCALES] == (1u << GROUPS) - 1u;
       fence_after();
-      if (PIECES == 2 && j > 0 && j % Sh::FLUSH == 0) {
+      if (j > 0 && (j & (flush - 1)) == 0) {
         wait_o_before(j);
-        if constexpr (Sh::SUM_SMEM) {
+        if constexpr (Sh::SUM_WS) {
+#pragma unroll 1
+          for (int d = 0; d < HD; d += 16) {
+            uint32_t o[16];
+            tmem_ld16(t_o + d, o);
+            tmem_wait_ld();
+            add_sums(d, j > flush, o);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              reinterpret_cast<uint4 *>(sums)[(d / 4 + i) * 128] =
+                  make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          }
+        } else if constexpr (Sh::SUM_SMEM) {
 #pragma unroll
           for (int d = 0; d < HD; d += 32) {
             float o[32];
@@ -780,7 +814,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
               float4 v = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-              if (j > Sh::FLUSH) {
+              if (j > flush) {
                 const float4 w = sums[(d + i) / 4 * 128];
                 v.x = fmaf(w.x, beta, v.x), v.y = fmaf(w.y, beta, v.y);
                 v.z = fmaf(w.z, beta, v.z), v.w = fmaf(w.w, beta, v.w);
@@ -793,14 +827,14 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
           for (int d = 0; d < HD; d += 32) {
             float o[32], v[32];
             const bool mine = d < sum_dims, both = d + 16 < sum_dims;
-            if (j > Sh::FLUSH) {
+            if (j > flush) {
               if (mine) kv_load_sum16(sum_out, sum_at + d, v);
               if (both) kv_load_sum16(sum_out, sum_at + d + 16, v + 16);
             }
             __syncwarp();
             tmem_ld32(t_o + d, o);
             tmem_wait_ld();
-            if (j > Sh::FLUSH) {
+            if (j > flush) {
 #pragma unroll
               for (int i = 0; i < 32; ++i) o[i] = fmaf(v[i], beta, o[i]);
             }
@@ -824,13 +858,26 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
     mbar_wait(o_final(x), 0, abort_w, c.status, 0x6800);
     fence_after();
     const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (Sh::SUM_WS && nj > flush) {
+#pragma unroll 1
+      for (int d = 0; d < HD; d += 16) {
+        uint32_t o[16];
+        tmem_ld16(t_o + d, o);
+        tmem_wait_ld();
+        add_sums(d, true, o);
+        tmem_st16(t_o + d, o);
+      }
+      tmem_wait_st();
+      // the rows' partial results go where the others' sums stand
+      if (splits > 1) asm volatile("bar.sync %0, 128;" ::"r"(1 + x) : "memory");
+    }
 #pragma unroll
     for (int d = 0; d < HD; d += 16) {
       uint32_t o[16];
       tmem_ld16(t_o + d, o);
       tmem_wait_ld();
       float v[16];
-      if (PIECES == 2 && nj > Sh::FLUSH && (Sh::SUM_SMEM || d < sum_dims)) {
+      if (!Sh::SUM_WS && nj > flush && (Sh::SUM_SMEM || d < sum_dims)) {
         if constexpr (Sh::SUM_SMEM) {
 #pragma unroll
           for (int i = 0; i < 16; i += 4) {
@@ -917,7 +964,7 @@ struct TilePlan {
 };
 
 template <int HD, int PIECES>
-TilePlan tile_plan(const KvView &c, int64_t tokens, int heads, int sms) {
+TilePlan tile_plan(const KvView &c, int dtype, int64_t tokens, int heads, int sms) {
   using Sh = TcShape<HD, PIECES>;
   TilePlan p{};
   const int64_t rows = tokens * (heads / c.heads);
@@ -927,8 +974,9 @@ TilePlan tile_plan(const KvView &c, int64_t tokens, int heads, int sms) {
   const int64_t tiles = ceil_div((int64_t)c.columns << c.page_log2, Sh::TOK);
   // one CTA an SM: too few of them share the tokens, four tiles each at least
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(sms / std::max<int64_t>(ctas, 1), tiles / 4));
-  p.ws_bytes = p.splits > 1 ? (size_t)p.splits * c.batch * c.heads * p.rows_padded * (HD + 2) * sizeof(float)
-                            : 0;
+  const size_t rows_all = (size_t)c.batch * c.heads * p.rows_padded;
+  if (p.splits > 1) p.ws_bytes = p.splits * rows_all * (HD + 2) * sizeof(float);
+  else if (Sh::SUM_WS && tiles > Sh::flush(dtype)) p.ws_bytes = rows_all * HD * sizeof(float);
   return p;
 }
 
@@ -940,7 +988,7 @@ int launch_tiles(const KvAttentionArgs &a, cudaStream_t stream) {
   if (rc != TT_OK) return rc;
   if ((int64_t)a.tokens * a.group > kKvMost || a.c.batch > 65535 || a.c.heads > 65535)
     return fail(TT_ERR_UNSUPPORTED, "tt_kv_attention: too many rows, heads or sequences");
-  const TilePlan p = tile_plan<HD, PIECES>(a.c, a.tokens, a.heads, sms);
+  const TilePlan p = tile_plan<HD, PIECES>(a.c, a.dtype, a.tokens, a.heads, sms);
   if ((int64_t)p.row_tiles * a.c.heads > INT32_MAX)
     return fail(TT_ERR_UNSUPPORTED, "tt_kv_attention: too many rows");
   auto *kern = kv_attention_tiles_kernel<HD, FMT, PIECES>;
@@ -981,12 +1029,12 @@ int for_tiles(const KvView &c, int dtype, F &&f) {
 
 }  // namespace
 
-size_t kv_attention_tiles_ws_bytes(const KvView &c, int64_t tokens, int heads) {
+size_t kv_attention_tiles_ws_bytes(const KvView &c, int dtype, int64_t tokens, int heads) {
   int sms = 0;
   if (kv_sm_count(&sms) != TT_OK) return 0;
   size_t n = 0;
-  for_tiles(c, TT_DTYPE_F32, [&](auto hd, auto, auto pieces) {  // the same for every type
-    n = tile_plan<decltype(hd)::value, decltype(pieces)::value>(c, tokens, heads, sms).ws_bytes;
+  for_tiles(c, dtype, [&](auto hd, auto, auto pieces) {
+    n = tile_plan<decltype(hd)::value, decltype(pieces)::value>(c, dtype, tokens, heads, sms).ws_bytes;
     return TT_OK;
   });
   return n;

@@ -399,7 +399,7 @@ size_t tt_kv_attention_workspace_bytes(const tt_kv_cache *cache, int64_t tokens,
   if (tokens <= 0 || tokens > INT32_MAX || c.batch == 0 || heads <= 0 || heads % c.heads != 0 ||
       tokens * (heads / c.heads) > kKvMost)
     return 0;
-  return kv_attention_ws_bytes(c, tokens, heads);
+  return kv_attention_ws_bytes(c, TT_DTYPE_F16, tokens, heads);  // 16-bit rows may need the most
 }
 
 int tt_kv_attention(const tt_kv_cache *cache, int dtype, const void *q, const int64_t *q_strides,
@@ -424,7 +424,7 @@ int tt_kv_attention(const tt_kv_cache *cache, int dtype, const void *q, const in
   if (q == out) return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_attention: out may not alias q");
   if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15)
     return fail(TT_ERR_INVALID_ARGUMENT, "tt_kv_attention: out and workspace must be 16-byte aligned");
-  const size_t need = kv_attention_ws_bytes(c, tokens, heads);
+  const size_t need = kv_attention_ws_bytes(c, dtype, tokens, heads);
   if (workspace_bytes < need || (need > 0 && workspace == nullptr))
     return fail(TT_ERR_WORKSPACE, "tt_kv_attention: workspace smaller than "
                                   "tt_kv_attention_workspace_bytes (" + std::to_string(need) + " bytes)");

@@ -188,10 +188,10 @@ struct KvSmemSet {
   std::atomic<bool> done[64] = {};
   int ensure(const void *kernel, size_t bytes, int regs = 0);
 };
-size_t kv_attention_ws_bytes(const KvView &c, int64_t tokens, int heads);
+size_t kv_attention_ws_bytes(const KvView &c, int dtype, int64_t tokens, int heads);
 int launch_kv_attention(const KvAttentionArgs &a, cudaStream_t stream);
 // kv_attention_tc.cu
-size_t kv_attention_tiles_ws_bytes(const KvView &c, int64_t tokens, int heads);
+size_t kv_attention_tiles_ws_bytes(const KvView &c, int dtype, int64_t tokens, int heads);
 int launch_kv_attention_tiles(const KvAttentionArgs &a, cudaStream_t stream);
 
 }  // namespace tt
