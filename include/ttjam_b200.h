@@ -348,7 +348,9 @@ int tt_test_gelu(const float *x, float *y, int64_t n, void *stream);
  * attention. A scale that tt_kv_write does not make (no power of two from 2^-64
  * to 2^63, NaN, or the 0 of a page never written) is latched too (0x5400), by the
  * attention and where tokens are appended to its page, and counts as NaN there;
- * tt_kv_read multiplies by it as it is.
+ * tt_kv_read multiplies by it as it is. A bounded wait of the attention that runs out
+ * is latched as TT_ERR_DEVICE_TIMEOUT, and its output is not meaningful. Without a
+ * status word (NULL) none of these is reported.
  * ------------------------------------------------------------------------ */
 
 #define TT_KV_E4M3 0 /* float8 e4m3 (torch.float8_e4m3fn) */
@@ -429,6 +431,16 @@ size_t tt_cached_workspace_bytes(const tt_config *cfg, int dtype, const tt_kv_ca
 int tt_forward_cached(const tt_config *cfg, const void *image, int dtype, const void *x,
                       const tt_kv_cache *caches, const int32_t *counts, int64_t batch, int64_t tokens,
                       void *y, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Test support: shows that a bounded wait of the attention for many rows that runs out
+ * ends its kernel cleanly. Arms a one-shot switch: in the next launch, in this
+ * process, of that kernel (tt_kv_attention or tt_forward_cached with 56 and more rows a
+ * key head, 40 where head_dim is above 64) no block learns that its queries
+ * are there. The waits that this holds up run out after 2^28 cycles, about 0.15 s:
+ * TT_ERR_DEVICE_TIMEOUT is latched in the cache's status word, the kernel waits for what it
+ * has issued, frees its tensor memory and returns; that call's output is not
+ * meaningful, later calls are unaffected. Returns TT_OK. */
+int tt_test_arm_kv_wait_timeout(void);
 
 /* Synchronises `stream`, reads and clears the cache's status word: *code receives
  * TT_OK or the first latched TT_ERR_DEVICE_*, *detail which check it was. */

@@ -45,6 +45,7 @@ EXPORTED = (
     "tt_host_workspace_bytes", "tt_forward_host", "tt_test_gelu",
     "tt_kv_write", "tt_kv_read", "tt_kv_attention", "tt_kv_attention_workspace_bytes",
     "tt_kv_read_status", "tt_forward_cached", "tt_cached_workspace_bytes",
+    "tt_test_arm_kv_wait_timeout",
 )
 
 # Element types of the typed entry points (TT_DTYPE_*), by torch dtype name.
@@ -151,6 +152,8 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
         lib.tt_test_gelu.argtypes = [vp, vp, i64, vp]
         lib.tt_test_arm_wait_timeout.restype = ctypes.c_int
         lib.tt_test_arm_wait_timeout.argtypes = [ctypes.c_int]
+        lib.tt_test_arm_kv_wait_timeout.restype = ctypes.c_int
+        lib.tt_test_arm_kv_wait_timeout.argtypes = []
         kvp, i64p = ctypes.POINTER(TTKVCache), ctypes.POINTER(i64)
         lib.tt_kv_write.restype = ctypes.c_int
         lib.tt_kv_write.argtypes = [kvp, ctypes.c_int, vp, vp, i64p, i64p, i64, vp, vp]

@@ -47,6 +47,9 @@
 namespace tt {
 namespace {
 
+// tt_test_arm_kv_wait_timeout: whether the next launch of the tile kernel takes the switch
+std::atomic<bool> g_armed_timeout{false};
+
 constexpr int kConvWarps = 4, kConvThreads = 32 * kConvWarps;
 
 template <int HD_, int PIECES>
@@ -346,7 +349,7 @@ __global__ void __launch_bounds__(TcShape<HD, PIECES>::THREADS, 1)
       mbar_init(o_done(x), 1), mbar_init(o_final(x), 1);
     }
     for (int i = 0; i < SCALES; ++i) mbar_init(sc_full(i), 1);
-    mbar_init(q_ready, 4 * active);
+    mbar_init(q_ready, 4 * active + a.test_hold_back);  // 1: an arrival that never comes
     mbar_init(drain_bar, 1);
     *abort_w = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -997,8 +1000,10 @@ int launch_tiles(const KvAttentionArgs &a, cudaStream_t stream) {
   const int set_rc = set.ensure(reinterpret_cast<const void *>(kern), Sh::SMEM,
                                 Sh::SHIFT_REGS ? Sh::START_REGS : 0);
   if (set_rc != TT_OK) return set_rc;
+  KvAttentionArgs args = a;
+  args.test_hold_back = g_armed_timeout.exchange(false);  // test switch: this launch takes it
   TT_CUDA_TRY(launch_kernel(kern, dim3(p.row_tiles * a.c.heads, a.c.batch, p.splits), dim3(Sh::THREADS),
-                            Sh::SMEM, stream, 1, a, p.row_tiles, p.splits));
+                            Sh::SMEM, stream, 1, args, p.row_tiles, p.splits));
   if (p.splits > 1)
     TT_CUDA_TRY(launch_kernel(kv_attention_tiles_join_kernel<HD, FMT>,
                               dim3((unsigned)ceil_div((int64_t)a.tokens * a.group * (HD / 4), 256),
@@ -1047,3 +1052,8 @@ int launch_kv_attention_tiles(const KvAttentionArgs &a, cudaStream_t stream) {
 }
 
 }  // namespace tt
+
+extern "C" int tt_test_arm_kv_wait_timeout(void) {
+  tt::g_armed_timeout.store(true);
+  return TT_OK;
+}

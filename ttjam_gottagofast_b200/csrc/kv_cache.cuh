@@ -174,6 +174,7 @@ struct KvAttentionArgs {
   int dtype, tokens, heads, group;  // dtype: of q
   float scale;
   bool q_vec;  // q's rows are 16-byte aligned
+  int test_hold_back;  // set by the tile kernel's launcher (tt_test_arm_kv_wait_timeout)
 };
 
 // kv_attention.cu
