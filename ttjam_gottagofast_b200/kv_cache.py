@@ -119,9 +119,9 @@ class KVCache:
         self.num_layers, self.num_pages = layers, pages
         self.kv_heads, self.page_size, self.head_dim = heads, page, hd
         self.batch, self.max_tokens = batch, max_tokens
-        # An upper bound on lengths, which holds while nothing else has written into
-        # them: torch's count of the writes is still _seen, and no graph advances them.
-        self._longest, self._seen, self._captured = 0, None, False
+        # An upper bound on lengths, which holds as long as nothing else has written into
+        # them: torch's count of the writes is still _seen. None: the bound is not kept.
+        self._longest, self._seen = 0, None
         self._status = torch.zeros(2, dtype=torch.int32, device=k.device)
         self._lib = _lib.load()
         self._c_write, self._c_read = self._lib.tt_kv_write, self._lib.tt_kv_read
@@ -145,17 +145,19 @@ class KVCache:
     def advance(self, tokens: int, new_tokens: Optional[torch.Tensor] = None) -> None:
         """Add `tokens` new tokens to every sequence, or new_tokens[b], at most
         `tokens` and not negative, to sequence b. Refuses what `max_tokens` has
-        no room for. The host keeps a bound on the lengths, and reads them from
-        the device only when that does not settle it: near `max_tokens`, after
-        the caller wrote into `lengths`, and in a cache whose advance was
-        captured. (While a CUDA graph is captured, and in its replays, the host
-        cannot know the lengths; one beyond the room is then latched on the
-        device.)"""
+        no room for. As long as `advance` and `reset` alone change the lengths, the
+        host keeps a bound on them, and reads them from the device only near
+        `max_tokens`. Once anything else has written into `lengths`, a graph with it
+        or with an `advance` in it was captured, or `lengths_changed` was called,
+        and in a cache over the caller's tensors, every call reads them, as a
+        replay may change them unseen. (While a CUDA graph is captured, and in its
+        replays, the host cannot know the lengths; one beyond the room is then
+        latched on the device.)"""
         if tokens < 0:
             raise ValueError("tokens must be >= 0")
         new_tokens = self._counts(new_tokens)
+        known = self._bound_holds()
         if not torch.cuda.is_current_stream_capturing():
-            known = self._seen is not None and self._seen == self._writes() and not self._captured
             if not known or self._longest + tokens > self.max_tokens:
                 grown = self.lengths + (tokens if new_tokens is None else new_tokens)
                 longest = int(grown.max()) if self.batch else 0
@@ -166,17 +168,26 @@ class KVCache:
             else:
                 self._longest += tokens
         else:
-            self._captured = True
+            self._seen = None
         self.lengths.add_(tokens if new_tokens is None else new_tokens)
-        self._seen = self._writes()
+        if self._seen is not None:
+            self._seen = self.lengths._version
 
     def reset(self) -> None:
         """Forget every token (lengths 0); the pages stay where they are."""
+        known = self._bound_holds() and not torch.cuda.is_current_stream_capturing()
         self.lengths.zero_()
-        self._longest, self._seen = 0, self._writes()
+        self._longest, self._seen = 0, self.lengths._version if known else None
 
-    def _writes(self) -> Optional[int]:
-        return None if self.lengths.is_inference() else self.lengths._version
+    def lengths_changed(self) -> None:
+        """Say that `lengths` changes by means that torch does not count (kernels of the
+        caller's own, `.data`): from now on `advance` reads it on every call."""
+        self._seen = None
+
+    def _bound_holds(self) -> bool:
+        if self._seen is not None and self._seen != self.lengths._version:
+            self._seen = None
+        return self._seen is not None
 
     # ---- the operators ------------------------------------------------------
     # What a call's shapes, strides and types decide (its checks, the constant
