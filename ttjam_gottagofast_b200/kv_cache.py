@@ -291,8 +291,11 @@ class KVCache:
     def read_device_status(self) -> Tuple[int, int]:
         """Synchronise, return and clear (code, detail) latched by the kernels' checks
         of lengths, counts, block-table entries and scales; (0, 0) when all were in range."""
+        if _current_device() != self._index:  # a default stream is the current device's
+            with torch.cuda.device(self.device):
+                return self.read_device_status()
         code, detail = ctypes.c_int32(0), ctypes.c_int32(0)
-        stream = torch.cuda.current_stream(self.device).cuda_stream
+        stream = _raw_stream(self._index)
         _lib.check(self._lib.tt_kv_read_status(self._structs[0], ctypes.byref(code),
                                                ctypes.byref(detail), stream),
                    "tt_kv_read_status", self._lib)
