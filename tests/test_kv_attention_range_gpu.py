@@ -143,3 +143,31 @@ def test_appending_to_a_page_with_such_a_scale(bad):
     cache.lengths.fill_(1)
     cache.write(x, x)
     assert torch.equal(cache.read(max_tokens=1)[0], x) and cache.read_device_status() == (0, 0)
+
+
+@pytest.mark.parametrize("tokens,heads,hd", [(1, 2, 64), (3, 2, 128), (70, 2, 64), (130, 1, 128), (60, 1, 256)])
+def test_moving_references_give_numbers(tokens, heads, hd):
+    """Scores that grow along the sequence, so that sums are rescaled all the way."""
+    cache, _ = kh.make(72, "int8", 2, 20, heads, hd, 64, [1100, 700])
+    order = torch.arange(20).float()
+    for b in range(2):
+        cache.k_scale[0, cache.block_table[b].long()] = torch.exp2(torch.floor(order / 3) - 6)[:, None].cuda()
+    want = kh.mirror(cache)
+    q = torch.randn((2, tokens, heads, hd), generator=torch.Generator().manual_seed(3)).cuda()
+    got = cache.attend(q)
+    exact, size, total, reach = ref.attend(want, q.cpu(), [tokens] * 2, hd ** -0.5)
+    bound, _ = kh.attention_bound(size, total, reach, hd, 1100, torch.float32)
+    assert not torch.isnan(exact).any() and _worst(got, exact, bound) <= 1
+
+
+def test_shared_pages_and_a_padded_batch_give_numbers():
+    """Two sequences over the same pages, read only, padded to more rows than a
+    sequence has room for."""
+    cache, _ = kh.make(75, "e4m3", 2, 2, 1, 32, 16, [32, 20])
+    cache.block_table[1] = cache.block_table[0]
+    want = kh.mirror(cache)
+    q = torch.randn((2, 40, 3, 32), generator=torch.Generator().manual_seed(4)).cuda()
+    got = cache.attend(q, new_tokens=torch.tensor([2, 1], dtype=torch.int32, device="cuda"))
+    exact, size, total, reach = ref.attend(want, q.cpu(), [2, 1], 32 ** -0.5)
+    bound, _ = kh.attention_bound(size, total, reach, 32, 32, torch.float32)
+    assert _worst(got, exact, bound) <= 1 and not got[0, 2:].any() and not got[1, 1:].any()
