@@ -44,12 +44,14 @@
 // the segments that ended up on several warps. Where no segment is longer than
 // kWhole steps, warps take whole ones, and nothing is left to join.
 //
-// Measured, one new token a sequence: 2 sequences of 100000, 16 heads of 64, int8, 78
-// to 80 us with the join, its first kernel at 5.5 TB/s of codes (0.84 of a plain
-// copy's rate), bound by memory and by instructions (0.54 of the issue slots); 64 of
-// up to 2048, e4m3, fp32, 37 us; 32 of up to 8192, 32 query heads on 4 of 128, fp16 on
-// e4m3, 43 us, bound by the latency between dependent instructions, as registers leave 12 warps an
-// SM. One short sequence: 8 us, a chain of loads (length, page, scale, codes).
+// Measured, one new token a sequence: 2 sequences of 100000, 16 heads of 64, int8, 80
+// to 82 us with the join, its first kernel at 5.5 TB/s of codes (0.83 of a plain
+// copy's rate), bound by memory and by instructions (0.53 of the issue slots); 64 of
+// up to 2048, e4m3, fp32, 38 us; 32 of up to 8192, 32 query heads on 4 of 128, fp16 on
+// e4m3, 44 us, bound by the latency between dependent instructions, as registers leave 12 warps an
+// SM. One short sequence: 8 us, a chain of loads (length, page, scale, codes). One sequence
+// of 100000 with a single key head of 128: 148 us for one row, 258 for eight, nearly all of it the
+// join, whose few blocks add up hundreds of partial results each.
 #include <math_constants.h>
 
 #include <algorithm>
@@ -899,10 +901,9 @@ int for_rows(const KvView &c, int64_t rows, F &&f) {
 // Rows of a key head from which the tile kernel takes over: it takes up to 128 rows in
 // the time of one, this file's kernel goes over the codes once for every 8. Measured,
 // e4m3, fp32 rows, this kernel / the tiles, us. 16 heads of 64: 16 sequences of 2000
-// tokens, 48 rows 85 / 94; 4 of 20000, 48 rows 167 / 160, 32 rows 119 / 161. 32 heads
-// of 128 on 4: 16 of 2000, 24 rows 33 / 39, 32 rows 39 / 39; 4 of 20000, 32 rows
-// 68 / 86, and 8 to 11 more for every 8 rows. (One short sequence costs 15 to 25 us
-// either way.)
+// tokens, 48 rows 88 / 93; 4 of 20000, 48 rows 172 / 163, 32 rows 122 / 162. 32 heads
+// of 128 on 4: 16 of 2000, 24 rows 35 / 42, 32 rows 41 / 41; 4 of 20000, 32 rows
+// 68 / 93, 48 rows 91 / 93. (One short sequence costs 15 to 25 us either way.)
 bool use_tiles(const KvView &c, int64_t tokens, int heads) {
   return tokens * (heads / c.heads) >= (c.hd <= 64 ? 56 : 40);
 }

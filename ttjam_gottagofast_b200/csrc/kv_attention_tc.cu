@@ -8,9 +8,9 @@
 // bits). 16-bit rows take one: q, scaled by a power of two to have its largest element
 // in [2^14, 2^15), is exact in it (bf16 elements below 2^-28 of the row's largest lose at
 // most 2^-39 of that). p takes two whatever the rows' type, so that a row has fp32
-// accuracy before its one rounding (the grouped prompt below takes 520 us; with one
-// piece of p 449, and outputs up to 2^-11 of their largest terms off); the sum of p is
-// taken before p is split, in fp32.
+// accuracy before its one rounding (one piece of p took 70 us less of the grouped prompt
+// below, and was up to 2^-11 of the largest terms off); the sum of p is taken before p is
+// split, in fp32.
 //
 // CTA = (row tile, key head, sequence, split of the tokens): MT tiles of 128 query
 // rows (row = token * group + head of the group) against tiles of 64 tokens.
@@ -30,9 +30,9 @@
 //             4 x 2048 fp32 rows behind 2048, 16 heads of 64. Two threads a row
 //             instead of one: 279 us, the same work in more instructions.)
 // Bound by the softmax groups' instructions, exp2 and reads of tensor memory at
-// head_dim 64 (fp32, 4 x 2048 rows behind 2048, 16 heads: 103 GFLOP counted once, 257
+// head_dim 64 (fp32, 4 x 2048 rows behind 2048, 16 heads: 103 GFLOP counted once, 264
 // us), by shared memory's rate under the products of 64 columns and the converters'
-// stores at 128 (bf16, 3 x 4096 rows, 32 heads on 4: 347 GFLOP, 520 us, 0.67 PFLOP/s).
+// stores at 128 (bf16, 3 x 4096 rows, 32 heads on 4: 347 GFLOP, 556 us, 0.62 PFLOP/s).
 // K and V tiles have a ring each. Every wait is bounded; one that gives up latches
 // TT_ERR_DEVICE_TIMEOUT in the cache's status word, and the kernel frees its tensor
 // memory and returns.
