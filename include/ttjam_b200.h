@@ -390,9 +390,12 @@ int tt_kv_write(const tt_kv_cache *cache, int dtype, const void *k, const void *
 int tt_kv_read(const tt_kv_cache *cache, int dtype, void *k, void *v, int64_t max_tokens,
                void *stream);
 
-/* Bytes of scratch tt_kv_attention needs for `tokens` rows of `heads` query heads
- * on the current device (0 when it needs none, or for invalid arguments). */
+/* Bytes of scratch tt_kv_attention needs for `tokens` rows of `heads` query heads of any
+ * type, or of element type `dtype`, on the current device (0 when it needs none, or for
+ * invalid arguments). Many 16-bit rows over long caches need as much as their fp32 values. */
 size_t tt_kv_attention_workspace_bytes(const tt_kv_cache *cache, int64_t tokens, int32_t heads);
+size_t tt_kv_attention_typed_workspace_bytes(const tt_kv_cache *cache, int dtype, int64_t tokens,
+                                             int32_t heads);
 
 /* Causal attention of new tokens over the cache, which holds their keys and
  * values already (tt_kv_write). q is [batch, tokens, heads, head_dim] with

@@ -108,3 +108,18 @@ def test_long_contexts_do_not_drift(hd, rows, batch, dtype):
         assert bool((off.abs() <= bound + half_step * (exact + bound)).all())
         bias += float((off / exact).mean()) / 2
     assert abs(bias) <= run / 2 + 5 * eps / 4 / (rows * hd * 2) ** 0.5
+
+
+def test_scratch_for_long_sums_is_asked_for_16_bit_rows_alone():
+    """The sums of many 16-bit rows over a long cache stand in scratch as fp32 values; fp32
+    rows have theirs in the output, and short caches need none."""
+    from ttjam_gottagofast_b200 import KVCache, _lib
+
+    lib = _lib.load()
+    need = lambda c, dtype: lib.tt_kv_attention_typed_workspace_bytes(c._structs[0], dtype, 256, 2)  # noqa: E731
+    values = 160 * 256 * 2 * 128 * 4
+    for room, wanted in ((4096, (0, 0, 0)), (8192, (0, values, 0)), (8256, (0, values, values))):
+        c = KVCache(160, room, 2, 128, page_size=64)
+        assert tuple(need(c, d) for d in (0, 1, 2)) == wanted
+        assert lib.tt_kv_attention_workspace_bytes(c._structs[0], 256, 2) == max(wanted)
+        assert need(c, 3) == 0

@@ -45,7 +45,7 @@ EXPORTED = (
     "tt_host_workspace_bytes", "tt_forward_host", "tt_test_gelu",
     "tt_kv_write", "tt_kv_read", "tt_kv_attention", "tt_kv_attention_workspace_bytes",
     "tt_kv_read_status", "tt_forward_cached", "tt_cached_workspace_bytes",
-    "tt_test_arm_kv_wait_timeout",
+    "tt_test_arm_kv_wait_timeout", "tt_kv_attention_typed_workspace_bytes",
 )
 
 # Element types of the typed entry points (TT_DTYPE_*), by torch dtype name.
@@ -161,6 +161,8 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
         lib.tt_kv_read.argtypes = [kvp, ctypes.c_int, vp, vp, i64, vp]
         lib.tt_kv_attention_workspace_bytes.restype = sz
         lib.tt_kv_attention_workspace_bytes.argtypes = [kvp, i64, i32]
+        lib.tt_kv_attention_typed_workspace_bytes.restype = sz
+        lib.tt_kv_attention_typed_workspace_bytes.argtypes = [kvp, ctypes.c_int, i64, i32]
         lib.tt_kv_attention.restype = ctypes.c_int
         lib.tt_kv_attention.argtypes = [kvp, ctypes.c_int, vp, i64p, i64, i32, vp,
                                         ctypes.c_float, vp, vp, sz, vp]

@@ -393,13 +393,19 @@ int tt_kv_read(const tt_kv_cache *cache, int dtype, void *k, void *v, int64_t ma
   return launch_kv_read(c, dtype, k, v, max_tokens, static_cast<cudaStream_t>(stream));
 }
 
-size_t tt_kv_attention_workspace_bytes(const tt_kv_cache *cache, int64_t tokens, int32_t heads) {
+size_t tt_kv_attention_typed_workspace_bytes(const tt_kv_cache *cache, int dtype, int64_t tokens,
+                                             int32_t heads) {
   KvView c;
-  if (kv_view(cache, "tt_kv_attention_workspace_bytes", &c) != TT_OK) return 0;
+  if (kv_view(cache, "tt_kv_attention_workspace_bytes", &c) != TT_OK || !dtype_ok(dtype)) return 0;
   if (tokens <= 0 || tokens > INT32_MAX || c.batch == 0 || heads <= 0 || heads % c.heads != 0 ||
       tokens * (heads / c.heads) > kKvMost)
     return 0;
-  return kv_attention_ws_bytes(c, TT_DTYPE_F16, tokens, heads);  // 16-bit rows may need the most
+  return kv_attention_ws_bytes(c, dtype, tokens, heads);
+}
+
+size_t tt_kv_attention_workspace_bytes(const tt_kv_cache *cache, int64_t tokens, int32_t heads) {
+  // float16 rows need the most
+  return tt_kv_attention_typed_workspace_bytes(cache, TT_DTYPE_F16, tokens, heads);
 }
 
 int tt_kv_attention(const tt_kv_cache *cache, int dtype, const void *q, const int64_t *q_strides,

@@ -264,11 +264,12 @@ class KVCache:
             self._check(q, "q", q.shape[2])
             if q.stride(3) != 1:
                 return self.attend(q.contiguous(), new_tokens, layer, scale, out)
+            dtype = _dtype_code(q, "q")
             with torch.cuda.device(self.device):
-                nbytes = self._lib.tt_kv_attention_workspace_bytes(self._structs[0], q.shape[1],
-                                                                   q.shape[2])
-            plan = self._keep(key, (self._struct(layer), _dtype_code(q, "q"), _strides(q),
-                                    q.shape[1], q.shape[2], nbytes))
+                nbytes = self._lib.tt_kv_attention_typed_workspace_bytes(self._structs[0], dtype,
+                                                                         q.shape[1], q.shape[2])
+            plan = self._keep(key, (self._struct(layer), dtype, _strides(q), q.shape[1],
+                                    q.shape[2], nbytes))
         struct, dtype, strides, n, heads, nbytes = plan
         counts = None if new_tokens is None else self._counts(new_tokens)
         if _current_device() != self._index:
