@@ -30,9 +30,9 @@
 //             4 x 2048 fp32 rows behind 2048, 16 heads of 64. Two threads a row
 //             instead of one: 279 us, the same work in more instructions.)
 // Bound by the softmax groups' instructions, exp2 and reads of tensor memory at
-// head_dim 64 (fp32, 4 x 2048 rows behind 2048, 16 heads: 103 GFLOP counted once, 264
+// head_dim 64 (fp32, 4 x 2048 rows behind 2048, 16 heads: 103 GFLOP counted once, 265
 // us), by shared memory's rate under the products of 64 columns and the converters'
-// stores at 128 (bf16, 3 x 4096 rows, 32 heads on 4: 347 GFLOP, 556 us, 0.62 PFLOP/s).
+// stores at 128 (bf16, 3 x 4096 rows, 32 heads on 4: 347 GFLOP, 560 us, 0.62 PFLOP/s).
 // K and V tiles have a ring each. Every wait is bounded; one that gives up latches
 // TT_ERR_DEVICE_TIMEOUT in the cache's status word, and the kernel frees its tensor
 // memory and returns.
@@ -63,7 +63,7 @@ struct TcShape {
   static constexpr uint32_t SLOT = BOXES * BOX;
   static constexpr uint32_t QBOX = 128 * 128;
   static constexpr uint32_t QBYTES = QT ? 0 : MT * PIECES * BOXES * QBOX;
-  static constexpr bool SUM_SMEM = HD == 64;  // see FLUSH
+  static constexpr bool SUM_SMEM = HD == 64;  // see flush()
   static constexpr uint32_t SUMS = SUM_SMEM ? MT * 128 * HD * 4 : 0;
   // Codes on their way, AHEAD tiles: up to head_dim 64 in shared memory, every thread's
   // own chunks, copied asynchronously (in registers, loads share the few scoreboards,
